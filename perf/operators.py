@@ -13,9 +13,11 @@ Five kinds:
 
 The cache's format.  A row is the 64 values of one token, head and k or v.  It has one scale byte
 s and 64 e4m3 codes: a code c stands for c 2^(s - 127), s = max(e - 7, 10) for e the biased
-exponent of the row's largest magnitude, and codes round to nearest even.  A row with an infinity
-or a NaN has s = 255 and codes 0 and stands for NaN.  A page of 16 tokens is 16640 bytes: the codes
-of k [head][token][dim], those of v [head][dim][token], then the scales [head][k, v][token].
+exponent of the row's largest magnitude, and codes round to nearest even (at s = 247, the last, they
+stop at 240).  A row with an infinity
+or a NaN has s = 255 and stands for NaN (its codes: NaN in k, 0 in v).  A page of 16 tokens is 16640
+bytes: the codes of k [head][token][dim], those of v [head][token / 4][dim % 16][dim / 16][token % 4]
+(four tokens of a dimension in a word), then the scales [head][k, v][token].
 
 Attention: out = sum_j p_j v_j / (sum_j p_j + exp(sink)), p_j = exp(q . k_j / 8), over the keys up
 to the query's position, and within the window where there is one.
@@ -267,7 +269,7 @@ def _run_own(x):
 _CONCENTRATION = float(np.float32(0.1 * math.log(32.0) + 1.0))
 
 
-def _quantise(x):
+def _quantise(x, code_of_bad):
     """[..., 64] bf16 -> (codes [..., 64] and scale bytes [...], uint8)."""
     x = x.float()
     amax = x.abs().amax(-1)
@@ -275,14 +277,16 @@ def _quantise(x):
     bad = exponent == 255
     s = torch.where(bad, 255, (exponent - 7).clamp(min=10))
     inverse = ((254 - s.clamp(max=247)) << 23).view(F32)       # 2^(127 - s)
-    codes = torch.where(bad[..., None], 0.0, x * inverse[..., None]).to(FP8)
+    most = torch.where(s == 247, 240.0, 256.0)[..., None]
+    x = torch.minimum(torch.maximum(x * inverse[..., None], -most), most)
+    codes = torch.where(bad[..., None], code_of_bad, x).to(FP8)
     return codes.view(torch.uint8), s.to(torch.uint8)
 
 
 def _parts(cache):
     """Views of the pages: codes of k and of v, scales."""
     return (cache[:, :CODES].unflatten(1, (KVH, PAGE, DIM)),
-            cache[:, CODES:2 * CODES].unflatten(1, (KVH, DIM, PAGE)),
+            cache[:, CODES:2 * CODES].unflatten(1, (KVH, PAGE // 4, DIM // 4, 4, 4)),
             cache[:, 2 * CODES:].unflatten(1, (KVH, 2, PAGE)))
 
 
@@ -290,8 +294,9 @@ def _put(cache, slots, k, v):
     """k, v [n, 8, 64] bf16 -> the rows at slots [n]."""
     kc, vc, sc = _parts(cache)
     page, at = slots // PAGE, slots % PAGE
-    kc[page, :, at], sc[page, :, 0, at] = _quantise(k)
-    vc[page, :, :, at], sc[page, :, 1, at] = _quantise(v)
+    kc[page, :, at], sc[page, :, 0, at] = _quantise(k, math.nan)
+    codes, sc[page, :, 1, at] = _quantise(v, 0.0)
+    vc[page, :, at // 4, :, :, at % 4] = codes.unflatten(-1, (4, DIM // 4)).transpose(-1, -2)
 
 
 def _get(cache, slots):
@@ -299,7 +304,8 @@ def _get(cache, slots):
     kc, vc, sc = _parts(cache)
     page, at = slots // PAGE, slots % PAGE
     out = []
-    for codes, s in ((kc[page, :, at], sc[page, :, 0, at]), (vc[page, :, :, at], sc[page, :, 1, at])):
+    v = vc[page, :, at // 4, :, :, at % 4].transpose(-1, -2).flatten(-2)
+    for codes, s in ((kc[page, :, at], sc[page, :, 0, at]), (v, sc[page, :, 1, at])):
         factor = torch.where(s == 255, math.nan, (s.int() << 23).view(F32))
         out.append(codes.view(FP8).float() * factor[..., None])
     return out
@@ -412,7 +418,7 @@ def _stored(a):
     top = np.abs(a).max(-1, keepdims=True)
     _, e = np.frexp(top)                          # top = f 2^e, f in [0.5, 1)
     unit = np.exp2(np.maximum(np.where(top > 0, e - 1 - 7, -200), -117).astype(np.float64))
-    c = a / unit
+    c = np.where(top >= 2.0 ** 127, np.clip(a / unit, -240.0, 240.0), a / unit)
     _, e = np.frexp(c)
     step = np.exp2(np.maximum(e - 1, -6) - 3.0)   # e4m3: 3 fraction bits, exponents from -6
     return np.rint(c / step) * step * unit
@@ -431,15 +437,16 @@ def _decoded(cache, pages, low, total):
     c = np.arange(256)
     e, f = (c >> 3) & 15, c & 7
     value = np.where(e == 0, f / 8.0 * 2.0 ** -6, (1 + f / 8.0) * np.exp2(e - 7.0))
-    value = np.where(c & 128, -value, value)
+    value = np.where((c & 127) == 127, np.nan, np.where(c & 128, -value, value))
     table = torch.from_numpy(value).to(DEV)
     mine = cache[pages]
     p = mine.shape[0]
     scale = torch.exp2(mine[:, 2 * CODES:].view(p, KVH, 2, PAGE).double() - 127.0)
     k = table[mine[:, :CODES].int()].view(p, KVH, PAGE, DIM) * scale[:, :, 0, :, None]
-    v = table[mine[:, CODES:2 * CODES].int()].view(p, KVH, DIM, PAGE) * scale[:, :, 1, None, :]
+    v = table[mine[:, CODES:2 * CODES].int()].view(p, KVH, PAGE // 4, DIM // 4, 4, 4)
+    v = v.permute(0, 1, 2, 5, 4, 3).reshape(p, KVH, PAGE, DIM) * scale[:, :, 1, :, None]
     k = k.permute(0, 2, 1, 3).reshape(p * PAGE, KVH, DIM)
-    v = v.permute(0, 3, 1, 2).reshape(p * PAGE, KVH, DIM)
+    v = v.permute(0, 2, 1, 3).reshape(p * PAGE, KVH, DIM)
     return k[low:total], v[low:total]
 
 
