@@ -123,17 +123,17 @@ int attn_qkv_rope_append(const uint16_t* qkv, const uint16_t* qkv_bias, int64_t 
                                             as_stream(stream)));
 }
 
-// Workspace of attn_decode: the arrival counts [batch][8] (int32, padded to
-// 256 bytes; zero before the first call, left zero by every call), then the
-// split partials o [batch][64][splits][64] and (m, l) [batch][64][splits][2].
-static size_t decode_counts_bytes(int64_t batch) {
-  return ((size_t)batch * kKvHeads * 4 + 255) & ~(size_t)255;
-}
+// Workspace of attn_decode: the arrival counts [65536][8] (int32; zero before the
+// first call, left zero by every call), then the split partials o
+// [batch][64][splits][64] and (m, l) [batch][64][splits][2].  The counts' place
+// does not depend on the batch: a call's partials never lie where a call of more
+// sequences on the same workspace counts.
+constexpr size_t kDecodeCounts = (size_t)65536 * kKvHeads * 4;
 
 size_t attn_decode_workspace_bytes(int64_t batch, int64_t max_span) {
   if (batch <= 0 || max_span <= 0) return 0;
   const size_t parts = (size_t)batch * kQHeads * (size_t)decode_splits(batch, max_span);
-  return decode_counts_bytes(batch) + parts * (kHeadDim + 2) * sizeof(float) + 256;
+  return kDecodeCounts + parts * (kHeadDim + 2) * sizeof(float) + 256;
 }
 
 int attn_decode(const uint16_t* q, int64_t batch, const void* kv_cache, int64_t num_pages,
@@ -152,7 +152,7 @@ int attn_decode(const uint16_t* q, int64_t batch, const void* kv_cache, int64_t 
   const int64_t splits = decode_splits(batch, max_span);
   if (splits > 65535) return MOE_ERR_SHAPE;
   int* arrive = (int*)workspace;
-  float* part_o = (float*)((char*)workspace + decode_counts_bytes(batch));
+  float* part_o = (float*)((char*)workspace + kDecodeCounts);
   float* part_ml = part_o + (size_t)batch * kQHeads * splits * kHeadDim;
   return status(attn_launch_decode(q, (int)batch, kv_cache, page_indptr, page_indices,
                                    (int)num_pages, kv_len, window, sm_scale, sinks, (int)splits,

@@ -54,9 +54,9 @@ MOE_API int attn_qkv_rope_append(const uint16_t* qkv, const uint16_t* qkv_bias, 
 
 /* Workspace of attn_decode for `batch` sequences attending to at most
  * max_span keys each (min(kv_len, window) for sliding layers).  Its first
- * 32 x batch bytes are arrival counts that must be zero before the first call
- * on the workspace; every call leaves them zero (zero the whole workspace
- * once when it is allocated). */
+ * 2 MB are arrival counts that must be zero before the first call on the
+ * workspace; every call leaves them zero, whatever its batch (zero the whole
+ * workspace once when it is allocated). */
 MOE_API size_t attn_decode_workspace_bytes(int64_t batch, int64_t max_span);
 
 /* Decode attention: one query token per sequence, q [batch, 64, 64] bf16 at

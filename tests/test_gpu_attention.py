@@ -803,3 +803,24 @@ def test_prefill_attention_shared_keys_window(A, window, qlens, prefix):
         rows = slice(q_indptr[b], q_indptr[b + 1])
         o, lse = AO.attention(q[rows], seqs.k[b], seqs.v[b], np.arange(L - ql, L), window)
         close(got[rows], AO.sink_scale(o, lse, sinks))
+
+
+def test_decode_attention_workspace_of_other_batches(A):
+    """One workspace for a long single sequence and for a batch: the partials of the one do not
+    lie where the other counts its splits."""
+    one, many = PagedSeqs(101, [3000]), PagedSeqs(102, [900] * 12)
+    rng = np.random.default_rng(103)
+    q = bf(rng.standard_normal((12, HQ, D)))
+    sinks = bf(rng.standard_normal(HQ))
+    ws = A.decode_workspace(12, 4096)
+
+    def run(seqs, n, w):
+        out = torch.zeros((n, HQ, D), dtype=torch.bfloat16, device="cuda")
+        A.decode(bf16_dev(q[:n]), seqs.cache, seqs.page_indptr, seqs.page_indices, seqs.kv_len,
+                 4096, 0, SCALE, bf16_dev(sinks), out, w)
+        return host_bf16(out)
+
+    want = [run(one, 1, A.decode_workspace(1, 4096)), run(many, 12, A.decode_workspace(12, 4096))]
+    for _ in range(2):
+        np.testing.assert_array_equal(run(one, 1, ws), want[0])
+        np.testing.assert_array_equal(run(many, 12, ws), want[1])
