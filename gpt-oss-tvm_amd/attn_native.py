@@ -43,6 +43,15 @@ _SIGS = {
                                    _P], _INT),
     "attn_sample_workspace_bytes": ([_I64], _SZ),
     "attn_sample_top_p": ([_P, _I64, _I64, _F, _F, _F, _P, _P, _SZ, _P], _INT),
+    "attn_qkv_rope_append_fp8": ([_P, _P, _I64, _P, _P, _P, _F, _P, _I64, _P, _P], _INT),
+    "attn_kv_quantize_fp8": ([_P, _I64, _P, _I64, _P, _I64, _P, _P], _INT),
+    "attn_kv_read_fp8": ([_P, _I64, _P, _I64, _P, _P, _P], _INT),
+    "attn_decode_fp8_workspace_bytes": ([_I64, _I64], _SZ),
+    "attn_decode_fp8": ([_P, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _F, _P, _P, _P, _SZ, _P],
+                        _INT),
+    "attn_prefill_fp8_workspace_bytes": ([_I64, _I64, _I64, _I64, _I32], _SZ),
+    "attn_prefill_fp8": ([_P, _I64, _P, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _F, _P, _P,
+                          _P, _SZ, _P], _INT),
 }
 for _name, (_args, _ret) in _SIGS.items():
     _fn = getattr(_lib, _name)
@@ -312,3 +321,149 @@ def rows_qkv_rope_append(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor,
     most 3072)."""
     return _qkv_fused(_lib.attn_rows_qkv_rope_append, "attn_rows_qkv_rope_append", x, W, bias,
                       positions, slots, inv_freq, concentration, kv_cache, q_out, norm_w, eps)
+
+
+# -- the 8-bit KV cache: [pages, 16640] uint8 a layer (format in include/attn_gfx950.h) ----------
+
+FP8_PAGE_BYTES = 16640
+
+
+def _expect_fp8(kv_cache: torch.Tensor) -> None:
+    _expect(kv_cache, "kv_cache", torch.uint8)
+    if kv_cache.dim() != 2 or kv_cache.shape[1] != FP8_PAGE_BYTES:
+        raise ValueError(f"kv_cache: expected [pages, {FP8_PAGE_BYTES}], "
+                         f"got {tuple(kv_cache.shape)}")
+    _current(kv_cache, "kv_cache")
+
+
+def _current(t: torch.Tensor, name: str) -> None:
+    """The launch goes to the current device's stream."""
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name}: on {t.device}, the current device is "
+                         f"cuda:{torch.cuda.current_device()}")
+
+
+def _on(device: torch.device, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if t.device != device:
+            raise ValueError(f"{name}: on {t.device}, kv_cache on {device}")
+
+
+def qkv_rope_append_fp8(qkv: torch.Tensor, bias: torch.Tensor, positions: torch.Tensor,
+                        slots: torch.Tensor, inv_freq: torch.Tensor, concentration: float,
+                        kv_cache: torch.Tensor, q_out: torch.Tensor) -> torch.Tensor:
+    """``qkv_rope_append`` into the 8-bit cache: q as there, k and v quantised as they
+    are written.  Slots inside the pool have to differ."""
+    _expect_fp8(kv_cache)
+    _expect(qkv, "qkv", torch.bfloat16)
+    if qkv.dim() != 2 or qkv.shape[1] != QKV_DIM:
+        raise ValueError(f"qkv: expected [n, {QKV_DIM}], got {tuple(qkv.shape)}")
+    n = qkv.shape[0]
+    _expect(bias, "bias", torch.bfloat16, (QKV_DIM,))
+    _expect(positions, "positions", torch.int32, (n,))
+    _expect(slots, "slots", torch.int32, (n,))
+    _expect(inv_freq, "inv_freq", torch.float32, (HEAD_DIM // 2,))
+    _expect(q_out, "q_out", torch.bfloat16, (n, Q_HEADS, HEAD_DIM))
+    _on(kv_cache.device, qkv=qkv, bias=bias, positions=positions, slots=slots, inv_freq=inv_freq,
+        q_out=q_out)
+    _check(_lib.attn_qkv_rope_append_fp8(_ptr(qkv), _ptr(bias), n, _ptr(positions), _ptr(slots),
+                                         _ptr(inv_freq), concentration, _ptr(kv_cache),
+                                         kv_cache.shape[0], _ptr(q_out), _stream()),
+           "attn_qkv_rope_append_fp8")
+    return q_out
+
+
+def kv_quantize_fp8(src: torch.Tensor, src_slots: torch.Tensor, kv_cache: torch.Tensor,
+                    slots: torch.Tensor) -> torch.Tensor:
+    """Rows of a bf16 cache ``src`` [pages, 2, 8, 16, 64] at ``src_slots`` [n] into the 8-bit
+    cache at ``slots`` [n] (which have to differ)."""
+    _expect_fp8(kv_cache)
+    _expect(src, "src", torch.bfloat16)
+    if src.dim() != 5 or tuple(src.shape[1:]) != (2, KV_HEADS, PAGE, HEAD_DIM):
+        raise ValueError(f"src: expected [pages, 2, {KV_HEADS}, {PAGE}, {HEAD_DIM}], "
+                         f"got {tuple(src.shape)}")
+    _expect(src_slots, "src_slots", torch.int32, (src_slots.numel(),))
+    n = src_slots.numel()
+    _expect(slots, "slots", torch.int32, (n,))
+    _on(kv_cache.device, src=src, src_slots=src_slots, slots=slots)
+    _check(_lib.attn_kv_quantize_fp8(_ptr(src), src.shape[0], _ptr(src_slots), n, _ptr(kv_cache),
+                                     kv_cache.shape[0], _ptr(slots), _stream()),
+           "attn_kv_quantize_fp8")
+    return kv_cache
+
+
+def kv_read_fp8(kv_cache: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor | None = None,
+                v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The rows at ``slots`` [n] back as bf16: k and v [n, 8, 64], exact."""
+    _expect_fp8(kv_cache)
+    _expect(slots, "slots", torch.int32, (slots.numel(),))
+    n = slots.numel()
+    outs = [torch.empty((n, KV_HEADS, HEAD_DIM), dtype=torch.bfloat16, device=kv_cache.device)
+            if t is None else t for t in (k_out, v_out)]
+    for t, name in zip(outs, ("k_out", "v_out")):
+        _expect(t, name, torch.bfloat16, (n, KV_HEADS, HEAD_DIM))
+    _on(kv_cache.device, slots=slots, k_out=outs[0], v_out=outs[1])
+    _check(_lib.attn_kv_read_fp8(_ptr(kv_cache), kv_cache.shape[0], _ptr(slots), n, _ptr(outs[0]),
+                                 _ptr(outs[1]), _stream()), "attn_kv_read_fp8")
+    return outs[0], outs[1]
+
+
+def decode_fp8_workspace_bytes(batch: int, max_span: int) -> int:
+    return int(_lib.attn_decode_fp8_workspace_bytes(batch, max_span))
+
+
+def decode_fp8_workspace(batch: int, max_span: int, device="cuda") -> torch.Tensor:
+    """A zeroed attn_decode_fp8 workspace (its arrival counts must be zero before
+    the first call; every call leaves them zero)."""
+    return torch.zeros(max(decode_fp8_workspace_bytes(batch, max_span), 256), dtype=torch.uint8,
+                       device=device)
+
+
+def _tables_fp8(q, kv_cache, page_indptr, page_indices, kv_len, sinks, out, batch):
+    _expect_fp8(kv_cache)
+    _expect(q, "q", torch.bfloat16, (q.shape[0], Q_HEADS, HEAD_DIM))
+    _expect(page_indptr, "page_indptr", torch.int32, (batch + 1,))
+    _expect(page_indices, "page_indices", torch.int32)
+    _expect(kv_len, "kv_len", torch.int32, (batch,))
+    _expect(sinks, "sinks", torch.bfloat16, (Q_HEADS,))
+    _expect(out, "out", torch.bfloat16, (q.shape[0], Q_HEADS, HEAD_DIM))
+    _on(kv_cache.device, q=q, page_indptr=page_indptr, page_indices=page_indices, kv_len=kv_len,
+        sinks=sinks, out=out)
+
+
+def decode_fp8(q: torch.Tensor, kv_cache: torch.Tensor, page_indptr: torch.Tensor,
+               page_indices: torch.Tensor, kv_len: torch.Tensor, max_span: int, window: int,
+               sm_scale: float, sinks: torch.Tensor, out: torch.Tensor,
+               workspace: torch.Tensor) -> torch.Tensor:
+    """``decode`` over the 8-bit cache: softmax with the sink as a further logit, rounded
+    once; ``workspace`` from ``decode_fp8_workspace`` (reused by calls that follow one
+    another)."""
+    batch = q.shape[0]
+    _tables_fp8(q, kv_cache, page_indptr, page_indices, kv_len, sinks, out, batch)
+    _expect(workspace, "workspace", torch.uint8)
+    _on(kv_cache.device, workspace=workspace)
+    _check(_lib.attn_decode_fp8(_ptr(q), batch, _ptr(kv_cache), kv_cache.shape[0],
+                                _ptr(page_indptr), _ptr(page_indices), _ptr(kv_len), max_span,
+                                window, sm_scale, _ptr(sinks), _ptr(out), _ptr(workspace),
+                                workspace.numel(), _stream()), "attn_decode_fp8")
+    return out
+
+
+def prefill_fp8(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, kv_cache: torch.Tensor,
+                page_indptr: torch.Tensor, page_indices: torch.Tensor, kv_len: torch.Tensor,
+                window: int, sm_scale: float, sinks: torch.Tensor, out: torch.Tensor,
+                max_kv_len: int = 0) -> torch.Tensor:
+    """``prefill`` over the 8-bit cache (the formula of ``decode_fp8``): causal attention of
+    each sequence's new tokens over its cached ones.  ``max_kv_len`` as there."""
+    batch = q_indptr.numel() - 1
+    _tables_fp8(q, kv_cache, page_indptr, page_indices, kv_len, sinks, out, batch)
+    _expect(q_indptr, "q_indptr", torch.int32, (batch + 1,))
+    _on(kv_cache.device, q_indptr=q_indptr)
+    n = q.shape[0]
+    need = _lib.attn_prefill_fp8_workspace_bytes(n, batch, max_q_len, max_kv_len, window)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _check(_lib.attn_prefill_fp8(_ptr(q), n, _ptr(q_indptr), batch, max_q_len, _ptr(kv_cache),
+                                 kv_cache.shape[0], _ptr(page_indptr), _ptr(page_indices),
+                                 _ptr(kv_len), max_kv_len, window, sm_scale, _ptr(sinks),
+                                 _ptr(out), _ptr(ws), need, _stream()), "attn_prefill_fp8")
+    return out

@@ -1,6 +1,7 @@
 // C ABI of the attention-block entry points: argument validation, then the
 // launchers of attn_kernels.hip.  Declarations and reference citations:
 // include/attn_gfx950.h.
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -14,7 +15,7 @@ int attn_launch_rms_norm(const void* x, int n, int H, const void* w, float eps, 
                          hipStream_t s);
 int attn_launch_qkv_rope_append(const void* qkv, const void* bias, int n, const int* positions,
                                 const int* slots, const float* inv_freq, float conc, void* cache,
-                                int num_pages, void* q_out, hipStream_t s);
+                                int num_pages, void* q_out, bool fp8, hipStream_t s);
 int attn_launch_decode(const void* q, int batch, const void* cache, const int* page_indptr,
                        const int* page_indices, int num_pages, const int* kv_len, int window,
                        float sm_scale, const void* sinks, int splits, int cps, float* part_o,
@@ -46,6 +47,20 @@ int attn_launch_rows_qkv(const void* x, int M, int K, const void* W, const void*
                          void* q_out, hipStream_t s);
 int attn_launch_sample(const void* logits, int batch, int V, float temperature, float top_p,
                        float uniform, int* out, void* state, hipStream_t s);
+int attn_launch_fp8_quantize(const void* src, int src_pages, const int* src_slots, int n,
+                             void* cache, int num_pages, const int* slots, hipStream_t s);
+int attn_launch_fp8_read(const void* cache, int num_pages, const int* slots, int n, void* k_out,
+                         void* v_out, hipStream_t s);
+int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const int* page_indptr,
+                           const int* page_indices, int num_pages, const int* kv_len,
+                           int64_t max_span, int window, float sm_scale, const void* sinks,
+                           int splits, float* part_o, float* part_ml, int* arrive, void* out,
+                           hipStream_t s);
+int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
+                          const void* cache, const int* page_indptr, const int* page_indices,
+                          int num_pages, const int* kv_len, int window, float sm_scale,
+                          const void* sinks, void* out, int splits, int rows, float* part_o,
+                          float* part_ml, hipStream_t s);
 }
 
 namespace {
@@ -107,10 +122,10 @@ int attn_rms_norm(const uint16_t* x, int64_t n, int64_t H, const uint16_t* w, fl
   return status(attn_launch_rms_norm(x, (int)n, (int)H, w, eps, out, as_stream(stream)));
 }
 
-int attn_qkv_rope_append(const uint16_t* qkv, const uint16_t* qkv_bias, int64_t n,
-                         const int32_t* positions, const int32_t* slots, const float* inv_freq,
-                         float concentration, void* kv_cache, int64_t num_pages, uint16_t* q_out,
-                         moe_stream_t stream) {
+static int rope_append(const uint16_t* qkv, const uint16_t* qkv_bias, int64_t n,
+                       const int32_t* positions, const int32_t* slots, const float* inv_freq,
+                       float concentration, void* kv_cache, int64_t num_pages, uint16_t* q_out,
+                       bool fp8, moe_stream_t stream) {
   if (n < 0 || n > kMaxTokens || num_pages <= 0 || num_pages > kMaxPages) return MOE_ERR_SHAPE;
   if (n == 0) return MOE_OK;
   if (!qkv || !qkv_bias || !positions || !slots || !inv_freq || !kv_cache || !q_out)
@@ -119,8 +134,16 @@ int attn_qkv_rope_append(const uint16_t* qkv, const uint16_t* qkv_bias, int64_t 
       !a4(slots) || !a4(inv_freq))
     return MOE_ERR_ALIGN;
   return status(attn_launch_qkv_rope_append(qkv, qkv_bias, (int)n, positions, slots, inv_freq,
-                                            concentration, kv_cache, (int)num_pages, q_out,
+                                            concentration, kv_cache, (int)num_pages, q_out, fp8,
                                             as_stream(stream)));
+}
+
+int attn_qkv_rope_append(const uint16_t* qkv, const uint16_t* qkv_bias, int64_t n,
+                         const int32_t* positions, const int32_t* slots, const float* inv_freq,
+                         float concentration, void* kv_cache, int64_t num_pages, uint16_t* q_out,
+                         moe_stream_t stream) {
+  return rope_append(qkv, qkv_bias, n, positions, slots, inv_freq, concentration, kv_cache,
+                     num_pages, q_out, false, stream);
 }
 
 // Workspace of attn_decode: the arrival counts [65536][8] (int32; zero before the
@@ -356,6 +379,137 @@ int attn_rows_qkv_rope_append(const uint16_t* x, int64_t M, int64_t K, const uin
                               int64_t num_pages, uint16_t* q_out, moe_stream_t stream) {
   return qkv_rope_append(kRowsQkvTokens, x, M, K, W, norm_w, eps, qkv_bias, positions, slots,
                          inv_freq, concentration, kv_cache, num_pages, q_out, stream);
+}
+
+// ---------------------------------------------------------------------------
+// The 8-bit cache
+
+int attn_qkv_rope_append_fp8(const uint16_t* qkv, const uint16_t* qkv_bias, int64_t n,
+                             const int32_t* positions, const int32_t* slots, const float* inv_freq,
+                             float concentration, void* kv_cache, int64_t num_pages,
+                             uint16_t* q_out, moe_stream_t stream) {
+  if (num_pages >= kMaxPages) return MOE_ERR_SHAPE;
+  return rope_append(qkv, qkv_bias, n, positions, slots, inv_freq, concentration, kv_cache,
+                     num_pages, q_out, true, stream);
+}
+
+int attn_kv_quantize_fp8(const void* src, int64_t src_pages, const int32_t* src_slots, int64_t n,
+                         void* kv_cache, int64_t num_pages, const int32_t* slots,
+                         moe_stream_t stream) {
+  if (n < 0 || n > kMaxTokens || src_pages <= 0 || src_pages >= kMaxPages || num_pages <= 0 ||
+      num_pages >= kMaxPages)
+    return MOE_ERR_SHAPE;
+  if (n == 0) return MOE_OK;
+  if (!src || !src_slots || !kv_cache || !slots) return MOE_ERR_NULL;
+  if (!a16(src) || !a16(kv_cache) || !a4(src_slots) || !a4(slots)) return MOE_ERR_ALIGN;
+  return status(attn_launch_fp8_quantize(src, (int)src_pages, src_slots, (int)n, kv_cache,
+                                         (int)num_pages, slots, as_stream(stream)));
+}
+
+int attn_kv_read_fp8(const void* kv_cache, int64_t num_pages, const int32_t* slots, int64_t n,
+                     uint16_t* k_out, uint16_t* v_out, moe_stream_t stream) {
+  if (n < 0 || n > kMaxTokens || num_pages <= 0 || num_pages >= kMaxPages) return MOE_ERR_SHAPE;
+  if (n == 0) return MOE_OK;
+  if (!kv_cache || !slots || !k_out || !v_out) return MOE_ERR_NULL;
+  if (!a16(kv_cache) || !a4(slots) || !a16(k_out) || !a16(v_out)) return MOE_ERR_ALIGN;
+  return status(attn_launch_fp8_read(kv_cache, (int)num_pages, slots, (int)n, k_out, v_out,
+                                     as_stream(stream)));
+}
+
+namespace {
+constexpr int64_t kFp8Block = 64;  // keys of a block of the 8-bit attention kernels
+// 64-key blocks that a span of keys can touch
+int64_t fp8_blocks(int64_t span) { return (span + 2 * (kFp8Block - 1)) / kFp8Block; }
+
+// Splits of a sequence's keys, at least 4 blocks each (a wave of the workgroup takes
+// one).  The kernel shares a sequence's own blocks out over at most kFp8DecWgs
+// workgroups' worth of them, whatever max_span is: the bound only trims the grid.
+constexpr int64_t kFp8SplitBlocks = 4, kFp8MaxSplits = 64, kFp8DecWgs = 2048;
+int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
+  const int64_t most = std::max<int64_t>(
+      1, std::min(kFp8MaxSplits, kFp8DecWgs / (batch * kKvHeads)));
+  return std::max<int64_t>(1, std::min(most, fp8_blocks(max_span) / kFp8SplitBlocks));
+}
+
+constexpr int64_t kFp8ChunkTokens = 8, kFp8ChunkWgs = 1024;
+int64_t fp8_chunk_splits(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
+  if (batch <= 0 || batch > kFp8ChunkWgs || max_q_len <= 0) return 1;  // (and no overflow below)
+  const int64_t wgs = (max_q_len + kFp8ChunkTokens - 1) / kFp8ChunkTokens * batch * kKvHeads;
+  const int64_t keys = window > 0 ? std::min(max_kv_len, window + kFp8ChunkTokens) : max_kv_len;
+  if (keys <= 0) return 1;
+  const int64_t most = std::min(kFp8MaxSplits, kFp8ChunkWgs / wgs);
+  return std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks));
+}
+}  // namespace
+
+// Workspace of attn_decode_fp8: arrival counts as attn_decode's, then the splits'
+// o [splits][batch][64][64] and (m, l) [splits][batch][64][2].
+size_t attn_decode_fp8_workspace_bytes(int64_t batch, int64_t max_span) {
+  if (batch <= 0 || batch > 65535 || max_span <= 0 || max_span > kMaxPages * kPage) return 0;
+  const size_t parts = (size_t)batch * kQHeads * (size_t)fp8_decode_splits(batch, max_span);
+  return kDecodeCounts + parts * (kHeadDim + 2) * sizeof(float);
+}
+
+int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cache, int64_t num_pages,
+                    const int32_t* page_indptr, const int32_t* page_indices, const int32_t* kv_len,
+                    int64_t max_span, int32_t window, float sm_scale, const uint16_t* sinks,
+                    uint16_t* out, void* workspace, size_t workspace_bytes, moe_stream_t stream) {
+  if (batch < 0 || batch > 65535 || num_pages <= 0 || num_pages >= kMaxPages) return MOE_ERR_SHAPE;
+  if (batch == 0) return MOE_OK;
+  if (max_span <= 0 || max_span > kMaxPages * kPage) return MOE_ERR_SHAPE;
+  if (!(sm_scale > 0.0f && sm_scale <= FLT_MAX)) return MOE_ERR_UNSUPPORTED;
+  if (!q || !kv_cache || !page_indptr || !page_indices || !kv_len || !sinks || !out || !workspace)
+    return MOE_ERR_NULL;
+  if (!a16(q) || !a16(kv_cache) || !a16(out) || !a16(workspace) || !a4(page_indptr) ||
+      !a4(page_indices) || !a4(kv_len) || ((uintptr_t)sinks & 1u))
+    return MOE_ERR_ALIGN;
+  if (workspace_bytes < attn_decode_fp8_workspace_bytes(batch, max_span)) return MOE_ERR_WORKSPACE;
+  const int64_t splits = fp8_decode_splits(batch, max_span);
+  float* part_o = (float*)((char*)workspace + kDecodeCounts);
+  return status(attn_launch_fp8_decode(q, (int)batch, kv_cache, page_indptr, page_indices,
+                                       (int)num_pages, kv_len, max_span, window, sm_scale, sinks,
+                                       (int)splits, part_o,
+                                       part_o + (size_t)splits * batch * kQHeads * kHeadDim,
+                                       (int*)workspace, out, as_stream(stream)));
+}
+
+// Workspace: the splits' o [splits][rows][64][64], then (m, l) [splits][rows][64][2]
+size_t attn_prefill_fp8_workspace_bytes(int64_t rows, int64_t batch, int64_t max_q_len,
+                                        int64_t max_kv_len, int32_t window) {
+  if (rows <= 0 || rows > kMaxTokens || batch <= 0 || max_q_len <= 0 || max_q_len > kMaxTokens)
+    return 0;
+  const int64_t splits = fp8_chunk_splits(batch, max_q_len, max_kv_len, window);
+  return splits <= 1 ? 0 : (size_t)(splits * rows * kQHeads * (kHeadDim + 2)) * sizeof(float);
+}
+
+int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
+                     int64_t max_q_len, const void* kv_cache, int64_t num_pages,
+                     const int32_t* page_indptr, const int32_t* page_indices,
+                     const int32_t* kv_len, int64_t max_kv_len, int32_t window, float sm_scale,
+                     const uint16_t* sinks, uint16_t* out, void* workspace, size_t workspace_bytes,
+                     moe_stream_t stream) {
+  if (rows < 0 || rows > kMaxTokens || batch < 0 || max_q_len < 0 || max_q_len > kMaxTokens ||
+      num_pages <= 0 || num_pages >= kMaxPages)
+    return MOE_ERR_SHAPE;
+  if (rows == 0 || batch == 0 || max_q_len == 0) return MOE_OK;
+  const int64_t tiles = (max_q_len + kFp8ChunkTokens - 1) / kFp8ChunkTokens;
+  if (batch > kMaxTokens || tiles * batch * kKvHeads >= ((int64_t)1 << 24)) return MOE_ERR_SHAPE;
+  if (!(sm_scale > 0.0f && sm_scale <= FLT_MAX)) return MOE_ERR_UNSUPPORTED;
+  if (!q || !q_indptr || !kv_cache || !page_indptr || !page_indices || !kv_len || !sinks || !out)
+    return MOE_ERR_NULL;
+  if (!a16(q) || !a16(kv_cache) || !a16(out) || !a4(q_indptr) || !a4(page_indptr) ||
+      !a4(page_indices) || !a4(kv_len) || ((uintptr_t)sinks & 1u))
+    return MOE_ERR_ALIGN;
+  const size_t need = attn_prefill_fp8_workspace_bytes(rows, batch, max_q_len, max_kv_len, window);
+  if (need && !workspace) return MOE_ERR_NULL;
+  if (need && !a16(workspace)) return MOE_ERR_ALIGN;
+  if (workspace_bytes < need) return MOE_ERR_WORKSPACE;
+  const int64_t splits = need ? fp8_chunk_splits(batch, max_q_len, max_kv_len, window) : 1;
+  float* part_o = (float*)workspace;
+  return status(attn_launch_fp8_chunk(
+      q, q_indptr, (int)batch, (int)max_q_len, kv_cache, page_indptr, page_indices, (int)num_pages,
+      kv_len, window, sm_scale, sinks, out, (int)splits, (int)rows, part_o,
+      need ? part_o + splits * rows * kQHeads * kHeadDim : nullptr, as_stream(stream)));
 }
 
 }  // extern "C"

@@ -1,0 +1,562 @@
+// The 8-bit paged KV cache (gfx950): rows of a bf16 cache put into it, rows read
+// back, and the attention of decode and of chunks of new tokens over it.  The
+// format and its page layout: attn_common.h.  (The QKV epilogue that appends to
+// it is qkv_rope_append_kernel<true> of attn_kernels.hip.)
+#include "attn_common.h"
+
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ---------------------------------------------------------------------------
+// Rows of a bf16 cache (by slot) into the 8-bit cache (by slot): one wave a token,
+// lane (k or v, head, quarter of 16 dims).  A decode step's fused projections
+// write their rows to a few bf16 pages; this puts them away.
+__global__ __launch_bounds__(256) void fp8_quantize_kernel(
+    const uint8_t* __restrict__ src, int src_pages, const int* __restrict__ src_slots, int n,
+    uint8_t* __restrict__ cache, int num_pages, const int* __restrict__ slots) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= n) return;
+  const int kv = lane >> 5, hk = (lane >> 2) & 7, part = lane & 3;
+  const int from = src_slots[i], slot = slots[i];
+  if (from < 0 || from >= src_pages * kPage) return;
+  const uint8_t* row = src + ((((size_t)(from / kPage) * 2 + kv) * kHkv + hk) * kPage +
+                              from % kPage) * (kD * 2) + part * 32;
+  const u32x4 a = *(const u32x4*)row, b = *(const u32x4*)(row + 16);
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    top = max(max(top, a[j] & 0x7FFFu), (a[j] >> 16) & 0x7FFFu);
+    top = max(max(top, b[j] & 0x7FFFu), (b[j] >> 16) & 0x7FFFu);
+  }
+  const uint32_t s = fp8_scale_of(quad_max(top));
+  u32x4 codes;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    codes[j] = j < 2 ? fp8_codes(a[2 * j], a[2 * j + 1], s, kv)
+                     : fp8_codes(b[2 * j - 4], b[2 * j - 3], s, kv);
+  uint8_t* const page = fp8_page(cache, slot, num_pages);
+  if (!page) return;
+  const int token = slot % kPage;
+  if (kv == 0) {
+    *(u32x4*)(page + hk * kFp8Head + token * kFp8Row + part * 16) = codes;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      page[fp8_v_at(hk, token, part * 16 + j)] = (uint8_t)(codes[j >> 2] >> (8 * (j & 3)));
+  }
+  if (part == 0) page[fp8_scale_at(hk, kv, token)] = (uint8_t)s;
+}
+
+// Rows by slot back to bf16, k and v [n, 8, 64]: exact (a code has four
+// significant bits, and no value is below bf16's normal range); a row of scale
+// 255 gives NaN, a slot outside the pool zeros.  One wave a token.
+__global__ __launch_bounds__(256) void fp8_read_kernel(const uint8_t* __restrict__ cache,
+                                                       int num_pages,
+                                                       const int* __restrict__ slots, int n,
+                                                       uint16_t* __restrict__ k_out,
+                                                       uint16_t* __restrict__ v_out) {
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (i >= n) return;
+  const int kv = lane >> 5, hk = (lane >> 2) & 7, part = lane & 3;
+  const int slot = slots[i];
+  const uint8_t* const page = fp8_page(const_cast<uint8_t*>(cache), slot, num_pages);
+  u32x4 codes = u32x4{0u, 0u, 0u, 0u};
+  uint32_t s = kFp8MinScale;
+  if (page) {
+    const int token = slot % kPage;
+    if (kv == 0) {
+      codes = *(const u32x4*)(page + hk * kFp8Head + token * kFp8Row + part * 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        codes[j >> 2] |= (uint32_t)page[fp8_v_at(hk, token, part * 16 + j)] << (8 * (j & 3));
+    }
+    s = page[fp8_scale_at(hk, kv, token)];
+  }
+  const float scale = __uint_as_float(min(s, kFp8BadScale - 1u) << 23);
+  u32x4 lo = __builtin_bit_cast(u32x4, fp8_to_bf16(codes[0], codes[1], scale));
+  u32x4 hi = __builtin_bit_cast(u32x4, fp8_to_bf16(codes[2], codes[3], scale));
+  if (s == kFp8BadScale) lo = hi = u32x4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+  uint16_t* const dst = (kv ? v_out : k_out) + ((size_t)i * kHkv + hk) * kD + part * 16;
+  *(u32x4*)dst = lo;
+  *(u32x4*)(dst + 8) = hi;
+}
+
+// ---------------------------------------------------------------------------
+// Attention.  For a query at position p of a sequence and the keys j <= p (and
+// > p - window, where there is one):
+//   out = sum_j p_j v_j / (sum_j p_j + exp(sink)),  p_j = exp(sm_scale q . k_j)
+// rounded to bf16 once.  (The bf16 cache's form rounds o, the sink's factor and
+// their product, as the operators it restates do.)  A query that sees no key gets
+// 0.  Scores, maxima, sums and outputs in fp32; exponents in units of log2.
+
+// o over the sum and the sink's share, at the reference point m (log2).  l is 0
+// only where no key was seen (m is a key's score, so its p is 1).
+__device__ __forceinline__ float sink_share(float l, float m, uint16_t sink) {
+  return l == 0.0f ? 0.0f : 1.0f / (l + __builtin_amdgcn_exp2f(fmaf(bf2f(sink), kLog2e, -m)));
+}
+
+// How many splits a tile's `blocks` blocks of 64 keys are shared out over, at most
+// `most`: one per 4 blocks (each of a workgroup's waves then has one).  It follows
+// from the keys and `most`, so a caller's larger bound on the keys changes nothing.
+constexpr int kFp8Block = 64;
+constexpr int kFp8SplitBlocks = 4;
+struct Shares {
+  int each, used;  // blocks of a split, splits with any
+  __device__ __forceinline__ Shares(int blocks, int most) {
+    const int n = max(1, min(blocks / kFp8SplitBlocks, most));
+    each = (blocks + n - 1) / n;
+    used = each > 0 ? (blocks + each - 1) / each : 0;
+  }
+};
+
+// The keys that a tile's tokens see: positions lo .. last (none if last < lo).
+struct Sight {
+  int lo, last, first, blocks;  // first block of 64, number of blocks
+  __device__ __forceinline__ Sight(int pos, int tokens, int window) {
+    lo = window > 0 ? max(0, pos - window + 1) : 0;
+    last = pos + tokens - 1;
+    first = lo / kFp8Block;
+    blocks = last >= lo ? last / kFp8Block - first + 1 : 0;
+  }
+};
+
+// Few tokens: decode (kDecode: one token a sequence) and tiles of 2 kCt tokens of
+// a chunk.  Bound by the cache's bytes, so nothing but loads is on the way: a wave
+// takes blocks of 64 keys (four pages) alone, from global memory to registers,
+// no LDS and no barrier before the end.  Both products run on
+// v_mfma_f32_16x16x32_bf16 over columns (token, head of the group):
+//  * S^T = K Q^T: row r of score tile kk is key 4 kk + r % 4 of the block's page
+//    r / 4, so lane (r, g) loads 16 of its dims, 16 g .. 16 g + 15, and result
+//    element i of lane (column, g) is key 4 kk + i of page g;
+//  * O^T = V^T P^T: the lane's P operand then is its own scores, slots 4 kk + i of
+//    two products; V^T's slots the same keys of page g, dims 16 dt + r, as the
+//    cache holds them.
+// Codes go to bf16 exactly (k with its scale, whose row a lane holds alone; v
+// without: its scales multiply p); pv enters as two bf16 pieces, about 16 bits.
+// The loads of a block are in flight during the products of the one before.
+struct RowsArgs {
+  const uint16_t* q;
+  const int* q_indptr;  // chunks only
+  const uint8_t* cache;
+  const int* page_indptr;
+  const int* page_indices;
+  const int* kv_len;
+  const uint16_t* sinks;
+  uint16_t* out;
+  float* part_o;   // [splits][rows][64][64]
+  float* part_ml;  // [splits][rows][64][2]
+  int* arrive;     // decode: [batch][8], left zero
+  int64_t max_span;
+  int num_pages, window, splits, rows, tiles;
+  float c2;        // sm_scale log2(e)
+};
+
+struct KvRegs {
+  u32x4 k[4], v[4], ks, vs;
+};
+
+template <int kCt, bool kDecode>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
+  constexpr int kCols = 16 * kCt;
+  __shared__ __align__(16) float obuf[4][16][kD + 4];  // one column tile of each wave
+  __shared__ float mbuf[4][kCols], lbuf[4][kCols];
+  // x: (sequence, tile, kv head), y: split
+  const int hk = blockIdx.x % kHkv, share = blockIdx.y;
+  const int b = blockIdx.x / kHkv / a.tiles, tile = blockIdx.x / kHkv % a.tiles;
+  const int qb = kDecode ? b : a.q_indptr[b];
+  const int qn = kDecode ? 1 : a.q_indptr[b + 1] - qb;
+  const int t0 = tile * 2 * kCt;
+  if (t0 >= qn) return;
+  const int nt = kDecode ? 1 : min(2 * kCt, qn - t0);
+  const int L = a.kv_len[b], pos = L - qn + t0;  // of the tile's first token
+  const Sight sight(pos, nt, a.window);
+  const Shares shares(sight.blocks, a.splits);
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, r = lane & 15, g = lane >> 4;
+  const int row0 = qb + t0;
+  const bool too_long = kDecode && (int64_t)sight.last + 1 - sight.lo > a.max_span;
+  if (share >= max(shares.used, 1) || (too_long && share > 0)) return;
+  if (too_long) {
+    for (int i = t; i < kGroup * kD; i += 256)
+      a.out[((size_t)row0 * kHq + hk * kGroup) * kD + i] = 0x7FC0;
+    return;
+  }
+  const PageList pages{a.page_indices + a.page_indptr[b],
+                       a.page_indptr[b + 1] - a.page_indptr[b], a.num_pages};
+  const int last_page = max(0, min(pages.count - 1, (L - 1) / kPage));
+  const int begin = share * shares.each, end = min(begin + shares.each, sight.blocks);
+
+  // Q operand of column tile ct: column r is token 2 ct + r / 8, head r % 8
+  bf16x8 qv[kCt][2];
+#pragma unroll
+  for (int ct = 0; ct < kCt; ++ct) {
+    const int row = row0 + min(2 * ct + (r >> 3), nt - 1);
+    const u32x4* src = (const u32x4*)(a.q + ((size_t)row * kHq + hk * kGroup + (r & 7)) * kD);
+    qv[ct][0] = moe::as_bf16x8(src[2 * g]);
+    qv[ct][1] = moe::as_bf16x8(src[2 * g + 1]);
+  }
+  f32x4 o[kCt][4];
+  float m[kCt], l[kCt];
+#pragma unroll
+  for (int ct = 0; ct < kCt; ++ct) {
+    m[ct] = -INFINITY;
+    l[ct] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // The wave's blocks: begin + wave, + 4, ...  Lane 4 j + p holds the page p of the
+  // j-th of 16 blocks.
+  int ids = 0;
+  auto fetch_ids = [&](int blk) {
+    const int i = (sight.first + blk + 4 * (lane >> 2)) * 4 + (lane & 3);
+    ids = pages.count > 0 ? pages.clamp(pages.ids[min(i, last_page)]) : 0;
+  };
+  auto load = [&](KvRegs& x, int j) {  // the j-th of the wave's 16 at hand
+    const uint8_t* kp = a.cache + (size_t)__shfl(ids, 4 * j + (r >> 2), kWave) * kFp8Page;
+    const uint8_t* vp = a.cache + (size_t)__shfl(ids, 4 * j + g, kWave) * kFp8Page;
+    const uint8_t* kr = kp + hk * kFp8Head + (r & 3) * kFp8Row + g * 16;
+    const uint8_t* vr = vp + kFp8V + hk * kFp8Head + r * 16;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) x.k[kk] = *(const u32x4*)(kr + kk * 4 * kFp8Row);
+#pragma unroll
+    for (int qd = 0; qd < 4; ++qd) x.v[qd] = *(const u32x4*)(vr + qd * 256);
+    x.ks = *(const u32x4*)(kp + kFp8Scales + hk * 2 * kPage);
+    x.vs = *(const u32x4*)(vp + kFp8Scales + hk * 2 * kPage + kPage);
+  };
+  auto compute = [&](KvRegs& x, int kb) {  // kb: the block's first key
+    const int key0 = kb + 16 * g;          // this lane's page
+    if (kb + kFp8Block > L) {  // stale codes past the sequence's end may be NaN
+#pragma unroll
+      for (int qd = 0; qd < 4; ++qd) {
+        const int n = min(max(L - (key0 + 4 * qd), 0), 4);
+        const uint32_t keep = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) x.v[qd][dt] &= keep;
+      }
+    }
+    bf16x8 ka[4][2];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+      const uint32_t s = min((x.ks[kk] >> (8 * (r & 3))) & 255u, kFp8BadScale - 1u);
+      const float scale = __uint_as_float(s << 23);
+      ka[kk][0] = fp8_to_bf16(x.k[kk][0], x.k[kk][1], scale);
+      ka[kk][1] = fp8_to_bf16(x.k[kk][2], x.k[kk][3], scale);
+    }
+    bf16x8 va[4][2];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) {
+      va[dt][0] = fp8_to_bf16(x.v[0][dt], x.v[1][dt], 1.0f);
+      va[dt][1] = fp8_to_bf16(x.v[2][dt], x.v[3][dt], 1.0f);
+    }
+    // every token of the tile sees the whole block
+    const bool whole = kb + kFp8Block - 1 <= pos && (a.window <= 0 || kb > sight.last - a.window);
+#pragma unroll
+    for (int ct = 0; ct < kCt; ++ct) {
+      f32x4 st[4];
+      float mx = -INFINITY;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) {
+        st[kk] = mfma_bf16(ka[kk][0], qv[ct][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        st[kk] = mfma_bf16(ka[kk][1], qv[ct][1], st[kk]);
+      }
+      if (!whole) {
+        const int p = pos + min(2 * ct + (r >> 3), nt - 1);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = key0 + 4 * kk + i;
+            const bool ok = key <= p && (a.window <= 0 || key > p - a.window);
+            st[kk][i] = ok ? st[kk][i] : -INFINITY;
+          }
+      }
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[kk][i]);
+      const float mn = fmaxf(m[ct], group_max(mx) * a.c2);
+      if (__any(mn > m[ct])) {
+        const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - mn);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[ct][dt][i] *= alpha;
+        l[ct] *= alpha;
+        m[ct] = mn;
+      }
+      const float mneg = m[ct] == -INFINITY ? 0.0f : -m[ct];
+      float ps = 0.f;
+      bf16x8 ph[2], pl[2];
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(st[kk][i], a.c2, mneg));
+          ps += p;
+          // a bad row's scale byte gives an infinite factor: NaN from its codes 0
+          const float f = __uint_as_float(((x.vs[kk] >> (8 * i)) & 255u) << 23);
+          const float pv = whole || st[kk][i] != -INFINITY ? p * f : 0.0f;
+          const __bf16 hi = (__bf16)pv;
+          ph[kk >> 1][4 * (kk & 1) + i] = hi;
+          pl[kk >> 1][4 * (kk & 1) + i] = (__bf16)(pv - (float)hi);
+        }
+      l[ct] += ps;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          o[ct][dt] = mfma_bf16(va[dt][h], ph[h], o[ct][dt]);
+          o[ct][dt] = mfma_bf16(va[dt][h], pl[h], o[ct][dt]);
+        }
+    }
+  };
+
+  for (int c0 = begin + wave; c0 < end; c0 += 64) {  // 16 of the wave's blocks
+    fetch_ids(c0);
+    const int n = min(16, (end - c0 + 3) / 4);
+    KvRegs x[2];
+    load(x[0], 0);
+    for (int j = 0; j < n; j += 2) {
+      if (j + 1 < n) load(x[1], j + 1);
+      compute(x[0], (sight.first + c0 + 4 * j) * kFp8Block);
+      if (j + 1 >= n) break;
+      if (j + 2 < n) load(x[0], j + 2);
+      compute(x[1], (sight.first + c0 + 4 * (j + 1)) * kFp8Block);
+    }
+  }
+
+  // The four waves' states merged, in wave order
+#pragma unroll
+  for (int ct = 0; ct < kCt; ++ct) {
+    float lt = l[ct];
+    lt += __shfl_xor(lt, 16, kWave);
+    lt += __shfl_xor(lt, 32, kWave);
+    if (g == 0) {
+      mbuf[wave][16 * ct + r] = m[ct];
+      lbuf[wave][16 * ct + r] = lt;
+    }
+  }
+  const bool alone = shares.used <= 1;
+#pragma unroll
+  for (int ct = 0; ct < kCt; ++ct) {
+    __syncthreads();  // the maxima are there; the last tile's o was read
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) *(f32x4*)&obuf[wave][r][16 * dt + 4 * g] = o[ct][dt];
+    __syncthreads();
+    const int col = t >> 4, d = (t & 15) * 4, cc = 16 * ct + col;
+    const int token = 2 * ct + (col >> 3), head = hk * kGroup + (col & 7);
+    if (token >= nt) continue;
+    float mt = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, mbuf[w][cc]);
+    f32x4 ot = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      // a wave that saw none of the column's keys: m = -inf, l = 0, o = 0
+      const float wgt = mbuf[w][cc] == -INFINITY && lbuf[w][cc] == 0.0f
+                            ? 0.0f : __builtin_amdgcn_exp2f(mbuf[w][cc] - mt);
+      lt = fmaf(lbuf[w][cc], wgt, lt);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ot[i] = fmaf(obuf[w][col][d + i], wgt, ot[i]);
+    }
+    const size_t at = (size_t)(row0 + token) * kHq + head;
+    if (alone) {
+      const float f = sink_share(lt, mt, a.sinks[head]);
+      uint16_t v4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v4[i] = f2bf(ot[i] * f);
+      *(uint2*)(a.out + at * kD + d) = make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
+                                                  (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
+    } else {
+      const size_t pt = (size_t)share * a.rows * kHq + at;
+      if constexpr (kDecode) {  // merged by a workgroup of this launch: device scope
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store_dev(a.part_o + pt * kD + d + i, ot[i]);
+        if (d == 0) {
+          store_dev(a.part_ml + pt * 2, mt);
+          store_dev(a.part_ml + pt * 2 + 1, lt);
+        }
+      } else {
+        *(f32x4*)(a.part_o + pt * kD + d) = ot;
+        if (d == 0) *(float2*)(a.part_ml + pt * 2) = make_float2(mt, lt);
+      }
+    }
+  }
+  if constexpr (kDecode) {
+    if (alone) return;
+    // The last of the head group's splits to finish merges them: its stores are
+    // done (vmcnt), the workgroup meets, one thread counts; the one that completes
+    // the count leaves it zero for the next call.
+    __shared__ int is_last;
+    moe::wait_vmcnt<0>();
+    __syncthreads();
+    if (t == 0) {
+      int* cnt = a.arrive + b * kHkv + hk;
+      const int prev = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      is_last = prev == shares.used - 1;
+      if (is_last) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!is_last) return;
+    // 32 threads a head: the weights exp2(m_s - m) of its splits to LDS, then two
+    // dimensions each over the splits in order, eight loads in flight.
+    __shared__ float wgt[kGroup][64];  // used <= 64
+    const int h = t >> 5, i0 = t & 31;
+    const size_t at = (size_t)row0 * kHq + hk * kGroup + h, step = (size_t)a.rows * kHq;
+    const int used = shares.used;
+    float ms[2], ls[2], mt = -INFINITY, lt = 0.f;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int s = i0 + 32 * j;
+      ms[j] = s < used ? load_dev(a.part_ml + (at + s * step) * 2) : -INFINITY;
+      ls[j] = s < used ? load_dev(a.part_ml + (at + s * step) * 2 + 1) : 0.0f;
+      mt = fmaxf(mt, ms[j]);
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) mt = fmaxf(mt, __shfl_xor(mt, off, kWave));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float w = ms[j] == -INFINITY && ls[j] == 0.0f ? 0.0f
+                                                          : __builtin_amdgcn_exp2f(ms[j] - mt);
+      if (i0 + 32 * j < used) wgt[h][i0 + 32 * j] = w;
+      lt = fmaf(ls[j], w, lt);
+    }
+#pragma unroll
+    for (int off = 16; off >= 1; off >>= 1) lt += __shfl_xor(lt, off, kWave);
+    __syncthreads();
+    const int d = i0 * 2;
+    float o0 = 0.f, o1 = 0.f;
+    for (int s0 = 0; s0 < used; s0 += 8) {
+      uint64_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = load_dev((const uint64_t*)(a.part_o + (at + min(s0 + i, used - 1) * step) * kD + d));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = s0 + i < used ? wgt[h][s0 + i] : 0.0f;
+        if (s0 + i < used) {
+          o0 = fmaf(__uint_as_float((uint32_t)v[i]), w, o0);
+          o1 = fmaf(__uint_as_float((uint32_t)(v[i] >> 32)), w, o1);
+        }
+      }
+    }
+    const float f = sink_share(lt, mt, a.sinks[hk * kGroup + h]);
+    *(uint32_t*)(a.out + at * kD + d) = (uint32_t)f2bf(o0 * f) | ((uint32_t)f2bf(o1 * f) << 16);
+  }
+}
+
+// The splits of a chunk's tiles merged: one wave four rows (token, head), a thread
+// four dimensions, eight splits' loads in flight.  `tokens`: of a tile.
+__global__ __launch_bounds__(256) void fp8_merge_kernel(RowsArgs a, int tokens) {
+  const int b = blockIdx.x / a.tiles, t0 = blockIdx.x % a.tiles * tokens;
+  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
+  const int i = blockIdx.y * 16 + (threadIdx.x >> 4);  // (token of the tile, head)
+  const int token = i / kHq, head = i % kHq, d = (threadIdx.x & 15) * 4;
+  if (token >= tokens || t0 + token >= qn) return;
+  const Sight sight(a.kv_len[b] - qn + t0, min(tokens, qn - t0), a.window);
+  const int used = Shares(sight.blocks, a.splits).used;
+  if (used <= 1) return;  // written already
+  const size_t at = (size_t)(qb + t0 + token) * kHq + head, step = (size_t)a.rows * kHq;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < used; s0 += 8) {
+    float2 ml[8];
+    f32x4 po[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const size_t pt = at + (size_t)min(s0 + j, used - 1) * step;
+      ml[j] = *(const float2*)(a.part_ml + pt * 2);
+      po[j] = *(const f32x4*)(a.part_o + pt * kD + d);
+    }
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mn = s0 + j < used ? fmaxf(mn, ml[j].x) : mn;
+    const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+    if (s0 > 0) {
+      l *= alpha;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] *= alpha;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (s0 + j >= used) continue;
+      const float w = ml[j].x == -INFINITY && ml[j].y == 0.0f
+                          ? 0.0f : __builtin_amdgcn_exp2f(ml[j].x - mn);
+      l = fmaf(ml[j].y, w, l);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = fmaf(po[j][q], w, o[q]);
+    }
+    m = mn;
+  }
+  const float f = sink_share(l, m, a.sinks[head]);
+  uint16_t v4[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v4[q] = f2bf(o[q] * f);
+  *(uint2*)(a.out + at * kD + d) = make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
+                                              (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
+}
+
+}  // namespace attn
+
+// ---------------------------------------------------------------------------
+// Launchers (argument checks live in the C ABI, attn_capi.hip)
+extern "C" {
+
+int attn_launch_fp8_quantize(const void* src, int src_pages, const int* src_slots, int n,
+                             void* cache, int num_pages, const int* slots, hipStream_t s) {
+  hipLaunchKernelGGL(attn::fp8_quantize_kernel, dim3((n + 3) / 4), dim3(256), 0, s,
+                     (const uint8_t*)src, src_pages, src_slots, n, (uint8_t*)cache, num_pages,
+                     slots);
+  return hipGetLastError() == hipSuccess ? 0 : -6;
+}
+
+int attn_launch_fp8_read(const void* cache, int num_pages, const int* slots, int n, void* k_out,
+                         void* v_out, hipStream_t s) {
+  hipLaunchKernelGGL(attn::fp8_read_kernel, dim3((n + 3) / 4), dim3(256), 0, s,
+                     (const uint8_t*)cache, num_pages, slots, n, (uint16_t*)k_out,
+                     (uint16_t*)v_out);
+  return hipGetLastError() == hipSuccess ? 0 : -6;
+}
+
+// part_o [splits][batch][64][64], part_ml [splits][batch][64][2], splits <= 64
+int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const int* page_indptr,
+                           const int* page_indices, int num_pages, const int* kv_len,
+                           int64_t max_span, int window, float sm_scale, const void* sinks,
+                           int splits, float* part_o, float* part_ml, int* arrive, void* out,
+                           hipStream_t s) {
+  if (splits < 1 || splits > 64) return -6;
+  const attn::RowsArgs a{(const uint16_t*)q, nullptr, (const uint8_t*)cache, page_indptr,
+                         page_indices, kv_len, (const uint16_t*)sinks, (uint16_t*)out, part_o,
+                         part_ml, arrive, max_span, num_pages, window, splits, batch, 1,
+                         sm_scale * attn::kLog2e};
+  hipLaunchKernelGGL((attn::fp8_rows_kernel<1, true>), dim3(attn::kHkv * batch, splits), dim3(256),
+                     0, s, a);
+  return hipGetLastError() == hipSuccess ? 0 : -6;
+}
+
+// part_o [splits][rows][64][64], part_ml [splits][rows][64][2] where splits > 1
+int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
+                          const void* cache, const int* page_indptr, const int* page_indices,
+                          int num_pages, const int* kv_len, int window, float sm_scale,
+                          const void* sinks, void* out, int splits, int rows, float* part_o,
+                          float* part_ml, hipStream_t s) {
+  constexpr int kTokens = 8;
+  const int tiles = (max_q_len + kTokens - 1) / kTokens;
+  const attn::RowsArgs a{(const uint16_t*)q, q_indptr, (const uint8_t*)cache, page_indptr,
+                         page_indices, kv_len, (const uint16_t*)sinks, (uint16_t*)out, part_o,
+                         part_ml, nullptr, 0, num_pages, window, splits, rows, tiles,
+                         sm_scale * attn::kLog2e};
+  hipLaunchKernelGGL((attn::fp8_rows_kernel<kTokens / 2, false>),
+                     dim3(attn::kHkv * batch * tiles, splits), dim3(256), 0, s, a);
+  if (hipGetLastError() != hipSuccess) return -6;
+  if (splits > 1) {
+    hipLaunchKernelGGL(attn::fp8_merge_kernel, dim3(batch * tiles, kTokens * attn::kHq / 16),
+                       dim3(256), 0, s, a, kTokens);
+    if (hipGetLastError() != hipSuccess) return -6;
+  }
+  return 0;
+}
+
+}  // extern "C"

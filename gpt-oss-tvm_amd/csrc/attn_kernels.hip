@@ -10,25 +10,10 @@
 //
 // Shapes fixed by gpt-oss: head_dim 64, 64 query heads, 8 key/value heads
 // (GQA groups of 8), pages of 16 tokens.  The host checks them.
-#include "moe_common.h"
+#include "attn_common.h"
 
 namespace attn {
 
-using moe::bf16x8;
-using moe::bf2f;
-using moe::f2bf;
-using moe::f32x4;
-using moe::kWave;
-using moe::load_dev;
-using moe::store_dev;
-using moe::u32x4;
-
-constexpr int kD = 64;          // head_dim
-constexpr int kHq = 64;         // query heads
-constexpr int kHkv = 8;         // key/value heads
-constexpr int kGroup = kHq / kHkv;
-constexpr int kPage = 16;       // tokens per page
-constexpr int kQkvHeads = kHq + 2 * kHkv;
 // bytes of one (page, k or v, head) block: 16 tokens x 64 dims x bf16
 constexpr int kHeadBlock = kPage * kD * 2;
 constexpr int kPageBytes = 2 * kHkv * kHeadBlock;  // 32 KB per page per layer
@@ -38,21 +23,6 @@ __device__ __forceinline__ const uint16_t* kv_row(const uint8_t* cache, int page
   return (const uint16_t*)(cache + (size_t)page * kPageBytes + (size_t)(kv * kHkv + hk) * kHeadBlock +
                            slot * (kD * 2));
 }
-
-// A sequence's page list: the page holding position pos.  The list index is
-// clamped to the sequence's pages and the page id to the pool, so a page table
-// that does not cover kv_len reads wrong keys instead of foreign memory (the
-// host sizes the tables; this only keeps a bad table from faulting).
-struct PageList {
-  const int* ids;
-  int count, pool;
-  // a table entry clamped into the pool (callers that read entries ahead
-  // clamp them at use)
-  __device__ __forceinline__ int clamp(int id) const { return min(max(id, 0), pool - 1); }
-  __device__ __forceinline__ int page_of(int pos) const {
-    return clamp(ids[max(min(pos / kPage, count - 1), 0)]);
-  }
-};
 
 // ---------------------------------------------------------------------------
 // RMSNorm (attention.py:80, nn.RMSNorm): sum of squares of the bf16 inputs in
@@ -141,9 +111,45 @@ __global__ __launch_bounds__(kRmsThreads) void rms_norm_kernel(const u32x4* __re
 // and stores.  (Four tokens a workgroup gained nothing: 2048, 4096, 6144 and 8192
 // tokens 10.0 -> 11.4, 18.8 -> 20.3, 25.0 -> 27.4 and 31.8 -> 33.2 us with qkv from
 // HBM, 4096 and 8192 from the cache 15.7 -> 15.5 and 26.6 -> 28.6.)
+
+// The quarter of a row that a thread of a quad holds (bf16 dims d .. d + 7 in lo,
+// d + 32 .. d + 39 in hi) to slot's place in the 8-bit cache, if it has one.
+__device__ __forceinline__ void store_row_fp8(u32x4 lo, u32x4 hi, int d, int slot, int kv, int hk,
+                                              uint8_t* __restrict__ cache, int num_pages) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    top = max(max(top, lo[i] & 0x7FFFu), (lo[i] >> 16) & 0x7FFFu);
+    top = max(max(top, hi[i] & 0x7FFFu), (hi[i] >> 16) & 0x7FFFu);
+  }
+  const uint32_t s = fp8_scale_of(quad_max(top));
+  uint32_t codes[4];  // dims d .. d + 3, d + 4 .. d + 7, then + 32
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    codes[i] = i < 2 ? fp8_codes(lo[2 * i], lo[2 * i + 1], s, kv)
+                     : fp8_codes(hi[2 * i - 4], hi[2 * i - 3], s, kv);
+  uint8_t* const page = fp8_page(cache, slot, num_pages);
+  if (!page) return;
+  const int token = slot % kPage;
+  if (kv == 0) {
+    uint8_t* const dst = page + hk * kFp8Head + token * kFp8Row + d;
+    *(uint2*)dst = make_uint2(codes[0], codes[1]);
+    *(uint2*)(dst + 32) = make_uint2(codes[2], codes[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      page[fp8_v_at(hk, token, d + (j & 7) + (j & 8) * 4)] =
+          (uint8_t)(codes[j >> 2] >> (8 * (j & 3)));
+  }
+  if ((d & 31) == 0) page[fp8_scale_at(hk, kv, token)] = (uint8_t)s;
+}
+
 constexpr int kRopeThreads = kQkvHeads * 4;  // 320: (head, quarter of its 32 pairs)
 constexpr int kRopeRow = 1 << 20;            // workgroups of a grid row
 
+// kFp8: k and v go to the 8-bit cache, after the same rounding to bf16: a row's
+// four threads meet for its largest magnitude (quad moves) and write 16 codes each.
+template <bool kFp8>
 __global__ __launch_bounds__(kRopeThreads) void qkv_rope_append_kernel(
     const uint16_t* __restrict__ qkv, const uint16_t* __restrict__ bias, int n,
     const int* __restrict__ positions, const int* __restrict__ slots,
@@ -193,6 +199,8 @@ __global__ __launch_bounds__(kRopeThreads) void qkv_rope_append_kernel(
   uint16_t* dst = nullptr;
   if (head < kHq) {
     dst = q_out + ((size_t)tok * kHq + head) * kD;
+  } else if constexpr (kFp8) {  // the last 64 threads, one wave
+    store_row_fp8(olo, ohi, d, slot, (head - kHq) / kHkv, (head - kHq) % kHkv, cache, num_pages);
   } else if (slot >= 0 && slot < num_pages * kPage) {  // other slots are not written
     const int kv = head < kHq + kHkv ? 0 : 1;
     const int hk = head - kHq - kv * kHkv;
@@ -599,20 +607,6 @@ constexpr int kPfWaves = 4;           // waves (query heads) per workgroup
 constexpr float kPfSlack = 8.0f;      // log2 headroom of the lazy softmax rescale
 constexpr int kPfHalves = kGroup / kPfWaves;  // workgroups per GQA group
 
-// max of x over lanes l, l ^ 16, l ^ 32, l ^ 48 (the four 16-lane rows) in
-// registers: swapping x with itself, v_permlane32_swap returns x of lanes
-// l & 31 and l | 32, v_permlane16_swap x of rows 2 (l / 32) and 2 (l / 32) + 1
-__device__ __forceinline__ float group_max(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  const float y = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(y), __float_as_uint(y), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-__device__ __forceinline__ f32x4 mfma_bf16(bf16x8 a, bf16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
 template <bool kSplit>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void prefill_kernel(
     const uint16_t* __restrict__ q, const int* __restrict__ q_indptr,
@@ -1005,14 +999,16 @@ int attn_launch_rms_norm(const void* x, int n, int H, const void* w, float eps, 
 
 int attn_launch_qkv_rope_append(const void* qkv, const void* bias, int n, const int* positions,
                                 const int* slots, const float* inv_freq, float conc, void* cache,
-                                int num_pages, void* q_out, hipStream_t s) {
+                                int num_pages, void* q_out, bool fp8, hipStream_t s) {
   // (2^24 tokens: in rows, as a launch holds less than 2^32 threads in each)
   const int rows = (n + attn::kRopeRow - 1) / attn::kRopeRow;
-  hipLaunchKernelGGL(attn::qkv_rope_append_kernel, dim3(rows > 1 ? attn::kRopeRow : n, rows),
-                     dim3(attn::kRopeThreads), 0, s, (const uint16_t*)qkv, (const uint16_t*)bias, n,
-                     positions, slots, inv_freq, conc, (uint8_t*)cache, num_pages,
-                     (uint16_t*)q_out);
-  return hipGetLastError() == hipSuccess ? 0 : -6;
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(rows > 1 ? attn::kRopeRow : n, rows), dim3(attn::kRopeThreads),
+                       0, s, (const uint16_t*)qkv, (const uint16_t*)bias, n, positions, slots,
+                       inv_freq, conc, (uint8_t*)cache, num_pages, (uint16_t*)q_out);
+    return hipGetLastError() == hipSuccess ? 0 : -6;
+  };
+  return fp8 ? go(attn::qkv_rope_append_kernel<true>) : go(attn::qkv_rope_append_kernel<false>);
 }
 
 int attn_launch_decode(const void* q, int batch, const void* cache, const int* page_indptr,

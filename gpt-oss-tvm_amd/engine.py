@@ -7,7 +7,8 @@ the GPU top-p sampler (``attn_sample_top_p``) with the reference's fixed
 parameters (temperature 0.7, top_p 0.9, uniform sample 0.5: engine.py:40).
 A chat loop drives it exactly as the reference's chat.py does: ``prefill``
 (or ``extend``) the prompt, ``sample``, then ``decode`` + ``sample`` per
-generated token, ``popn`` to roll the cache back.
+generated token, ``popn`` to roll the cache back.  ``kv_dtype`` torch.float8_e4m3fn
+keeps the cache in 8 bits: half its bytes in memory and in every decode step.
 """
 from __future__ import annotations
 
@@ -25,7 +26,8 @@ class Engine:
     next_seq_id = 0
 
     def __init__(self, model_path: str | Path | None = None, config: GPTOssConfig | None = None,
-                 device: str = "cuda", max_total_seq_len: int | None = None):
+                 device: str = "cuda", max_total_seq_len: int | None = None,
+                 kv_dtype: torch.dtype = torch.bfloat16):
         if model_path is not None:
             self.model_path = Path(model_path)
             self.config = config or GPTOssConfig.from_file(self.model_path / "config.json")
@@ -40,7 +42,8 @@ class Engine:
             weights.TorchCheckpoint(self.model_path, self.device).load_into(self.model)
         cw = self.config.context_window_size or 40960
         self.paged_kv_cache = self.model.create_paged_kv_cache(
-            1, max_total_seq_len or cw, self.config.prefill_chunk_size, 16, self.device)
+            1, max_total_seq_len or cw, self.config.prefill_chunk_size, 16, self.device,
+            dtype=kv_dtype)
         self.sample_parameters = {"temperature": 0.7, "top_p": 0.9, "random_seed": 0.5}
         self._sample_ws = A.sample_workspace(1, self.device)
         self._token = torch.zeros(1, dtype=torch.int32, device=self.device)

@@ -14,6 +14,11 @@ pre-norm, bias, RoPE and cache append (QKV) or the bias and residual (output)
 fused; for more as library GEMMs (``torch.nn.functional.linear`` without bias,
 hipBLASLt) followed by the HIP epilogue kernels.  Everything else runs in the HIP
 kernels of libmoe_gfx950 (attn_native): there is no other path.
+
+Over an 8-bit cache (``PagedKVCache(dtype=torch.float8_e4m3fn)``) k and v are
+quantised as they are written -- by the RoPE epilogue, or from the bf16 rows
+that the fused projections leave in the cache's staging pages -- and the 8-bit
+forms of the attention kernels read them.
 """
 from __future__ import annotations
 
@@ -151,26 +156,33 @@ class AttentionBlock(torch.nn.Module):
             t, norm_w = x2, self.norm.weight
             if n > A.ROWS_NORM_MAX_TOKENS:
                 t, norm_w = A.rms_norm(x2, norm_w, self.eps), None
-            A.rows_qkv_rope_append(t, self.qkv.weight, self.qkv.bias, tables.positions,
-                                   tables.slots, self.inv_freq, self.concentration, layer, q,
-                                   norm_w=norm_w, eps=self.eps)
+            rows, slots = ((cache.staging, cache.staging_slots[:n]) if cache.fp8
+                           else (layer, tables.slots))
+            A.rows_qkv_rope_append(t, self.qkv.weight, self.qkv.bias, tables.positions, slots,
+                                   self.inv_freq, self.concentration, rows, q, norm_w=norm_w,
+                                   eps=self.eps)
+            if cache.fp8:
+                A.kv_quantize_fp8(rows, slots, layer, tables.slots)
         else:
             t = A.rms_norm(x2, self.norm.weight, self.eps)
             qkv = F.linear(t, self.qkv.weight)
-            A.qkv_rope_append(qkv, self.qkv.bias, tables.positions, tables.slots, self.inv_freq,
-                              self.concentration, layer, q)
+            append = A.qkv_rope_append_fp8 if cache.fp8 else A.qkv_rope_append
+            append(qkv, self.qkv.bias, tables.positions, tables.slots, self.inv_freq,
+                   self.concentration, layer, q)
         o = torch.empty_like(q)
         window = self._window(tables)
         if tables.is_decode:
             span = cache.static_span or tables.max_kv_len
             span = min(span, window) if window > 0 else span
             ws = cache.decode_workspace(tables.batch, span)
-            A.decode(q, layer, tables.page_indptr, tables.page_indices, tables.kv_len, span,
-                     window, self.sm_scale, self.sinks, o, ws)
+            decode = A.decode_fp8 if cache.fp8 else A.decode
+            decode(q, layer, tables.page_indptr, tables.page_indices, tables.kv_len, span,
+                   window, self.sm_scale, self.sinks, o, ws)
         else:
-            A.prefill(q, tables.q_indptr, tables.max_q_len, layer, tables.page_indptr,
-                      tables.page_indices, tables.kv_len, window, self.sm_scale, self.sinks, o,
-                      tables.max_kv_len)
+            prefill = A.prefill_fp8 if cache.fp8 else A.prefill
+            prefill(q, tables.q_indptr, tables.max_q_len, layer, tables.page_indptr,
+                    tables.page_indices, tables.kv_len, window, self.sm_scale, self.sinks, o,
+                    tables.max_kv_len)
         o2 = o.view(n, A.Q_HEADS * A.HEAD_DIM)
         if fused_out:
             return A.rows_bias_residual(o2, self.out.weight, self.out.bias, x2).view(x.shape)

@@ -21,6 +21,11 @@ Sliding window: the reference's cache keeps only the window's pages for its
 "mha_sliding" layers; this cache keeps every token and the kernels attend to
 the last ``window`` positions in those layers, which gives the same result
 with one page table for all layers.
+
+With ``dtype=torch.float8_e4m3fn`` the cache holds 8-bit rows with a scale byte
+each (the format of include/attn_gfx950.h): one uint8 tensor [layers, pages,
+16640], half a bf16 cache's bytes, quantised as it is written and read by the
+8-bit attention kernels.  The tables are the same.
 """
 from __future__ import annotations
 
@@ -29,6 +34,8 @@ import dataclasses
 import torch
 
 PAGE_SIZE = 16
+FP8_PAGE_BYTES = 16640  # of a page of an 8-bit cache
+STAGED = 64             # tokens of the largest fused decode projection
 
 
 @dataclasses.dataclass
@@ -66,8 +73,22 @@ class PagedKVCache:
         self.num_pages = num_pages
         self.max_batch = max_batch
         self.max_tokens = max_tokens
-        self.data = torch.zeros((num_layers, num_pages, 2, kv_heads, PAGE_SIZE, head_dim),
-                                dtype=dtype, device=device)
+        self.fp8 = dtype == torch.float8_e4m3fn
+        if self.fp8:
+            if (kv_heads, head_dim) != (8, 64):
+                raise ValueError("the 8-bit cache is built for 8 key/value heads of 64")
+            self.data = torch.zeros((num_layers, num_pages, FP8_PAGE_BYTES), dtype=torch.uint8,
+                                    device=device)
+            # where the fused decode projections append a step's bf16 rows, to be quantised
+            # from there (every layer in turn, on one stream)
+            self.staging = torch.zeros((STAGED // PAGE_SIZE, 2, kv_heads, PAGE_SIZE, head_dim),
+                                       dtype=torch.bfloat16, device=device)
+            self.staging_slots = torch.arange(STAGED, dtype=torch.int32, device=device)
+        elif dtype.itemsize != 2:
+            raise ValueError(f"a cache holds bf16 or float8_e4m3fn rows, not {dtype}")
+        else:
+            self.data = torch.zeros((num_layers, num_pages, 2, kv_heads, PAGE_SIZE, head_dim),
+                                    dtype=dtype, device=device)
         self.free = list(range(num_pages - 1, -1, -1))  # pop() hands out page 0 first
         self.seqs: dict[int, _Seq] = {}
         # The forward tables live in one device buffer at fixed offsets (kernels
@@ -104,10 +125,12 @@ class PagedKVCache:
         to at most `span` keys; grown here only (``reserve_decode`` sizes it
         up front for callers that capture the forward in a graph)."""
         import attn_native
-        need = attn_native.decode_workspace_bytes(batch, span)
-        if self._decode_ws is None or self._decode_ws.numel() < need:
+        size, make = ((attn_native.decode_fp8_workspace_bytes, attn_native.decode_fp8_workspace)
+                      if self.fp8 else
+                      (attn_native.decode_workspace_bytes, attn_native.decode_workspace))
+        if self._decode_ws is None or self._decode_ws.numel() < size(batch, span):
             # a buffer a captured graph holds stays alive in _decode_ws_held
-            self._decode_ws = attn_native.decode_workspace(batch, span, self.data.device)
+            self._decode_ws = make(batch, span, self.data.device)
         return self._decode_ws
 
     def reserve_decode(self, batch: int, span: int, for_graph: bool = False) -> None:
@@ -155,6 +178,49 @@ class PagedKVCache:
 
     def seq_len(self, seq_id: int) -> int:
         return self.seqs[seq_id].length
+
+    # -- a sequence's rows -----------------------------------------------------------
+    def slots_of(self, seq_id: int, start: int = 0, stop: int | None = None) -> torch.Tensor:
+        """The cache slots (page * 16 + offset) of a sequence's tokens start .. stop - 1."""
+        s = self.seqs[seq_id]
+        stop = s.length if stop is None else stop
+        if not 0 <= start <= stop <= s.length:
+            raise ValueError(f"tokens {start}..{stop} of a sequence of {s.length}")
+        return torch.tensor([s.pages[p // PAGE_SIZE] * PAGE_SIZE + p % PAGE_SIZE
+                             for p in range(start, stop)], dtype=torch.int32,
+                            device=self.data.device)
+
+    def read(self, seq_id: int, layer: int, start: int = 0,
+             stop: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """k and v [n, kv_heads, head_dim] of a sequence's tokens start .. stop - 1 in one layer
+        (an 8-bit cache's as the bf16 values that its rows stand for)."""
+        slots = self.slots_of(seq_id, start, stop)
+        if self.fp8:
+            import attn_native
+            return attn_native.kv_read_fp8(self.layer(layer), slots)
+        page, at = slots.long() // PAGE_SIZE, slots.long() % PAGE_SIZE
+        data = self.layer(layer)
+        return data[page, 0, :, at], data[page, 1, :, at]
+
+    def quantize_from(self, seq_id: int, source: "PagedKVCache", source_id: int) -> None:
+        """A new sequence ``seq_id`` of this 8-bit cache with the tokens and the window of
+        ``source_id`` of a bf16 cache of as many layers: its rows quantised, in every layer."""
+        import attn_native
+        if not self.fp8 or source.fp8 or source.num_layers != self.num_layers:
+            raise ValueError("quantize_from takes a sequence of a bf16 cache into an 8-bit cache "
+                             "of as many layers")
+        old = source.seqs[source_id]
+        need = -(-old.length // PAGE_SIZE)
+        if need > len(self.free):
+            raise MemoryError(f"KV cache full: {need} pages needed, {len(self.free)} free")
+        self.add_sequence(seq_id)
+        s = self.seqs[seq_id]
+        s.pages = [self.free.pop() for _ in range(need)]
+        s.length, s.window = old.length, old.window
+        if s.length:
+            mine, theirs = self.slots_of(seq_id), source.slots_of(source_id)
+            for i in range(self.num_layers):
+                attn_native.kv_quantize_fp8(source.layer(i), theirs, self.layer(i), mine)
 
     # -- one forward ---------------------------------------------------------------
     def begin_forward(self, seq_ids, append_lengths) -> ForwardTables:

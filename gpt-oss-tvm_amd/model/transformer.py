@@ -123,10 +123,11 @@ class GPTOssForCausalLM(torch.nn.Module):
 
     def create_paged_kv_cache(self, max_batch_size: int, max_total_seq_len: int,
                               prefill_chunk_size: int, page_size: int = 16,
-                              device="cuda") -> PagedKVCache:
-        """model/transformer.py:153-175: one page pool for every layer."""
+                              device="cuda", dtype=torch.bfloat16) -> PagedKVCache:
+        """model/transformer.py:153-175: one page pool for every layer; ``dtype``
+        torch.float8_e4m3fn holds 8-bit rows (half the bytes)."""
         if page_size != 16:
             raise ValueError("the attention kernels use pages of 16 tokens")
         pages = -(-max_total_seq_len // page_size) + max_batch_size
         return PagedKVCache(self.num_hidden_layers, pages, max_batch_size,
-                            max(prefill_chunk_size, max_batch_size), device=device)
+                            max(prefill_chunk_size, max_batch_size), device=device, dtype=dtype)

@@ -175,6 +175,79 @@ MOE_API int attn_sample_top_p(const uint16_t* logits, int64_t batch, int64_t voc
                               float temperature, float top_p, float uniform, int32_t* out_ids,
                               void* workspace, size_t workspace_bytes, moe_stream_t stream);
 
+/* ---- The 8-bit KV cache -------------------------------------------------------
+ * Half a bf16 cache's bytes; the page tables, slots and positions are the same.
+ * A row is the 64 values of one token, kv head and k or v: e4m3 codes (OCP, nearest
+ * even) and one E8M0 scale byte s; code c stands for c 2^(s - 127).  With e the
+ * biased exponent of the row's largest magnitude s = max(e - 7, 10): values are off
+ * by at most 2^-4 of themselves or 2^-17 of the row's largest (or 2^-127).  (At s =
+ * 247 codes stop at 240, as 256 would stand for 2^128.)  A row with an infinity or a NaN has s = 255 and stands for NaN:
+ * queries that see its token get NaN, others are not affected.
+ * One layer's cache is [num_pages][16640] bytes.  A page: k codes [8 heads][16
+ * tokens][64 dims]; at 8192 v codes [8][token / 4][dim % 16][dim / 16][token % 4]; at
+ * 16384 scales [8][k, v][16].  It needs no initialisation: what lies past a
+ * sequence's kv_len is never used. */
+#define ATTN_FP8_PAGE_BYTES 16640
+
+/* attn_qkv_rope_append into the 8-bit cache: q_out is the same bit for bit, and k
+ * and v are the rows it would append, quantised.  The slots of a call inside the
+ * pool have to differ (as there: a slot listed twice holds a mixture). */
+MOE_API int attn_qkv_rope_append_fp8(const uint16_t* qkv, const uint16_t* qkv_bias, int64_t n,
+                                     const int32_t* positions, const int32_t* slots,
+                                     const float* inv_freq, float concentration, void* kv_cache,
+                                     int64_t num_pages, uint16_t* q_out, moe_stream_t stream);
+
+/* Rows of a bf16 cache [src_pages, 2, 8, 16, 64] into the 8-bit one: the row at
+ * src_slots[i] to slots[i], i < n.  Puts away the rows that the fused decode
+ * projections appended to a few bf16 pages; moves a sequence from one kind of
+ * cache to the other.  Where either slot lies outside its pool nothing is written;
+ * the other slots have to differ. */
+MOE_API int attn_kv_quantize_fp8(const void* src, int64_t src_pages, const int32_t* src_slots,
+                                 int64_t n, void* kv_cache, int64_t num_pages,
+                                 const int32_t* slots, moe_stream_t stream);
+
+/* The rows at slots[i] back as bf16, k_out and v_out [n, 8, 64]: exact, NaN for a row of
+ * scale 255, 0 for a slot outside the pool. */
+MOE_API int attn_kv_read_fp8(const void* kv_cache, int64_t num_pages, const int32_t* slots,
+                             int64_t n, uint16_t* k_out, uint16_t* v_out, moe_stream_t stream);
+
+/* Workspace of attn_decode_fp8, a pure function of its arguments (0 where the call
+ * would be refused).  Its first 2 MB are arrival counts, as attn_decode's: zero
+ * before the first call, left zero by every call, whatever its batch.  Calls on
+ * one workspace have to follow one another (one stream, or events). */
+MOE_API size_t attn_decode_fp8_workspace_bytes(int64_t batch, int64_t max_span);
+
+/* attn_decode over the 8-bit cache.  out = sum_j p_j v_j / (sum_j p_j +
+ * exp(sinks[h])), p_j = exp(sm_scale q . k_j), over the last `window` keys (window >
+ * 0) or all: the softmax with the sink as a further logit, in fp32 with one rounding
+ * to bf16 (attn_decode rounds as the operators it restates do).  A sequence with no
+ * key (kv_len 0) gets 0, one whose span exceeds max_span NaN.  sm_scale > 0.  The
+ * result of a sequence follows from its keys and the batch size, not from
+ * max_span. */
+MOE_API int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cache,
+                            int64_t num_pages, const int32_t* page_indptr,
+                            const int32_t* page_indices, const int32_t* kv_len, int64_t max_span,
+                            int32_t window, float sm_scale, const uint16_t* sinks, uint16_t* out,
+                            void* workspace, size_t workspace_bytes, moe_stream_t stream);
+
+/* attn_prefill over the 8-bit cache, with attn_decode_fp8's formula: each sequence's new
+ * tokens (appended already) causally over its cached keys.  q has `rows` rows;
+ * rows outside q_indptr's ranges are left as they are.  max_q_len bounds every
+ * q_len, max_kv_len kv_len (it only chooses how the keys of few query tiles are
+ * shared out over workgroups; 0: unknown, not shared out).  A sequence's last bits
+ * may change with the other sequences of the call and with the bounds.  The
+ * workspace (none where attn_prefill_fp8_workspace_bytes is 0) needs no
+ * initialisation. */
+MOE_API size_t attn_prefill_fp8_workspace_bytes(int64_t rows, int64_t batch, int64_t max_q_len,
+                                                int64_t max_kv_len, int32_t window);
+MOE_API int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr,
+                             int64_t batch, int64_t max_q_len, const void* kv_cache,
+                             int64_t num_pages, const int32_t* page_indptr,
+                             const int32_t* page_indices, const int32_t* kv_len,
+                             int64_t max_kv_len, int32_t window, float sm_scale,
+                             const uint16_t* sinks, uint16_t* out, void* workspace,
+                             size_t workspace_bytes, moe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

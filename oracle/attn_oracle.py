@@ -194,6 +194,87 @@ class AttnParams:
     out_b: np.ndarray    # [H]
 
 
+# -- the 8-bit cache (include/attn_gfx950.h) --------------------------------------
+
+FP8_PAGE_BYTES, FP8_V, FP8_SCALES = 16640, 8192, 16384
+
+
+def e4m3_values() -> np.ndarray:
+    """The 256 values of OCP e4m3 (bias 7, subnormals, NaN at 0x7F and 0xFF), fp64."""
+    c = np.arange(256)
+    e, f = (c >> 3) & 15, c & 7
+    mag = np.where(e == 0, f * 2.0 ** -9, (8 + f) * np.exp2(e - 10.0))
+    mag[(c & 127) == 127] = np.nan
+    return np.where(c & 128, -mag, mag)
+
+
+def fp8_quantize(rows_bf16: np.ndarray, is_v: bool) -> tuple[np.ndarray, np.ndarray]:
+    """Rows [..., 64] of bf16 bits -> (e4m3 codes [..., 64], scale bytes [...]):
+    s = max(e - 7, 10), e the biased exponent of the row's largest magnitude, code =
+    nearest e4m3 value to v 2^(127 - s), ties to the even code (at most 240 at s = 247,
+    where 256 would stand for 2^128); a row with an infinity or a NaN gets s = 255 and
+    codes 0x7F (k) or 0 (v)."""
+    e = ((rows_bf16 & 0x7FFF) >> 7).max(axis=-1).astype(np.int64)
+    s = np.where(e == 255, 255, np.maximum(e - 7, 10))
+    x = bf16_to_f32(rows_bf16).astype(np.float64) * np.exp2(127.0 - s)[..., None]
+    bad = (s == 255)[..., None]
+    mag = np.minimum(np.abs(np.where(bad, 0.0, x)), np.where(s == 247, 240.0, 256.0)[..., None])
+    table = e4m3_values()[:127]                  # ascending, 0 .. 448
+    hi = np.searchsorted(table, mag)             # table[hi - 1] < mag <= table[hi]
+    lo = np.maximum(hi - 1, 0)
+    up, down = table[hi] - mag, mag - table[lo]
+    code = np.where((up < down) | ((up == down) & (hi % 2 == 0)), hi, lo)
+    code = code | np.where((rows_bf16 & 0x8000) != 0, 128, 0)
+    code = np.where(bad, 0 if is_v else 0x7F, code)
+    return code.astype(np.uint8), s.astype(np.uint8)
+
+
+def fp8_dequantize(codes: np.ndarray, scales: np.ndarray) -> np.ndarray:
+    """The values that rows of codes stand for, fp64 (NaN for scale 255)."""
+    s = scales.astype(np.float64)
+    return e4m3_values()[codes] * np.where(s == 255, np.nan, np.exp2(s - 127.0))[..., None]
+
+
+def fp8_put(cache: np.ndarray, slots: np.ndarray, k_bf16: np.ndarray, v_bf16: np.ndarray) -> None:
+    """Rows k, v [n, 8, 64] into the pages of cache [pages, 16640] uint8."""
+    kc, ks = fp8_quantize(k_bf16, False)
+    vc, vs = fp8_quantize(v_bf16, True)
+    d = np.arange(HEAD_DIM)
+    for i, slot in enumerate(slots):
+        page, t = divmod(int(slot), 16)
+        for h in range(N_KV_HEADS):
+            base = h * 1024
+            cache[page, base + t * 64:base + t * 64 + 64] = kc[i, h]
+            cache[page, FP8_V + base + t // 4 * 256 + d % 16 * 16 + d // 16 * 4 + t % 4] = vc[i, h]
+            cache[page, FP8_SCALES + h * 32 + t] = ks[i, h]
+            cache[page, FP8_SCALES + h * 32 + 16 + t] = vs[i, h]
+
+
+def attention_sink(q: np.ndarray, k: np.ndarray, v: np.ndarray, q_pos: np.ndarray, window: int,
+                   sinks: np.ndarray, sm_scale: float = 0.125):
+    """fp64 softmax attention with the sink as a further logit.  q [n, 64, 64], k, v [L, 8,
+    64], sinks [64] -> (out [n, 64, 64], the same sum over |v|, the largest sum_d |q_d k_d|
+    sm_scale of each (row, head) over its keys)."""
+    n, L = q.shape[0], k.shape[0]
+    out, mag, size = (np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:2]))
+    for i in range(n):
+        p = int(q_pos[i])
+        lo = max(0, p - window + 1) if window > 0 else 0
+        kk, vv = k[lo:p + 1], v[lo:p + 1]
+        if p + 1 <= lo:
+            continue
+        for h in range(N_KV_HEADS):
+            rows = slice(8 * h, 8 * h + 8)
+            s = q[i, rows] @ kk[:, h].T * sm_scale
+            top = np.maximum(s.max(axis=1), sinks[rows])
+            w = np.exp(s - top[:, None])
+            den = w.sum(axis=1) + np.exp(sinks[rows] - top)
+            out[i, rows] = w @ vv[:, h] / den[:, None]
+            mag[i, rows] = w @ np.abs(vv[:, h]) / den[:, None]
+            size[i, rows] = (np.abs(q[i, rows]) @ np.abs(kk[:, h]).T).max(axis=1) * sm_scale
+    return out, mag, size
+
+
 def split_qkv(qkv_bf16: np.ndarray, hq: int = N_Q_HEADS, hkv: int = N_KV_HEADS, d: int = HEAD_DIM):
     """attention.py:206-210: [n, (Hq + 2 Hkv) D] -> q [n, Hq, D], k, v [n, Hkv, D]."""
     x = qkv_bf16.reshape(qkv_bf16.shape[0], hq + 2 * hkv, d)
