@@ -59,8 +59,8 @@ int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const in
 int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
                           const void* cache, const int* page_indptr, const int* page_indices,
                           int num_pages, const int* kv_len, int window, float sm_scale,
-                          const void* sinks, void* out, int splits, int rows, float* part_o,
-                          float* part_ml, hipStream_t s);
+                          const void* sinks, void* out, int tokens, int splits, int rows,
+                          float* part_o, float* part_ml, hipStream_t s);
 }
 
 namespace {
@@ -431,11 +431,15 @@ int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
   return std::max<int64_t>(1, std::min(most, fp8_blocks(max_span) / kFp8SplitBlocks));
 }
 
-constexpr int64_t kFp8ChunkTokens = 8, kFp8ChunkWgs = 1024;
+// Tokens of a chunk's query tile.
+int64_t fp8_tile(int64_t max_q_len) { return max_q_len <= 8 ? 8 : 32; }
+
+constexpr int64_t kFp8ChunkWgs = 512;
 int64_t fp8_chunk_splits(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
   if (batch <= 0 || batch > kFp8ChunkWgs || max_q_len <= 0) return 1;  // (and no overflow below)
-  const int64_t wgs = (max_q_len + kFp8ChunkTokens - 1) / kFp8ChunkTokens * batch * kKvHeads;
-  const int64_t keys = window > 0 ? std::min(max_kv_len, window + kFp8ChunkTokens) : max_kv_len;
+  const int64_t tokens = fp8_tile(max_q_len);
+  const int64_t wgs = (max_q_len + tokens - 1) / tokens * batch * kKvHeads;
+  const int64_t keys = window > 0 ? std::min(max_kv_len, window + tokens) : max_kv_len;
   if (keys <= 0) return 1;
   const int64_t most = std::min(kFp8MaxSplits, kFp8ChunkWgs / wgs);
   return std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks));
@@ -492,7 +496,7 @@ int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, i
       num_pages <= 0 || num_pages >= kMaxPages)
     return MOE_ERR_SHAPE;
   if (rows == 0 || batch == 0 || max_q_len == 0) return MOE_OK;
-  const int64_t tiles = (max_q_len + kFp8ChunkTokens - 1) / kFp8ChunkTokens;
+  const int64_t tokens = fp8_tile(max_q_len), tiles = (max_q_len + tokens - 1) / tokens;
   if (batch > kMaxTokens || tiles * batch * kKvHeads >= ((int64_t)1 << 24)) return MOE_ERR_SHAPE;
   if (!(sm_scale > 0.0f && sm_scale <= FLT_MAX)) return MOE_ERR_UNSUPPORTED;
   if (!q || !q_indptr || !kv_cache || !page_indptr || !page_indices || !kv_len || !sinks || !out)
@@ -508,7 +512,7 @@ int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, i
   float* part_o = (float*)workspace;
   return status(attn_launch_fp8_chunk(
       q, q_indptr, (int)batch, (int)max_q_len, kv_cache, page_indptr, page_indices, (int)num_pages,
-      kv_len, window, sm_scale, sinks, out, (int)splits, (int)rows, part_o,
+      kv_len, window, sm_scale, sinks, out, (int)tokens, (int)splits, (int)rows, part_o,
       need ? part_o + splits * rows * kQHeads * kHeadDim : nullptr, as_stream(stream)));
 }
 
