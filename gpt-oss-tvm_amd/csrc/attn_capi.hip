@@ -431,18 +431,26 @@ int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
   return std::max<int64_t>(1, std::min(most, fp8_blocks(max_span) / kFp8SplitBlocks));
 }
 
-// Tokens of a chunk's query tile.
-int64_t fp8_tile(int64_t max_q_len) { return max_q_len <= 8 ? 8 : 32; }
-
+// Tokens of a chunk's query tile, and how many splits its keys are shared out over.
+// Up to 8 tokens take the kernel that loads alone bind.  Longer chunks are split so
+// far that their workgroups fit the chip at once (two a CU), and take tiles of 64
+// tokens without a window where those are two rounds of the chip.
 constexpr int64_t kFp8ChunkWgs = 512;
-int64_t fp8_chunk_splits(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
-  if (batch <= 0 || batch > kFp8ChunkWgs || max_q_len <= 0) return 1;  // (and no overflow below)
-  const int64_t tokens = fp8_tile(max_q_len);
+struct Fp8Chunk {
+  int64_t tokens, splits, tiles;  // tiles of the longest sequence
+};
+Fp8Chunk fp8_chunk(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
+  auto make = [&](int64_t tokens, int64_t splits) {
+    return Fp8Chunk{tokens, splits, (max_q_len + tokens - 1) / tokens};
+  };
+  if (max_q_len > 8 && window <= 0 && (max_q_len + 63) / 64 * kKvHeads >= (512 + batch - 1) / batch)
+    return make(64, 1);
+  const int64_t tokens = max_q_len <= 8 ? 8 : 32;
   const int64_t wgs = (max_q_len + tokens - 1) / tokens * batch * kKvHeads;
   const int64_t keys = window > 0 ? std::min(max_kv_len, window + tokens) : max_kv_len;
-  if (keys <= 0) return 1;
+  if (keys <= 0) return make(tokens, 1);
   const int64_t most = std::min(kFp8MaxSplits, kFp8ChunkWgs / wgs);
-  return std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks));
+  return make(tokens, std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks)));
 }
 }  // namespace
 
@@ -480,9 +488,10 @@ int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cache, int6
 // Workspace: the splits' o [splits][rows][64][64], then (m, l) [splits][rows][64][2]
 size_t attn_prefill_fp8_workspace_bytes(int64_t rows, int64_t batch, int64_t max_q_len,
                                         int64_t max_kv_len, int32_t window) {
-  if (rows <= 0 || rows > kMaxTokens || batch <= 0 || max_q_len <= 0 || max_q_len > kMaxTokens)
+  if (rows <= 0 || rows > kMaxTokens || batch <= 0 || batch > kMaxTokens || max_q_len <= 0 ||
+      max_q_len > kMaxTokens)
     return 0;
-  const int64_t splits = fp8_chunk_splits(batch, max_q_len, max_kv_len, window);
+  const int64_t splits = fp8_chunk(batch, max_q_len, max_kv_len, window).splits;
   return splits <= 1 ? 0 : (size_t)(splits * rows * kQHeads * (kHeadDim + 2)) * sizeof(float);
 }
 
@@ -496,8 +505,9 @@ int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, i
       num_pages <= 0 || num_pages >= kMaxPages)
     return MOE_ERR_SHAPE;
   if (rows == 0 || batch == 0 || max_q_len == 0) return MOE_OK;
-  const int64_t tokens = fp8_tile(max_q_len), tiles = (max_q_len + tokens - 1) / tokens;
-  if (batch > kMaxTokens || tiles * batch * kKvHeads >= ((int64_t)1 << 24)) return MOE_ERR_SHAPE;
+  if (batch > kMaxTokens) return MOE_ERR_SHAPE;  // (and no overflow below)
+  const Fp8Chunk chunk = fp8_chunk(batch, max_q_len, max_kv_len, window);
+  if (chunk.tiles * batch * kKvHeads >= ((int64_t)1 << 22)) return MOE_ERR_SHAPE;
   if (!(sm_scale > 0.0f && sm_scale <= FLT_MAX)) return MOE_ERR_UNSUPPORTED;
   if (!q || !q_indptr || !kv_cache || !page_indptr || !page_indices || !kv_len || !sinks || !out)
     return MOE_ERR_NULL;
@@ -508,12 +518,12 @@ int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, i
   if (need && !workspace) return MOE_ERR_NULL;
   if (need && !a16(workspace)) return MOE_ERR_ALIGN;
   if (workspace_bytes < need) return MOE_ERR_WORKSPACE;
-  const int64_t splits = need ? fp8_chunk_splits(batch, max_q_len, max_kv_len, window) : 1;
   float* part_o = (float*)workspace;
   return status(attn_launch_fp8_chunk(
       q, q_indptr, (int)batch, (int)max_q_len, kv_cache, page_indptr, page_indices, (int)num_pages,
-      kv_len, window, sm_scale, sinks, out, (int)tokens, (int)splits, (int)rows, part_o,
-      need ? part_o + splits * rows * kQHeads * kHeadDim : nullptr, as_stream(stream)));
+      kv_len, window, sm_scale, sinks, out, (int)chunk.tokens, (int)chunk.splits, (int)rows,
+      part_o, need ? part_o + chunk.splits * rows * kQHeads * kHeadDim : nullptr,
+      as_stream(stream)));
 }
 
 }  // extern "C"

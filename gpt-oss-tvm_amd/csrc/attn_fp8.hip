@@ -449,11 +449,11 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
   }
 }
 
-// Long chunks: a workgroup takes 32 tokens x the 8 heads of a kv head (256 columns
-// (token, head)) through the sequence's keys in blocks of 64; a wave 8 tokens, two
-// column tiles of 32.  Bound by the vector ALUs and the matrix cores (a score
-// costs one exponential and four multiply-adds of 64 dims in all), so both are
-// kept short:
+// Long chunks: a workgroup takes kTokens tokens x the 8 heads of a kv head (columns
+// (token, head)) through the sequence's keys in blocks of 64, a wave 4 tokens: one
+// column tile of 32.  Bound by the vector ALUs (per 32 x 32 scores 16 exponentials,
+// 16 multiply-adds, 8 conversions and 8 dot products of a wave against 8 matrix
+// products), so:
 //  * v_mfma_f32_32x32x16_bf16: S^T = K Q^T leaves lane (column l % 32, half h =
 //    l / 32) the keys 8 (i / 4) + 4 h + i % 4 of a 32-key tile in elements i = 0 ..
 //    15, which are, packed to bf16, the operands of two products O^T += V^T P^T over 16
@@ -467,13 +467,24 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
 //    1, which fp32 and bf16 carry; a wave takes new maxima, rescales and computes its
 //    p anew only when some column's sum over a tile passes 2^24 (or m is not set:
 //    -m = inf gives an infinite or NaN sum).
+//  * 128 registers, so that four waves share a SIMD: a wave alone issues a vector
+//    instruction every 8 cycles, and one's matrix products run under the others'
+//    exponentials.  (64 columns a wave, two waves, with the products of one tile and the
+//    exponentials of the next interleaved by hand: the same time at 4096 tokens.)
 // The next block's codes are loaded to registers during a block's products, then
 // converted once for all waves, k with its scale, v with its keys', into LDS (bf16,
 // rows of 128 bytes whose 16-byte units are XORed with the row's bits 1 .. 3, so
 // 16 rows of one unit spread over all banks); one barrier per block.
 // A row that must not be used (255) is NaN in k and 0 in v.
-constexpr int kTileTokens = 32;
+//
+// 64 tokens halve the conversions per column, but a CU holds one workgroup and not
+// two, the last ones leave more of the chip idle, and a window's edges are masked in
+// more columns: 4096 tokens 157 us against 161, 2048 tokens 72 against 54, 4096 with
+// window 128 44 against 33.  So they are taken without a window where they are two
+// rounds or more of the chip.
 constexpr float kTileMost = 16777216.0f;  // 2^24
+constexpr int kTileBytes = kFp8Block * kD * 2;
+constexpr int tile_threads(int tokens) { return 16 * tokens; }
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
@@ -485,78 +496,73 @@ __device__ __forceinline__ float half_max(float x) {
   return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
-template <bool kSplit>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void fp8_tile_kernel(
-    RowsArgs a) {
-  __shared__ __align__(16) uint8_t kt[2][kFp8Block * kD * 2];
-  __shared__ __align__(16) uint8_t vt[2][kD * kFp8Block * 2];
+template <int kTokens, bool kSplit>
+__global__ __launch_bounds__(tile_threads(kTokens)) __attribute__((amdgpu_waves_per_eu(4))) void
+fp8_tile_kernel(RowsArgs a) {
+  __shared__ __align__(16) uint8_t kt[2][kTileBytes];
+  __shared__ __align__(16) uint8_t vt[2][kTileBytes];
   // x: (tile from the last, which sees the most keys; sequence; kv head), y: split
-  const int hk = blockIdx.x % kHkv, rest = blockIdx.x / kHkv, batch = gridDim.x / kHkv / a.tiles;
+  const int hk = blockIdx.x % kHkv, total = gridDim.x / kHkv, batch = total / a.tiles;
+  int rest = blockIdx.x / kHkv;
+  // An XCD's 32 CUs take the second 32 workgroups beside the first: in reverse, so that
+  // the longest has the shortest beside it (2048 tokens 59 -> 54 us)
+  if (kTokens == 32 && rest >= 32 && rest < 64) rest = min(total, 64) - 1 - (rest - 32);
   const int b = rest % batch, tile = a.tiles - 1 - rest / batch;
-  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb, t0 = tile * kTileTokens;
+  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb, t0 = tile * kTokens;
   if (t0 >= qn) return;
-  const int nt = min(kTileTokens, qn - t0), row0 = qb + t0;
+  const int nt = min(kTokens, qn - t0), row0 = qb + t0;
   const int L = a.kv_len[b], pos = L - qn + t0;
   const Sight sight(pos, nt, a.window);
   const Shares shares(sight.blocks, kSplit ? a.splits : 1);
   const int share = kSplit ? blockIdx.y : 0;
   if (share >= max(shares.used, 1)) return;
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, c = lane & 31, h = lane >> 5;
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+  const int c = lane & 31, h = lane >> 5;
   const PageList pages{a.page_indices + a.page_indptr[b],
                        a.page_indptr[b + 1] - a.page_indptr[b], a.num_pages};
   const int last_page = max(0, min(pages.count - 1, (L - 1) / kPage));
   const int begin = sight.first + share * shares.each;
   const int end = min(begin + shares.each, sight.first + sight.blocks);
 
-  bf16x8 qv[2][4];
-  int qpos[2];
-#pragma unroll
-  for (int ct = 0; ct < 2; ++ct) {
-    const int token = min(8 * wave + 4 * ct + (c >> 3), nt - 1);
-    const u32x4* src =
-        (const u32x4*)(a.q + ((size_t)(row0 + token) * kHq + hk * kGroup + (c & 7)) * kD);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) qv[ct][s] = moe::as_bf16x8(src[2 * s + h]);
-    qpos[ct] = pos + token;
-  }
-  f32x16 o[2][2];
-  float mneg[2], l[2];
-#pragma unroll
-  for (int ct = 0; ct < 2; ++ct) {
-    mneg[ct] = INFINITY;
-    l[ct] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[ct][dt][i] = 0.f;
-  }
-
-  // Staging: wave w takes page w of the block, lane the 16 dims 16 (l % 4) .. of
-  // its key l / 4 and the four keys of quad l / 16 in v's unit l % 16.
-  u32x4 kr, vr;
-  uint32_t ksc, vsc;
-  auto page_id = [&](int blk) {
-    return pages.count > 0 ? pages.ids[min(4 * blk + wave, last_page)] : 0;
+  // Staging: waves 0 .. 3 take k, waves 4 .. 7 v of page `wave & 3` of a block: lane
+  // the 16 dims 16 (l % 4) .. of key l / 4, or the four keys of quad l / 16 in v's unit
+  // l % 16; both take their keys' scales.
+  const int mine = wave & 3, quad = 4 * mine + (lane >> 4);
+  const bool is_v = wave & 4, stages = kTokens == 32 || wave < 8;
+  const unsigned part = (is_v ? kFp8V : 0) + hk * kFp8Head + lane * 16;
+  const unsigned spart = kFp8Scales + hk * 2 * kPage + (lane >> 4) * 4;
+  struct Raw {
+    u32x4 codes;
+    uint32_t ks, vs;
   };
-  auto load = [&](int id) {
-    const uint8_t* page = a.cache + (size_t)(unsigned)pages.clamp(id) * kFp8Page;
-    kr = *(const u32x4*)(page + hk * kFp8Head + lane * 16);
-    vr = *(const u32x4*)(page + kFp8V + hk * kFp8Head + lane * 16);
-    ksc = *(const uint32_t*)(page + kFp8Scales + hk * 2 * kPage + (lane >> 4) * 4);
-    vsc = *(const uint32_t*)(page + kFp8Scales + hk * 2 * kPage + kPage + (lane >> 4) * 4);
+  // the pages of 64 blocks at a time, one a lane (past the last block: its last page again)
+  int ids = 0;
+  auto fetch_ids = [&](int blk) {
+    ids = pages.count > 0 ? pages.clamp(pages.ids[min(4 * (blk + lane) + mine, last_page)]) : 0;
   };
-  auto store = [&](int buf, int kb) {
-    const int byte = 8 * ((lane >> 2) & 3), key = 16 * wave + (lane >> 2);
-    const uint32_t sk = (ksc >> byte) & 255u, sv = (vsc >> byte) & 255u;
-    const bool bad = max(sk, sv) == kFp8BadScale;
-    const float scale = __uint_as_float(min(sk, kFp8BadScale - 1u) << 23);
+  auto load = [&](Raw& x, int blk) {
+    const int i = (blk - begin) & 63;
+    if (i == 0 && blk > begin) fetch_ids(blk);
+    const uint8_t* page = a.cache + (size_t)(unsigned)__builtin_amdgcn_readlane(ids, i) * kFp8Page;
+    x.codes = *(const u32x4*)(page + part);
+    x.ks = *(const uint32_t*)(page + spart);
+    x.vs = *(const uint32_t*)(page + spart + kPage);
+  };
+  auto store = [&](Raw& x, int buf, int kb) {
+    if (!is_v) {
+      const int byte = 8 * ((lane >> 2) & 3), key = 16 * mine + (lane >> 2);
+      const uint32_t sk = (x.ks >> byte) & 255u, sv = (x.vs >> byte) & 255u;
+      const bool bad = max(sk, sv) == kFp8BadScale;
+      const float scale = __uint_as_float(min(sk, kFp8BadScale - 1u) << 23);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) kr[j] = bad ? kFp8NanCodes : kr[j];
-    uint8_t* row = kt[buf] + key * 128;
-    const int x = (key >> 1) & 7, u = 2 * (lane & 3);
-    *(bf16x8*)(row + ((u ^ x) << 4)) = fp8_to_bf16(kr[0], kr[1], scale);
-    *(bf16x8*)(row + (((u + 1) ^ x) << 4)) = fp8_to_bf16(kr[2], kr[3], scale);
-    const int quad = t >> 4, n = quad & 7, r = lane & 15;
+      for (int j = 0; j < 4; ++j) x.codes[j] = bad ? kFp8NanCodes : x.codes[j];
+      uint8_t* row = kt[buf] + key * 128;
+      const int swz = (key >> 1) & 7, u = 2 * (lane & 3);
+      *(bf16x8*)(row + ((u ^ swz) << 4)) = fp8_to_bf16(x.codes[0], x.codes[1], scale);
+      *(bf16x8*)(row + (((u + 1) ^ swz) << 4)) = fp8_to_bf16(x.codes[2], x.codes[3], scale);
+      return;
+    }
+    const int n = quad & 7, r = lane & 15;
     const int unit = 4 * (quad >> 3) + 2 * (n >> 2) + (n & 1), half = (n >> 1) & 1;
     uint32_t keep = ~0u;
     if (kb + kFp8Block > L) {  // stale codes past the sequence's end may be NaN
@@ -566,10 +572,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
     float s[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      s[j] = __uint_as_float(min((vsc >> (8 * j)) & 255u, kFp8BadScale - 1u) << 23);
+      s[j] = __uint_as_float(min((x.vs >> (8 * j)) & 255u, kFp8BadScale - 1u) << 23);
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) {
-      const uint32_t w = vr[dt] & keep;
+      const uint32_t w = x.codes[dt] & keep;
       auto pair = [&](float s0, float s1, auto hi) {  // two keys, each with its scale
         const auto x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s0, decltype(hi)::value);
         const auto x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s1, decltype(hi)::value);
@@ -582,133 +588,135 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
     }
   };
 
-  if (begin < end) {
-    load(page_id(begin));
-    store(0, begin * kFp8Block);
+  // the first blocks' codes and q are on their way at once
+  Raw raw, raw0;
+  if (stages && begin < end) {
+    fetch_ids(begin);
+    load(raw0, begin);
+    load(raw, begin + 1);
   }
-  int next_id = begin + 1 < end ? page_id(begin + 1) : 0;
-  __syncthreads();
+  const int token = min(4 * wave + (c >> 3), nt - 1);
+  const uint16_t sink = a.sinks[hk * kGroup + (c & 7)];
+  bf16x8 qv[4];
+  {
+    const u32x4* src =
+        (const u32x4*)(a.q + ((size_t)(row0 + token) * kHq + hk * kGroup + (c & 7)) * kD);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qv[s] = moe::as_bf16x8(src[2 * s + h]);
+  }
+  const int qpos = pos + token - 4 * h;  // element i's key is 8 (i / 4) + i % 4 from 4 h on
+  const unsigned reach = a.window > 0 ? a.window : 0x7FFFFFFFu;  // keys back that a token sees
+  const moe::bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+  f32x16 o[2];
+  float mneg = INFINITY, l = 0.f;
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+
+  if (stages && begin < end) store(raw0, 0, begin * kFp8Block);
+  moe::lds_barrier();
   int buf = 0;
-  for (int blk = begin; blk < end; ++blk) {
-    const int kb = blk * kFp8Block;
-    const bool more = blk + 1 < end;
-    if (more) {
-      load(next_id);  // in flight during this block's products
-      if (blk + 2 < end) next_id = page_id(blk + 2);
-    }
-    const bool whole = kb + kFp8Block - 1 <= pos && (a.window <= 0 || kb > sight.last - a.window);
-    bf16x8 ka[4], va[2][2];
-    auto read_k = [&](int kt32) {
-      const int key = 32 * kt32 + c;
+  auto run = [&](auto masked, int from, int to) __attribute__((always_inline)) {
+    for (int blk = from; blk < to; ++blk) {
+      const int kb = blk * kFp8Block;
 #pragma unroll
-      for (int s = 0; s < 4; ++s)
-        ka[s] = *(const bf16x8*)(kt[buf] + key * 128 + (((2 * s + h) ^ ((key >> 1) & 7)) << 4));
-    };
-    auto read_v = [&](int kt32) {
+      for (int kt32 = 0; kt32 < 2; ++kt32) {
+        f32x16 s;
 #pragma unroll
-      for (int dt = 0; dt < 2; ++dt)
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          const bf16x8 ka = *(const bf16x8*)(kt[buf] + (32 * kt32 + c) * 128 +
+                                             (((2 * st + h) ^ ((c >> 1) & 7)) << 4));
+          s = mfma32(ka, qv[st], s);
+        }
+        if constexpr (decltype(masked)::value) {
+          const int back = qpos - kb - 32 * kt32;  // of the first element's key behind the token
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            s[i] = (unsigned)(back - 8 * (i >> 2) - (i & 3)) < reach ? s[i] : -INFINITY;
+        }
+        moe::bf16x2 p[8];
+        float ps;
+        auto exps = [&](float mn) __attribute__((always_inline)) {
+          ps = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            p[i][0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i], a.c2, mn));
+            p[i][1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], a.c2, mn));
+            ps = __builtin_amdgcn_fdot2_f32_bf16(p[i], ones, ps, false);
+          }
+        };
+        exps(mneg);
+        if (__any(!(ps < kTileMost))) {
+          float mx = s[0];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+          const float m = -mneg, mn = fmaxf(m, half_max(mx) * a.c2);
+          const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+          for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+          l *= alpha;
+          mneg = -mn;
+          exps(mn == -INFINITY ? 0.0f : -mn);
+        }
+        l += ps;
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          const int d = 32 * dt + c;
-          va[dt][m] = *(const bf16x8*)(vt[buf] + d * 128 +
-                                       (((4 * kt32 + 2 * m + h) ^ ((d >> 1) & 7)) << 4));
-        }
-    };
-    auto scores = [&](f32x16& s, int ct) {
+          bf16x8 pb;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = 0.f;
+          for (int j = 0; j < 8; ++j) pb[j] = p[4 * m + (j >> 1)][j & 1];
 #pragma unroll
-      for (int st = 0; st < 4; ++st) s = mfma32(ka[st], qv[ct][st], s);
-    };
-    auto softmax_pv = [&](f32x16& s, int kt32, int ct) {
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = kb + 32 * kt32 + 8 * (i >> 2) + 4 * h + (i & 3);
-          const bool ok = key <= qpos[ct] && (a.window <= 0 || key > qpos[ct] - a.window);
-          s[i] = ok ? s[i] : -INFINITY;
+          for (int dt = 0; dt < 2; ++dt) {
+            const bf16x8 va = *(const bf16x8*)(vt[buf] + (32 * dt + c) * 128 +
+                                               (((4 * kt32 + 2 * m + h) ^ ((c >> 1) & 7)) << 4));
+            o[dt] = mfma32(va, pb, o[dt]);
+          }
         }
       }
-      moe::bf16x2 pk[8];
-      float ps;
-      const moe::bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
-      auto exps = [&](float mn) {
-        ps = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          pk[i][0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i], a.c2, mn));
-          pk[i][1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], a.c2, mn));
-          ps = __builtin_amdgcn_fdot2_f32_bf16(pk[i], ones, ps, false);
-        }
-      };
-      exps(mneg[ct]);
-      if (__any(!(ps < kTileMost))) {
-        float mx = s[0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        const float m = -mneg[ct], mn = fmaxf(m, half_max(mx) * a.c2);
-        const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-#pragma unroll
-        for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[ct][dt][i] *= alpha;
-        l[ct] *= alpha;
-        mneg[ct] = -mn;
-        exps(mn == -INFINITY ? 0.0f : -mn);
-      }
-      l[ct] += ps;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        bf16x8 p;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = pk[4 * m + (j >> 1)][j & 1];
-#pragma unroll
-        for (int dt = 0; dt < 2; ++dt) o[ct][dt] = mfma32(va[dt][m], p, o[ct][dt]);
-      }
-    };
-    f32x16 s0, s1;
-    read_k(0);
-    scores(s0, 0);
-    scores(s1, 1);
-    read_v(0);
-    read_k(1);
-    softmax_pv(s0, 0, 0);
-    scores(s0, 0);
-    softmax_pv(s1, 0, 1);
-    scores(s1, 1);
-    read_v(1);
-    softmax_pv(s0, 1, 0);
-    softmax_pv(s1, 1, 1);
-    if (more) store(buf ^ 1, kb + kFp8Block);
-    __syncthreads();
-    buf ^= 1;
-  }
+      if (stages && blk + 1 < end) store(raw, buf ^ 1, kb + kFp8Block);
+      if (stages && blk + 2 < end) load(raw, blk + 2);  // in flight during the next block's products
+      moe::lds_barrier();
+      buf ^= 1;
+    }
+  };
+  // blocks that every token sees whole: from whole0 to whole1
+  const int whole1 = max(begin, min(end, (pos + 1) / kFp8Block));
+  const int whole0 = min(whole1, a.window <= 0 ? begin
+                                               : max(begin, (sight.last - a.window) / kFp8Block + 1));
+  run(std::true_type{}, begin, whole0);
+  run(std::false_type{}, whole0, whole1);
+  run(std::true_type{}, whole1, end);
+
+  const float lt = l + __shfl_xor(l, 32, kWave);
   const bool alone = shares.used <= 1;
-#pragma unroll
-  for (int ct = 0; ct < 2; ++ct) {
-    const float lt = l[ct] + __shfl_xor(l[ct], 32, kWave);
-    const int token = 8 * wave + 4 * ct + (c >> 3), head = hk * kGroup + (c & 7);
-    if (token >= nt) continue;
-    const size_t at = (size_t)(row0 + token) * kHq + head;
-    const float f = alone ? sink_share(lt, -mneg[ct], a.sinks[head]) : 1.0f;
-    const size_t pt = (size_t)share * a.rows * kHq + at;
+  if (4 * wave + (c >> 3) >= nt) return;
+  const size_t at = (size_t)(row0 + token) * kHq + hk * kGroup + (c & 7);
+  if (alone) {
+    const float f = sink_share(lt, -mneg, sink);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const int d = 32 * dt + 2 * i + 4 * h;
-        if (alone) {
-          uint16_t v4[4];
+        uint16_t v4[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) v4[j] = f2bf(o[ct][dt][i + j] * f);
-          *(uint2*)(a.out + at * kD + d) = make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
-                                                      (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
-        } else {
-          *(f32x4*)(a.part_o + pt * kD + d) =
-              f32x4{o[ct][dt][i], o[ct][dt][i + 1], o[ct][dt][i + 2], o[ct][dt][i + 3]};
-        }
+        for (int j = 0; j < 4; ++j) v4[j] = f2bf(o[dt][i + j] * f);
+        *(uint2*)(a.out + at * kD + 32 * dt + 2 * i + 4 * h) =
+            make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
+                       (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
       }
-    if (!alone && h == 0) *(float2*)(a.part_ml + pt * 2) = make_float2(-mneg[ct], lt);
+  } else {
+    const size_t pt = (size_t)share * a.rows * kHq + at;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *(f32x4*)(a.part_o + pt * kD + 32 * dt + 2 * i + 4 * h) =
+            f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+    if (h == 0) *(float2*)(a.part_ml + pt * 2) = make_float2(-mneg, lt);
   }
 }
 
@@ -801,26 +809,32 @@ int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const in
   return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
-// tokens: of a tile, 8 or 32; part_o [splits][rows][64][64], part_ml
+// tokens: of a tile, 8, 32 or (not split) 64; part_o [splits][rows][64][64], part_ml
 // [splits][rows][64][2] where splits > 1
 int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
                           const void* cache, const int* page_indptr, const int* page_indices,
                           int num_pages, const int* kv_len, int window, float sm_scale,
                           const void* sinks, void* out, int tokens, int splits, int rows,
                           float* part_o, float* part_ml, hipStream_t s) {
-  if (tokens != 8 && tokens != attn::kTileTokens) return -6;
+  if (tokens != 8 && tokens != 32 && !(tokens == 64 && splits == 1)) return -6;
   const int tiles = (max_q_len + tokens - 1) / tokens;
   const attn::RowsArgs a{(const uint16_t*)q, q_indptr, (const uint8_t*)cache, page_indptr,
                          page_indices, kv_len, (const uint16_t*)sinks, (uint16_t*)out, part_o,
                          part_ml, nullptr, 0, num_pages, window, splits, rows, tiles,
                          sm_scale * attn::kLog2e};
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(attn::kHkv * batch * tiles, splits), dim3(256), 0, s, a);
+  auto go = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3(attn::kHkv * batch * tiles, splits), dim3(threads), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -6;
   };
-  const int rc = tokens != attn::kTileTokens ? go(attn::fp8_rows_kernel<4, false>)
-                 : splits > 1                ? go(attn::fp8_tile_kernel<true>)
-                                             : go(attn::fp8_tile_kernel<false>);
+  int rc = -6;
+  if (tokens == 8)
+    rc = go(attn::fp8_rows_kernel<4, false>, 256);
+  else if (tokens == 64)
+    rc = go(attn::fp8_tile_kernel<64, false>, attn::tile_threads(64));
+  else if (splits > 1)
+    rc = go(attn::fp8_tile_kernel<32, true>, attn::tile_threads(32));
+  else
+    rc = go(attn::fp8_tile_kernel<32, false>, attn::tile_threads(32));
   if (rc || splits == 1) return rc;
   hipLaunchKernelGGL(attn::fp8_merge_kernel, dim3(batch * tiles, tokens * attn::kHq / 16),
                      dim3(256), 0, s, a, tokens);

@@ -325,6 +325,15 @@ def test_prefill_long(A, window):
     check_prefill(A, seqs, [2100], window, 42, 2100, rows, scale=12.0)
 
 
+@pytest.mark.parametrize("window", [0, 128])
+def test_prefill_many_tiles(A, window):
+    """A ragged batch whose query tiles are two rounds of the chip (the larger tiles)."""
+    qlens, prefix = [512, 1, 64, 65, 130, 0, 257, 511], [0, 700, 3, 64, 1, 9, 300, 77]
+    seqs = Seqs(45, [p + q for p, q in zip(prefix, qlens)])
+    rows = np.array([0, 1, 3, 4, 31, 32, 63, 64, 100, 129, 200, 255, 256, 400, 510, 511])
+    check_prefill(A, seqs, qlens, window, 46, 777, rows)
+
+
 def test_prefill_creeping_maximum(A):
     """Scores that rise block by block, slowly and by large steps, and ones that fall: the
     running reference point of the softmax has to follow."""
