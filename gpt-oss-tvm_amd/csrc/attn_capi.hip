@@ -54,8 +54,8 @@ int attn_launch_fp8_read(const void* cache, int num_pages, const int* slots, int
 int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const int* page_indptr,
                            const int* page_indices, int num_pages, const int* kv_len,
                            int64_t max_span, int window, float sm_scale, const void* sinks,
-                           int splits, float* part_o, float* part_ml, int* arrive, void* out,
-                           hipStream_t s);
+                           int splits, int least, float* part_o, float* part_ml, int* arrive,
+                           void* out, hipStream_t s);
 int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
                           const void* cache, const int* page_indptr, const int* page_indices,
                           int num_pages, const int* kv_len, int window, float sm_scale,
@@ -420,37 +420,49 @@ namespace {
 constexpr int64_t kFp8Block = 64;  // keys of a block of the 8-bit attention kernels
 // 64-key blocks that a span of keys can touch
 int64_t fp8_blocks(int64_t span) { return (span + 2 * (kFp8Block - 1)) / kFp8Block; }
+// Blocks that a split has at least (a wave of the workgroup takes one), splits at most.
+constexpr int64_t kFp8SplitBlocks = 4, kFp8MaxSplits = 64;
 
-// Splits of a sequence's keys, at least 4 blocks each (a wave of the workgroup takes
-// one).  The kernel shares a sequence's own blocks out over at most kFp8DecWgs
-// workgroups' worth of them, whatever max_span is: the bound only trims the grid.
-constexpr int64_t kFp8SplitBlocks = 4, kFp8MaxSplits = 64, kFp8DecWgs = 2048;
+// Decode: blocks that a split has at least, and splits at most.  A split costs its start
+// and its part of the merge, so a batch that fills the chip with a workgroup a head
+// (64 sequences) is split only where sequences are longer than 64 blocks (64 of 1024 to
+// 4096 keys: 38.7 us, in halves 41.0; 16 of up to 2000: 13.7 in halves, 12.2 in
+// quarters).  One sequence alone takes more than 32 where they have 16 blocks each (131072
+// keys: 37.3 us in 32, 34.8 in 64; 20000 keys: 15.3 in 32, 18.9 in 64).
+int64_t fp8_decode_least(int64_t batch) {
+  return batch >= 64 ? 64 : std::max(kFp8SplitBlocks, batch / 2);
+}
 int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
-  const int64_t most = std::max<int64_t>(
-      1, std::min(kFp8MaxSplits, kFp8DecWgs / (batch * kKvHeads)));
-  return std::max<int64_t>(1, std::min(most, fp8_blocks(max_span) / kFp8SplitBlocks));
+  const int64_t least = fp8_decode_least(batch), most = batch == 1 ? kFp8MaxSplits : 32;
+  return std::min(most, (fp8_blocks(max_span) + least - 1) / least);
 }
 
-// Tokens of a chunk's query tile, and how many splits its keys are shared out over.
-// Up to 8 tokens take the kernel that loads alone bind.  Longer chunks are split so
-// far that their workgroups fit the chip at once (two a CU), and take tiles of 64
-// tokens without a window where those are two rounds of the chip.
-constexpr int64_t kFp8ChunkWgs = 512;
+// Tokens of a chunk's query tile, and how many splits its keys are shared out over: as
+// many as let its workgroups fit the chip at once (two a CU).
+//  * 64 of more than 32 tokens, without a window, where they are two rounds of the chip.
+//  * 2 or 4 tokens (the loads bind) up to 24 tokens, and for longer chunks where there
+//    are few of these tiles over few keys; us in tiles of 4 and of 32, tokens over
+//    cached: 16 sequences of 24 over 2000 33.1 and 36.4; 64 over 6000 25.3 and 30.2; 200
+//    over 500 13.5 and 21.1, over 6000 63 and 48; 64 sequences of 32 over 300 55.7 and 37.8.
+constexpr int64_t kFp8ChunkWgs = 512, kFp8FewTokens = 24, kFp8FewTiles = 64, kFp8FewKeys = 200000;
 struct Fp8Chunk {
   int64_t tokens, splits, tiles;  // tiles of the longest sequence
 };
 Fp8Chunk fp8_chunk(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
-  auto make = [&](int64_t tokens, int64_t splits) {
-    return Fp8Chunk{tokens, splits, (max_q_len + tokens - 1) / tokens};
-  };
-  if (max_q_len > 8 && window <= 0 && (max_q_len + 63) / 64 * kKvHeads >= (512 + batch - 1) / batch)
-    return make(64, 1);
-  const int64_t tokens = max_q_len <= 8 ? 8 : 32;
-  const int64_t wgs = (max_q_len + tokens - 1) / tokens * batch * kKvHeads;
+  auto tiles_of = [&](int64_t tokens) { return (max_q_len + tokens - 1) / tokens; };
+  if (window <= 0 && max_q_len > 32 && tiles_of(64) * kKvHeads >= (512 + batch - 1) / batch)
+    return Fp8Chunk{64, 1, tiles_of(64)};
+  const int64_t reach = window > 0 ? std::min(max_kv_len, window + max_q_len) : max_kv_len;
+  const int64_t small = tiles_of(4) <= kFp8FewTiles ? tiles_of(4) * std::min(batch, kFp8FewTiles + 1)
+                                                    : kFp8FewTiles + 1;  // tiles of 4, or too many
+  const bool few = max_q_len <= kFp8FewTokens ||
+                   (small <= kFp8FewTiles && reach > 0 && small * reach <= kFp8FewKeys);
+  const int64_t tokens = max_q_len <= 2 ? 2 : few ? 4 : 32;
   const int64_t keys = window > 0 ? std::min(max_kv_len, window + tokens) : max_kv_len;
-  if (keys <= 0) return make(tokens, 1);
-  const int64_t most = std::min(kFp8MaxSplits, kFp8ChunkWgs / wgs);
-  return make(tokens, std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks)));
+  if (keys <= 0 || batch > kFp8ChunkWgs) return Fp8Chunk{tokens, 1, tiles_of(tokens)};
+  const int64_t most = std::min<int64_t>(kFp8MaxSplits, kFp8ChunkWgs / (tiles_of(tokens) * batch * kKvHeads));
+  return Fp8Chunk{tokens, std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks)),
+                  tiles_of(tokens)};
 }
 }  // namespace
 
@@ -480,7 +492,7 @@ int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cache, int6
   float* part_o = (float*)((char*)workspace + kDecodeCounts);
   return status(attn_launch_fp8_decode(q, (int)batch, kv_cache, page_indptr, page_indices,
                                        (int)num_pages, kv_len, max_span, window, sm_scale, sinks,
-                                       (int)splits, part_o,
+                                       (int)splits, (int)fp8_decode_least(batch), part_o,
                                        part_o + (size_t)splits * batch * kQHeads * kHeadDim,
                                        (int*)workspace, out, as_stream(stream)));
 }

@@ -99,16 +99,16 @@ __device__ __forceinline__ float sink_share(float l, float m, uint16_t sink) {
   return l == 0.0f ? 0.0f : 1.0f / (l + __builtin_amdgcn_exp2f(fmaf(bf2f(sink), kLog2e, -m)));
 }
 
-// How many splits a tile's `blocks` blocks of 64 keys are shared out over, at most
-// `most`: one per 4 blocks (each of a workgroup's waves then has one).  It follows
-// from the keys and `most`, so a caller's larger bound on the keys changes nothing.
+// How many splits a tile's `blocks` blocks of 64 keys are shared out over: as many as
+// have `least` blocks, more than 32 only where they have 16, at most `most`.  It follows
+// from the keys and not from the caller's bound on them, which only trims the grid.
 constexpr int kFp8Block = 64;
-constexpr int kFp8SplitBlocks = 4;
+constexpr float kFp8Most = 16777216.0f;  // 2^24
 struct Shares {
   int each, used;  // blocks of a split, splits with any
-  __device__ __forceinline__ Shares(int blocks, int most) {
-    const int n = max(1, min(blocks / kFp8SplitBlocks, most));
-    each = (blocks + n - 1) / n;
+  __device__ __forceinline__ Shares(int blocks, int most, int least) {
+    const int n = min(min(most, (blocks + least - 1) / least), max(32, (blocks + 15) / 16));
+    each = n > 0 ? (blocks + n - 1) / n : 0;
     used = each > 0 ? (blocks + each - 1) / each : 0;
   }
 };
@@ -124,23 +124,9 @@ struct Sight {
   }
 };
 
-// Few tokens: decode (kDecode: one token a sequence) and tiles of 2 kCt tokens of
-// a chunk.  Bound by the cache's bytes, so nothing but loads is on the way: a wave
-// takes blocks of 64 keys (four pages) alone, from global memory to registers,
-// no LDS and no barrier before the end.  Both products run on
-// v_mfma_f32_16x16x32_bf16 over columns (token, head of the group):
-//  * S^T = K Q^T: row r of score tile kk is key 4 kk + r % 4 of the block's page
-//    r / 4, so lane (r, g) loads 16 of its dims, 16 g .. 16 g + 15, and result
-//    element i of lane (column, g) is key 4 kk + i of page g;
-//  * O^T = V^T P^T: the lane's P operand then is its own scores, slots 4 kk + i of
-//    two products; V^T's slots the same keys of page g, dims 16 dt + r, as the
-//    cache holds them.
-// Codes go to bf16 exactly (k with its scale, whose row a lane holds alone; v
-// without: its scales multiply p); pv enters as two bf16 pieces, about 16 bits.
-// The loads of a block are in flight during the products of the one before.
 struct RowsArgs {
   const uint16_t* q;
-  const int* q_indptr;  // chunks only
+  const int* q_indptr;  // chunks
   const uint8_t* cache;
   const int* page_indptr;
   const int* page_indices;
@@ -151,39 +137,329 @@ struct RowsArgs {
   float* part_ml;  // [splits][rows][64][2]
   int* arrive;     // decode: [batch][8], left zero
   int64_t max_span;
-  int num_pages, window, splits, rows, tiles;
+  int num_pages, window, splits, least, rows, tiles;
   float c2;        // sm_scale log2(e)
 };
 
-struct KvRegs {
-  u32x4 k[4], v[4], ks, vs;
-};
+// Decode: one token a sequence.  Bound by the cache's bytes, so nothing but loads is on
+// the way: a wave takes blocks of 64 keys (four pages) alone, from global memory to
+// registers, no LDS and no barrier before the end; a load takes the 1 KB that a page
+// holds of a kv head's k or v, past the caches (nontemporal: read once; 7.1 TB/s
+// against 6.3 in a kernel that only loads).  Both products run on
+// v_mfma_f32_16x16x32_bf16 with the 8 heads of a kv head in columns 0 .. 7 and again
+// in 8 .. 15:
+//  * S^T = K Q^T: row r of a page's score tile is its key r, so lane (r, g) loads dims
+//    16 g .. 16 g + 15 of it, and result element i of lane (column, g) is key 4 g + i;
+//  * O^T = V^T P^T over two pages: the lane's P operand then is its own scores, slot
+//    4 kk + i for page kk of the two; V^T's slots the same keys, dims 16 dt + r, as the
+//    cache holds them.
+// Columns 0 .. 7 keep the scores of the block's first two pages and 8 .. 15 those of
+// the others, each column with a softmax state of its own, so that every lane's
+// exponential is of use; each half's products give one half of the columns, the other
+// is not looked at.
+// Codes go to bf16 exactly (k with its scale, whose row a lane holds alone; v
+// without: its scales multiply p); pv enters as two bf16 pieces, about 16 bits.
+// k of the next block is in flight from the scores on, v from the products on.
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void fp8_decode_kernel(
+    RowsArgs a) {
+  constexpr int kStates = 8;  // of a head in a workgroup: 4 waves, two halves
+  __shared__ __align__(16) float obuf[4][16][kD + 4];
+  __shared__ float mbuf[4][16], lbuf[4][16];
+  // x: (sequence, kv head), y: split
+  const int hk = blockIdx.x % kHkv, b = blockIdx.x / kHkv, share = blockIdx.y;
+  const int L = a.kv_len[b], pos = L - 1;
+  const Sight sight(pos, 1, a.window);
+  const Shares shares(sight.blocks, a.splits, a.least);
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int lane = t & 63, r = lane & 15, g = lane >> 4;
+  const bool second = r >= 8;
+  const bool too_long = (int64_t)sight.last + 1 - sight.lo > a.max_span;
+  if (share >= max(shares.used, 1) || (too_long && share > 0)) return;
+  if (too_long) {
+    for (int i = t; i < kGroup * kD; i += 256)
+      a.out[((size_t)b * kHq + hk * kGroup) * kD + i] = 0x7FC0;
+    return;
+  }
+  const PageList pages{a.page_indices + a.page_indptr[b],
+                       a.page_indptr[b + 1] - a.page_indptr[b], a.num_pages};
+  const int last_page = max(0, min(pages.count - 1, (L - 1) / kPage));
+  const int begin = share * shares.each, end = min(begin + shares.each, sight.blocks);
+  const unsigned reach = a.window > 0 ? a.window : 0x7FFFFFFFu;  // keys back that it sees
 
-template <int kCt, bool kDecode>
-__global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
+  // The wave's blocks: begin + wave, + 4, ...  Lane 4 j + p holds the page p of the
+  // j-th of 16 blocks.
+  int ids = 0;
+  auto fetch_ids = [&](int blk) {
+    const int i = (sight.first + blk + 4 * (lane >> 2)) * 4 + (lane & 3);
+    ids = pages.count > 0 ? pages.clamp(pages.ids[min(i, last_page)]) : 0;
+  };
+  u32x4 k[4], v[4];      // of the block's pages
+  uint32_t ks[4], vs[2];  // k's scale of key r; v's of keys 4 g .. of the lane's own pages
+  const unsigned k_at = hk * kFp8Head + r * kFp8Row + g * 16;
+  const unsigned v_at = kFp8V + hk * kFp8Head + lane * 16;
+  const unsigned s_at = kFp8Scales + hk * 2 * kPage;
+  auto page_of = [&](int j, int p) {  // of the j-th block at hand
+    return a.cache + (size_t)(unsigned)__builtin_amdgcn_readlane(ids, 4 * j + p) * kFp8Page;
+  };
+  auto load_k = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const uint8_t* page = page_of(j, p);
+      k[p] = __builtin_nontemporal_load((const u32x4*)(page + k_at));
+      ks[p] = page[s_at + r];
+    }
+  };
+  auto load_v = [&](int j) __attribute__((always_inline)) {
+    const uint8_t* page[4];
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      page[p] = page_of(j, p);
+      v[p] = __builtin_nontemporal_load((const u32x4*)(page[p] + v_at));
+    }
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+      vs[kk] = *(const uint32_t*)((second ? page[2 + kk] : page[kk]) + s_at + kPage + 4 * g);
+  };
+  fetch_ids(begin + wave);
+
+  // Q operand: column r is head r % 8
+  bf16x8 qv[2];
+  {
+    const u32x4* src = (const u32x4*)(a.q + ((size_t)b * kHq + hk * kGroup + (r & 7)) * kD);
+    qv[0] = moe::as_bf16x8(src[2 * g]);
+    qv[1] = moe::as_bf16x8(src[2 * g + 1]);
+  }
+  f32x4 o[2][4];
+  float mneg = INFINITY, l = 0.f;  // minus the column's reference point (not set: inf)
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) o[x][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  for (int c0 = begin + wave; c0 < end; c0 += 64) {  // 16 of the wave's blocks
+    if (c0 != begin + wave) fetch_ids(c0);
+    const int n = min(16, (end - c0 + 3) / 4);
+    load_k(0);
+    load_v(0);
+    for (int j = 0; j < n; ++j) {
+      const int kb = (sight.first + c0 + 4 * j) * kFp8Block;
+      f32x4 st[2];
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        f32x4 s[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const u32x4 kp = k[2 * x + kk];
+          const float scale = __uint_as_float(min(ks[2 * x + kk], kFp8BadScale - 1u) << 23);
+          s[x] = mfma_bf16(fp8_to_bf16(kp[0], kp[1], scale), qv[0], f32x4{0.f, 0.f, 0.f, 0.f});
+          s[x] = mfma_bf16(fp8_to_bf16(kp[2], kp[3], scale), qv[1], s[x]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st[kk][i] = second ? s[1][i] : s[0][i];
+      }
+      if (j + 1 < n) load_k(j + 1);
+      // every key of the block is seen
+      const bool whole = kb + kFp8Block - 1 <= pos && (a.window <= 0 || kb > pos - a.window);
+      const int back = pos - (kb + (second ? 32 : 0) + 4 * g);  // of the lane's first key
+      if (!whole) {
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            st[kk][i] = (unsigned)(back - 16 * kk - i) < reach ? st[kk][i] : -INFINITY;
+      }
+      float p[8], ps;
+      auto exps = [&](float mn) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          p[i] = __builtin_amdgcn_exp2f(fmaf(st[i >> 2][i & 3], a.c2, mn));
+        ps = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+      };
+      exps(mneg);
+      if (__any(!(ps < kFp8Most))) {
+        float mx = st[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, st[i >> 2][i & 3]);
+        const float mo = -mneg, mn = fmaxf(mo, group_max(mx) * a.c2);
+        const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mo - mn);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[x][dt][i] *= alpha;
+        l *= alpha;
+        mneg = -mn;
+        exps(mn == -INFINITY ? 0.0f : -mn);
+      }
+      l += ps;
+      bf16x8 ph, pl;
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // times v's scale.  A bad row's byte gives an infinite factor: NaN from its
+          // codes 0; a hidden key's p of 0 stays 0
+          float pv = p[4 * kk + i] * __uint_as_float(((vs[kk] >> (8 * i)) & 255u) << 23);
+          if (!whole) pv = (unsigned)(back - 16 * kk - i) < reach ? pv : 0.0f;
+          const __bf16 hi = (__bf16)pv;
+          ph[4 * kk + i] = hi;
+          pl[4 * kk + i] = (__bf16)(pv - (float)hi);
+        }
+      if (kb + kFp8Block > L) {  // stale codes past the sequence's end may be NaN
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const int left = min(max(L - (kb + 16 * p + 4 * g), 0), 4);
+          const uint32_t keep = left == 4 ? ~0u : (1u << (8 * left)) - 1u;
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) v[p][dt] &= keep;
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const bf16x8 va = fp8_to_bf16(v[2 * x][dt], v[2 * x + 1][dt], 1.0f);
+          o[x][dt] = mfma_bf16(va, ph, o[x][dt]);
+          o[x][dt] = mfma_bf16(va, pl, o[x][dt]);
+        }
+      if (j + 1 < n) load_v(j + 1);
+    }
+  }
+
+  // The eight states of a head merged, in a fixed order: 32 threads a head, two
+  // dimensions each
+  l += __shfl_xor(l, 16, kWave);
+  l += __shfl_xor(l, 32, kWave);
+  if (g == 0) {
+    mbuf[wave][r] = -mneg;
+    lbuf[wave][r] = l;
+  }
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) {
+    f32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = second ? o[1][dt][i] : o[0][dt][i];
+    *(f32x4*)&obuf[wave][r][16 * dt + 4 * g] = w;
+  }
+  __syncthreads();
+  const int h = t >> 5, i0 = t & 31, d = 2 * i0;
+  // the weight of a state; one that saw no key: m = -inf, l = 0, o = 0
+  auto weight = [](float m, float l, float top) {
+    return m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+  };
+  float mt = -INFINITY, lt = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+  for (int s = 0; s < kStates; ++s) mt = fmaxf(mt, mbuf[s >> 1][h + 8 * (s & 1)]);
+#pragma unroll
+  for (int s = 0; s < kStates; ++s) {
+    const int w = s >> 1, c = h + 8 * (s & 1);
+    const float wgt = weight(mbuf[w][c], lbuf[w][c], mt);
+    lt = fmaf(lbuf[w][c], wgt, lt);
+    const float2 ow = *(const float2*)&obuf[w][c][d];
+    o0 = fmaf(ow.x, wgt, o0);
+    o1 = fmaf(ow.y, wgt, o1);
+  }
+  const size_t at = (size_t)b * kHq + hk * kGroup + h, step = (size_t)a.rows * kHq;
+  const uint16_t sink = a.sinks[hk * kGroup + h];
+  auto write = [&](float l_all, float m_all) {
+    const float f = sink_share(l_all, m_all, sink);
+    *(uint32_t*)(a.out + at * kD + d) = (uint32_t)f2bf(o0 * f) | ((uint32_t)f2bf(o1 * f) << 16);
+  };
+  const int used = shares.used;
+  if (used <= 1) {
+    write(lt, mt);
+    return;
+  }
+  // to be merged by a workgroup of this launch: device scope
+  const size_t pt = at + (size_t)share * step;
+  store_dev((uint64_t*)(a.part_o + pt * kD + d),
+            (uint64_t)__float_as_uint(o0) | ((uint64_t)__float_as_uint(o1) << 32));
+  if (i0 == 0)
+    store_dev((uint64_t*)(a.part_ml + pt * 2),
+              (uint64_t)__float_as_uint(mt) | ((uint64_t)__float_as_uint(lt) << 32));
+  // The last of the head group's splits to finish merges them: its stores are
+  // done (vmcnt), the workgroup meets, one thread counts; the one that completes
+  // the count leaves it zero for the next call.
+  __shared__ int is_last;
+  moe::wait_vmcnt<0>();
+  __syncthreads();
+  if (t == 0) {
+    int* cnt = a.arrive + b * kHkv + hk;
+    const int prev = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    is_last = prev == used - 1;
+    if (is_last) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!is_last) return;
+  // The states (a lane a split, its weights to LDS) and o (a thread two dimensions, over the
+  // splits in order, sixteen loads in flight, the first beside the states').
+  __shared__ float wgt[kGroup][64];  // used <= 64
+  float ms[2], ls[2];
+  mt = -INFINITY;
+  lt = o0 = o1 = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int s = i0 + 32 * j;
+    uint64_t ml = (uint64_t)0xFF800000u;  // m = -inf, l = 0
+    if (s < used) ml = load_dev((const uint64_t*)(a.part_ml + (at + s * step) * 2));
+    ms[j] = __uint_as_float((uint32_t)ml);
+    ls[j] = __uint_as_float((uint32_t)(ml >> 32));
+  }
+  for (int s0 = 0; s0 < used; s0 += 16) {
+    uint64_t po[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      po[i] = load_dev((const uint64_t*)(a.part_o + (at + min(s0 + i, used - 1) * step) * kD + d));
+    if (s0 == 0) {
+      mt = fmaxf(ms[0], ms[1]);
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) mt = fmaxf(mt, __shfl_xor(mt, off, kWave));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float w = weight(ms[j], ls[j], mt);
+        if (i0 + 32 * j < used) wgt[h][i0 + 32 * j] = w;
+        lt = fmaf(ls[j], w, lt);
+      }
+#pragma unroll
+      for (int off = 16; off >= 1; off >>= 1) lt += __shfl_xor(lt, off, kWave);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (s0 + i < used) {
+        o0 = fmaf(__uint_as_float((uint32_t)po[i]), wgt[h][s0 + i], o0);
+        o1 = fmaf(__uint_as_float((uint32_t)(po[i] >> 32)), wgt[h][s0 + i], o1);
+      }
+  }
+  write(lt, mt);
+}
+
+// Chunks of few tokens (drafts under verification): a tile of 2 kCt tokens in kCt tiles
+// of 16 columns (token, head), by decode's loads and products; p enters as one
+// bf16 rounding, as in the long chunks' form.  More tokens take more such tiles,
+// which find the keys in the cache: four column tiles a wave spill (16 sequences of 5
+// tokens over up to 4000 keys: 54 us in tiles of 8, 29 in tiles of 4).
+template <int kCt>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void fp8_rows_kernel(
+    RowsArgs a) {
   constexpr int kCols = 16 * kCt;
   __shared__ __align__(16) float obuf[4][16][kD + 4];  // one column tile of each wave
   __shared__ float mbuf[4][kCols], lbuf[4][kCols];
   // x: (sequence, tile, kv head), y: split
   const int hk = blockIdx.x % kHkv, share = blockIdx.y;
   const int b = blockIdx.x / kHkv / a.tiles, tile = blockIdx.x / kHkv % a.tiles;
-  const int qb = kDecode ? b : a.q_indptr[b];
-  const int qn = kDecode ? 1 : a.q_indptr[b + 1] - qb;
+  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
   const int t0 = tile * 2 * kCt;
   if (t0 >= qn) return;
-  const int nt = kDecode ? 1 : min(2 * kCt, qn - t0);
+  const int nt = min(2 * kCt, qn - t0);
   const int L = a.kv_len[b], pos = L - qn + t0;  // of the tile's first token
   const Sight sight(pos, nt, a.window);
-  const Shares shares(sight.blocks, a.splits);
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, r = lane & 15, g = lane >> 4;
+  const Shares shares(sight.blocks, a.splits, a.least);
+  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int lane = t & 63, r = lane & 15, g = lane >> 4;
   const int row0 = qb + t0;
-  const bool too_long = kDecode && (int64_t)sight.last + 1 - sight.lo > a.max_span;
-  if (share >= max(shares.used, 1) || (too_long && share > 0)) return;
-  if (too_long) {
-    for (int i = t; i < kGroup * kD; i += 256)
-      a.out[((size_t)row0 * kHq + hk * kGroup) * kD + i] = 0x7FC0;
-    return;
-  }
+  if (share >= max(shares.used, 1)) return;
   const PageList pages{a.page_indices + a.page_indptr[b],
                        a.page_indptr[b + 1] - a.page_indptr[b], a.num_pages};
   const int last_page = max(0, min(pages.count - 1, (L - 1) / kPage));
@@ -198,11 +474,12 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
     qv[ct][0] = moe::as_bf16x8(src[2 * g]);
     qv[ct][1] = moe::as_bf16x8(src[2 * g + 1]);
   }
+  const unsigned reach = a.window > 0 ? a.window : 0x7FFFFFFFu;
   f32x4 o[kCt][4];
-  float m[kCt], l[kCt];
+  float mneg[kCt], l[kCt];  // minus the columns' reference points (not set: inf)
 #pragma unroll
   for (int ct = 0; ct < kCt; ++ct) {
-    m[ct] = -INFINITY;
+    mneg[ct] = INFINITY;
     l[ct] = 0.f;
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt) o[ct][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -215,118 +492,128 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
     const int i = (sight.first + blk + 4 * (lane >> 2)) * 4 + (lane & 3);
     ids = pages.count > 0 ? pages.clamp(pages.ids[min(i, last_page)]) : 0;
   };
-  auto load = [&](KvRegs& x, int j) {  // the j-th of the wave's 16 at hand
-    const uint8_t* kp = a.cache + (size_t)__shfl(ids, 4 * j + (r >> 2), kWave) * kFp8Page;
-    const uint8_t* vp = a.cache + (size_t)__shfl(ids, 4 * j + g, kWave) * kFp8Page;
-    const uint8_t* kr = kp + hk * kFp8Head + (r & 3) * kFp8Row + g * 16;
-    const uint8_t* vr = vp + kFp8V + hk * kFp8Head + r * 16;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) x.k[kk] = *(const u32x4*)(kr + kk * 4 * kFp8Row);
-#pragma unroll
-    for (int qd = 0; qd < 4; ++qd) x.v[qd] = *(const u32x4*)(vr + qd * 256);
-    x.ks = *(const u32x4*)(kp + kFp8Scales + hk * 2 * kPage);
-    x.vs = *(const u32x4*)(vp + kFp8Scales + hk * 2 * kPage + kPage);
+  u32x4 k[4], v[4];       // of the block's pages
+  uint32_t ks[4], vs[4];  // k's scale of key r; v's of keys 4 g ..
+  const unsigned k_at = hk * kFp8Head + r * kFp8Row + g * 16;
+  const unsigned v_at = kFp8V + hk * kFp8Head + lane * 16;
+  const unsigned s_at = kFp8Scales + hk * 2 * kPage;
+  auto page_of = [&](int j, int p) {  // of the j-th block at hand
+    return a.cache + (size_t)(unsigned)__builtin_amdgcn_readlane(ids, 4 * j + p) * kFp8Page;
   };
-  auto compute = [&](KvRegs& x, int kb) {  // kb: the block's first key
-    const int key0 = kb + 16 * g;          // this lane's page
-    if (kb + kFp8Block > L) {  // stale codes past the sequence's end may be NaN
+  auto load_k = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
-      for (int qd = 0; qd < 4; ++qd) {
-        const int n = min(max(L - (key0 + 4 * qd), 0), 4);
-        const uint32_t keep = n == 4 ? ~0u : (1u << (8 * n)) - 1u;
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) x.v[qd][dt] &= keep;
-      }
+    for (int p = 0; p < 4; ++p) {
+      const uint8_t* page = page_of(j, p);
+      k[p] = __builtin_nontemporal_load((const u32x4*)(page + k_at));
+      ks[p] = page[s_at + r];
     }
+  };
+  auto load_v = [&](int j) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const uint8_t* page = page_of(j, p);
+      v[p] = __builtin_nontemporal_load((const u32x4*)(page + v_at));
+      vs[p] = *(const uint32_t*)(page + s_at + kPage + 4 * g);
+    }
+  };
+  auto block = [&](int kb, int next) __attribute__((always_inline)) {  // kb: its first key
     bf16x8 ka[4][2];
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      const uint32_t s = min((x.ks[kk] >> (8 * (r & 3))) & 255u, kFp8BadScale - 1u);
-      const float scale = __uint_as_float(s << 23);
-      ka[kk][0] = fp8_to_bf16(x.k[kk][0], x.k[kk][1], scale);
-      ka[kk][1] = fp8_to_bf16(x.k[kk][2], x.k[kk][3], scale);
+    for (int p = 0; p < 4; ++p) {
+      const float scale = __uint_as_float(min(ks[p], kFp8BadScale - 1u) << 23);
+      ka[p][0] = fp8_to_bf16(k[p][0], k[p][1], scale);
+      ka[p][1] = fp8_to_bf16(k[p][2], k[p][3], scale);
     }
-    bf16x8 va[4][2];
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) {
-      va[dt][0] = fp8_to_bf16(x.v[0][dt], x.v[1][dt], 1.0f);
-      va[dt][1] = fp8_to_bf16(x.v[2][dt], x.v[3][dt], 1.0f);
-    }
+    if (next >= 0) load_k(next);  // in flight during the rest
     // every token of the tile sees the whole block
     const bool whole = kb + kFp8Block - 1 <= pos && (a.window <= 0 || kb > sight.last - a.window);
+    bf16x8 pb[kCt][2];
 #pragma unroll
     for (int ct = 0; ct < kCt; ++ct) {
       f32x4 st[4];
-      float mx = -INFINITY;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        st[kk] = mfma_bf16(ka[kk][0], qv[ct][0], f32x4{0.f, 0.f, 0.f, 0.f});
-        st[kk] = mfma_bf16(ka[kk][1], qv[ct][1], st[kk]);
+      for (int p = 0; p < 4; ++p) {
+        st[p] = mfma_bf16(ka[p][0], qv[ct][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        st[p] = mfma_bf16(ka[p][1], qv[ct][1], st[p]);
       }
+      // the token's position behind the lane's first key; it sees `reach` keys back
+      const int back = pos + min(2 * ct + (r >> 3), nt - 1) - (kb + 4 * g);
       if (!whole) {
-        const int p = pos + min(2 * ct + (r >> 3), nt - 1);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
+        for (int p = 0; p < 4; ++p)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = key0 + 4 * kk + i;
-            const bool ok = key <= p && (a.window <= 0 || key > p - a.window);
-            st[kk][i] = ok ? st[kk][i] : -INFINITY;
-          }
+          for (int i = 0; i < 4; ++i)
+            st[p][i] = (unsigned)(back - 16 * p - i) < reach ? st[p][i] : -INFINITY;
       }
+      f32x4 e[4];
+      float ps;
+      auto exps = [&](float mn) __attribute__((always_inline)) {
+        ps = 0.f;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
+        for (int p = 0; p < 4; ++p) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[kk][i]);
-      const float mn = fmaxf(m[ct], group_max(mx) * a.c2);
-      if (__any(mn > m[ct])) {
-        const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - mn);
+          for (int i = 0; i < 4; ++i) e[p][i] = __builtin_amdgcn_exp2f(fmaf(st[p][i], a.c2, mn));
+          ps += (e[p][0] + e[p][1]) + (e[p][2] + e[p][3]);
+        }
+      };
+      exps(mneg[ct]);
+      if (__any(!(ps < kFp8Most))) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, st[p][i]);
+        const float mo = -mneg[ct], mn = fmaxf(mo, group_max(mx) * a.c2);
+        const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mo - mn);
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[ct][dt][i] *= alpha;
         l[ct] *= alpha;
-        m[ct] = mn;
+        mneg[ct] = -mn;
+        exps(mn == -INFINITY ? 0.0f : -mn);
       }
-      const float mneg = m[ct] == -INFINITY ? 0.0f : -m[ct];
-      float ps = 0.f;
-      bf16x8 ph[2], pl[2];
+      l[ct] += ps;
+      // times v's scales.  A bad row's byte gives an infinite factor: NaN from its
+      // codes 0; a hidden key's p of 0 stays 0
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
+      for (int p = 0; p < 4; ++p)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(st[kk][i], a.c2, mneg));
-          ps += p;
-          // a bad row's scale byte gives an infinite factor: NaN from its codes 0
-          const float f = __uint_as_float(((x.vs[kk] >> (8 * i)) & 255u) << 23);
-          const float pv = whole || st[kk][i] != -INFINITY ? p * f : 0.0f;
-          const __bf16 hi = (__bf16)pv;
-          ph[kk >> 1][4 * (kk & 1) + i] = hi;
-          pl[kk >> 1][4 * (kk & 1) + i] = (__bf16)(pv - (float)hi);
-        }
-      l[ct] += ps;
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          o[ct][dt] = mfma_bf16(va[dt][h], ph[h], o[ct][dt]);
-          o[ct][dt] = mfma_bf16(va[dt][h], pl[h], o[ct][dt]);
+          float pv = e[p][i] * __uint_as_float(((vs[p] >> (8 * i)) & 255u) << 23);
+          if (!whole) pv = (unsigned)(back - 16 * p - i) < reach ? pv : 0.0f;
+          pb[ct][p >> 1][4 * (p & 1) + i] = (__bf16)pv;
         }
     }
+    if (kb + kFp8Block > L) {  // stale codes past the sequence's end may be NaN
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int left = min(max(L - (kb + 16 * p + 4 * g), 0), 4);
+        const uint32_t keep = left == 4 ? ~0u : (1u << (8 * left)) - 1u;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) v[p][dt] &= keep;
+      }
+    }
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) {
+      const bf16x8 v0 = fp8_to_bf16(v[0][dt], v[1][dt], 1.0f);
+      const bf16x8 v1 = fp8_to_bf16(v[2][dt], v[3][dt], 1.0f);
+#pragma unroll
+      for (int ct = 0; ct < kCt; ++ct) {
+        o[ct][dt] = mfma_bf16(v0, pb[ct][0], o[ct][dt]);
+        o[ct][dt] = mfma_bf16(v1, pb[ct][1], o[ct][dt]);
+      }
+    }
+    if (next >= 0) load_v(next);
   };
 
   for (int c0 = begin + wave; c0 < end; c0 += 64) {  // 16 of the wave's blocks
     fetch_ids(c0);
     const int n = min(16, (end - c0 + 3) / 4);
-    KvRegs x[2];
-    load(x[0], 0);
-    for (int j = 0; j < n; j += 2) {
-      if (j + 1 < n) load(x[1], j + 1);
-      compute(x[0], (sight.first + c0 + 4 * j) * kFp8Block);
-      if (j + 1 >= n) break;
-      if (j + 2 < n) load(x[0], j + 2);
-      compute(x[1], (sight.first + c0 + 4 * (j + 1)) * kFp8Block);
-    }
+    load_k(0);
+    load_v(0);
+    for (int j = 0; j < n; ++j)
+      block((sight.first + c0 + 4 * j) * kFp8Block, j + 1 < n ? j + 1 : -1);
   }
 
   // The four waves' states merged, in wave order
@@ -336,7 +623,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
     lt += __shfl_xor(lt, 16, kWave);
     lt += __shfl_xor(lt, 32, kWave);
     if (g == 0) {
-      mbuf[wave][16 * ct + r] = m[ct];
+      mbuf[wave][16 * ct + r] = -mneg[ct];
       lbuf[wave][16 * ct + r] = lt;
     }
   }
@@ -373,79 +660,9 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
                                                   (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
     } else {
       const size_t pt = (size_t)share * a.rows * kHq + at;
-      if constexpr (kDecode) {  // merged by a workgroup of this launch: device scope
-#pragma unroll
-        for (int i = 0; i < 4; ++i) store_dev(a.part_o + pt * kD + d + i, ot[i]);
-        if (d == 0) {
-          store_dev(a.part_ml + pt * 2, mt);
-          store_dev(a.part_ml + pt * 2 + 1, lt);
-        }
-      } else {
-        *(f32x4*)(a.part_o + pt * kD + d) = ot;
-        if (d == 0) *(float2*)(a.part_ml + pt * 2) = make_float2(mt, lt);
-      }
+      *(f32x4*)(a.part_o + pt * kD + d) = ot;
+      if (d == 0) *(float2*)(a.part_ml + pt * 2) = make_float2(mt, lt);
     }
-  }
-  if constexpr (kDecode) {
-    if (alone) return;
-    // The last of the head group's splits to finish merges them: its stores are
-    // done (vmcnt), the workgroup meets, one thread counts; the one that completes
-    // the count leaves it zero for the next call.
-    __shared__ int is_last;
-    moe::wait_vmcnt<0>();
-    __syncthreads();
-    if (t == 0) {
-      int* cnt = a.arrive + b * kHkv + hk;
-      const int prev = __hip_atomic_fetch_add(cnt, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      is_last = prev == shares.used - 1;
-      if (is_last) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!is_last) return;
-    // 32 threads a head: the weights exp2(m_s - m) of its splits to LDS, then two
-    // dimensions each over the splits in order, eight loads in flight.
-    __shared__ float wgt[kGroup][64];  // used <= 64
-    const int h = t >> 5, i0 = t & 31;
-    const size_t at = (size_t)row0 * kHq + hk * kGroup + h, step = (size_t)a.rows * kHq;
-    const int used = shares.used;
-    float ms[2], ls[2], mt = -INFINITY, lt = 0.f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int s = i0 + 32 * j;
-      ms[j] = s < used ? load_dev(a.part_ml + (at + s * step) * 2) : -INFINITY;
-      ls[j] = s < used ? load_dev(a.part_ml + (at + s * step) * 2 + 1) : 0.0f;
-      mt = fmaxf(mt, ms[j]);
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mt = fmaxf(mt, __shfl_xor(mt, off, kWave));
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float w = ms[j] == -INFINITY && ls[j] == 0.0f ? 0.0f
-                                                          : __builtin_amdgcn_exp2f(ms[j] - mt);
-      if (i0 + 32 * j < used) wgt[h][i0 + 32 * j] = w;
-      lt = fmaf(ls[j], w, lt);
-    }
-#pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) lt += __shfl_xor(lt, off, kWave);
-    __syncthreads();
-    const int d = i0 * 2;
-    float o0 = 0.f, o1 = 0.f;
-    for (int s0 = 0; s0 < used; s0 += 8) {
-      uint64_t v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = load_dev((const uint64_t*)(a.part_o + (at + min(s0 + i, used - 1) * step) * kD + d));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float w = s0 + i < used ? wgt[h][s0 + i] : 0.0f;
-        if (s0 + i < used) {
-          o0 = fmaf(__uint_as_float((uint32_t)v[i]), w, o0);
-          o1 = fmaf(__uint_as_float((uint32_t)(v[i] >> 32)), w, o1);
-        }
-      }
-    }
-    const float f = sink_share(lt, mt, a.sinks[hk * kGroup + h]);
-    *(uint32_t*)(a.out + at * kD + d) = (uint32_t)f2bf(o0 * f) | ((uint32_t)f2bf(o1 * f) << 16);
   }
 }
 
@@ -482,7 +699,6 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(RowsArgs a) {
 // more columns: 4096 tokens 157 us against 161, 2048 tokens 72 against 54, 4096 with
 // window 128 44 against 33.  So they are taken without a window where they are two
 // rounds or more of the chip.
-constexpr float kTileMost = 16777216.0f;  // 2^24
 constexpr int kTileBytes = kFp8Block * kD * 2;
 constexpr int tile_threads(int tokens) { return 16 * tokens; }
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
@@ -513,7 +729,7 @@ fp8_tile_kernel(RowsArgs a) {
   const int nt = min(kTokens, qn - t0), row0 = qb + t0;
   const int L = a.kv_len[b], pos = L - qn + t0;
   const Sight sight(pos, nt, a.window);
-  const Shares shares(sight.blocks, kSplit ? a.splits : 1);
+  const Shares shares(sight.blocks, kSplit ? a.splits : 1, a.least);
   const int share = kSplit ? blockIdx.y : 0;
   if (share >= max(shares.used, 1)) return;
   const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
@@ -582,7 +798,8 @@ fp8_tile_kernel(RowsArgs a) {
         return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x1),
                                      __builtin_bit_cast(uint32_t, x0), 0x07060100u);
       };
-      const uint32_t p0 = pair(s[0], s[1], std::false_type{}), p1 = pair(s[2], s[3], std::true_type{});
+      const uint32_t p0 = pair(s[0], s[1], std::false_type{});
+      const uint32_t p1 = pair(s[2], s[3], std::true_type{});
       const int d = 16 * dt + r;
       *(uint2*)(vt[buf] + d * 128 + ((unit ^ ((d >> 1) & 7)) << 4) + 8 * half) = make_uint2(p0, p1);
     }
@@ -649,7 +866,7 @@ fp8_tile_kernel(RowsArgs a) {
           }
         };
         exps(mneg);
-        if (__any(!(ps < kTileMost))) {
+        if (__any(!(ps < kFp8Most))) {
           float mx = s[0];
 #pragma unroll
           for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
@@ -678,15 +895,15 @@ fp8_tile_kernel(RowsArgs a) {
         }
       }
       if (stages && blk + 1 < end) store(raw, buf ^ 1, kb + kFp8Block);
-      if (stages && blk + 2 < end) load(raw, blk + 2);  // in flight during the next block's products
+      if (stages && blk + 2 < end) load(raw, blk + 2);  // in flight during the next's products
       moe::lds_barrier();
       buf ^= 1;
     }
   };
   // blocks that every token sees whole: from whole0 to whole1
   const int whole1 = max(begin, min(end, (pos + 1) / kFp8Block));
-  const int whole0 = min(whole1, a.window <= 0 ? begin
-                                               : max(begin, (sight.last - a.window) / kFp8Block + 1));
+  const int seen0 = (sight.last - a.window) / kFp8Block + 1;
+  const int whole0 = min(whole1, a.window <= 0 ? begin : max(begin, seen0));
   run(std::true_type{}, begin, whole0);
   run(std::false_type{}, whole0, whole1);
   run(std::true_type{}, whole1, end);
@@ -729,7 +946,7 @@ __global__ __launch_bounds__(256) void fp8_merge_kernel(RowsArgs a, int tokens) 
   const int token = i / kHq, head = i % kHq, d = (threadIdx.x & 15) * 4;
   if (token >= tokens || t0 + token >= qn) return;
   const Sight sight(a.kv_len[b] - qn + t0, min(tokens, qn - t0), a.window);
-  const int used = Shares(sight.blocks, a.splits).used;
+  const int used = Shares(sight.blocks, a.splits, a.least).used;
   if (used <= 1) return;  // written already
   const size_t at = (size_t)(qb + t0 + token) * kHq + head, step = (size_t)a.rows * kHq;
   float m = -INFINITY, l = 0.f;
@@ -797,38 +1014,40 @@ int attn_launch_fp8_read(const void* cache, int num_pages, const int* slots, int
 int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const int* page_indptr,
                            const int* page_indices, int num_pages, const int* kv_len,
                            int64_t max_span, int window, float sm_scale, const void* sinks,
-                           int splits, float* part_o, float* part_ml, int* arrive, void* out,
-                           hipStream_t s) {
+                           int splits, int least, float* part_o, float* part_ml, int* arrive,
+                           void* out, hipStream_t s) {
   if (splits < 1 || splits > 64) return -6;
   const attn::RowsArgs a{(const uint16_t*)q, nullptr, (const uint8_t*)cache, page_indptr,
                          page_indices, kv_len, (const uint16_t*)sinks, (uint16_t*)out, part_o,
-                         part_ml, arrive, max_span, num_pages, window, splits, batch, 1,
+                         part_ml, arrive, max_span, num_pages, window, splits, least, batch, 1,
                          sm_scale * attn::kLog2e};
-  hipLaunchKernelGGL((attn::fp8_rows_kernel<1, true>), dim3(attn::kHkv * batch, splits), dim3(256),
+  hipLaunchKernelGGL(attn::fp8_decode_kernel, dim3(attn::kHkv * batch, splits), dim3(256),
                      0, s, a);
   return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
-// tokens: of a tile, 8, 32 or (not split) 64; part_o [splits][rows][64][64], part_ml
+// tokens: of a tile, 2, 4, 32 or (not split) 64; part_o [splits][rows][64][64], part_ml
 // [splits][rows][64][2] where splits > 1
 int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
                           const void* cache, const int* page_indptr, const int* page_indices,
                           int num_pages, const int* kv_len, int window, float sm_scale,
                           const void* sinks, void* out, int tokens, int splits, int rows,
                           float* part_o, float* part_ml, hipStream_t s) {
-  if (tokens != 8 && tokens != 32 && !(tokens == 64 && splits == 1)) return -6;
+  if (tokens == 64 && splits != 1) return -6;
   const int tiles = (max_q_len + tokens - 1) / tokens;
   const attn::RowsArgs a{(const uint16_t*)q, q_indptr, (const uint8_t*)cache, page_indptr,
                          page_indices, kv_len, (const uint16_t*)sinks, (uint16_t*)out, part_o,
-                         part_ml, nullptr, 0, num_pages, window, splits, rows, tiles,
+                         part_ml, nullptr, 0, num_pages, window, splits, 4, rows, tiles,
                          sm_scale * attn::kLog2e};
   auto go = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3(attn::kHkv * batch * tiles, splits), dim3(threads), 0, s, a);
     return hipGetLastError() == hipSuccess ? 0 : -6;
   };
   int rc = -6;
-  if (tokens == 8)
-    rc = go(attn::fp8_rows_kernel<4, false>, 256);
+  if (tokens == 2)
+    rc = go(attn::fp8_rows_kernel<1>, 256);
+  else if (tokens == 4)
+    rc = go(attn::fp8_rows_kernel<2>, 256);
   else if (tokens == 64)
     rc = go(attn::fp8_tile_kernel<64, false>, attn::tile_threads(64));
   else if (splits > 1)
