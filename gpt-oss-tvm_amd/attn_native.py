@@ -326,27 +326,36 @@ def rows_qkv_rope_append(x: torch.Tensor, W: torch.Tensor, bias: torch.Tensor,
 # -- the 8-bit KV cache: [pages, 16640] uint8 a layer (format in include/attn_gfx950.h) ----------
 
 FP8_PAGE_BYTES = 16640
+_BF16, _I32T, _F32T, _U8 = torch.bfloat16, torch.int32, torch.float32, torch.uint8
 
 
-def _expect_fp8(kv_cache: torch.Tensor) -> None:
-    _expect(kv_cache, "kv_cache", torch.uint8)
-    if kv_cache.dim() != 2 or kv_cache.shape[1] != FP8_PAGE_BYTES:
+def _refuse(t, name, dtype, shape, index):
+    """Says what is wrong with an argument that a wrapper's quick check did not pass."""
+    _expect(t, name, dtype, shape)
+    raise ValueError(f"{name}: on {t.device}, expected cuda:{index}, the current device")
+
+
+def _need(t, name, dtype, shape, index):
+    """``_expect``, and on the current device: the launch goes to its stream.  One line
+    where all is well: a call's checks cost as much host time as a short kernel runs."""
+    if not (type(t) in _TENSORS and t.dtype is dtype and t.get_device() == index
+            and t.shape == shape and t.is_contiguous()):
+        _refuse(t, name, dtype, shape, index)
+
+
+_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
+def _need_fp8(kv_cache):
+    """Of an 8-bit cache on the current device: its pages, the device's index and stream."""
+    if not isinstance(kv_cache, torch.Tensor) or kv_cache.dim() != 2:
+        _expect(kv_cache, "kv_cache", _U8)
         raise ValueError(f"kv_cache: expected [pages, {FP8_PAGE_BYTES}], "
                          f"got {tuple(kv_cache.shape)}")
-    _current(kv_cache, "kv_cache")
-
-
-def _current(t: torch.Tensor, name: str) -> None:
-    """The launch goes to the current device's stream."""
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name}: on {t.device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
-
-
-def _on(device: torch.device, **tensors: torch.Tensor) -> None:
-    for name, t in tensors.items():
-        if t.device != device:
-            raise ValueError(f"{name}: on {t.device}, kv_cache on {device}")
+    index, pages = kv_cache.get_device(), kv_cache.shape[0]
+    _need(kv_cache, "kv_cache", _U8, (pages, FP8_PAGE_BYTES),
+          torch.cuda.current_device() if index >= 0 else None)
+    return pages, index, _stream()
 
 
 def qkv_rope_append_fp8(qkv: torch.Tensor, bias: torch.Tensor, positions: torch.Tensor,
@@ -354,21 +363,17 @@ def qkv_rope_append_fp8(qkv: torch.Tensor, bias: torch.Tensor, positions: torch.
                         kv_cache: torch.Tensor, q_out: torch.Tensor) -> torch.Tensor:
     """``qkv_rope_append`` into the 8-bit cache: q as there, k and v quantised as they
     are written.  Slots inside the pool have to differ."""
-    _expect_fp8(kv_cache)
-    _expect(qkv, "qkv", torch.bfloat16)
-    if qkv.dim() != 2 or qkv.shape[1] != QKV_DIM:
-        raise ValueError(f"qkv: expected [n, {QKV_DIM}], got {tuple(qkv.shape)}")
+    pages, dev, stream = _need_fp8(kv_cache)
     n = qkv.shape[0]
-    _expect(bias, "bias", torch.bfloat16, (QKV_DIM,))
-    _expect(positions, "positions", torch.int32, (n,))
-    _expect(slots, "slots", torch.int32, (n,))
-    _expect(inv_freq, "inv_freq", torch.float32, (HEAD_DIM // 2,))
-    _expect(q_out, "q_out", torch.bfloat16, (n, Q_HEADS, HEAD_DIM))
-    _on(kv_cache.device, qkv=qkv, bias=bias, positions=positions, slots=slots, inv_freq=inv_freq,
-        q_out=q_out)
-    _check(_lib.attn_qkv_rope_append_fp8(_ptr(qkv), _ptr(bias), n, _ptr(positions), _ptr(slots),
-                                         _ptr(inv_freq), concentration, _ptr(kv_cache),
-                                         kv_cache.shape[0], _ptr(q_out), _stream()),
+    _need(qkv, "qkv", _BF16, (n, QKV_DIM), dev)
+    _need(bias, "bias", _BF16, (QKV_DIM,), dev)
+    _need(positions, "positions", _I32T, (n,), dev)
+    _need(slots, "slots", _I32T, (n,), dev)
+    _need(inv_freq, "inv_freq", _F32T, (HEAD_DIM // 2,), dev)
+    _need(q_out, "q_out", _BF16, (n, Q_HEADS, HEAD_DIM), dev)
+    _check(_lib.attn_qkv_rope_append_fp8(qkv.data_ptr(), bias.data_ptr(), n, positions.data_ptr(),
+                                         slots.data_ptr(), inv_freq.data_ptr(), concentration,
+                                         kv_cache.data_ptr(), pages, q_out.data_ptr(), stream),
            "attn_qkv_rope_append_fp8")
     return q_out
 
@@ -377,35 +382,36 @@ def kv_quantize_fp8(src: torch.Tensor, src_slots: torch.Tensor, kv_cache: torch.
                     slots: torch.Tensor) -> torch.Tensor:
     """Rows of a bf16 cache ``src`` [pages, 2, 8, 16, 64] at ``src_slots`` [n] into the 8-bit
     cache at ``slots`` [n] (which have to differ)."""
-    _expect_fp8(kv_cache)
-    _expect(src, "src", torch.bfloat16)
-    if src.dim() != 5 or tuple(src.shape[1:]) != (2, KV_HEADS, PAGE, HEAD_DIM):
-        raise ValueError(f"src: expected [pages, 2, {KV_HEADS}, {PAGE}, {HEAD_DIM}], "
-                         f"got {tuple(src.shape)}")
-    _expect(src_slots, "src_slots", torch.int32, (src_slots.numel(),))
-    n = src_slots.numel()
-    _expect(slots, "slots", torch.int32, (n,))
-    _on(kv_cache.device, src=src, src_slots=src_slots, slots=slots)
-    _check(_lib.attn_kv_quantize_fp8(_ptr(src), src.shape[0], _ptr(src_slots), n, _ptr(kv_cache),
-                                     kv_cache.shape[0], _ptr(slots), _stream()),
+    pages, dev, stream = _need_fp8(kv_cache)
+    src_pages, n = src.shape[0], src_slots.numel()
+    _need(src, "src", _BF16, (src_pages, 2, KV_HEADS, PAGE, HEAD_DIM), dev)
+    _need(src_slots, "src_slots", _I32T, (n,), dev)
+    _need(slots, "slots", _I32T, (n,), dev)
+    _check(_lib.attn_kv_quantize_fp8(src.data_ptr(), src_pages, src_slots.data_ptr(), n,
+                                     kv_cache.data_ptr(), pages, slots.data_ptr(), stream),
            "attn_kv_quantize_fp8")
     return kv_cache
 
 
 def kv_read_fp8(kv_cache: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor | None = None,
                 v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """The rows at ``slots`` [n] back as bf16: k and v [n, 8, 64], exact."""
-    _expect_fp8(kv_cache)
-    _expect(slots, "slots", torch.int32, (slots.numel(),))
+    """The rows at ``slots`` [n] back as bf16: k and v [n, 8, 64], exact.  Where neither output
+    is given they are the halves of one new tensor."""
+    pages, dev, stream = _need_fp8(kv_cache)
     n = slots.numel()
-    outs = [torch.empty((n, KV_HEADS, HEAD_DIM), dtype=torch.bfloat16, device=kv_cache.device)
-            if t is None else t for t in (k_out, v_out)]
-    for t, name in zip(outs, ("k_out", "v_out")):
-        _expect(t, name, torch.bfloat16, (n, KV_HEADS, HEAD_DIM))
-    _on(kv_cache.device, slots=slots, k_out=outs[0], v_out=outs[1])
-    _check(_lib.attn_kv_read_fp8(_ptr(kv_cache), kv_cache.shape[0], _ptr(slots), n, _ptr(outs[0]),
-                                 _ptr(outs[1]), _stream()), "attn_kv_read_fp8")
-    return outs[0], outs[1]
+    _need(slots, "slots", _I32T, (n,), dev)
+    shape = (n, KV_HEADS, HEAD_DIM)
+    if k_out is None and v_out is None:
+        k_out, v_out = torch.empty((2, *shape), dtype=_BF16, device=kv_cache.device).unbind()
+    else:
+        k_out, v_out = (torch.empty(shape, dtype=_BF16, device=kv_cache.device) if t is None else t
+                        for t in (k_out, v_out))
+        _need(k_out, "k_out", _BF16, shape, dev)
+        _need(v_out, "v_out", _BF16, shape, dev)
+    _check(_lib.attn_kv_read_fp8(kv_cache.data_ptr(), pages, slots.data_ptr(), n,
+                                 k_out.data_ptr(), v_out.data_ptr(), stream),
+           "attn_kv_read_fp8")
+    return k_out, v_out
 
 
 def decode_fp8_workspace_bytes(batch: int, max_span: int) -> int:
@@ -419,16 +425,14 @@ def decode_fp8_workspace(batch: int, max_span: int, device="cuda") -> torch.Tens
                        device=device)
 
 
-def _tables_fp8(q, kv_cache, page_indptr, page_indices, kv_len, sinks, out, batch):
-    _expect_fp8(kv_cache)
-    _expect(q, "q", torch.bfloat16, (q.shape[0], Q_HEADS, HEAD_DIM))
-    _expect(page_indptr, "page_indptr", torch.int32, (batch + 1,))
-    _expect(page_indices, "page_indices", torch.int32)
-    _expect(kv_len, "kv_len", torch.int32, (batch,))
-    _expect(sinks, "sinks", torch.bfloat16, (Q_HEADS,))
-    _expect(out, "out", torch.bfloat16, (q.shape[0], Q_HEADS, HEAD_DIM))
-    _on(kv_cache.device, q=q, page_indptr=page_indptr, page_indices=page_indices, kv_len=kv_len,
-        sinks=sinks, out=out)
+def _need_tables(q, page_indptr, page_indices, kv_len, sinks, out, batch, dev):
+    n = q.shape[0]
+    _need(q, "q", _BF16, (n, Q_HEADS, HEAD_DIM), dev)
+    _need(page_indptr, "page_indptr", _I32T, (batch + 1,), dev)
+    _need(page_indices, "page_indices", _I32T, page_indices.shape, dev)
+    _need(kv_len, "kv_len", _I32T, (batch,), dev)
+    _need(sinks, "sinks", _BF16, (Q_HEADS,), dev)
+    _need(out, "out", _BF16, (n, Q_HEADS, HEAD_DIM), dev)
 
 
 def decode_fp8(q: torch.Tensor, kv_cache: torch.Tensor, page_indptr: torch.Tensor,
@@ -438,14 +442,15 @@ def decode_fp8(q: torch.Tensor, kv_cache: torch.Tensor, page_indptr: torch.Tenso
     """``decode`` over the 8-bit cache: softmax with the sink as a further logit, rounded
     once; ``workspace`` from ``decode_fp8_workspace`` (reused by calls that follow one
     another)."""
+    pages, dev, stream = _need_fp8(kv_cache)
     batch = q.shape[0]
-    _tables_fp8(q, kv_cache, page_indptr, page_indices, kv_len, sinks, out, batch)
-    _expect(workspace, "workspace", torch.uint8)
-    _on(kv_cache.device, workspace=workspace)
-    _check(_lib.attn_decode_fp8(_ptr(q), batch, _ptr(kv_cache), kv_cache.shape[0],
-                                _ptr(page_indptr), _ptr(page_indices), _ptr(kv_len), max_span,
-                                window, sm_scale, _ptr(sinks), _ptr(out), _ptr(workspace),
-                                workspace.numel(), _stream()), "attn_decode_fp8")
+    _need_tables(q, page_indptr, page_indices, kv_len, sinks, out, batch, dev)
+    _need(workspace, "workspace", _U8, workspace.shape, dev)
+    _check(_lib.attn_decode_fp8(q.data_ptr(), batch, kv_cache.data_ptr(), pages,
+                                page_indptr.data_ptr(), page_indices.data_ptr(), kv_len.data_ptr(),
+                                max_span, window, sm_scale, sinks.data_ptr(), out.data_ptr(),
+                                workspace.data_ptr(), workspace.numel(), stream),
+           "attn_decode_fp8")
     return out
 
 
@@ -455,15 +460,15 @@ def prefill_fp8(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, kv_cach
                 max_kv_len: int = 0) -> torch.Tensor:
     """``prefill`` over the 8-bit cache (the formula of ``decode_fp8``): causal attention of
     each sequence's new tokens over its cached ones.  ``max_kv_len`` as there."""
-    batch = q_indptr.numel() - 1
-    _tables_fp8(q, kv_cache, page_indptr, page_indices, kv_len, sinks, out, batch)
-    _expect(q_indptr, "q_indptr", torch.int32, (batch + 1,))
-    _on(kv_cache.device, q_indptr=q_indptr)
-    n = q.shape[0]
+    pages, dev, stream = _need_fp8(kv_cache)
+    n, batch = q.shape[0], q_indptr.numel() - 1
+    _need_tables(q, page_indptr, page_indices, kv_len, sinks, out, batch, dev)
+    _need(q_indptr, "q_indptr", _I32T, (batch + 1,), dev)
     need = _lib.attn_prefill_fp8_workspace_bytes(n, batch, max_q_len, max_kv_len, window)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _check(_lib.attn_prefill_fp8(_ptr(q), n, _ptr(q_indptr), batch, max_q_len, _ptr(kv_cache),
-                                 kv_cache.shape[0], _ptr(page_indptr), _ptr(page_indices),
-                                 _ptr(kv_len), max_kv_len, window, sm_scale, _ptr(sinks),
-                                 _ptr(out), _ptr(ws), need, _stream()), "attn_prefill_fp8")
+    ws = torch.empty(need, dtype=_U8, device=q.device) if need else None
+    _check(_lib.attn_prefill_fp8(q.data_ptr(), n, q_indptr.data_ptr(), batch, max_q_len,
+                                 kv_cache.data_ptr(), pages, page_indptr.data_ptr(),
+                                 page_indices.data_ptr(), kv_len.data_ptr(), max_kv_len, window,
+                                 sm_scale, sinks.data_ptr(), out.data_ptr(), _ptr(ws), need,
+                                 stream), "attn_prefill_fp8")
     return out
