@@ -93,6 +93,47 @@ __device__ __forceinline__ int fp8_scale_at(int head, int kv, int token) {
   return kFp8Scales + (head * 2 + kv) * kPage + token;
 }
 
+// v's codes and the scales lie four tokens to a word.  Kernels that go over tokens by
+// their slots take them in runs: a run begins at a multiple of four, or where a slot does
+// not follow the one before, so a run of four is a quad whose words one wave moves
+// whole, whatever the tokens' order and wherever sequences begin; shorter ones go byte by
+// byte.  A wave or workgroup takes the runs that begin at tokens first .. first + 3.
+struct SlotRuns {
+  uint32_t begins;  // bit t: a run begins at token first + t (or there is no such token)
+  __device__ __forceinline__ SlotRuns(const int* __restrict__ slots, int first, int n) {
+    uint32_t slot[8];  // of the tokens first - 1 .. first + 6
+#pragma unroll
+    for (int t = 0; t < 8; ++t) slot[t] = (uint32_t)slots[min(max(first - 1 + t, 0), n - 1)];
+    begins = 0;
+#pragma unroll
+    for (int t = 0; t < 7; ++t) {
+      const bool follows = first + t > 0 && first + t < n && slot[t + 1] % 4 != 0 &&
+                           slot[t + 1] == slot[t] + 1;
+      begins |= (follows ? 0u : 1u) << t;
+    }
+  }
+  // length (1 to 4) of the run that begins at token first + t
+  __device__ __forceinline__ int length(int t) const {
+    return __builtin_ctz(begins >> (t + 1) | 8u) + 1;
+  }
+};
+// whether a run of `length` tokens from `slot` on is a quad of the pool
+__device__ __forceinline__ bool fp8_quad(int slot, int length, int num_pages) {
+  return length == 4 && slot >= 0 && slot < num_pages * kPage;
+}
+
+// Four words of four bytes, transposed.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+  const uint32_t ab = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u);
+  const uint32_t cd = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t ab2 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+  const uint32_t cd2 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  w[0] = __builtin_amdgcn_perm(cd, ab, 0x05040100u);
+  w[1] = __builtin_amdgcn_perm(cd, ab, 0x07060302u);
+  w[2] = __builtin_amdgcn_perm(cd2, ab2, 0x05040100u);
+  w[3] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302u);
+}
+
 // scale byte of a row whose largest magnitude has the bf16 bits `top`
 __device__ __forceinline__ uint32_t fp8_scale_of(uint32_t top) {
   const uint32_t e = top >> 7;

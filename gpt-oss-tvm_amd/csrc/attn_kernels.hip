@@ -149,6 +149,10 @@ constexpr int kRopeRow = 1 << 20;            // workgroups of a grid row
 
 // kFp8: k and v go to the 8-bit cache, after the same rounding to bf16: a row's
 // four threads meet for its largest magnitude (quad moves) and write 16 codes each.
+// v's go byte by byte, four tokens to a word: neighbours in one L2 join them there
+// (8192 tokens 51.5 us, 53.4 with neighbours on different XCDs).  Four tokens a
+// workgroup, v's codes leaving in words, took 54.5 us, and 12.5 for 333 tokens where
+// one has 9.0.
 template <bool kFp8>
 __global__ __launch_bounds__(kRopeThreads) void qkv_rope_append_kernel(
     const uint16_t* __restrict__ qkv, const uint16_t* __restrict__ bias, int n,
@@ -158,7 +162,11 @@ __global__ __launch_bounds__(kRopeThreads) void qkv_rope_append_kernel(
 #pragma clang fp contract(off)
   __shared__ float cs[32], sn[32];
   const int t = threadIdx.x;
-  const int tok = blockIdx.x + blockIdx.y * kRopeRow;
+  int tok = blockIdx.x + blockIdx.y * kRopeRow;
+  if (kFp8 && (tok | 127) < n) {  // 16 tokens in a row go to one of the eight XCDs
+    const int r = tok % 128;
+    tok += (r % 8) * 16 + r / 8 - r;
+  }
   if (tok >= n) return;
   const int head = t >> 2, d = (t & 3) * 8;
   const size_t col = (size_t)head * kD + d;

@@ -109,6 +109,42 @@ def test_quantize_and_read_bit_exact(A, n, order):
         np.testing.assert_array_equal(got.double().cpu().numpy(), values(rows, is_v))
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_quantize_and_read_runs(A, seed):
+    """Runs of tokens of all lengths from all places in a quad, upwards and downwards, up to the
+    pool's last slot; source slots outside their pool in places, whose rows are not written."""
+    rng = np.random.default_rng(300 + seed)
+    pages = 40
+    free, runs = np.ones(pages * PAGE, dtype=bool), [np.arange(pages * PAGE - 6, pages * PAGE)]
+    free[runs[0]] = False
+    for _ in range(90):
+        a, length = rng.integers(0, pages * PAGE - 12), rng.integers(1, 12)
+        run = np.arange(a, a + length)
+        if free[run].all():
+            free[run] = False
+            runs.append(run[::-1] if rng.random() < 0.2 else run)
+    slots = np.concatenate([runs[i] for i in rng.permutation(len(runs))])
+    n = len(slots)
+    k, v = rows_of(rng, n), rows_of(rng, n)
+    mine = rng.permutation(pages * PAGE)[:n]
+    src = np.zeros((pages, 2, HKV, PAGE, D), dtype=np.uint16)
+    src[mine // PAGE, 0, :, mine % PAGE] = k
+    src[mine // PAGE, 1, :, mine % PAGE] = v
+    bad = rng.random(n) < 0.05
+    cache = u8_dev(untouched(pages))
+    A.kv_quantize_fp8(bf16_dev(src), i32_dev(np.where(bad, pages * PAGE, mine)), cache,
+                      i32_dev(slots))
+    want = untouched(pages)
+    AO.fp8_put(want, slots[~bad], k[~bad], v[~bad])
+    np.testing.assert_array_equal(cache.cpu().numpy(), want)
+    AO.fp8_put(want, slots, k, v)
+    out = rng.random(n) < 0.05
+    gk, gv = A.kv_read_fp8(u8_dev(want), i32_dev(np.where(out, -slots - 1, slots)))
+    for got, rows, is_v in ((gk, k, False), (gv, v, True)):
+        ref = np.where(out[:, None, None], 0.0, values(rows, is_v))
+        np.testing.assert_array_equal(got.double().cpu().numpy(), ref)
+
+
 def test_quantize_and_read_slots_outside(A):
     rng = np.random.default_rng(7)
     src = bf(rng.standard_normal((2, 2, HKV, PAGE, D)))
