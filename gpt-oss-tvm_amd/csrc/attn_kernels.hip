@@ -112,10 +112,15 @@ __global__ __launch_bounds__(kRmsThreads) void rms_norm_kernel(const u32x4* __re
 // tokens 10.0 -> 11.4, 18.8 -> 20.3, 25.0 -> 27.4 and 31.8 -> 33.2 us with qkv from
 // HBM, 4096 and 8192 from the cache 15.7 -> 15.5 and 26.6 -> 28.6.)
 
-// The quarter of a row that a thread of a quad holds (bf16 dims d .. d + 7 in lo,
-// d + 32 .. d + 39 in hi) to slot's place in the 8-bit cache, if it has one.
-__device__ __forceinline__ void store_row_fp8(u32x4 lo, u32x4 hi, int d, int slot, int kv, int hk,
-                                              uint8_t* __restrict__ cache, int num_pages) {
+// The quarters of a token's k and v rows that the lanes of a wave hold (lane (k or v,
+// head, quarter d / 8): bf16 dims d .. d + 7 in lo, d + 32 .. d + 39 in hi) to slot's place
+// in the 8-bit cache, if it has one.  v's codes change lanes through LDS (vrow, 512
+// bytes): four tokens share each word of them, and a wave writes a head's 64 bytes in
+// one store of 256 bytes' span.
+__device__ __forceinline__ void store_token_fp8(u32x4 lo, u32x4 hi, int slot,
+                                                uint8_t* __restrict__ cache, int num_pages,
+                                                uint8_t* vrow) {
+  const int lane = threadIdx.x & 63, kv = lane >> 5, hk = (lane >> 2) & 7, d = (lane & 3) * 8;
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -131,17 +136,20 @@ __device__ __forceinline__ void store_row_fp8(u32x4 lo, u32x4 hi, int d, int slo
   uint8_t* const page = fp8_page(cache, slot, num_pages);
   if (!page) return;
   const int token = slot % kPage;
+  const uint2 left = make_uint2(codes[0], codes[1]), right = make_uint2(codes[2], codes[3]);
   if (kv == 0) {
-    uint8_t* const dst = page + hk * kFp8Head + token * kFp8Row + d;
-    *(uint2*)dst = make_uint2(codes[0], codes[1]);
-    *(uint2*)(dst + 32) = make_uint2(codes[2], codes[3]);
+    uint8_t* const row = page + hk * kFp8Head + token * kFp8Row + d;
+    *(uint2*)row = left;
+    *(uint2*)(row + 32) = right;
   } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      page[fp8_v_at(hk, token, d + (j & 7) + (j & 8) * 4)] =
-          (uint8_t)(codes[j >> 2] >> (8 * (j & 3)));
+    *(uint2*)(vrow + hk * kD + d) = left;
+    *(uint2*)(vrow + hk * kD + d + 32) = right;
   }
-  if ((d & 31) == 0) page[fp8_scale_at(hk, kv, token)] = (uint8_t)s;
+  if (d == 0) page[fp8_scale_at(hk, kv, token)] = (uint8_t)s;
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (one wave wrote vrow and reads it)
+  const int dim = (lane >> 2) + 16 * (lane & 3);
+#pragma unroll
+  for (int h = 0; h < kHkv; ++h) page[fp8_v_at(h, token, dim)] = vrow[h * kD + dim];
 }
 
 constexpr int kRopeThreads = kQkvHeads * 4;  // 320: (head, quarter of its 32 pairs)
@@ -149,10 +157,10 @@ constexpr int kRopeRow = 1 << 20;            // workgroups of a grid row
 
 // kFp8: k and v go to the 8-bit cache, after the same rounding to bf16: a row's
 // four threads meet for its largest magnitude (quad moves) and write 16 codes each.
-// v's go byte by byte, four tokens to a word: neighbours in one L2 join them there
-// (8192 tokens 51.5 us, 53.4 with neighbours on different XCDs).  Four tokens a
-// workgroup, v's codes leaving in words, took 54.5 us, and 12.5 for 333 tokens where
-// one has 9.0.
+// v's codes of four tokens share words: neighbours in one L2 join them there (8192
+// tokens and their read back 42.4 us, 44.2 with neighbours on different XCDs, 53.3 with
+// v's codes stored by the lanes that made them).  Four tokens a workgroup, v's codes
+// leaving in words, took 54.5 us, and 12.5 for 333 tokens where one has 9.0.
 template <bool kFp8>
 __global__ __launch_bounds__(kRopeThreads) void qkv_rope_append_kernel(
     const uint16_t* __restrict__ qkv, const uint16_t* __restrict__ bias, int n,
@@ -208,7 +216,8 @@ __global__ __launch_bounds__(kRopeThreads) void qkv_rope_append_kernel(
   if (head < kHq) {
     dst = q_out + ((size_t)tok * kHq + head) * kD;
   } else if constexpr (kFp8) {  // the last 64 threads, one wave
-    store_row_fp8(olo, ohi, d, slot, (head - kHq) / kHkv, (head - kHq) % kHkv, cache, num_pages);
+    __shared__ alignas(8) uint8_t vrow[kHkv * kD];
+    store_token_fp8(olo, ohi, slot, cache, num_pages, vrow);
   } else if (slot >= 0 && slot < num_pages * kPage) {  // other slots are not written
     const int kv = head < kHq + kHkv ? 0 : 1;
     const int hk = head - kHq - kv * kHkv;
