@@ -438,13 +438,19 @@ int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
 }
 
 // Tokens of a chunk's query tile, and how many splits its keys are shared out over: as
-// many as let its workgroups fit the chip at once (two a CU).
+// many as let its workgroups fit the chip at once (two a CU; three of several tiles of 2).
 //  * 64 of more than 32 tokens, without a window, where they are two rounds of the chip.
-//  * 2 or 4 tokens (the loads bind) up to 24 tokens, and for longer chunks where there
-//    are few of these tiles over few keys; us in tiles of 4 and of 32, tokens over
-//    cached: 16 sequences of 24 over 2000 33.1 and 36.4; 64 over 6000 25.3 and 30.2; 200
-//    over 500 13.5 and 21.1, over 6000 63 and 48; 64 sequences of 32 over 300 55.7 and 37.8.
-constexpr int64_t kFp8ChunkWgs = 512, kFp8FewTokens = 24, kFp8FewTiles = 64, kFp8FewKeys = 200000;
+//  * 4 tokens up to 24 tokens, and for longer chunks where there are few of these tiles
+//    over few keys; us in tiles of 4 and of 32, tokens over cached: 16 sequences of 24
+//    over 2000 33.1 and 36.4; 64 over 6000 25.3 and 30.2; 200 over 500 13.5 and 21.1, over
+//    6000 63 and 48; 64 sequences of 32 over 300 55.7 and 37.8.
+//  * 2 tokens of up to 2 and of 5 to 12: a wave's blocks take half as long, and three
+//    workgroups share a CU; us in tiles of 4 and of 2, sequences of tokens over up to
+//    cached: 16 of 5 over 4000 29.3 and 25.7, 128 of 5 over 1000 52.3 and 37.5, one of 9
+//    over 8000 18.1 and 16.4, 16 of 12 over 4000 39.5 and 37.0; but 16 of 3 over 4000
+//    21.1 and 22.7, 16 of 16 over 4000 33.3 and 42.9.
+constexpr int64_t kFp8ChunkWgs = 512, kFp8PairWgs = 768, kFp8PairTokens = 12, kFp8FewTokens = 24,
+                  kFp8FewTiles = 64, kFp8FewKeys = 200000;
 struct Fp8Chunk {
   int64_t tokens, splits, tiles;  // tiles of the longest sequence
 };
@@ -457,10 +463,12 @@ Fp8Chunk fp8_chunk(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t
                                                     : kFp8FewTiles + 1;  // tiles of 4, or too many
   const bool few = max_q_len <= kFp8FewTokens ||
                    (small <= kFp8FewTiles && reach > 0 && small * reach <= kFp8FewKeys);
-  const int64_t tokens = max_q_len <= 2 ? 2 : few ? 4 : 32;
+  const bool pairs = max_q_len <= 2 || (max_q_len > 4 && max_q_len <= kFp8PairTokens);
+  const int64_t tokens = pairs ? 2 : few ? 4 : 32;
+  const int64_t wgs = pairs && max_q_len > 2 ? kFp8PairWgs : kFp8ChunkWgs;
   const int64_t keys = window > 0 ? std::min(max_kv_len, window + tokens) : max_kv_len;
   if (keys <= 0 || batch > kFp8ChunkWgs) return Fp8Chunk{tokens, 1, tiles_of(tokens)};
-  const int64_t most = std::min<int64_t>(kFp8MaxSplits, kFp8ChunkWgs / (tiles_of(tokens) * batch * kKvHeads));
+  const int64_t most = std::min(kFp8MaxSplits, wgs / (tiles_of(tokens) * batch * kKvHeads));
   return Fp8Chunk{tokens, std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks)),
                   tiles_of(tokens)};
 }

@@ -538,9 +538,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void f
 
 // Chunks of few tokens (drafts under verification): a tile of 2 kCt tokens in kCt tiles
 // of 16 columns (token, head), by decode's loads and products; p enters as one
-// bf16 rounding, as in the long chunks' form.  More tokens take more such tiles,
-// which find the keys in the cache: four column tiles a wave spill (16 sequences of 5
-// tokens over up to 4000 keys: 54 us in tiles of 8, 29 in tiles of 4).
+// bf16 rounding, as in the long chunks' form.  More tokens take more such tiles, which
+// read the keys again.  Bound by a wave's own instructions over its blocks: 16 sequences
+// of 5 tokens over up to 4000 keys take 54 us in one tile of 8 (its four column tiles a
+// wave spill), 29 in tiles of 4, 25.7 in tiles of 2.
 template <int kCt>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void fp8_rows_kernel(
     RowsArgs a) {

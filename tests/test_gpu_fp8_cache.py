@@ -352,6 +352,17 @@ def test_prefill_shared_keys(A, qlens, prefix, window):
     check_prefill(A, seqs, qlens, window, 31, 4 * max(lengths), rows)   # a bound far above
 
 
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("longest", [1, 2, 3, 4, 5, 6, 12, 13])
+def test_prefill_few_tokens(A, longest, window):
+    """Drafts of up to `longest` tokens over caches of all lengths, their keys in shares."""
+    rng = np.random.default_rng(longest)
+    qlens = [longest, 1, 0, *rng.integers(1, longest + 1, 4).tolist()]
+    prefix = [2500, 0, 70, 63, 64, 1100, 255]
+    seqs = Seqs(500 + longest, [p + n for p, n in zip(prefix, qlens)])
+    check_prefill(A, seqs, qlens, window, 501 + longest, bound=2500 + longest)
+
+
 @pytest.mark.parametrize("window", [0, 128])
 def test_prefill_long(A, window):
     """A long prompt at sampled rows: sharp scores, the row maximum anywhere."""
