@@ -456,11 +456,13 @@ struct Fp8Chunk {
 };
 Fp8Chunk fp8_chunk(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
   auto tiles_of = [&](int64_t tokens) { return (max_q_len + tokens - 1) / tokens; };
+  max_kv_len = std::min(max_kv_len, kMaxPages * kPage);  // (and no overflow below)
   if (window <= 0 && max_q_len > 32 && tiles_of(64) * kKvHeads >= (512 + batch - 1) / batch)
     return Fp8Chunk{64, 1, tiles_of(64)};
   const int64_t reach = window > 0 ? std::min(max_kv_len, window + max_q_len) : max_kv_len;
-  const int64_t small = tiles_of(4) <= kFp8FewTiles ? tiles_of(4) * std::min(batch, kFp8FewTiles + 1)
-                                                    : kFp8FewTiles + 1;  // tiles of 4, or too many
+  const int64_t small = tiles_of(4) <= kFp8FewTiles  // tiles of 4, or too many
+                            ? tiles_of(4) * std::min(batch, kFp8FewTiles + 1)
+                            : kFp8FewTiles + 1;
   const bool few = max_q_len <= kFp8FewTokens ||
                    (small <= kFp8FewTiles && reach > 0 && small * reach <= kFp8FewKeys);
   const bool pairs = max_q_len <= 2 || (max_q_len > 4 && max_q_len <= kFp8PairTokens);
@@ -505,14 +507,22 @@ int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cache, int6
                                        (int*)workspace, out, as_stream(stream)));
 }
 
-// Workspace: the splits' o [splits][rows][64][64], then (m, l) [splits][rows][64][2]
+// Workspace: the splits' o [splits][rows][64][64], then (m, l) [splits][rows][64][2], rows
+// the tokens of the sequences' tiles, whatever rows q has beside them (a split call's
+// workgroups are few, so at most 35 MB).
+int64_t fp8_chunk_rows(const Fp8Chunk& chunk, int64_t batch) {
+  return chunk.tokens * chunk.tiles * batch;
+}
+
 size_t attn_prefill_fp8_workspace_bytes(int64_t rows, int64_t batch, int64_t max_q_len,
                                         int64_t max_kv_len, int32_t window) {
   if (rows <= 0 || rows > kMaxTokens || batch <= 0 || batch > kMaxTokens || max_q_len <= 0 ||
       max_q_len > kMaxTokens)
     return 0;
-  const int64_t splits = fp8_chunk(batch, max_q_len, max_kv_len, window).splits;
-  return splits <= 1 ? 0 : (size_t)(splits * rows * kQHeads * (kHeadDim + 2)) * sizeof(float);
+  const Fp8Chunk chunk = fp8_chunk(batch, max_q_len, max_kv_len, window);
+  if (chunk.splits <= 1) return 0;
+  return (size_t)(chunk.splits * fp8_chunk_rows(chunk, batch) * kQHeads * (kHeadDim + 2)) *
+         sizeof(float);
 }
 
 int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
@@ -539,10 +549,12 @@ int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, i
   if (need && !a16(workspace)) return MOE_ERR_ALIGN;
   if (workspace_bytes < need) return MOE_ERR_WORKSPACE;
   float* part_o = (float*)workspace;
+  const int64_t part_rows = need ? fp8_chunk_rows(chunk, batch) : 0;
   return status(attn_launch_fp8_chunk(
       q, q_indptr, (int)batch, (int)max_q_len, kv_cache, page_indptr, page_indices, (int)num_pages,
-      kv_len, window, sm_scale, sinks, out, (int)chunk.tokens, (int)chunk.splits, (int)rows,
-      part_o, need ? part_o + chunk.splits * rows * kQHeads * kHeadDim : nullptr,
+      kv_len, window, sm_scale, sinks, out, (int)chunk.tokens, (int)chunk.splits,
+      (int)part_rows, part_o,
+      need ? part_o + chunk.splits * part_rows * kQHeads * kHeadDim : nullptr,
       as_stream(stream)));
 }
 

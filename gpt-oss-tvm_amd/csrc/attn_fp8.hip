@@ -218,7 +218,7 @@ struct Shares {
 struct Sight {
   int lo, last, first, blocks;  // first block of 64, number of blocks
   __device__ __forceinline__ Sight(int pos, int tokens, int window) {
-    lo = window > 0 ? max(0, pos - window + 1) : 0;
+    lo = window > 0 && pos >= window ? pos - window + 1 : 0;
     last = pos + tokens - 1;
     first = lo / kFp8Block;
     blocks = last >= lo ? last / kFp8Block - first + 1 : 0;
@@ -234,7 +234,7 @@ struct RowsArgs {
   const int* kv_len;
   const uint16_t* sinks;
   uint16_t* out;
-  float* part_o;   // [splits][rows][64][64]
+  float* part_o;   // [splits][rows][64][64], rows: sequences, or a chunk's tiles' tokens
   float* part_ml;  // [splits][rows][64][2]
   int* arrive;     // decode: [batch][8], left zero
   int64_t max_span;
@@ -761,7 +761,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
       *(uint2*)(a.out + at * kD + d) = make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
                                                   (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
     } else {
-      const size_t pt = (size_t)share * a.rows * kHq + at;
+      const size_t row = (size_t)share * a.rows + blockIdx.x / kHkv * (2 * kCt) + token;
+      const size_t pt = row * kHq + head;
       *(f32x4*)(a.part_o + pt * kD + d) = ot;
       if (d == 0) *(float2*)(a.part_ml + pt * 2) = make_float2(mt, lt);
     }
@@ -810,7 +811,8 @@ __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
 }
 // max over lanes l and l ^ 32
 __device__ __forceinline__ float half_max(float x) {
-  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  const uint32_t u = __float_as_uint(x);
+  const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
   return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
@@ -1028,7 +1030,8 @@ fp8_tile_kernel(RowsArgs a) {
                        (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
       }
   } else {
-    const size_t pt = (size_t)share * a.rows * kHq + at;
+    const size_t pt = ((size_t)share * a.rows + (b * a.tiles + tile) * kTokens + token) * kHq +
+                      hk * kGroup + (c & 7);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
@@ -1050,7 +1053,8 @@ __global__ __launch_bounds__(256) void fp8_merge_kernel(RowsArgs a, int tokens) 
   const Sight sight(a.kv_len[b] - qn + t0, min(tokens, qn - t0), a.window);
   const int used = Shares(sight.blocks, a.splits, a.least).used;
   if (used <= 1) return;  // written already
-  const size_t at = (size_t)(qb + t0 + token) * kHq + head, step = (size_t)a.rows * kHq;
+  const size_t at = ((size_t)blockIdx.x * tokens + token) * kHq + head;
+  const size_t step = (size_t)a.rows * kHq;
   float m = -INFINITY, l = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < used; s0 += 8) {
@@ -1086,8 +1090,9 @@ __global__ __launch_bounds__(256) void fp8_merge_kernel(RowsArgs a, int tokens) 
   uint16_t v4[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) v4[q] = f2bf(o[q] * f);
-  *(uint2*)(a.out + at * kD + d) = make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
-                                              (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
+  *(uint2*)(a.out + ((size_t)(qb + t0 + token) * kHq + head) * kD + d) =
+      make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
+                 (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
 }
 
 }  // namespace attn

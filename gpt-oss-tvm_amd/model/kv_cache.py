@@ -84,7 +84,7 @@ class PagedKVCache:
             self.staging = torch.zeros((STAGED // PAGE_SIZE, 2, kv_heads, PAGE_SIZE, head_dim),
                                        dtype=torch.bfloat16, device=device)
             self.staging_slots = torch.arange(STAGED, dtype=torch.int32, device=device)
-        elif dtype.itemsize != 2:
+        elif dtype.is_floating_point and dtype.itemsize == 1:
             raise ValueError(f"a cache holds bf16 or float8_e4m3fn rows, not {dtype}")
         else:
             self.data = torch.zeros((num_layers, num_pages, 2, kv_heads, PAGE_SIZE, head_dim),
@@ -206,9 +206,10 @@ class PagedKVCache:
         """A new sequence ``seq_id`` of this 8-bit cache with the tokens and the window of
         ``source_id`` of a bf16 cache of as many layers: its rows quantised, in every layer."""
         import attn_native
-        if not self.fp8 or source.fp8 or source.num_layers != self.num_layers:
+        if (not self.fp8 or source.fp8 or source.num_layers != self.num_layers
+                or source.data.device != self.data.device):
             raise ValueError("quantize_from takes a sequence of a bf16 cache into an 8-bit cache "
-                             "of as many layers")
+                             "of as many layers on the same device")
         old = source.seqs[source_id]
         need = -(-old.length // PAGE_SIZE)
         if need > len(self.free):

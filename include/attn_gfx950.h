@@ -181,8 +181,9 @@ MOE_API int attn_sample_top_p(const uint16_t* logits, int64_t batch, int64_t voc
  * even) and one E8M0 scale byte s; code c stands for c 2^(s - 127).  With e the
  * biased exponent of the row's largest magnitude s = max(e - 7, 10): values are off
  * by at most 2^-4 of themselves or 2^-17 of the row's largest (or 2^-127).  (At s =
- * 247 codes stop at 240, as 256 would stand for 2^128.)  A row with an infinity or a NaN has s = 255 and stands for NaN:
- * queries that see its token get NaN, others are not affected.
+ * 247 codes stop at 240, as 256 would stand for 2^128.)  A row with an infinity or a
+ * NaN has s = 255 and stands for NaN: queries that see its token get NaN, others are
+ * not affected.
  * One layer's cache is [num_pages][16640] bytes.  A page: k codes [8 heads][16
  * tokens][64 dims]; at 8192 v codes [8][token / 4][dim % 16][dim / 16][token % 4]; at
  * 16384 scales [8][k, v][16].  It needs no initialisation: what lies past a
@@ -223,7 +224,8 @@ MOE_API size_t attn_decode_fp8_workspace_bytes(int64_t batch, int64_t max_span);
  * to bf16 (attn_decode rounds as the operators it restates do).  A sequence with no
  * key (kv_len 0) gets 0, one whose span exceeds max_span NaN.  sm_scale > 0.  The
  * result of a sequence follows from its keys and the batch size, not from
- * max_span. */
+ * max_span.  The sums are fp32 with weights of up to 2^24: |v| above 2^80 may give an
+ * infinity. */
 MOE_API int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cache,
                             int64_t num_pages, const int32_t* page_indptr,
                             const int32_t* page_indices, const int32_t* kv_len, int64_t max_span,
@@ -237,7 +239,7 @@ MOE_API int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cac
  * shared out over workgroups; 0: unknown, not shared out).  A sequence's last bits
  * may change with the other sequences of the call and with the bounds.  The
  * workspace (none where attn_prefill_fp8_workspace_bytes is 0) needs no
- * initialisation. */
+ * initialisation; calls on one have to follow one another. */
 MOE_API size_t attn_prefill_fp8_workspace_bytes(int64_t rows, int64_t batch, int64_t max_q_len,
                                                 int64_t max_kv_len, int32_t window);
 MOE_API int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr,

@@ -74,7 +74,8 @@ def test_host_cache():
     with pytest.raises(ValueError):
         PagedKVCache(1, 2, 1, 16, kv_heads=4, device="cpu", dtype=FP8)
     with pytest.raises(ValueError):
-        PagedKVCache(1, 2, 1, 16, device="cpu", dtype=torch.float32)
+        PagedKVCache(1, 2, 1, 16, device="cpu", dtype=torch.float8_e5m2)
+    assert PagedKVCache(1, 2, 1, 16, device="cpu", dtype=torch.float32).data.dtype == torch.float32
     b = PagedKVCache(num_layers=3, num_pages=8, max_batch=2, max_tokens=64, device="cpu")
     assert not b.fp8
     with pytest.raises(ValueError):
@@ -149,6 +150,12 @@ def test_refusals():
     for batch in (-1, 0, (1 << 60) + 1, (1 << 62) + 3, (1 << 63) - 1):
         assert size(300, batch, 300, 6300, 0) == 0, batch
     need = size(5, 1, 5, 4000, 0)
+    assert size(1 << 20, 1, 5, 4000, 0) == need         # rows behind the sequences cost nothing
+    assert size(5, 1, 5, (1 << 63) - 1, 0) == size(5, 1, 5, 1 << 31, 0) < 1 << 28
+    for batch in (1, 3, 40, 512):                       # a call's parts are bounded
+        for longest in (1, 2, 4, 7, 12, 24, 30, 33, 100, 300, 2000):
+            for window in (0, 128):
+                assert size(9, batch, longest, 1 << 20, window) <= 64 << 20, (batch, longest)
 
     def pre(q=p, rows=5, batch=1, longest=5, pages=8, most_kv=4000, scale=0.125, out=p, ws=p,
             bytes_=need):

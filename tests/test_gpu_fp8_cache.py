@@ -427,6 +427,27 @@ def test_prefill_more_queries_than_keys(A):
     within(got[20:30], q[20:30], seqs.kd[0], seqs.vd[0], np.arange(10), 0, sinks, U)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 20])
+def test_window_of_any_size(A, window):
+    """As no window, also where a chunk begins before its sequence's first token."""
+    seqs = Seqs(75, [10, 300])
+    rng = np.random.default_rng(76)
+    q, sinks = bf(rng.standard_normal((40, HQ, D))), bf(rng.standard_normal(HQ))
+    none, _ = run_prefill(A, seqs, q, [30, 10], sinks, 0, 0)
+    got, _ = run_prefill(A, seqs, q, [30, 10], sinks, window, 0)
+    within(got[20:30], q[20:30], seqs.kd[0], seqs.vd[0], np.arange(10), 0, sinks, U)
+    within(got[30:], q[30:], seqs.kd[1], seqs.vd[1], np.arange(290, 300), 0, sinks, U)
+    assert not got[:20].any() and not none[:20].any()
+    np.testing.assert_array_equal(run_decode(A, seqs, q[:2], sinks, window, 300),
+                                  run_decode(A, seqs, q[:2], sinks, 0, 300))
+
+
+@pytest.mark.parametrize("n", [5, 40])
+def test_prefill_rows_behind(A, n):
+    """A few tokens at the head of a long buffer, their keys shared out over workgroups."""
+    check_prefill(A, Seqs(77, [2100, 900]), [n, 3], 0, 78, bound=2100, extra=4000)
+
+
 def test_pages_past_32_bits(A):
     """Pages beyond the fourth GiB of a layer's cache, by every entry point."""
     pool = (4 << 30) // AO.FP8_PAGE_BYTES + 1200
