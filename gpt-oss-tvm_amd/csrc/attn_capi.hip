@@ -59,8 +59,8 @@ int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const in
 int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
                           const void* cache, const int* page_indptr, const int* page_indices,
                           int num_pages, const int* kv_len, int window, float sm_scale,
-                          const void* sinks, void* out, int tokens, int splits, int rows,
-                          float* part_o, float* part_ml, hipStream_t s);
+                          const void* sinks, void* out, int tokens, int splits, int halves,
+                          int rows, float* part_o, float* part_ml, hipStream_t s);
 }
 
 namespace {
@@ -449,10 +449,18 @@ int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
 //    cached: 16 of 5 over 4000 29.3 and 25.7, 128 of 5 over 1000 52.3 and 37.5, one of 9
 //    over 8000 18.1 and 16.4, 16 of 12 over 4000 39.5 and 37.0; but 16 of 3 over 4000
 //    21.1 and 22.7, 16 of 16 over 4000 33.3 and 42.9.
+//  * Two splits of 32 tokens make the halves of one workgroup, joined in LDS: half the parts
+//    to be written and merged, none for two; us without and with: 1000 over 1000 59.9
+//    and 45.2, 700 29.5 and 21.8, 300 over 6000 59.3 and 56.7, 128 over 16000 62.7 and 57.2.
+//    Of an odd number one is given up, which pays from seven on (280 over 4000 45.7 and
+//    43.8) or over few keys: three, 550 over 1000 39.2 and 35.9, over 1500 44.5 and 43.6,
+//    over 2500 55.5 and 59.1, over 6000 93 and 114; five, 380 over 3000 47.2 and 48.2.
+constexpr int64_t kFp8OddSplits = 7, kFp8OddKeys = 600;
 constexpr int64_t kFp8ChunkWgs = 512, kFp8PairWgs = 768, kFp8PairTokens = 12, kFp8FewTokens = 24,
                   kFp8FewTiles = 64, kFp8FewKeys = 200000;
 struct Fp8Chunk {
   int64_t tokens, splits, tiles;  // tiles of the longest sequence
+  int64_t halves = 1;             // of a split, one workgroup's
 };
 Fp8Chunk fp8_chunk(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
   auto tiles_of = [&](int64_t tokens) { return (max_q_len + tokens - 1) / tokens; };
@@ -471,8 +479,11 @@ Fp8Chunk fp8_chunk(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t
   const int64_t keys = window > 0 ? std::min(max_kv_len, window + tokens) : max_kv_len;
   if (keys <= 0 || batch > kFp8ChunkWgs) return Fp8Chunk{tokens, 1, tiles_of(tokens)};
   const int64_t most = std::min(kFp8MaxSplits, wgs / (tiles_of(tokens) * batch * kKvHeads));
-  return Fp8Chunk{tokens, std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks)),
-                  tiles_of(tokens)};
+  const int64_t splits = std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kFp8SplitBlocks));
+  const bool pays = splits % 2 == 0 || splits >= kFp8OddSplits || keys <= kFp8OddKeys * splits;
+  if (tokens == 32 && splits > 1 && pays)
+    return Fp8Chunk{tokens, splits / 2, tiles_of(tokens), 2};
+  return Fp8Chunk{tokens, splits, tiles_of(tokens)};
 }
 }  // namespace
 
@@ -553,7 +564,7 @@ int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, i
   return status(attn_launch_fp8_chunk(
       q, q_indptr, (int)batch, (int)max_q_len, kv_cache, page_indptr, page_indices, (int)num_pages,
       kv_len, window, sm_scale, sinks, out, (int)chunk.tokens, (int)chunk.splits,
-      (int)part_rows, part_o,
+      (int)chunk.halves, (int)part_rows, part_o,
       need ? part_o + chunk.splits * part_rows * kQHeads * kHeadDim : nullptr,
       as_stream(stream)));
 }

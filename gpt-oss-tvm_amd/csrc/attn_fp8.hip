@@ -804,10 +804,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
 // two, the last ones leave more of the chip idle, and a window's edges are masked in
 // more columns: 4096 tokens 157 us against 161, 2048 tokens 72 against 54, 4096 with
 // window 128 44 against 33.  So they are taken without a window where they are two
-// rounds or more of the chip.  At 4096 tokens 865 to 905 TFLOP/s (a library product of
-// 8192^3 reaches 1314), 300 over 6000 in 6 shares 56 us (537).
+// rounds or more of the chip.  With kHalves = 2 the workgroup's second half takes the
+// other blocks of its share, and the states meet in LDS.  At 4096 tokens 865 to 905
+// TFLOP/s (a library product of 8192^3 reaches 1314), 300 over 6000 530 with the merge.
 constexpr int kTileBytes = kFp8Block * kD * 2;
-constexpr int tile_threads(int tokens) { return 16 * tokens; }
+constexpr int tile_threads(int tokens, int halves) { return 16 * tokens * halves; }
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
 
 __device__ __forceinline__ f32x16 mfma32(bf16x8 a, bf16x8 b, f32x16 c) {
@@ -820,11 +821,11 @@ __device__ __forceinline__ float half_max(float x) {
   return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
 }
 
-template <int kTokens, bool kSplit>
-__global__ __launch_bounds__(tile_threads(kTokens)) __attribute__((amdgpu_waves_per_eu(4))) void
-fp8_tile_kernel(RowsArgs a) {
-  __shared__ __align__(16) uint8_t kt[2][kTileBytes];
-  __shared__ __align__(16) uint8_t vt[2][kTileBytes];
+template <int kTokens, bool kSplit, int kHalves>
+__global__ __launch_bounds__(tile_threads(kTokens, kHalves))
+__attribute__((amdgpu_waves_per_eu(4))) void fp8_tile_kernel(RowsArgs a) {
+  constexpr int kWaves = kTokens / 4;  // of a half
+  __shared__ __align__(16) uint8_t lds[kHalves][2][2][kTileBytes];
   // x: (tile from the last, which sees the most keys; sequence; kv head), y: split
   const int hk = blockIdx.x % kHkv, total = gridDim.x / kHkv, batch = total / a.tiles;
   int rest = blockIdx.x / kHkv;
@@ -840,19 +841,25 @@ fp8_tile_kernel(RowsArgs a) {
   const Shares shares(sight.blocks, kSplit ? a.splits : 1, a.least);
   const int share = kSplit ? blockIdx.y : 0;
   if (share >= max(shares.used, 1)) return;
-  const int t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6) % kWaves;
+  const int half = kHalves == 1 ? 0 : __builtin_amdgcn_readfirstlane(t >> 6) / kWaves;
   const int c = lane & 31, h = lane >> 5;
   const PageList pages{a.page_indices + a.page_indptr[b],
                        a.page_indptr[b + 1] - a.page_indptr[b], a.num_pages};
   const int last_page = max(0, min(pages.count - 1, (L - 1) / kPage));
-  const int begin = sight.first + share * shares.each;
-  const int end = min(begin + shares.each, sight.first + sight.blocks);
+  const int begin0 = sight.first + share * shares.each;
+  const int end0 = min(begin0 + shares.each, sight.first + sight.blocks);
+  const int most = (end0 - begin0 + kHalves - 1) / kHalves;  // blocks of a half
+  const int begin = begin0 + half * most, end = min(begin + most, end0);
+  uint8_t(*const kt)[kTileBytes] = lds[half][0];
+  uint8_t(*const vt)[kTileBytes] = lds[half][1];
 
   // Staging: waves 0 .. 3 take k, waves 4 .. 7 v of page `wave & 3` of a block: lane
   // the 16 dims 16 (l % 4) .. of key l / 4, or the four keys of quad l / 16 in v's unit
   // l % 16; both take their keys' scales.
   const int mine = wave & 3, quad = 4 * mine + (lane >> 4);
-  const bool is_v = wave & 4, stages = kTokens == 32 || wave < 8;
+  const bool is_v = wave & 4, stages = kWaves == 8 || wave < 8;
   const unsigned part = (is_v ? kFp8V : 0) + hk * kFp8Head + lane * 16;
   const unsigned spart = kFp8Scales + hk * 2 * kPage + (lane >> 4) * 4;
   struct Raw {
@@ -1016,7 +1023,36 @@ fp8_tile_kernel(RowsArgs a) {
   run(std::false_type{}, whole0, whole1);
   run(std::true_type{}, whole1, end);
 
-  const float lt = l + __shfl_xor(l, 32, kWave);
+  float lt = l + __shfl_xor(l, 32, kWave);
+  if constexpr (kHalves == 2) {
+    // the second half's states into the first's, through the tiles' LDS
+    __shared__ float2 ml[kWaves][32];
+    for (int i = max(end - begin, 0); i < most; ++i) moe::lds_barrier();
+    f32x4* const part = (f32x4*)&lds[0][0][0][0] + wave * 8 * kWave + lane;
+    if (half == 1) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        part[q * kWave] = f32x4{o[q >> 2][4 * (q & 3)], o[q >> 2][4 * (q & 3) + 1],
+                                o[q >> 2][4 * (q & 3) + 2], o[q >> 2][4 * (q & 3) + 3]};
+      if (h == 0) ml[wave][c] = make_float2(-mneg, lt);
+    }
+    moe::lds_barrier();
+    if (half == 1) return;
+    const float2 other = ml[wave][c];
+    const float m = fmaxf(-mneg, other.x);
+    const float w0 = -mneg == -INFINITY && lt == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(-mneg - m);
+    const float w1 =
+        other.x == -INFINITY && other.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(other.x - m);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const f32x4 po = part[q * kWave];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[q >> 2][4 * (q & 3) + j] = fmaf(po[j], w1, o[q >> 2][4 * (q & 3) + j] * w0);
+    }
+    lt = fmaf(other.y, w1, lt * w0);
+    mneg = -m;
+  }
   const bool alone = shares.used <= 1;
   if (4 * wave + (c >> 3) >= nt) return;
   const size_t at = (size_t)(row0 + token) * kHq + hk * kGroup + (c & 7);
@@ -1142,13 +1178,13 @@ int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const in
 int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
                           const void* cache, const int* page_indptr, const int* page_indices,
                           int num_pages, const int* kv_len, int window, float sm_scale,
-                          const void* sinks, void* out, int tokens, int splits, int rows,
-                          float* part_o, float* part_ml, hipStream_t s) {
-  if (tokens == 64 && splits != 1) return -6;
+                          const void* sinks, void* out, int tokens, int splits, int halves,
+                          int rows, float* part_o, float* part_ml, hipStream_t s) {
+  if (tokens == 64 ? splits != 1 || halves != 1 : tokens != 32 && halves != 1) return -6;
   const int tiles = (max_q_len + tokens - 1) / tokens;
   const attn::RowsArgs a{(const uint16_t*)q, q_indptr, (const uint8_t*)cache, page_indptr,
                          page_indices, kv_len, (const uint16_t*)sinks, (uint16_t*)out, part_o,
-                         part_ml, nullptr, 0, num_pages, window, splits, 4, rows, tiles,
+                         part_ml, nullptr, 0, num_pages, window, splits, 4 * halves, rows, tiles,
                          sm_scale * attn::kLog2e};
   auto go = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3(attn::kHkv * batch * tiles, splits), dim3(threads), 0, s, a);
@@ -1160,11 +1196,13 @@ int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max
   else if (tokens == 4)
     rc = go(attn::fp8_rows_kernel<2>, 256);
   else if (tokens == 64)
-    rc = go(attn::fp8_tile_kernel<64, false>, attn::tile_threads(64));
+    rc = go(attn::fp8_tile_kernel<64, false, 1>, attn::tile_threads(64, 1));
+  else if (halves == 2)
+    rc = go(attn::fp8_tile_kernel<32, true, 2>, attn::tile_threads(32, 2));
   else if (splits > 1)
-    rc = go(attn::fp8_tile_kernel<32, true>, attn::tile_threads(32));
+    rc = go(attn::fp8_tile_kernel<32, true, 1>, attn::tile_threads(32, 1));
   else
-    rc = go(attn::fp8_tile_kernel<32, false>, attn::tile_threads(32));
+    rc = go(attn::fp8_tile_kernel<32, false, 1>, attn::tile_threads(32, 1));
   if (rc || splits == 1) return rc;
   hipLaunchKernelGGL(attn::fp8_merge_kernel, dim3(batch * tiles, tokens * attn::kHq / 16),
                      dim3(256), 0, s, a, tokens);

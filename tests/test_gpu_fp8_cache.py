@@ -352,6 +352,36 @@ def test_prefill_shared_keys(A, qlens, prefix, window):
     check_prefill(A, seqs, qlens, window, 31, 4 * max(lengths), rows)   # a bound far above
 
 
+@pytest.mark.parametrize("qlens,prefix", [
+    ([700], [0]), ([1000], [1000]), ([400], [400]), ([130], [2300]),
+    ([64, 33, 0, 1], [1500, 40, 9, 0]),
+    ([520, 3, 40], [0, 600, 1]), ([30] * 9, list(range(0, 1800, 200)))])
+def test_prefill_shared_keys_in_halves(A, qlens, prefix):
+    """Tiles whose keys two halves of a workgroup take: of none, one and many blocks, in one share
+    and in several, with scores that leave one half all the weight."""
+    lengths = [p + q for p, q in zip(prefix, qlens)]
+    seqs = Seqs(32, lengths)
+    rows = np.array([0, 1, 31, 32, 63, 64, 65, 100, 127, 128, 299, 399, 511, 640, 699, 999])
+    for scale in (2.0, 8.0):
+        check_prefill(A, seqs, qlens, 0, 33, max(lengths), rows, scale=scale)
+
+
+def test_prefill_bad_rows_in_halves(A):
+    """As test_prefill_bad_rows, with the bad tokens in either half of a tile's keys."""
+    L, n = 1500, 700
+    seqs0 = Seqs(62, [L])
+    k, v = [x.copy() for x in seqs0.k], [x.copy() for x in seqs0.v]
+    k[0][100, 2, 5], v[0][1200, 6, 9], k[0][1499, 1, 0] = NAN_ROW, 0xFF80, 0x7F80
+    seqs = Seqs(62, [L], k=k, v=v)
+    rows = np.array([0, 350, 398, 399, 400, 401, 600, 698, 699])
+    _, _, got = check_prefill(A, seqs, [n], 0, 63, L, rows)
+    bad = np.isnan(O.bf16_to_f32(got)).any(axis=-1)
+    pos = np.arange(L - n, L)
+    for h, j in ((2, 100), (6, 1200), (1, 1499)):
+        np.testing.assert_array_equal(bad[:, 8 * h], pos >= j)
+    assert not bad[:, [0, 24, 32, 40, 56]].any()
+
+
 @pytest.mark.parametrize("window", [0, 100])
 @pytest.mark.parametrize("longest", [1, 2, 3, 4, 5, 6, 12, 13])
 def test_prefill_few_tokens(A, longest, window):
