@@ -440,10 +440,12 @@ int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
 // Tokens of a chunk's query tile, and how many splits its keys are shared out over: as
 // many as let its workgroups fit the chip at once (two a CU; three of several tiles of 2).
 //  * 64 of more than 32 tokens, without a window, where they are two rounds of the chip.
-//  * 4 tokens up to 24 tokens, and for longer chunks where there are few of these tiles
-//    over few keys; us in tiles of 4 and of 32, tokens over cached: 16 sequences of 24
-//    over 2000 33.1 and 36.4; 64 over 6000 25.3 and 30.2; 200 over 500 13.5 and 21.1, over
-//    6000 63 and 48; 64 sequences of 32 over 300 55.7 and 37.8.
+//  * 4 tokens up to 24 tokens, where their tiles are two rounds of the chip or less, and
+//    for longer chunks where there are few of these tiles over few keys; us in tiles of
+//    4 and of 32, (sequences of) tokens over (up to) cached: 16 of 24 over 2000 33.2 and
+//    34.5, 32 of 16 over 4000 65.7 and 74, of 20 over 1000 31.6 and 27.3, 64 of 16 over 1000
+//    49.5 and 40.8; 64 over 6000 25.6 and 26.8, 128 over 3000 26.3 and 32, 200 over 500 13.4
+//    and 21.8, 100 over 6000 38.2 and 35.0.
 //  * 2 tokens of up to 2 and of 5 to 12: a wave's blocks take half as long, and three
 //    workgroups share a CU; us in tiles of 4 and of 2, sequences of tokens over up to
 //    cached: 16 of 5 over 4000 29.3 and 25.7, 128 of 5 over 1000 52.3 and 37.5, one of 9
@@ -457,7 +459,7 @@ int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
 //    over 2500 55.5 and 59.1, over 6000 93 and 114; five, 380 over 3000 47.2 and 48.2.
 constexpr int64_t kFp8OddSplits = 7, kFp8OddKeys = 600;
 constexpr int64_t kFp8ChunkWgs = 512, kFp8PairWgs = 768, kFp8PairTokens = 12, kFp8FewTokens = 24,
-                  kFp8FewTiles = 64, kFp8FewKeys = 200000;
+                  kFp8FewTiles = 64, kFp8FewKeys = 130000;
 struct Fp8Chunk {
   int64_t tokens, splits, tiles;  // tiles of the longest sequence
   int64_t halves = 1;             // of a split, one workgroup's
@@ -471,7 +473,8 @@ Fp8Chunk fp8_chunk(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t
   const int64_t small = tiles_of(4) <= kFp8FewTiles  // tiles of 4, or too many
                             ? tiles_of(4) * std::min(batch, kFp8FewTiles + 1)
                             : kFp8FewTiles + 1;
-  const bool few = max_q_len <= kFp8FewTokens ||
+  const bool rounds = tiles_of(4) == 1 || tiles_of(4) * batch <= 2 * kFp8FewTiles;
+  const bool few = (max_q_len <= kFp8FewTokens && rounds) ||
                    (small <= kFp8FewTiles && reach > 0 && small * reach <= kFp8FewKeys);
   const bool pairs = max_q_len <= 2 || (max_q_len > 4 && max_q_len <= kFp8PairTokens);
   const int64_t tokens = pairs ? 2 : few ? 4 : 32;
