@@ -206,10 +206,12 @@ class PagedKVCache:
         """A new sequence ``seq_id`` of this 8-bit cache with the tokens and the window of
         ``source_id`` of a bf16 cache of as many layers: its rows quantised, in every layer."""
         import attn_native
-        if (not self.fp8 or source.fp8 or source.num_layers != self.num_layers
+        if (not self.fp8 or source.data.dtype != torch.bfloat16
+                or source.data.shape[2:] != self.staging.shape[1:]
+                or source.num_layers != self.num_layers
                 or source.data.device != self.data.device):
             raise ValueError("quantize_from takes a sequence of a bf16 cache into an 8-bit cache "
-                             "of as many layers on the same device")
+                             "of as many layers and the same heads on the same device")
         old = source.seqs[source_id]
         need = -(-old.length // PAGE_SIZE)
         if need > len(self.free):
@@ -218,10 +220,14 @@ class PagedKVCache:
         s = self.seqs[seq_id]
         s.pages = [self.free.pop() for _ in range(need)]
         s.length, s.window = old.length, old.window
-        if s.length:
-            mine, theirs = self.slots_of(seq_id), source.slots_of(source_id)
-            for i in range(self.num_layers):
-                attn_native.kv_quantize_fp8(source.layer(i), theirs, self.layer(i), mine)
+        try:
+            if s.length:
+                mine, theirs = self.slots_of(seq_id), source.slots_of(source_id)
+                for i in range(self.num_layers):
+                    attn_native.kv_quantize_fp8(source.layer(i), theirs, self.layer(i), mine)
+        except Exception:  # its rows are not there: no sequence
+            self.remove_sequence(seq_id)
+            raise
 
     # -- one forward ---------------------------------------------------------------
     def begin_forward(self, seq_ids, append_lengths) -> ForwardTables:

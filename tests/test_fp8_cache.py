@@ -90,6 +90,21 @@ def test_host_cache():
     assert 1 not in c.seqs and len(c.free) == 6
 
 
+@pytest.mark.parametrize("source", [dict(dtype=torch.float32), dict(dtype=torch.float16),
+                                    dict(kv_heads=4), dict(head_dim=32), dict()])
+def test_refused_move_leaves_the_cache(source):
+    """A sequence that quantize_from does not take (or whose rows a launch does not: here, on the
+    CPU, the last) is not in the cache afterwards, and its pages are free."""
+    c = PagedKVCache(num_layers=2, num_pages=8, max_batch=2, max_tokens=64, device="cpu", dtype=FP8)
+    b = PagedKVCache(num_layers=2, num_pages=8, max_batch=2, max_tokens=64, device="cpu", **source)
+    b.add_sequence(5)
+    b.begin_forward([5], [20])
+    free = list(c.free)
+    with pytest.raises(ValueError):
+        c.quantize_from(1, b, 5)
+    assert 1 not in c.seqs and c.free == free and b.seq_len(5) == 20
+
+
 def test_bf16_cache_reads_its_rows():
     c = PagedKVCache(num_layers=1, num_pages=4, max_batch=1, max_tokens=64, device="cpu")
     c.data.copy_(torch.randn(c.data.shape))
