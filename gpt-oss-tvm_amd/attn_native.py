@@ -338,12 +338,9 @@ def _refuse(t, name, dtype, shape, index):
 def _need(t, name, dtype, shape, index):
     """``_expect``, and on the current device: the launch goes to its stream.  One line
     where all is well: a call's checks cost as much host time as a short kernel runs."""
-    if not (type(t) in _TENSORS and t.dtype is dtype and t.get_device() == index
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index
             and t.shape == shape and t.is_contiguous()):
         _refuse(t, name, dtype, shape, index)
-
-
-_TENSORS = (torch.Tensor, torch.nn.Parameter)
 
 
 def _need_fp8(kv_cache):

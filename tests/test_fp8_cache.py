@@ -189,3 +189,16 @@ def test_refusals():
     with pytest.raises(TypeError):
         A.kv_read_fp8(cpu.view(torch.int8), slots)
     assert A.FP8_PAGE_BYTES == FP8_PAGE_BYTES == AO.FP8_PAGE_BYTES
+
+
+class Named(torch.Tensor):
+    """A tensor of a caller's own class."""
+
+
+def test_tensors_of_any_class():
+    import attn_native as A
+    t = torch.zeros((3, 8), dtype=torch.bfloat16)
+    for x in (t, torch.nn.Parameter(t, requires_grad=False), t.as_subclass(Named)):
+        A._need(x, "x", torch.bfloat16, (3, 8), -1)        # -1: the index of a CPU tensor
+        with pytest.raises(ValueError, match="GPU"):
+            A._need(x, "x", torch.bfloat16, (3, 8), 0)

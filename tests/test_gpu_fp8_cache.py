@@ -699,3 +699,23 @@ def test_engine_graph_equals_eager(A):
     for (a, s), (b, t) in zip(want, graphed(3)):
         assert torch.equal(a, b) and s == t
     assert eng.get_kv_total_seq_len() == 140 + 2 + 100 + 3
+
+
+def test_tensors_of_any_class(A):
+    """Arguments of a caller's own class of tensor, as the bf16 cache's wrappers take them."""
+    class Named(torch.Tensor):
+        pass
+
+    rng = np.random.default_rng(130)
+    seqs = Seqs(131, [40])
+    q, sinks = bf16_dev(bf(rng.standard_normal((1, HQ, D)))), bf16_dev(bf(rng.standard_normal(HQ)))
+    ws, out = A.decode_fp8_workspace(1, 40), torch.empty_like(q)
+    want = A.decode_fp8(q, *seqs.tables(), 40, 0, SCALE, sinks, out, ws).clone()
+    args = [t.as_subclass(Named) for t in (q, *seqs.tables())]
+    out.zero_()
+    A.decode_fp8(*args, 40, 0, SCALE, sinks.as_subclass(Named), out.as_subclass(Named), ws)
+    assert torch.equal(out, want)
+    slots = i32_dev(np.arange(5))
+    for a, b in zip(A.kv_read_fp8(args[1], slots.as_subclass(Named)),
+                    A.kv_read_fp8(seqs.cache, slots)):
+        np.testing.assert_array_equal(host_bf16(a), host_bf16(b))
