@@ -343,6 +343,20 @@ def _need(t, name, dtype, shape, index):
         _refuse(t, name, dtype, shape, index)
 
 
+def _count(t, name, dtype):
+    """The rows of an argument: its first dimension."""
+    try:
+        return t.shape[0]
+    except (AttributeError, IndexError):
+        _expect(t, name, dtype)
+        raise ValueError(f"{name}: expected rows, got a single value") from None
+
+
+def _shape(t):
+    """The shape of an argument that may have any (None where it is no tensor)."""
+    return getattr(t, "shape", None)
+
+
 def _need_fp8(kv_cache):
     """Of an 8-bit cache on the current device: its pages, the device's index and stream."""
     if not isinstance(kv_cache, torch.Tensor) or kv_cache.dim() != 2:
@@ -361,7 +375,7 @@ def qkv_rope_append_fp8(qkv: torch.Tensor, bias: torch.Tensor, positions: torch.
     """``qkv_rope_append`` into the 8-bit cache: q as there, k and v quantised as they
     are written.  Slots inside the pool have to differ."""
     pages, dev, stream = _need_fp8(kv_cache)
-    n = qkv.shape[0]
+    n = _count(qkv, "qkv", _BF16)
     _need(qkv, "qkv", _BF16, (n, QKV_DIM), dev)
     _need(bias, "bias", _BF16, (QKV_DIM,), dev)
     _need(positions, "positions", _I32T, (n,), dev)
@@ -380,7 +394,7 @@ def kv_quantize_fp8(src: torch.Tensor, src_slots: torch.Tensor, kv_cache: torch.
     """Rows of a bf16 cache ``src`` [pages, 2, 8, 16, 64] at ``src_slots`` [n] into the 8-bit
     cache at ``slots`` [n] (which have to differ)."""
     pages, dev, stream = _need_fp8(kv_cache)
-    src_pages, n = src.shape[0], src_slots.numel()
+    src_pages, n = _count(src, "src", _BF16), _count(src_slots, "src_slots", _I32T)
     _need(src, "src", _BF16, (src_pages, 2, KV_HEADS, PAGE, HEAD_DIM), dev)
     _need(src_slots, "src_slots", _I32T, (n,), dev)
     _need(slots, "slots", _I32T, (n,), dev)
@@ -395,7 +409,7 @@ def kv_read_fp8(kv_cache: torch.Tensor, slots: torch.Tensor, k_out: torch.Tensor
     """The rows at ``slots`` [n] back as bf16: k and v [n, 8, 64], exact.  Where neither output
     is given they are the halves of one new tensor."""
     pages, dev, stream = _need_fp8(kv_cache)
-    n = slots.numel()
+    n = _count(slots, "slots", _I32T)
     _need(slots, "slots", _I32T, (n,), dev)
     shape = (n, KV_HEADS, HEAD_DIM)
     if k_out is None and v_out is None:
@@ -423,10 +437,10 @@ def decode_fp8_workspace(batch: int, max_span: int, device="cuda") -> torch.Tens
 
 
 def _need_tables(q, page_indptr, page_indices, kv_len, sinks, out, batch, dev):
-    n = q.shape[0]
+    n = _count(q, "q", _BF16)
     _need(q, "q", _BF16, (n, Q_HEADS, HEAD_DIM), dev)
     _need(page_indptr, "page_indptr", _I32T, (batch + 1,), dev)
-    _need(page_indices, "page_indices", _I32T, page_indices.shape, dev)
+    _need(page_indices, "page_indices", _I32T, _shape(page_indices), dev)
     _need(kv_len, "kv_len", _I32T, (batch,), dev)
     _need(sinks, "sinks", _BF16, (Q_HEADS,), dev)
     _need(out, "out", _BF16, (n, Q_HEADS, HEAD_DIM), dev)
@@ -440,9 +454,9 @@ def decode_fp8(q: torch.Tensor, kv_cache: torch.Tensor, page_indptr: torch.Tenso
     once; ``workspace`` from ``decode_fp8_workspace`` (reused by calls that follow one
     another)."""
     pages, dev, stream = _need_fp8(kv_cache)
-    batch = q.shape[0]
+    batch = _count(q, "q", _BF16)
     _need_tables(q, page_indptr, page_indices, kv_len, sinks, out, batch, dev)
-    _need(workspace, "workspace", _U8, workspace.shape, dev)
+    _need(workspace, "workspace", _U8, _shape(workspace), dev)
     _check(_lib.attn_decode_fp8(q.data_ptr(), batch, kv_cache.data_ptr(), pages,
                                 page_indptr.data_ptr(), page_indices.data_ptr(), kv_len.data_ptr(),
                                 max_span, window, sm_scale, sinks.data_ptr(), out.data_ptr(),
@@ -458,9 +472,9 @@ def prefill_fp8(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, kv_cach
     """``prefill`` over the 8-bit cache (the formula of ``decode_fp8``): causal attention of
     each sequence's new tokens over its cached ones.  ``max_kv_len`` as there."""
     pages, dev, stream = _need_fp8(kv_cache)
-    n, batch = q.shape[0], q_indptr.numel() - 1
-    _need_tables(q, page_indptr, page_indices, kv_len, sinks, out, batch, dev)
+    n, batch = _count(q, "q", _BF16), _count(q_indptr, "q_indptr", _I32T) - 1
     _need(q_indptr, "q_indptr", _I32T, (batch + 1,), dev)
+    _need_tables(q, page_indptr, page_indices, kv_len, sinks, out, batch, dev)
     need = _lib.attn_prefill_fp8_workspace_bytes(n, batch, max_q_len, max_kv_len, window)
     ws = torch.empty(need, dtype=_U8, device=q.device) if need else None
     _check(_lib.attn_prefill_fp8(q.data_ptr(), n, q_indptr.data_ptr(), batch, max_q_len,

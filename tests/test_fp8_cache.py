@@ -202,3 +202,32 @@ def test_tensors_of_any_class():
         A._need(x, "x", torch.bfloat16, (3, 8), -1)        # -1: the index of a CPU tensor
         with pytest.raises(ValueError, match="GPU"):
             A._need(x, "x", torch.bfloat16, (3, 8), 0)
+
+
+def test_arguments_that_are_no_tensors(monkeypatch):
+    """None, an array or a single value where a tensor of rows belongs: a TypeError or a
+    ValueError that names it, before any launch."""
+    import attn_native as A
+    monkeypatch.setattr(A, "_need_fp8", lambda cache: (4, -1, None))   # as if on this device
+    cache = torch.zeros((4, FP8_PAGE_BYTES), dtype=torch.uint8)
+    i32, bf16 = torch.zeros(3, dtype=torch.int32), torch.bfloat16
+    q, sinks = torch.zeros((2, 64, 64), dtype=bf16), torch.zeros(64, dtype=bf16)
+    src = torch.zeros((1, 2, 8, 16, 64), dtype=bf16)
+    for bad in (None, np.zeros((2, 64, 64), dtype=np.float32), 5, torch.zeros((), dtype=bf16),
+                torch.zeros((), dtype=torch.int32)):
+        for name, call in (
+                ("qkv", lambda: A.qkv_rope_append_fp8(bad, None, i32, i32, None, 1.0, cache, q)),
+                ("src", lambda: A.kv_quantize_fp8(bad, i32, cache, i32)),
+                ("src_slots", lambda: A.kv_quantize_fp8(src, bad, cache, i32)),
+                ("slots", lambda: A.kv_read_fp8(cache, bad)),
+                ("q", lambda: A.decode_fp8(bad, cache, i32, i32, i32[:2], 9, 0, 0.1, sinks, q,
+                                           None)),
+                ("page_indices", lambda: A.decode_fp8(
+                    q, cache, i32, bad if getattr(bad, "dtype", None) != torch.int32 else "0",
+                    i32[:2], 9, 0, 0.1, sinks, q, None)),
+                ("workspace", lambda: A.decode_fp8(q, cache, i32, i32, i32[:2], 9, 0, 0.1, sinks,
+                                                   q, bad)),
+                ("q_indptr", lambda: A.prefill_fp8(q, bad, 1, cache, i32, i32, i32[:2], 0, 0.1,
+                                                   sinks, q))):
+            with pytest.raises((TypeError, ValueError), match=f"^{name}: "):
+                call()
