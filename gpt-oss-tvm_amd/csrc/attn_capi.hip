@@ -550,8 +550,9 @@ int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, i
     return MOE_ERR_SHAPE;
   if (rows == 0 || batch == 0 || max_q_len == 0) return MOE_OK;
   if (batch > kMaxTokens) return MOE_ERR_SHAPE;  // (and no overflow below)
+  // as many tiles of 64 tokens as a launch of attn_prefill holds
+  if ((max_q_len + 63) / 64 * batch >= ((int64_t)1 << 24)) return MOE_ERR_SHAPE;
   const Fp8Chunk chunk = fp8_chunk(batch, max_q_len, max_kv_len, window);
-  if (chunk.tiles * batch * kKvHeads >= ((int64_t)1 << 22)) return MOE_ERR_SHAPE;
   if (!(sm_scale > 0.0f && sm_scale <= FLT_MAX)) return MOE_ERR_UNSUPPORTED;
   if (!q || !q_indptr || !kv_cache || !page_indptr || !page_indices || !kv_len || !sinks || !out)
     return MOE_ERR_NULL;

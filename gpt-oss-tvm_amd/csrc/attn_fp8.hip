@@ -1174,7 +1174,9 @@ int attn_launch_fp8_decode(const void* q, int batch, const void* cache, const in
 }
 
 // tokens: of a tile, 2, 4, 32 or (not split) 64; part_o [splits][rows][64][64], part_ml
-// [splits][rows][64][2] where splits > 1
+// [splits][rows][64][2] where splits > 1.  A launch holds less than 2^32 threads: more
+// tiles go in launches of some sequences each, which are never split ones (their
+// workgroups fit the chip at once).
 int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max_q_len,
                           const void* cache, const int* page_indptr, const int* page_indices,
                           int num_pages, const int* kv_len, int window, float sm_scale,
@@ -1182,31 +1184,38 @@ int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max
                           int rows, float* part_o, float* part_ml, hipStream_t s) {
   if (tokens == 64 ? splits != 1 || halves != 1 : tokens != 32 && halves != 1) return -6;
   const int tiles = (max_q_len + tokens - 1) / tokens;
-  const attn::RowsArgs a{(const uint16_t*)q, q_indptr, (const uint8_t*)cache, page_indptr,
-                         page_indices, kv_len, (const uint16_t*)sinks, (uint16_t*)out, part_o,
-                         part_ml, nullptr, 0, num_pages, window, splits, 4 * halves, rows, tiles,
-                         sm_scale * attn::kLog2e};
-  auto go = [&](auto kernel, int threads) {
-    hipLaunchKernelGGL(kernel, dim3(attn::kHkv * batch * tiles, splits), dim3(threads), 0, s, a);
-    return hipGetLastError() == hipSuccess ? 0 : -6;
-  };
-  int rc = -6;
-  if (tokens == 2)
-    rc = go(attn::fp8_rows_kernel<1>, 256);
-  else if (tokens == 4)
-    rc = go(attn::fp8_rows_kernel<2>, 256);
-  else if (tokens == 64)
-    rc = go(attn::fp8_tile_kernel<64, false, 1>, attn::tile_threads(64, 1));
-  else if (halves == 2)
-    rc = go(attn::fp8_tile_kernel<32, true, 2>, attn::tile_threads(32, 2));
-  else if (splits > 1)
-    rc = go(attn::fp8_tile_kernel<32, true, 1>, attn::tile_threads(32, 1));
-  else
-    rc = go(attn::fp8_tile_kernel<32, false, 1>, attn::tile_threads(32, 1));
-  if (rc || splits == 1) return rc;
-  hipLaunchKernelGGL(attn::fp8_merge_kernel, dim3(batch * tiles, tokens * attn::kHq / 16),
-                     dim3(256), 0, s, a, tokens);
-  return hipGetLastError() == hipSuccess ? 0 : -6;
+  const int threads = tokens >= 32 ? attn::tile_threads(tokens, halves) : 256;
+  const int64_t room = (((int64_t)1 << 32) - 1) / ((int64_t)threads * attn::kHkv * tiles);
+  if (room < 1 || (splits > 1 && batch > room)) return -6;
+  for (int b = 0, most = (int)(room < batch ? room : batch); b < batch; b += most) {
+    const int group = batch - b < most ? batch - b : most;
+    const attn::RowsArgs a{(const uint16_t*)q, q_indptr + b, (const uint8_t*)cache,
+                           page_indptr + b, page_indices, kv_len + b, (const uint16_t*)sinks,
+                           (uint16_t*)out, part_o, part_ml, nullptr, 0, num_pages, window, splits,
+                           4 * halves, rows, tiles, sm_scale * attn::kLog2e};
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(attn::kHkv * group * tiles, splits), dim3(threads), 0, s, a);
+    };
+    if (tokens == 2)
+      go(attn::fp8_rows_kernel<1>);
+    else if (tokens == 4)
+      go(attn::fp8_rows_kernel<2>);
+    else if (tokens == 64)
+      go(attn::fp8_tile_kernel<64, false, 1>);
+    else if (halves == 2)
+      go(attn::fp8_tile_kernel<32, true, 2>);
+    else if (splits > 1)
+      go(attn::fp8_tile_kernel<32, true, 1>);
+    else
+      go(attn::fp8_tile_kernel<32, false, 1>);
+    if (hipGetLastError() != hipSuccess) return -6;
+    if (splits > 1) {
+      hipLaunchKernelGGL(attn::fp8_merge_kernel, dim3(group * tiles, tokens * attn::kHq / 16),
+                         dim3(256), 0, s, a, tokens);
+      if (hipGetLastError() != hipSuccess) return -6;
+    }
+  }
+  return 0;
 }
 
 }  // extern "C"

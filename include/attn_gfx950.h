@@ -239,7 +239,9 @@ MOE_API int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cac
  * shared out over workgroups; 0: unknown, not shared out).  A sequence's last bits
  * may change with the other sequences of the call and with the bounds.  The
  * workspace (none where attn_prefill_fp8_workspace_bytes is 0) needs no
- * initialisation; calls on one have to follow one another. */
+ * initialisation; calls on one have to follow one another.  Limits: rows, batch and
+ * max_q_len up to 2^24, and fewer than 2^24 tiles of 64 tokens, ceil(max_q_len / 64) x
+ * batch. */
 MOE_API size_t attn_prefill_fp8_workspace_bytes(int64_t rows, int64_t batch, int64_t max_q_len,
                                                 int64_t max_kv_len, int32_t window);
 MOE_API int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr,

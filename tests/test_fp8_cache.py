@@ -191,6 +191,25 @@ def test_refusals():
     assert A.FP8_PAGE_BYTES == FP8_PAGE_BYTES == AO.FP8_PAGE_BYTES
 
 
+def test_chunks_of_many_sequences():
+    """The sizes that attn_prefill takes: up to 2^24 tiles of 64 tokens (checked before the
+    pointers, so a call without them says which check it came to)."""
+    import attn_native  # noqa: F401  (the entry points' signatures)
+    import moe_native
+    lib, codes = moe_native.lib(), header_codes()
+    p = ctypes.c_void_p(0x1000)
+
+    def pre(batch, longest, window=0):
+        return lib.attn_prefill_fp8(None, 1 << 20, p, batch, longest, p, 8, p, p, p, 1 << 20,
+                                    window, 0.125, p, p, None, 0, None)
+    for window in (0, 128):
+        for batch, longest in ((2048, 16384), (65535, 16384), (1, 1 << 24), (63, 1 << 24),
+                               (600000, 7), ((1 << 24) - 1, 1)):
+            assert pre(batch, longest, window) == codes["MOE_ERR_NULL"], (batch, longest)
+        for batch, longest in ((65536, 16384), (64, 1 << 24), (1 << 24, 1)):
+            assert pre(batch, longest, window) == codes["MOE_ERR_SHAPE"], (batch, longest)
+
+
 class Named(torch.Tensor):
     """A tensor of a caller's own class."""
 

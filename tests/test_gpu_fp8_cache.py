@@ -719,3 +719,34 @@ def test_tensors_of_any_class(A):
     for a, b in zip(A.kv_read_fp8(args[1], slots.as_subclass(Named)),
                     A.kv_read_fp8(seqs.cache, slots)):
         np.testing.assert_array_equal(host_bf16(a), host_bf16(b))
+
+
+@pytest.mark.parametrize("longest,batch,window,threads,tokens", [
+    (600, 60000, 0, 1024, 64), (600, 60000, 128, 512, 32), (7, 600000, 0, 256, 2)])
+def test_prefill_more_tiles_than_a_launch(A, longest, batch, window, threads, tokens):
+    """Tiles of the longest sequence for so many sequences (nearly all of them empty here) that
+    they go in several launches: sequences at the ends and on both sides of the border."""
+    border = ((1 << 32) - 1) // (threads * HKV * -(-longest // tokens))
+    assert border + 1 < batch
+    at = np.array([0, border - 1, border, border + 1, batch - 1])
+    qlens = np.minimum([70, 5, 33, 64, 1], longest)
+    lengths = qlens + [0, 40, 300, 0, 200]
+    small = Seqs(140, lengths.tolist())
+    q_len, kv_len, pages = (np.zeros(batch, dtype=np.int32) for _ in range(3))
+    q_len[at], kv_len[at], pages[at] = qlens, lengths, -(-lengths // PAGE)
+    q_indptr, page_indptr = (np.concatenate([[0], np.cumsum(x)]) for x in (q_len, pages))
+    rng = np.random.default_rng(141)
+    n = int(q_indptr[-1])
+    q, sinks = bf(rng.standard_normal((n, HQ, D)) * 2.0), bf(rng.standard_normal(HQ))
+    out = torch.full((n + 2, HQ, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    qd = torch.zeros((n + 2, HQ, D), dtype=torch.bfloat16, device="cuda")
+    qd[:n] = bf16_dev(q)
+    A.prefill_fp8(qd, i32_dev(q_indptr), longest, small.cache, i32_dev(page_indptr),
+                  small.page_indices, i32_dev(kv_len), window, SCALE, bf16_dev(sinks), out,
+                  int(lengths.max()))
+    got = host_bf16(out)
+    assert (got[n:] == 0x40E0).all()
+    for i, b in enumerate(at):
+        rows = slice(q_indptr[b], q_indptr[b + 1])
+        within(got[rows], q[rows], small.kd[i], small.vd[i],
+               np.arange(lengths[i] - qlens[i], lengths[i]), window, sinks, U)
