@@ -440,17 +440,18 @@ int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
 // Tokens of a chunk's query tile, and how many splits its keys are shared out over: as
 // many as let its workgroups fit the chip at once (two a CU; three of several tiles of 2).
 //  * 64 of more than 32 tokens, without a window, where they are two rounds of the chip.
-//  * 4 tokens up to 24 tokens, where their tiles are two rounds of the chip or less, and
+//  * 4 tokens up to 20 tokens, where their tiles are two rounds of the chip or less, and
 //    for longer chunks where there are few of these tiles over few keys; us in tiles of
-//    4 and of 32, (sequences of) tokens over (up to) cached: 16 of 24 over 2000 33.2 and
-//    34.5, 32 of 16 over 4000 65.7 and 74, of 20 over 1000 31.6 and 27.3, 64 of 16 over 1000
-//    49.5 and 40.8; 64 over 6000 25.6 and 26.8, 128 over 3000 26.3 and 32, 200 over 500 13.4
-//    and 21.8, 100 over 6000 38.2 and 35.0.
+//    4 and of 32, (sequences of) tokens over (up to) cached: 16 of 20 over 2000 29.0 and
+//    33.1, of 24 over 2000 37.0 and 34.9, 32 of 16 over 4000 74.2 and 75.2, of 20 over 1000
+//    33.6 and 26.8, 64 of 16 over 1000 53.3 and 41.3; 8 of 24 over 1000 15.8 and 23.1, 24 over
+//    8000 22.0 and 25.5, 64 over 6000 27.9 and 25.7, 128 over 3000 28.2 and 30.2, 200 over 500
+//    14.2 and 21.7, 100 over 6000 42.3 and 35.5.
 //  * 2 tokens of up to 2 and of 5 to 12: a wave's blocks take half as long, and three
 //    workgroups share a CU; us in tiles of 4 and of 2, sequences of tokens over up to
-//    cached: 16 of 5 over 4000 29.3 and 25.7, 128 of 5 over 1000 52.3 and 37.5, one of 9
-//    over 8000 18.1 and 16.4, 16 of 12 over 4000 39.5 and 37.0; but 16 of 3 over 4000
-//    21.1 and 22.7, 16 of 16 over 4000 33.3 and 42.9.
+//    cached: 16 of 5 over 4000 31.8 and 27.1, 128 of 5 over 1000 56.1 and 39.6, one of 9
+//    over 8000 18.7 and 16.7, 16 of 12 over 4000 44.0 and 40.4; but 16 of 3 over 4000
+//    22.2 and 23.8, 16 of 16 over 4000 37.2 and 47.1.
 //  * Two splits of 32 tokens make the halves of one workgroup, joined in LDS: half the parts
 //    to be written and merged, none for two; us without and with: 1000 over 1000 59.9
 //    and 45.2, 700 29.5 and 21.8, 300 over 6000 59.3 and 56.7, 128 over 16000 62.7 and 57.2.
@@ -458,7 +459,7 @@ int64_t fp8_decode_splits(int64_t batch, int64_t max_span) {
 //    43.8) or over few keys: three, 550 over 1000 39.2 and 35.9, over 1500 44.5 and 43.6,
 //    over 2500 55.5 and 59.1, over 6000 93 and 114; five, 380 over 3000 47.2 and 48.2.
 constexpr int64_t kFp8OddSplits = 7, kFp8OddKeys = 600;
-constexpr int64_t kFp8ChunkWgs = 512, kFp8PairWgs = 768, kFp8PairTokens = 12, kFp8FewTokens = 24,
+constexpr int64_t kFp8ChunkWgs = 512, kFp8PairWgs = 768, kFp8PairTokens = 12, kFp8FewTokens = 20,
                   kFp8FewTiles = 64, kFp8FewKeys = 130000;
 struct Fp8Chunk {
   int64_t tokens, splits, tiles;  // tiles of the longest sequence

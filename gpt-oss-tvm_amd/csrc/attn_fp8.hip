@@ -540,11 +540,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4))) void f
 }
 
 // Chunks of few tokens (drafts under verification): a tile of 2 kCt tokens in kCt tiles
-// of 16 columns (token, head), by decode's loads and products; p enters as one
-// bf16 rounding, as in the long chunks' form.  More tokens take more such tiles, which
-// read the keys again.  Bound by a wave's own instructions over its blocks: 16 sequences
-// of 5 tokens over up to 4000 keys take 54 us in one tile of 8 (its four column tiles a
-// wave spill), 29 in tiles of 4, 25.7 in tiles of 2.
+// of 16 columns (token, head), by decode's loads and products, p in two bf16 pieces as
+// there: a token gets the same weights whether it is decoded or verified.  (One bf16
+// rounding of p, whatever p's sum takes, is 6 to 10% faster: 16 sequences of 5 tokens over
+// up to 4000 keys 25.5 us; its errors against 64 bits 0.0020 to 0.0022 where decode's
+// and this form's are 0.0017.)  More tokens take more such tiles, which read the
+// keys again.  Bound by a wave's own instructions over its blocks: the 16 sequences
+// of 5 tokens take 31.8 us in tiles of 4, 27.1 in tiles of 2 (one tile of 8, whose four
+// column tiles a wave spill, took twice as long).
 template <int kCt>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void fp8_rows_kernel(
     RowsArgs a) {
@@ -632,7 +635,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
     if (next >= 0) load_k(next);  // in flight during the rest
     // every token of the tile sees the whole block
     const bool whole = kb + kFp8Block - 1 <= pos && (a.window <= 0 || kb > sight.last - a.window);
-    bf16x8 pb[kCt][2];
+    bf16x8 ph[kCt][2], pl[kCt][2];
 #pragma unroll
     for (int ct = 0; ct < kCt; ++ct) {
       f32x4 st[4];
@@ -687,7 +690,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
         for (int i = 0; i < 4; ++i) {
           float pv = e[p][i] * __uint_as_float(((vs[p] >> (8 * i)) & 255u) << 23);
           if (!whole) pv = (unsigned)(back - 16 * p - i) < reach ? pv : 0.0f;
-          pb[ct][p >> 1][4 * (p & 1) + i] = (__bf16)pv;
+          const __bf16 hi = (__bf16)pv;
+          ph[ct][p >> 1][4 * (p & 1) + i] = hi;
+          pl[ct][p >> 1][4 * (p & 1) + i] = (__bf16)(pv - (float)hi);
         }
     }
     if (kb + kFp8Block > L) {  // stale codes past the sequence's end may be NaN
@@ -705,8 +710,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
       const bf16x8 v1 = fp8_to_bf16(v[2][dt], v[3][dt], 1.0f);
 #pragma unroll
       for (int ct = 0; ct < kCt; ++ct) {
-        o[ct][dt] = mfma_bf16(v0, pb[ct][0], o[ct][dt]);
-        o[ct][dt] = mfma_bf16(v1, pb[ct][1], o[ct][dt]);
+        o[ct][dt] = mfma_bf16(v0, ph[ct][0], o[ct][dt]);
+        o[ct][dt] = mfma_bf16(v0, pl[ct][0], o[ct][dt]);
+        o[ct][dt] = mfma_bf16(v1, ph[ct][1], o[ct][dt]);
+        o[ct][dt] = mfma_bf16(v1, pl[ct][1], o[ct][dt]);
       }
     }
     if (next >= 0) load_v(next);
@@ -784,7 +791,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
 //    product m reads quads 4 m + h and 4 m + 2 + h as one 16-byte unit.
 //  * p enters as one bf16 rounding, and the sum takes the rounded p (v_dot2): a
 //    weight is off by at most half a bf16 step, as the output's own rounding is,
-//    and where few keys matter the two cancel.
+//    and where few keys matter the two cancel.  (The cached values' own half step is
+//    sixteen times as large.)  Errors against 64 bits 0.0020 to 0.0021; in two pieces, as decode has
+//    p, 0.0017, for half as many products again and 40 more vector instructions a
+//    tile: 4096 tokens 223 us instead of 151, 300 over 6000 72 instead of 55.
 //  * No row maximum: the softmax's reference point m is the maximum of the
 //    first keys a column sees, and stays.  Larger scores only make p larger than
 //    1, which fp32 and bf16 carry; a wave takes new maxima, rescales and computes its

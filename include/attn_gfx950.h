@@ -233,7 +233,11 @@ MOE_API int attn_decode_fp8(const uint16_t* q, int64_t batch, const void* kv_cac
                             void* workspace, size_t workspace_bytes, moe_stream_t stream);
 
 /* attn_prefill over the 8-bit cache, with attn_decode_fp8's formula: each sequence's new
- * tokens (appended already) causally over its cached keys.  q has `rows` rows;
+ * tokens (appended already) causally over its cached keys.  Calls of few tokens a sequence
+ * (up to 20 where they leave the chip room, fewer beside many others) are computed as
+ * attn_decode_fp8's.  In longer ones the p_j are rounded to bf16 (their sum is taken of
+ * the rounded ones, in fp32): a key's weight is off by up to 2^-8 of itself, where the cache
+ * holds its values to 2^-4.  q has `rows` rows;
  * rows outside q_indptr's ranges are left as they are.  max_q_len bounds every
  * q_len, max_kv_len kv_len (it only chooses how the keys of few query tiles are
  * shared out over workgroups; 0: unknown, not shared out).  A sequence's last bits

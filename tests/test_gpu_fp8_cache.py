@@ -750,3 +750,23 @@ def test_prefill_more_tiles_than_a_launch(A, longest, batch, window, threads, to
         rows = slice(q_indptr[b], q_indptr[b + 1])
         within(got[rows], q[rows], small.kd[i], small.vd[i],
                np.arange(lengths[i] - qlens[i], lengths[i]), window, sinks, U)
+
+
+@pytest.mark.parametrize("longest", [1, 2, 3, 4, 5, 8, 12, 16, 20])
+def test_prefill_few_tokens_as_exact_as_decode(A, longest):
+    """Drafts of up to `longest` tokens keep their probabilities to decode's two bf16 pieces
+    (2^-16), alone and in shares: flat scores over few keys, whose roundings do not average out,
+    and sharp ones."""
+    qlens = [longest, 1, longest, max(1, longest - 1), longest]
+    lengths = [n + p for n, p in zip(qlens, [0, 2, 5, 40, 1300])]
+    seqs = Seqs(600 + longest, lengths)
+    indptr = np.concatenate([[0], np.cumsum(qlens)])
+    rng = np.random.default_rng(601)
+    for scale, bound in ((0.25, 0), (0.25, max(lengths)), (4.0, max(lengths))):
+        q = bf(rng.standard_normal((sum(qlens), HQ, D)) * scale)
+        sinks = bf(rng.standard_normal(HQ))
+        got, _ = run_prefill(A, seqs, q, qlens, sinks, 0, bound)
+        for b, (L, n) in enumerate(zip(lengths, qlens)):
+            rows = slice(indptr[b], indptr[b + 1])
+            within(got[rows], q[rows], seqs.kd[b], seqs.vd[b], np.arange(L - n, L), 0, sinks,
+                   2.0 ** -16)
