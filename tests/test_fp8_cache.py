@@ -250,3 +250,11 @@ def test_arguments_that_are_no_tensors(monkeypatch):
                                                    sinks, q))):
             with pytest.raises((TypeError, ValueError), match=f"^{name}: "):
                 call()
+
+
+def test_staging_holds_the_fused_projections():
+    """A step that takes the fused QKV projection finds a staging row for each of its tokens."""
+    import attn_native as A
+    c = PagedKVCache(1, 2, 1, 16, device="cpu", dtype=FP8)
+    assert c.staging_slots.numel() == c.staging.shape[0] * A.PAGE >= A.ROWS_QKV_MAX_TOKENS
+    assert A.ROWS_QKV_MAX_TOKENS >= A.GEMV_MAX_TOKENS

@@ -770,3 +770,181 @@ def test_prefill_few_tokens_as_exact_as_decode(A, longest):
             rows = slice(indptr[b], indptr[b + 1])
             within(got[rows], q[rows], seqs.kd[b], seqs.vd[b], np.arange(L - n, L), 0, sinks,
                    2.0 ** -16)
+
+
+class LongSeqs(Seqs):
+    """Sequences of any length on a pool of `pool` pages of random rows, each page of a sequence
+    any page of the pool: a page read in another's place shows."""
+
+    def __init__(self, seed, lengths, pool=300):
+        super().__init__(seed, [pool * PAGE])
+        rng = np.random.default_rng(seed + 1)
+        order = self.page_indices.cpu().numpy()        # order[i]: where tokens 16 i .. lie
+        lists = [rng.integers(0, pool, -(-L // PAGE)) for L in lengths]
+        rows = [(p[:, None] * PAGE + np.arange(PAGE)).ravel()[:L] for p, L in zip(lists, lengths)]
+        self.kd, self.vd = [self.kd[0][r] for r in rows], [self.vd[0][r] for r in rows]
+        self.lengths = lengths
+        self.page_indptr = i32_dev(np.concatenate([[0], np.cumsum([len(p) for p in lists])]))
+        self.page_indices = i32_dev(order[np.concatenate(lists)])
+        self.kv_len = i32_dev(np.array(lengths))
+
+
+@pytest.mark.parametrize("lengths", [[33000], [40000], [70000], [140000, 90]])
+def test_decode_long(A, lengths):
+    """Against the oracle: one sequence in 33 to 64 splits, and splits of more than 64 blocks,
+    whose waves fetch a second set of page ids (two sequences: at most 32 splits)."""
+    seqs = LongSeqs(700, lengths)
+    check_decode(A, seqs, 0, 701)
+    check_decode(A, seqs, 0, 702, scale=4.0)
+
+
+def parts(A, rows, batch, longest, most_kv, window):
+    """Rows of the parts that a chunk call's shares leave for the merge: shares x the tokens of
+    its tiles."""
+    size = A._lib.attn_prefill_fp8_workspace_bytes(rows, batch, longest, most_kv, window)
+    assert size % (HQ * (D + 2) * 4) == 0
+    return size // (HQ * (D + 2) * 4)
+
+
+@pytest.mark.parametrize("qlens,prefix,bound,window", [
+    ([2], [9000], 0, 0), ([4], [9000], 0, 0), ([12, 1], [9000, 70], 0, 0),   # tiles of 2 and 4
+    ([40], [9000], 0, 0), ([40, 3], [9000, 100], 0, 8000),                   # of 32, whole
+    ([30] + [1] * 31, [9000] + [50] * 31, 9030, 0),                          # two halves
+    ([4200], [0], 4200, 0), ([40] + [33] * 63, [9000] + [5] * 63, 9040, 0)])  # of 64
+def test_prefill_more_blocks_than_page_ids_at_hand(A, qlens, prefix, bound, window):
+    """More than 64 blocks of keys for one workgroup, or half of one: its waves fetch a second
+    and third set of page ids."""
+    lengths = [p + q for p, q in zip(prefix, qlens)]
+    assert parts(A, sum(qlens), len(qlens), max(qlens), bound, window) == 0      # one share
+    rows = np.array([0, 1, 2, 3, 11, 29, 31, 32, 39, 2000, 4095, 4096, 4097, 4170, 4199])
+    seqs = LongSeqs(710, lengths)
+    check_prefill(A, seqs, qlens, window, 711, bound, rows)
+    check_prefill(A, seqs, qlens, window, 712, bound, rows, scale=4.0)
+
+
+@pytest.mark.parametrize("qlen,prefix,window,shares", [
+    (550, 2500, 0, 3), (380, 3000, 0, 5), (550, 6000, 4000, 3), (300, 6000, 2000, 3)])
+def test_prefill_shared_keys_in_odd_shares(A, qlen, prefix, window, shares):
+    """Tiles of 32 tokens in an odd number of shares, each a workgroup's (the first three: as many
+    as fit the chip, 512 workgroups) or two halves' (the last), with and without a window."""
+    L, tiles = qlen + prefix, -(-qlen // 32)
+    assert parts(A, qlen, 1, qlen, L, window) == shares * 32 * tiles
+    assert shares == 512 // (8 * tiles) // (2 if qlen == 300 else 1)
+    rows = np.array([0, 1, 31, 32, 33, 160, qlen // 2, qlen - 33, qlen - 32, qlen - 31, qlen - 1])
+    seqs = LongSeqs(720, [L])
+    for scale in (2.0, 8.0):
+        check_prefill(A, seqs, [qlen], window, 721, L, rows, scale=scale)
+
+
+def test_prefill_larger_tiles_sharp_scores(A):
+    """Tiles of 64 tokens (a batch of two rounds of the chip): scores of +-100 and more, and ones
+    that rise or fall slowly and by large steps along the keys."""
+    qlens, prefix = [512, 64, 1, 130, 3, 33, 400, 100], [100, 0, 700, 9, 64, 31, 300, 77]
+    lengths = [p + q for p, q in zip(prefix, qlens)]
+    rows = np.array([0, 1, 3, 31, 32, 63, 64, 129, 255, 256, 399, 511])
+    check_prefill(A, Seqs(730, lengths), qlens, 0, 731, 700, rows, scale=12.0)
+    rng = np.random.default_rng(732)
+    for step in (0.02, 3.0, -3.0):
+        k = []
+        for L in lengths:
+            x = rng.standard_normal((L, HKV, D)) * 0.05
+            x[:, :, 0] += step * (np.arange(L)[:, None] // 16 - (0 if step > 0 else L // 16))
+            k.append(bf(x))
+        seqs = Seqs(733, lengths, k=k)
+        q = rng.standard_normal((sum(qlens), HQ, D)) * 0.1
+        q[:, :, 0] = 8.0
+        q, sinks = bf(q), bf(np.zeros(HQ))
+        got, indptr = run_prefill(A, seqs, q, qlens, sinks, 0, 700)
+        for b, (L, n) in enumerate(zip(lengths, qlens)):
+            pick = np.unique(np.clip(rows, 0, n - 1))
+            at = indptr[b] + pick
+            within(got[at], q[at], seqs.kd[b], seqs.vd[b], L - n + pick, 0, sinks, U)
+
+
+def test_prefill_larger_tiles_bad_rows(A):
+    """Tiles of 64 tokens: a NaN in k, infinities in v and k reach the queries that see them, in
+    their kv head, and no others; what lies past the sequences' ends reaches none."""
+    qlens, prefix = [512, 64, 1, 130, 3, 33, 400, 100], [100, 0, 700, 9, 64, 31, 300, 77]
+    lengths = [p + q for p, q in zip(prefix, qlens)]
+    seqs0 = Seqs(740, lengths)
+    k, v = [x.copy() for x in seqs0.k], [x.copy() for x in seqs0.v]
+    k[0][150, 2, 5], v[0][500, 6, 9], k[0][611, 1, 0] = NAN_ROW, 0xFF80, 0x7F80
+    seqs = Seqs(740, lengths, k=k, v=v)
+    rows = np.array([0, 49, 50, 51, 399, 400, 401, 510, 511])
+    _, _, got = check_prefill(A, seqs, qlens, 0, 741, 700, rows)
+    bad = np.isnan(O.bf16_to_f32(got)).any(axis=-1)
+    pos = np.arange(100, 612)
+    for h, j in ((2, 150), (6, 500), (1, 611)):
+        np.testing.assert_array_equal(bad[:512, 8 * h:8 * h + 8],
+                                      np.repeat((pos >= j)[:, None], 8, 1))
+    assert not bad[512:].any() and not bad[:, [0, 24, 32, 40, 56]].any()
+
+
+def test_captured_writes(A):
+    """A step that appends, quantises, attends and reads, on another stream and captured: before
+    each run the rows that it writes are replaced by others, so that only its own writes give the
+    outputs and the cache that the eager step left."""
+    from test_gpu_attention import _inv_freq_dev
+    rng = np.random.default_rng(750)
+    seqs = Seqs(751, [700, 90])
+    cache, ids = seqs.cache, seqs.page_indices.cpu().numpy()
+    ends = [int(x) for x in seqs.page_indptr[1:].cpu().numpy()]
+
+    def slot(b, pos):
+        return ids[(0 if b == 0 else ends[0]) + pos // PAGE] * PAGE + pos % PAGE
+
+    appended = i32_dev(np.array([slot(0, 698), slot(0, 699), slot(1, 89)]))
+    moved = i32_dev(np.array([slot(0, 690), slot(0, 691), slot(1, 80)]))
+    both = torch.cat([appended, moved])
+
+    def draw(*shape):
+        return bf16_dev(bf(rng.standard_normal(shape)))
+
+    qkv, bias, src = draw(3, (HQ + 2 * HKV) * D), draw((HQ + 2 * HKV) * D), draw(1, 2, HKV, PAGE, D)
+    pos, three, six = (i32_dev(np.array(x)) for x in ([698, 699, 89], [0, 1, 2], range(6)))
+    inv, conc = _inv_freq_dev()
+    q, qc, sinks, n = draw(2, HQ, D), draw(8, HQ, D), draw(HQ), 4
+    qi = i32_dev(np.array([0, n, 2 * n]))
+    ws = A.decode_fp8_workspace(2, 700)
+
+    def step():
+        qn = torch.empty((3, HQ, D), dtype=torch.bfloat16, device="cuda")
+        out, oc = torch.empty_like(q), torch.empty_like(qc)
+        A.qkv_rope_append_fp8(qkv, bias, pos, appended, inv, conc, cache, qn)
+        A.kv_quantize_fp8(src, three, cache, moved)
+        A.decode_fp8(q, *seqs.tables(), 700, 0, SCALE, sinks, out, ws)
+        A.prefill_fp8(qc, qi, n, *seqs.tables(), 0, SCALE, sinks, oc, 700)
+        return (qn, out, oc, *A.kv_read_fp8(cache, both))
+
+    def expect():
+        """What the step gives and leaves; then other rows in the places that it writes."""
+        want = [t.clone() for t in step()], cache.clone()
+        A.kv_quantize_fp8(draw(1, 2, HKV, PAGE, D), six, cache, both)
+        assert not torch.equal(cache, want[1])
+        return want
+
+    def same(got, want):
+        for a, b in zip(got, want[0]):
+            assert torch.equal(a, b)
+        assert torch.equal(cache, want[1])
+
+    want = expect()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    same(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(4):
+        qkv.copy_(draw(*qkv.shape))
+        src.copy_(draw(*src.shape))
+        q.mul_(-1.0)
+        want = expect()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        same(held, want)
+    assert int(ws[:2 << 20].count_nonzero()) == 0
