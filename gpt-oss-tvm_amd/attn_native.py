@@ -469,8 +469,9 @@ def prefill_fp8(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, kv_cach
                 page_indptr: torch.Tensor, page_indices: torch.Tensor, kv_len: torch.Tensor,
                 window: int, sm_scale: float, sinks: torch.Tensor, out: torch.Tensor,
                 max_kv_len: int = 0) -> torch.Tensor:
-    """``prefill`` over the 8-bit cache (the formula of ``decode_fp8``): causal attention of
-    each sequence's new tokens over its cached ones.  ``max_kv_len`` as there."""
+    """``prefill`` over the 8-bit cache (the formula of ``decode_fp8``; in calls of more than a
+    few tokens a sequence the probabilities are rounded to bf16): causal attention of each
+    sequence's new tokens over its cached ones.  ``max_kv_len`` as there."""
     pages, dev, stream = _need_fp8(kv_cache)
     n, batch = _count(q, "q", _BF16), _count(q_indptr, "q_indptr", _I32T) - 1
     _need(q_indptr, "q_indptr", _I32T, (batch + 1,), dev)

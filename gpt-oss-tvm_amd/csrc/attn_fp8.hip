@@ -14,8 +14,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Rows of a bf16 cache (by slot) quantised into the 8-bit cache, and rows read back.
 // Bound by their bytes.  A wave takes four tokens' runs; lane (k or v, head, quarter of
 // 16 dims).  A wave a token, v's codes moved byte by byte, had 49 us for 40960 rows read
-// where runs have 23.6 (5.4 TB/s), and 5.4 us for 1000 where they have 5.6.  40960 rows
-// are quantised in 31 us (4.1 TB/s).
+// where runs have 23.6, and 5.4 us for 1000 where they have 5.6.  40960 rows are
+// quantised in 31 us (4.1 TB/s).  (The 23.6 us, 5.4 TB/s, are of passes over three caches of
+// 43 MB into one output of 84 MB, which the last-level cache holds between them; a copy
+// of 2 GB reaches 4.95.)
 
 template <int kRun>
 __device__ __forceinline__ void quantize_run(const uint8_t* __restrict__ src, int src_pages,
@@ -792,18 +794,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void f
 //  * p enters as one bf16 rounding, and the sum takes the rounded p (v_dot2): a
 //    weight is off by at most half a bf16 step, as the output's own rounding is,
 //    and where few keys matter the two cancel.  (The cached values' own half step is
-//    sixteen times as large.)  Errors against 64 bits 0.0020 to 0.0021; in two pieces, as decode has
-//    p, 0.0017, for half as many products again and 40 more vector instructions a
-//    tile: 4096 tokens 223 us instead of 151, 300 over 6000 72 instead of 55.
+//    sixteen times as large.)  Errors against 64 bits are 0.0020 to 0.0021; in two
+//    pieces, as decode has p, 0.0017, for half as many products again and 40 more
+//    vector instructions a tile: 4096 tokens 223 us instead of 151, 300 over 6000 72
+//    instead of 55.
 //  * No row maximum: the softmax's reference point m is the maximum of the
 //    first keys a column sees, and stays.  Larger scores only make p larger than
 //    1, which fp32 and bf16 carry; a wave takes new maxima, rescales and computes its
 //    p anew only when some column's sum over a tile passes 2^24 (or m is not set:
 //    -m = inf gives an infinite or NaN sum).
-//  * 128 registers, so that four waves share a SIMD: a wave alone issues a vector
-//    instruction every 8 cycles, and one's matrix products run under the others'
-//    exponentials.  (64 columns a wave, two waves, with the products of one tile and the
-//    exponentials of the next interleaved by hand: the same time at 4096 tokens.)
+//  * 128 registers (the form in halves spills one), so that four waves share a SIMD: a
+//    wave alone issues a vector instruction every 8 cycles, and one's matrix products can
+//    run under the others' exponentials.  They do so little: at 4096 tokens the matrix
+//    cores are busy 36% of the time and the vector units 55%.  (64 columns a wave,
+//    two waves, with the products of one tile and the exponentials of the next
+//    interleaved by hand: the same time.)
 // The next block's codes are loaded to registers during a block's products, then
 // converted once for all waves, k with its scale, v with its keys', into LDS (bf16,
 // rows of 128 bytes whose 16-byte units are XORed with the row's bits 1 .. 3, so
