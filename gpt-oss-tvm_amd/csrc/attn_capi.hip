@@ -61,6 +61,22 @@ int attn_launch_fp8_chunk(const void* q, const int* q_indptr, int batch, int max
                           int num_pages, const int* kv_len, int window, float sm_scale,
                           const void* sinks, void* out, int tokens, int splits, int halves,
                           int rows, float* part_o, float* part_ml, hipStream_t s);
+int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_len,
+                     const void* mask, int words, const int* positions, const void* cache,
+                     bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
+                     const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
+                     hipStream_t s);
+int attn_launch_tree_commit(void* cache, int layers, int num_pages, bool fp8,
+                            const int* page_indptr, const int* page_indices, const int* kv_len,
+                            const int* q_indptr, int batch, int rows, int max_q_len,
+                            const int* tokens, const int* parents, const int* chosen, int* path,
+                            int* count, int* next, hipStream_t s);
+int attn_launch_copy_pages(void* cache, int layers, int num_pages, int page_bytes, const int* src,
+                           const int* dst, int n, hipStream_t s);
+size_t attn_beam_state_bytes(int rows, int vocab, int k);
+int attn_launch_beam(const void* logits, bool f32, const float* scores, int batch, int width,
+                     int vocab, int k, float* out_scores, int* out_beams, int* out_tokens,
+                     void* state, hipStream_t s);
 }
 
 namespace {
@@ -572,6 +588,156 @@ int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, i
       (int)chunk.halves, (int)part_rows, part_o,
       need ? part_o + chunk.splits * part_rows * kQHeads * kHeadDim : nullptr,
       as_stream(stream)));
+}
+
+// ---------------------------------------------------------------------------
+// Several continuations of a sequence: trees of drafted tokens, beams
+
+namespace {
+constexpr int64_t kTreeNodes = 1024;  // of a sequence
+constexpr int64_t kBeams = 64;        // of a request, and continuations of one that are chosen
+constexpr int64_t kMaxBatch = 65535, kMaxLayers = 65535;
+
+int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
+         int64_t max_q_len, const int32_t* tree_mask, int64_t mask_words, const int32_t* positions,
+         const void* kv_cache, int64_t num_pages, const int32_t* page_indptr,
+         const int32_t* page_indices, const int32_t* kv_len, int64_t max_kv_len, int32_t window,
+         float sm_scale, const uint16_t* sinks, uint16_t* out, void* workspace,
+         size_t workspace_bytes, bool fp8, moe_stream_t stream) {
+  if (rows < 0 || rows > kMaxTokens || batch < 0 || batch > kMaxBatch || max_q_len < 0 ||
+      max_q_len > kTreeNodes || num_pages <= 0 || num_pages >= kMaxPages || max_kv_len < 0)
+    return MOE_ERR_SHAPE;
+  if (rows == 0 || batch == 0 || max_q_len == 0) return MOE_OK;
+  if (mask_words < (max_q_len + 31) / 32 || mask_words > kTreeNodes / 32) return MOE_ERR_SHAPE;
+  if (!(sm_scale > 0.0f && sm_scale <= FLT_MAX)) return MOE_ERR_UNSUPPORTED;
+  if (!q || !q_indptr || !tree_mask || !positions || !kv_cache || !page_indptr || !page_indices ||
+      !kv_len || !sinks || !out)
+    return MOE_ERR_NULL;
+  if (!a16(q) || !a16(kv_cache) || !a16(out) || !a4(q_indptr) || !a4(tree_mask) ||
+      !a4(positions) || !a4(page_indptr) || !a4(page_indices) || !a4(kv_len) ||
+      ((uintptr_t)sinks & 1u))
+    return MOE_ERR_ALIGN;
+  const size_t need = attn_tree_workspace_bytes(batch, max_q_len, max_kv_len, window);
+  if (need && !workspace) return MOE_ERR_NULL;
+  if (need && !a16(workspace)) return MOE_ERR_ALIGN;
+  if (workspace_bytes < need) return MOE_ERR_WORKSPACE;
+  return status(attn_launch_tree(q, q_indptr, (int)batch, (int)max_q_len, tree_mask,
+                                 (int)mask_words, positions, kv_cache, fp8, page_indptr,
+                                 page_indices, (int)num_pages, kv_len, window, sm_scale, sinks, out,
+                                 as_stream(stream)));
+}
+
+int tree_commit(void* kv_cache, int64_t layers, int64_t num_pages, const int32_t* page_indptr,
+                const int32_t* page_indices, const int32_t* kv_len, const int32_t* q_indptr,
+                int64_t batch, int64_t rows, int64_t max_q_len, const int32_t* tokens,
+                const int32_t* parents, const int32_t* chosen, int32_t* path, int32_t* count,
+                int32_t* next, bool fp8, moe_stream_t stream) {
+  if (layers <= 0 || layers > kMaxLayers || num_pages <= 0 || num_pages >= kMaxPages || batch < 0 ||
+      batch > kMaxBatch || rows < 0 || rows > kMaxTokens || max_q_len < 0 ||
+      max_q_len > kTreeNodes)
+    return MOE_ERR_SHAPE;
+  if (batch == 0) return MOE_OK;
+  if (!kv_cache || !page_indptr || !page_indices || !kv_len || !q_indptr || !count || !next ||
+      (rows > 0 && (!tokens || !parents || !chosen || !path)))
+    return MOE_ERR_NULL;
+  if (!a16(kv_cache) || !a4(page_indptr) || !a4(page_indices) || !a4(kv_len) || !a4(q_indptr) ||
+      !a4(tokens) || !a4(parents) || !a4(chosen) || !a4(path) || !a4(count) || !a4(next))
+    return MOE_ERR_ALIGN;
+  return status(attn_launch_tree_commit(kv_cache, (int)layers, (int)num_pages, fp8, page_indptr,
+                                        page_indices, kv_len, q_indptr, (int)batch, (int)rows,
+                                        (int)max_q_len, tokens, parents, chosen, path, count, next,
+                                        as_stream(stream)));
+}
+}  // namespace
+
+size_t attn_tree_workspace_bytes(int64_t batch, int64_t max_q_len, int64_t max_kv_len,
+                                 int32_t window) {
+  return 0;
+}
+
+int attn_tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
+              int64_t max_q_len, const int32_t* tree_mask, int64_t mask_words,
+              const int32_t* positions, const void* kv_cache, int64_t num_pages,
+              const int32_t* page_indptr, const int32_t* page_indices, const int32_t* kv_len,
+              int64_t max_kv_len, int32_t window, float sm_scale, const uint16_t* sinks,
+              uint16_t* out, void* workspace, size_t workspace_bytes, moe_stream_t stream) {
+  return tree(q, rows, q_indptr, batch, max_q_len, tree_mask, mask_words, positions, kv_cache,
+              num_pages, page_indptr, page_indices, kv_len, max_kv_len, window, sm_scale, sinks,
+              out, workspace, workspace_bytes, false, stream);
+}
+
+int attn_tree_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
+                  int64_t max_q_len, const int32_t* tree_mask, int64_t mask_words,
+                  const int32_t* positions, const void* kv_cache, int64_t num_pages,
+                  const int32_t* page_indptr, const int32_t* page_indices, const int32_t* kv_len,
+                  int64_t max_kv_len, int32_t window, float sm_scale, const uint16_t* sinks,
+                  uint16_t* out, void* workspace, size_t workspace_bytes, moe_stream_t stream) {
+  return tree(q, rows, q_indptr, batch, max_q_len, tree_mask, mask_words, positions, kv_cache,
+              num_pages, page_indptr, page_indices, kv_len, max_kv_len, window, sm_scale, sinks,
+              out, workspace, workspace_bytes, true, stream);
+}
+
+int attn_tree_commit(void* kv_cache, int64_t layers, int64_t num_pages, const int32_t* page_indptr,
+                     const int32_t* page_indices, const int32_t* kv_len, const int32_t* q_indptr,
+                     int64_t batch, int64_t rows, int64_t max_q_len, const int32_t* tokens,
+                     const int32_t* parents, const int32_t* chosen, int32_t* path, int32_t* count,
+                     int32_t* next, moe_stream_t stream) {
+  return tree_commit(kv_cache, layers, num_pages, page_indptr, page_indices, kv_len, q_indptr,
+                     batch, rows, max_q_len, tokens, parents, chosen, path, count, next, false,
+                     stream);
+}
+
+int attn_tree_commit_fp8(void* kv_cache, int64_t layers, int64_t num_pages,
+                         const int32_t* page_indptr, const int32_t* page_indices,
+                         const int32_t* kv_len, const int32_t* q_indptr, int64_t batch,
+                         int64_t rows, int64_t max_q_len, const int32_t* tokens,
+                         const int32_t* parents, const int32_t* chosen, int32_t* path,
+                         int32_t* count, int32_t* next, moe_stream_t stream) {
+  return tree_commit(kv_cache, layers, num_pages, page_indptr, page_indices, kv_len, q_indptr,
+                     batch, rows, max_q_len, tokens, parents, chosen, path, count, next, true,
+                     stream);
+}
+
+int attn_kv_copy_pages(void* kv_cache, int64_t layers, int64_t num_pages, int64_t page_bytes,
+                       const int32_t* src_pages, const int32_t* dst_pages, int64_t n,
+                       moe_stream_t stream) {
+  if (layers <= 0 || layers > kMaxLayers || num_pages <= 0 || num_pages >= kMaxPages ||
+      page_bytes <= 0 || page_bytes % 16 || page_bytes > (1 << 20) || n < 0 || n > kMaxTokens)
+    return MOE_ERR_SHAPE;
+  if (n == 0) return MOE_OK;
+  if (!kv_cache || !src_pages || !dst_pages) return MOE_ERR_NULL;
+  if (!a16(kv_cache) || !a4(src_pages) || !a4(dst_pages)) return MOE_ERR_ALIGN;
+  return status(attn_launch_copy_pages(kv_cache, (int)layers, (int)num_pages, (int)page_bytes,
+                                       src_pages, dst_pages, (int)n, as_stream(stream)));
+}
+
+size_t attn_beam_workspace_bytes(int64_t batch, int64_t width, int64_t vocab, int64_t k) {
+  if (batch <= 0 || batch > kMaxBatch || width <= 0 || width > kBeams || vocab <= 0 ||
+      vocab >= ((int64_t)1 << 30) || k <= 0 || k > kBeams || k > width * vocab)
+    return 0;
+  return attn_beam_state_bytes((int)(batch * width), (int)vocab, (int)k);
+}
+
+int attn_beam_top_k(const void* logits, int32_t logits_f32, int64_t batch, int64_t width,
+                    int64_t vocab, const float* scores, int64_t k, float* out_scores,
+                    int32_t* out_beams, int32_t* out_tokens, void* workspace,
+                    size_t workspace_bytes, moe_stream_t stream) {
+  if (batch < 0 || batch > kMaxBatch || width <= 0 || vocab <= 0 || vocab >= ((int64_t)1 << 30) ||
+      k <= 0)
+    return MOE_ERR_SHAPE;
+  if (width > kBeams || k > kBeams) return MOE_ERR_UNSUPPORTED;
+  if (k > width * vocab) return MOE_ERR_SHAPE;
+  if (batch == 0) return MOE_OK;
+  if (!logits || !scores || !out_scores || !out_beams || !out_tokens || !workspace)
+    return MOE_ERR_NULL;
+  if (!a16(logits) || !a4(scores) || !a4(out_scores) || !a4(out_beams) || !a4(out_tokens) ||
+      !a16(workspace))
+    return MOE_ERR_ALIGN;
+  if (workspace_bytes < attn_beam_workspace_bytes(batch, width, vocab, k))
+    return MOE_ERR_WORKSPACE;
+  return status(attn_launch_beam(logits, logits_f32 != 0, scores, (int)batch, (int)width,
+                                 (int)vocab, (int)k, out_scores, out_beams, out_tokens, workspace,
+                                 as_stream(stream)));
 }
 
 }  // extern "C"

@@ -256,6 +256,93 @@ MOE_API int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_i
                              const uint16_t* sinks, uint16_t* out, void* workspace,
                              size_t workspace_bytes, moe_stream_t stream);
 
+/* ---- Trees of drafted tokens ------------------------------------------------------
+ * A draft of several continuations of a sequence, verified in one forward.  Node 0 is the
+ * last token that was sampled; every other node comes after its parent.  The sequence's
+ * nodes are appended as a chunk's tokens are: node i at index kv_len[b] - q_len + i of its
+ * pages (q_len = q_indptr[b + 1] - q_indptr[b] nodes, kv_len counting them), q, k and v rotated
+ * at its position, the cached tokens' number plus its depth. */
+
+/* attn_prefill with a tree's mask.  tree_mask [rows][mask_words]: bit j % 32 of word j / 32 of a
+ * row: it sees node j of its sequence (any mask; of a tree: the node and its ancestors; bits
+ * past q_len are not looked at).  Every row sees the cached keys; with a window > 0 only
+ * keys of positions above its own minus the window, a node's position being positions[row] (one
+ * before the cached tokens' end counts as their end).  out = sum_j p_j v_j / (sum_j p_j +
+ * exp(sinks[h])), p_j = exp(sm_scale q . k_j), with one rounding to bf16 as attn_decode_fp8 has it
+ * (attn_decode and attn_prefill round o, the sink's factor and their product); a row that
+ * sees no key gets 0.  Keys that a row does not see do not affect it, whatever they
+ * hold; infinities and NaN in those that it sees go where the formula takes them (8-bit cache:
+ * their rows stand for NaN).  Rows outside q_indptr's ranges are left as they are.
+ * max_q_len bounds every q_len: at most 1024, and 32 mask_words.  max_kv_len bounds kv_len;
+ * it only chooses how the keys are shared out over workgroups (0: unknown, not shared
+ * out), so last bits may change with it and with the other sequences of the call.  The
+ * workspace (none where attn_tree_workspace_bytes is 0) needs no initialisation; calls on
+ * one have to follow one another.  sm_scale > 0. */
+MOE_API size_t attn_tree_workspace_bytes(int64_t batch, int64_t max_q_len, int64_t max_kv_len,
+                                         int32_t window);
+MOE_API int attn_tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
+                      int64_t max_q_len, const int32_t* tree_mask, int64_t mask_words,
+                      const int32_t* positions, const void* kv_cache, int64_t num_pages,
+                      const int32_t* page_indptr, const int32_t* page_indices,
+                      const int32_t* kv_len, int64_t max_kv_len, int32_t window, float sm_scale,
+                      const uint16_t* sinks, uint16_t* out, void* workspace,
+                      size_t workspace_bytes, moe_stream_t stream);
+/* The same over the 8-bit cache. */
+MOE_API int attn_tree_fp8(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
+                          int64_t max_q_len, const int32_t* tree_mask, int64_t mask_words,
+                          const int32_t* positions, const void* kv_cache, int64_t num_pages,
+                          const int32_t* page_indptr, const int32_t* page_indices,
+                          const int32_t* kv_len, int64_t max_kv_len, int32_t window,
+                          float sm_scale, const uint16_t* sinks, uint16_t* out, void* workspace,
+                          size_t workspace_bytes, moe_stream_t stream);
+
+/* After verification.  tokens, parents (within the sequence's tree, -1 for node 0) and chosen
+ * (the token that the model takes after a node) [rows], rows as in q_indptr, which starts at 0.
+ * The walk of a sequence goes from node 0 to the child of the node at hand whose token is the
+ * chosen one (the lowest of several), until there is none.  count[b]: nodes on the path
+ * (0 for a sequence without nodes); path[q_indptr[b] + i]: its i-th node, -1 from count[b] on
+ * and in rows past q_indptr[batch]; next[b]: the token chosen after the last of them (-1
+ * without nodes).  The rows of k and v of the path's i-th node move to index kv_len[b] - q_len
+ * + i, in each of `layers` caches that lie one after the other, [layers][num_pages] pages.
+ * A sequence's last q_len tokens must lie on pages of its own. */
+MOE_API int attn_tree_commit(void* kv_cache, int64_t layers, int64_t num_pages,
+                             const int32_t* page_indptr, const int32_t* page_indices,
+                             const int32_t* kv_len, const int32_t* q_indptr, int64_t batch,
+                             int64_t rows, int64_t max_q_len, const int32_t* tokens,
+                             const int32_t* parents, const int32_t* chosen, int32_t* path,
+                             int32_t* count, int32_t* next, moe_stream_t stream);
+MOE_API int attn_tree_commit_fp8(void* kv_cache, int64_t layers, int64_t num_pages,
+                                 const int32_t* page_indptr, const int32_t* page_indices,
+                                 const int32_t* kv_len, const int32_t* q_indptr, int64_t batch,
+                                 int64_t rows, int64_t max_q_len, const int32_t* tokens,
+                                 const int32_t* parents, const int32_t* chosen, int32_t* path,
+                                 int32_t* count, int32_t* next, moe_stream_t stream);
+
+/* ---- Beams -------------------------------------------------------------------------
+ * Pages src_pages[i] -> dst_pages[i], i < n, in each of `layers` caches that lie one after the
+ * other (page_bytes: 32768, or ATTN_FP8_PAGE_BYTES): what a sequence that shares its pages
+ * with others writes to next.  A source may be named more than once; destinations have to
+ * differ, from one another and from the sources.  Where either id lies outside the pool
+ * nothing is written. */
+MOE_API int attn_kv_copy_pages(void* kv_cache, int64_t layers, int64_t num_pages,
+                               int64_t page_bytes, const int32_t* src_pages,
+                               const int32_t* dst_pages, int64_t n, moe_stream_t stream);
+
+/* The k best continuations of each request over its beams and the vocabulary: logits [batch,
+ * width, vocab] bf16, or fp32 where logits_f32 is not 0; scores [batch, width] fp32, the beams'
+ * own (-inf: a beam that has ended, or is not there yet).  The score of token t after beam b is
+ * scores[b] + logits[b][t] - log sum exp(logits[b]), summed and compared in fp64 and rounded once
+ * to fp32; a row of logits without a maximum (a NaN, +inf, nothing but -inf) and a score of
+ * NaN give -inf.  In descending order, equal ones by beam, then token: out_scores, out_beams (0
+ * .. width - 1 within the request) and out_tokens [batch, k].  width and k up to 64, k at
+ * most width * vocab.  The workspace needs no initialisation; calls on one have to follow
+ * one another. */
+MOE_API size_t attn_beam_workspace_bytes(int64_t batch, int64_t width, int64_t vocab, int64_t k);
+MOE_API int attn_beam_top_k(const void* logits, int32_t logits_f32, int64_t batch, int64_t width,
+                            int64_t vocab, const float* scores, int64_t k, float* out_scores,
+                            int32_t* out_beams, int32_t* out_tokens, void* workspace,
+                            size_t workspace_bytes, moe_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

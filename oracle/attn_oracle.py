@@ -275,6 +275,52 @@ def attention_sink(q: np.ndarray, k: np.ndarray, v: np.ndarray, q_pos: np.ndarra
     return out, mag, size
 
 
+def attention_seen(q: np.ndarray, k: np.ndarray, v: np.ndarray, seen: np.ndarray,
+                   sinks: np.ndarray, sm_scale: float = 0.125):
+    """``attention_sink`` with any mask: seen [n, L] bool, row i sees key j.  Keys that no row
+    sees may hold anything; a row that sees none gets 0."""
+    out, mag, size = (np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:2]))
+    for i in range(q.shape[0]):
+        kk, vv = k[seen[i]], v[seen[i]]
+        if not len(kk):
+            continue
+        for h in range(N_KV_HEADS):
+            rows = slice(8 * h, 8 * h + 8)
+            s = q[i, rows] @ kk[:, h].T * sm_scale
+            top = np.maximum(s.max(axis=1), sinks[rows])
+            w = np.exp(s - top[:, None])
+            den = w.sum(axis=1) + np.exp(sinks[rows] - top)
+            out[i, rows] = w @ vv[:, h] / den[:, None]
+            mag[i, rows] = w @ np.abs(vv[:, h]) / den[:, None]
+            size[i, rows] = (np.abs(q[i, rows]) @ np.abs(kk[:, h]).T).max(axis=1) * sm_scale
+    return out, mag, size
+
+
+def tree_walk(tokens, parents, chosen) -> list:
+    """The nodes of a tree from node 0 on along the chosen tokens (the lowest child of several)."""
+    path = [0] if len(tokens) else []
+    while path:
+        after = [j for j in range(path[-1] + 1, len(tokens))
+                 if parents[j] == path[-1] and tokens[j] == chosen[path[-1]]]
+        if not after:
+            break
+        path.append(after[0])
+    return path
+
+
+def beam_top_k(logits: np.ndarray, scores: np.ndarray, k: int):
+    """logits [width, vocab], scores [width] -> (scores fp64, beams, tokens) of the k best
+    continuations: by score in fp64, then beam, then token."""
+    x = logits.astype(np.float64)
+    with np.errstate(all="ignore"):
+        top = x.max(axis=1, keepdims=True)
+        s = scores.astype(np.float64)[:, None] + (
+            (x - top) - np.log(np.exp(x - top).sum(axis=1, keepdims=True)))
+    s = np.where(np.isnan(s), -np.inf, s).ravel()
+    order = np.argsort(-s, kind="stable")[:k]
+    return s[order], order // x.shape[1], order % x.shape[1]
+
+
 def split_qkv(qkv_bf16: np.ndarray, hq: int = N_Q_HEADS, hkv: int = N_KV_HEADS, d: int = HEAD_DIM):
     """attention.py:206-210: [n, (Hq + 2 Hkv) D] -> q [n, Hq, D], k, v [n, Hkv, D]."""
     x = qkv_bf16.reshape(qkv_bf16.shape[0], hq + 2 * hkv, d)
