@@ -65,6 +65,7 @@ int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_le
                      const void* mask, int words, const int* positions, const void* cache,
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
                      const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
+                     int tokens, int splits, int least, float* part_o, float* part_ml,
                      hipStream_t s);
 int attn_launch_tree_commit(void* cache, int layers, int num_pages, bool fp8,
                             const int* page_indptr, const int* page_indices, const int* kv_len,
@@ -598,6 +599,23 @@ constexpr int64_t kTreeNodes = 1024;  // of a sequence
 constexpr int64_t kBeams = 64;        // of a request, and continuations of one that are chosen
 constexpr int64_t kMaxBatch = 65535, kMaxLayers = 65535;
 
+// Tokens of a tree's tile, and how many splits its keys are shared out over: as many as let its
+// workgroups fit the chip at once (two a CU), each of kTreeLeast blocks or more.
+constexpr int64_t kTreeLeast = 4, kTreeWgs = 512, kTreeMaxSplits = 64;
+struct TreePlan {
+  int64_t tokens, tiles, splits;
+};
+TreePlan tree_plan(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
+  const int64_t tokens = max_q_len <= 4 ? 4 : max_q_len <= 8 ? 8 : max_q_len <= 16 ? 16 : 32;
+  const int64_t tiles = (max_q_len + tokens - 1) / tokens;
+  max_kv_len = std::min(max_kv_len, kMaxPages * kPage);  // (and no overflow below)
+  const int64_t keys = window > 0 ? std::min(max_kv_len, window + max_q_len) : max_kv_len;
+  if (keys <= 0) return TreePlan{tokens, tiles, 1};
+  const int64_t most = std::min(kTreeMaxSplits, kTreeWgs / (tiles * batch * kKvHeads));
+  return TreePlan{tokens, tiles,
+                  std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kTreeLeast))};
+}
+
 int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
          int64_t max_q_len, const int32_t* tree_mask, int64_t mask_words, const int32_t* positions,
          const void* kv_cache, int64_t num_pages, const int32_t* page_indptr,
@@ -621,9 +639,14 @@ int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch
   if (need && !workspace) return MOE_ERR_NULL;
   if (need && !a16(workspace)) return MOE_ERR_ALIGN;
   if (workspace_bytes < need) return MOE_ERR_WORKSPACE;
+  const TreePlan plan = tree_plan(batch, max_q_len, max_kv_len, window);
+  float* part_o = (float*)workspace;
+  const int64_t parts = plan.splits * plan.tokens * plan.tiles * batch;
   return status(attn_launch_tree(q, q_indptr, (int)batch, (int)max_q_len, tree_mask,
                                  (int)mask_words, positions, kv_cache, fp8, page_indptr,
                                  page_indices, (int)num_pages, kv_len, window, sm_scale, sinks, out,
+                                 (int)plan.tokens, (int)plan.splits, (int)kTreeLeast, part_o,
+                                 need ? part_o + parts * kQHeads * kHeadDim : nullptr,
                                  as_stream(stream)));
 }
 
@@ -652,7 +675,11 @@ int tree_commit(void* kv_cache, int64_t layers, int64_t num_pages, const int32_t
 
 size_t attn_tree_workspace_bytes(int64_t batch, int64_t max_q_len, int64_t max_kv_len,
                                  int32_t window) {
-  return 0;
+  if (batch <= 0 || batch > kMaxBatch || max_q_len <= 0 || max_q_len > kTreeNodes) return 0;
+  const TreePlan plan = tree_plan(batch, max_q_len, max_kv_len, window);
+  if (plan.splits <= 1) return 0;
+  return (size_t)(plan.splits * plan.tokens * plan.tiles * batch * kQHeads * (kHeadDim + 2)) *
+         sizeof(float);
 }
 
 int attn_tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,

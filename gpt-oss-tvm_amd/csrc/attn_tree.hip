@@ -3,14 +3,24 @@
 // A sequence of c cached tokens holds its tree's node i at index c + i of its pages; node i sees
 // the cached keys (those of the window, where there is one) and the nodes that its mask has:
 //   out = sum_j p_j v_j / (sum_j p_j + exp(sink)),  p_j = exp(sm_scale q . k_j)
-// rounded to bf16 once; a node that sees no key gets 0.
+// rounded to bf16 once; a node that sees no key gets 0.  Scores, sums and outputs in fp32,
+// exponents in units of log2.
+#include <type_traits>
+
 #include "attn_common.h"
 
 namespace attn {
 
-constexpr int kHeadBytes = kPage * kD * 2;           // of a bf16 page's k or v of one head
+constexpr int kHeadBytes = kPage * kD * 2;  // of a bf16 page's k or v of one head
 constexpr int kBfPage = 2 * kHkv * kHeadBytes;
 constexpr float kTreeLog2e = 1.4426950408889634f;
+constexpr float kTreeMost = 16777216.0f;    // 2^24
+constexpr int kTreeBlock = 64;              // keys
+constexpr int kTreeHalf = kTreeBlock * kD * 2;  // bytes of a block's k or v in LDS
+
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+typedef __attribute__((__vector_size__(4 * sizeof(short)))) short s16x4;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
 struct TreeArgs {
   const uint16_t* q;
@@ -23,99 +33,524 @@ struct TreeArgs {
   const int* kv_len;
   const uint16_t* sinks;
   uint16_t* out;
-  int words, num_pages, window;
-  float c2;  // sm_scale log2(e)
+  float* part_o;   // [splits][tiles' tokens][64][64]
+  float* part_ml;  // [splits][tiles' tokens][64][2]
+  int words, num_pages, window, tiles, splits, least, rows;
+  float c2;        // sm_scale log2(e)
 };
 
-// One token and kv head a workgroup, 32 threads a head: a thread a key of 32 for the scores,
-// two dimensions for the output.
-template <bool kFp8>
-__global__ __launch_bounds__(256) void tree_kernel(TreeArgs a) {
-  const int b = blockIdx.y, node = blockIdx.x / kHkv, hk = blockIdx.x % kHkv;
-  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
-  if (node >= qn) return;
-  const int row = qb + node, L = a.kv_len[b], cached = L - qn;
-  const int t = threadIdx.x, h = t >> 5, i = t & 31, head = hk * kGroup + h;
+__device__ __forceinline__ f32x16 tree_mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// The blocks of 64 keys that a sequence's nodes look at, and how they are shared out: over
+// as many splits as have `least` blocks, at most `most`.  It follows from the keys and not
+// from the caller's bound on them, which only trims the grid.
+struct TreeSpan {
+  int first, blocks;  // first block, number of blocks
+  int each, used;     // blocks of a split, splits with any
+  __device__ __forceinline__ TreeSpan(int cached, int total, int window, int most, int least) {
+    // positions are at or past the cached tokens' end
+    const int lo = window > 0 ? max(0, cached - window + 1) : 0;
+    first = lo / kTreeBlock;
+    blocks = total > lo ? (total - 1) / kTreeBlock - first + 1 : 0;
+    const int n = min(most, (blocks + least - 1) / least);
+    each = n > 0 ? (blocks + n - 1) / n : 0;
+    used = each > 0 ? (blocks + each - 1) / each : 0;
+  }
+};
+
+// o over the sum and the sink's share, at the reference point m (log2).  l is 0 only where no
+// key was seen (or none with a score above -inf).
+__device__ __forceinline__ float tree_share(float l, float m, uint16_t sink) {
+  return l == 0.0f ? 0.0f
+                   : 1.0f / (l + __builtin_amdgcn_exp2f(fmaf(bf2f(sink), kTreeLog2e, -m)));
+}
+// The weight of a partial state at the reference point `top`; one that saw no key: m = -inf, l = 0.
+__device__ __forceinline__ float tree_weight(float m, float l, float top) {
+  return m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// A tile of 4 kC tokens x the 8 heads of a kv head, a wave 4 tokens (32 columns); kK groups of kC
+// waves take every kK-th block of 64 keys.  A group stages its blocks through LDS as bf16, k in
+// rows of 128 bytes whose 16-byte units are XORed with the row's bits 1 .. 3; v of a bf16 cache
+// in rows too, read through the transposing LDS load, v of the 8-bit cache as the rows of
+// V^T, whose operand order its pages have.
+//  * S^T = K Q^T: lane (column l % 32, half h = l / 32) has the keys 8 (i / 4) + 4 h + i % 4 of a
+//    32-key tile in elements i = 0 .. 15, which are, packed to bf16, the operands of two
+//    products O^T += V^T P^T over 16 keys each.
+//  * p enters as one bf16 rounding, and the sum takes the rounded p: a weight is off by at most
+//    half a bf16 step, as the output's own rounding is.
+//  * No running maximum: the reference point is the maximum of the first keys that a column
+//    sees, and is renewed only when a tile's sum passes 2^24.
+//  * Blocks that every token of a wave sees whole take no mask; in the others (the tree's own, a
+//    window's edge) a lane has its token's 32 bits of a tile.
+template <bool kFp8, int kC, int kK>
+__global__ __launch_bounds__(64 * kC * kK)
+__attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs a) {
+  constexpr int kBufs = kC == 1 ? 1 : 2;        // one wave needs no second buffer
+  constexpr int kUnits = (kFp8 ? 8 : 16) / kC;  // 1 KB loads of a block that a wave makes
+  __shared__ __align__(16) uint8_t lds[kK][kBufs][2][kTreeHalf];
+  // x: (sequence, tile, kv head), y: split
+  const int hk = blockIdx.x % kHkv, share = blockIdx.y;
+  const int b = blockIdx.x / kHkv / a.tiles, tile = blockIdx.x / kHkv % a.tiles;
+  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb, t0 = tile * 4 * kC;
+  if (t0 >= qn) return;
+  const int nt = min(4 * kC, qn - t0), row0 = qb + t0;
   const PageList pages{a.page_indices + a.page_indptr[b],
                        a.page_indptr[b + 1] - a.page_indptr[b], a.num_pages};
-  const int pos = max(a.positions[row], cached);
-  const int lo = a.window > 0 ? pos - a.window + 1 : 0;  // the first position that is seen
-  const uint16_t* const q = a.q + ((size_t)row * kHq + head) * kD;
-  auto seen = [&](int key) {
-    if (key < 0 || key >= L || pages.count <= 0) return false;
-    if (key < cached) return key >= lo;
-    const int j = key - cached;
-    return (a.mask[(size_t)row * a.words + (j >> 5)] >> (j & 31) & 1) != 0 &&
-           max(a.positions[qb + j], cached) >= lo;
+  const int L = pages.count > 0 ? a.kv_len[b] : 0, cached = max(L - qn, 0);
+  const TreeSpan span(cached, L, a.window, a.splits, a.least);
+  if (share >= max(span.used, 1)) return;
+  const int t = threadIdx.x, lane = t & 63, c = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), cw = wave % kC, kg = wave / kC;
+  const bool active = 4 * cw < nt;
+  const int last_page = max(0, min(pages.count - 1, (L - 1) / kPage));
+  const int begin = span.first + share * span.each;
+  const int end = min(begin + span.each, span.first + span.blocks);
+  const int steps = (end - begin + kK - 1) / kK;  // of every group
+  constexpr int kPageSize = kFp8 ? kFp8Page : kBfPage;
+
+  // Staging.  The group's i-th block is begin + kg + kK i; lane 4 j + p holds its page p for
+  // the j-th of 16 blocks.
+  int ids = 0;
+  auto fetch_ids = [&](int i) {
+    const int page = (begin + kg + kK * (i + (lane >> 2))) * 4 + (lane & 3);
+    ids = pages.clamp(pages.ids[min(page, last_page)]);
   };
-  auto value = [&](const uint8_t* page, int kv, int slot, int d) {
-    if constexpr (kFp8) {
-      const uint32_t s = page[fp8_scale_at(hk, kv, slot)];
-      const uint8_t code =
-          kv ? page[fp8_v_at(hk, slot, d)] : page[hk * kFp8Head + slot * kFp8Row + d];
-      return s == kFp8BadScale ? NAN : moe::e4m3_byte<0>(code) * __uint_as_float(s << 23);
-    } else {
-      return bf2f(((const uint16_t*)(page + (kv * kHkv + hk) * kHeadBytes))[slot * kD + d]);
-    }
+  struct Raw {
+    u32x4 data[kUnits];
+    uint32_t ks[kFp8 ? kUnits : 1], vs[kFp8 ? kUnits : 1];
   };
-  auto page_at = [&](int key) {
-    return a.cache + (size_t)pages.page_of(key) * (kFp8 ? kFp8Page : kBfPage);
-  };
-  float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int k0 = max(min(lo, cached), 0) & ~31; k0 < L; k0 += 32) {
-    const int key = k0 + i;
-    float s = -INFINITY;
-    if (seen(key)) {
-      const uint8_t* page = page_at(key);
-      s = 0.f;
-      for (int d = 0; d < kD; ++d) s = fmaf(bf2f(q[d]), value(page, 0, key % kPage, d), s);
-      s *= a.c2;
-    }
-    float mx = s;
+  // unit u of the wave: load u kC + cw of the block: bf16 [k, v][page][half of its rows], 8-bit
+  // [k, v][page]
+  auto load = [&](Raw& x, int i) __attribute__((always_inline)) {
+    if ((i & 15) == 0 && i > 0) fetch_ids(i);
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, kWave));
-    const float mn = fmaxf(m, mx);
-    const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float p = s == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s - mn);
-    m = mn;
-    l = l * alpha + p;
-    o0 *= alpha;
-    o1 *= alpha;
-    for (int j = 0; j < 32; ++j) {
-      const float pj = __shfl(p, (t & 32) + j, kWave);
-      if (!seen(k0 + j)) continue;
-      const uint8_t* page = page_at(k0 + j);
-      o0 = fmaf(pj, value(page, 1, (k0 + j) % kPage, 2 * i), o0);
-      o1 = fmaf(pj, value(page, 1, (k0 + j) % kPage, 2 * i + 1), o1);
+    for (int u = 0; u < kUnits; ++u) {
+      const int id = u * kC + cw;
+      const int p = kFp8 ? id & 3 : (id >> 1) & 3, kv = kFp8 ? id >> 2 : id >> 3;
+      const uint8_t* page = a.cache + (size_t)(unsigned)__builtin_amdgcn_readlane(
+                                          ids, 4 * (i & 15) + p) * kPageSize;
+      if constexpr (kFp8) {
+        x.data[u] = *(const u32x4*)(page + (kv ? kFp8V : 0) + hk * kFp8Head + lane * 16);
+        const uint8_t* s = page + kFp8Scales + hk * 2 * kPage + (lane >> 4) * 4;
+        if (!kv) x.ks[u] = *(const uint32_t*)s;
+        x.vs[u] = *(const uint32_t*)(s + kPage);
+      } else {
+        x.data[u] = *(const u32x4*)(page + (kv * kHkv + hk) * kHeadBytes + (id & 1) * 1024 +
+                                    lane * 16);
+      }
     }
+  };
+  auto store = [&](Raw& x, uint8_t* kt, uint8_t* vt, int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      const int id = u * kC + cw;
+      const int p = kFp8 ? id & 3 : (id >> 1) & 3, kv = kFp8 ? id >> 2 : id >> 3;
+      if constexpr (!kFp8) {
+        const int key = kPage * p + 8 * (id & 1) + (lane >> 3), part = lane & 7;
+        const int at = kv ? part ^ ((key & 2) << 1) : part ^ ((key >> 1) & 7);
+        *(u32x4*)((kv ? vt : kt) + key * 128 + (at << 4)) = x.data[u];
+      } else if (!kv) {
+        // 16 dims of key lane / 4; a row that must not be used (255) is NaN in k and 0 in v
+        const int byte = 8 * ((lane >> 2) & 3), key = kPage * p + (lane >> 2);
+        const uint32_t sk = (x.ks[u] >> byte) & 255u, sv = (x.vs[u] >> byte) & 255u;
+        const bool bad = max(sk, sv) == kFp8BadScale;
+        const float scale = __uint_as_float(min(sk, kFp8BadScale - 1u) << 23);
+        u32x4 w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = bad ? kFp8NanCodes : x.data[u][j];
+        uint8_t* row = kt + key * 128;
+        const int swz = (key >> 1) & 7, at = 2 * (lane & 3);
+        *(bf16x8*)(row + ((at ^ swz) << 4)) = fp8_to_bf16(w[0], w[1], scale);
+        *(bf16x8*)(row + (((at + 1) ^ swz) << 4)) = fp8_to_bf16(w[2], w[3], scale);
+      } else {
+        // four keys (quad lane / 16 of the page) of the dims r, 16 + r, 32 + r, 48 + r.  A 16-byte
+        // unit of V^T's rows holds two quads: 4 m + h' and 4 m + 2 + h' for the product m of a
+        // 32-key tile and the lanes' half h'.
+        const int quad = 4 * p + (lane >> 4), r = lane & 15, n = quad & 7;
+        const int unit = 4 * (quad >> 3) + 2 * (n >> 2) + (n & 1), part = (n >> 1) & 1;
+        uint32_t keep = ~0u;
+        if (kb + kTreeBlock > L) {  // stale codes past the sequence's end may be NaN
+          const int m = min(max(L - (kb + 4 * quad), 0), 4);
+          keep = m == 4 ? ~0u : (1u << (8 * m)) - 1u;
+        }
+        float s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          s[j] = __uint_as_float(min((x.vs[u] >> (8 * j)) & 255u, kFp8BadScale - 1u) << 23);
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) {
+          const uint32_t w = x.data[u][dt] & keep;
+          const auto a0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s[0], false);
+          const auto a1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s[1], false);
+          const auto a2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s[2], true);
+          const auto a3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s[3], true);
+          const uint32_t p0 = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, a1),
+                                                    __builtin_bit_cast(uint32_t, a0), 0x07060100u);
+          const uint32_t p1 = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, a3),
+                                                    __builtin_bit_cast(uint32_t, a2), 0x07060100u);
+          const int d = 16 * dt + r;
+          *(uint2*)(vt + d * 128 + ((unit ^ ((d >> 1) & 7)) << 4) + 8 * part) = make_uint2(p0, p1);
+        }
+      }
+    }
+  };
+
+  // whether the group has an i-th block; the first blocks' loads and q are on their way at once
+  auto mine = [&](int i) { return begin + kg + kK * i < end; };
+  Raw raw;
+  if (mine(0)) {
+    fetch_ids(0);
+    load(raw, 0);
   }
+  const int token = min(4 * cw + (c >> 3), nt - 1), row = row0 + token;
+  const uint16_t sink = a.sinks[hk * kGroup + (c & 7)];
+  const int pos = max(a.positions[row], cached);
+  const uint32_t* const bits = a.mask + (size_t)row * a.words;
+  const uint32_t bits0 = bits[0], bits1 = a.words > 1 ? bits[1] : 0u;  // most trees' all
+  bf16x8 qv[4];
+  {
+    const u32x4* src = (const u32x4*)(a.q + ((size_t)row * kHq + hk * kGroup + (c & 7)) * kD);
 #pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) l += __shfl_xor(l, off, kWave);
-  const float f =
-      l == 0.0f ? 0.0f
-                : 1.0f / (l + __builtin_amdgcn_exp2f(fmaf(bf2f(a.sinks[head]), kTreeLog2e, -m)));
-  *(uint32_t*)(a.out + ((size_t)row * kHq + head) * kD + 2 * i) =
-      (uint32_t)f2bf(o0 * f) | ((uint32_t)f2bf(o1 * f) << 16);
+    for (int s = 0; s < 4; ++s) qv[s] = moe::as_bf16x8(src[2 * s + h]);
+  }
+  // the furthest position of the wave's tokens: where a window begins that all of them see
+  int far = max(pos, __shfl_xor(pos, 8, kWave));
+  far = __builtin_amdgcn_readfirstlane(max(far, __shfl_xor(far, 16, kWave)));
+  const int seen_from = a.window > 0 ? far - a.window : -1;  // the last key that not all see
+
+  // The lane's token's bits of the keys k0 .. k0 + 31
+  auto seen = [&](int k0) {
+    auto first_of = [](int n) { return n >= 32 ? ~0u : (1u << max(n, 0)) - 1u; };
+    auto word = [&](int w) {
+      return w == 0 ? bits0 : w == 1 ? bits1 : w < a.words ? bits[w] : 0u;
+    };
+    const int from = k0 - cached;  // the first key's node
+    const int lowest = a.window > 0 ? pos - a.window + 1 : 0;  // position
+    uint32_t nodes = 0u;
+    if (from >= 0) {
+      const int w = from >> 5, s = from & 31;
+      nodes = word(w) >> s;
+      if (s) nodes |= word(w + 1) << (32 - s);
+    } else if (from > -32) {
+      nodes = bits0 << -from;
+    }
+    nodes &= first_of(L - k0);
+    if (lowest > cached) {  // nodes before the window: a window shorter than the tree
+      for (uint32_t left = nodes; left; left &= left - 1u) {
+        const int i = __builtin_ctz(left);
+        if (max(a.positions[qb + from + i], cached) < lowest) nodes &= ~(1u << i);
+      }
+    }
+    return (first_of(cached - k0) & ~first_of(lowest - k0)) | nodes;
+  };
+
+  f32x16 o[2];
+  float mneg = INFINITY, l = 0.f;  // minus the column's reference point (not set: inf)
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+  const moe::bf16x2 ones = {(__bf16)1.0f, (__bf16)1.0f};
+
+  // where the lane reads in a block's tiles: k of its key c, step st at ^ 32 st; v of the 8-bit
+  // cache of its dim c, product m and 32-key tile n at ^ (32 m + 64 n); of a bf16 cache the quarter
+  // i % 4 of 16 dims of key i / 4 of four (i = lane % 16), the upper 32 dims at ^ 64
+  const int k_at = c * 128 + ((h ^ ((c >> 1) & 7)) << 4);
+  const int v_at = kFp8 ? k_at
+                        : (4 * h + ((lane >> 2) & 3)) * 128 + ((lane >> 4) & 1) * 32 +
+                              (lane & 3) * 8 + ((lane >> 3) & 1) * 64;
+  auto tile32 = [&](auto masked, const uint8_t* kt, const uint8_t* vt, int kb, int kt32)
+      __attribute__((always_inline)) {
+    constexpr bool kMasked = decltype(masked)::value;
+    f32x16 s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      const bf16x8 ka = *(const bf16x8*)(kt + 4096 * kt32 + (k_at ^ (32 * st)));
+      s = tree_mfma(ka, qv[st], s);
+    }
+    uint32_t see = ~0u;
+    if constexpr (kMasked) {
+      see = seen(kb + 32 * kt32);
+      const uint32_t mine = see >> (4 * h);
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
+    }
+    moe::bf16x2 p[8];
+    float ps;
+    auto exps = [&](float mn) __attribute__((always_inline)) {
+      ps = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i][0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i], a.c2, mn));
+        p[i][1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], a.c2, mn));
+        ps = __builtin_amdgcn_fdot2_f32_bf16(p[i], ones, ps, false);
+      }
+    };
+    exps(mneg);
+    if (__any(!(ps < kTreeMost))) {
+      float mx = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      const uint32_t u = __float_as_uint(mx);
+      const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+      mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+      const float m = -mneg, mn = fmaxf(m, mx * a.c2);
+      const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+      l *= alpha;
+      mneg = -mn;
+      exps(mn == -INFINITY ? 0.0f : -mn);
+    }
+    l += ps;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      bf16x8 pb;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) pb[j] = p[4 * m + (j >> 1)][j & 1];
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt) {
+        bf16x8 va;
+        if constexpr (kFp8) {
+          va = *(const bf16x8*)(vt + 4096 * dt + (v_at ^ (32 * m + 64 * kt32)));
+        } else {
+          u32x4 w;  // dim c of 32 dt of the keys 16 m + 8 j + 4 h ..
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4)(vt + 4096 * kt32 + 2048 * m + 1024 * j + (v_at ^ (64 * dt))));
+            const uint2 pair = __builtin_bit_cast(uint2, four);
+            w[2 * j] = pair.x;
+            w[2 * j + 1] = pair.y;
+          }
+          va = moe::as_bf16x8(w);
+          if constexpr (kMasked) {
+            // An infinity or a NaN must not meet the probability 0 of who does not see its key: it
+            // goes in by a product of its own, the largest number for it and for who sees it,
+            // whose square is past fp32's range
+            const __bf16 big = (__bf16)3.3895314e38f, none = (__bf16)0.0f;
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              bad |= ((w[j >> 1] >> (16 * (j & 1))) & 0x7F80u) == 0x7F80u;
+            if (__any(bad)) {
+              bf16x8 marks, who;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const bool x = ((w[j >> 1] >> (16 * (j & 1))) & 0x7F80u) == 0x7F80u;
+                marks[j] = x ? big : none;
+                va[j] = x ? none : va[j];
+                who[j] = see >> (16 * m + 8 * (j >> 2) + 4 * h + (j & 3)) & 1u ? big : none;
+              }
+              o[dt] = tree_mfma(marks, who, o[dt]);
+            }
+          }
+        }
+        o[dt] = tree_mfma(va, pb, o[dt]);
+      }
+    }
+  };
+  auto compute = [&](auto masked, int buf, int i) __attribute__((always_inline)) {
+    const int kb = (begin + kg + kK * i) * kTreeBlock;
+    const uint8_t *kt = lds[kg][buf][0], *vt = lds[kg][buf][1];
+    if constexpr (decltype(masked)::value) {
+#pragma unroll 1  // (registers)
+      for (int kt32 = 0; kt32 < 2; ++kt32) tile32(masked, kt, vt, kb, kt32);
+    } else {
+      tile32(masked, kt, vt, kb, 0);
+      tile32(masked, kt, vt, kb, 1);
+    }
+  };
+  auto put = [&](int buf, int i) __attribute__((always_inline)) {
+    store(raw, lds[kg][buf][0], lds[kg][buf][1], (begin + kg + kK * i) * kTreeBlock);
+  };
+
+  if (mine(0)) put(0, 0);
+  if (mine(1)) load(raw, 1);
+  if constexpr (kC > 1) moe::lds_barrier();
+  int i = 0;
+  auto run = [&](auto masked, int to) __attribute__((always_inline)) {
+    for (; i < to; ++i) {
+      const int buf = kBufs == 1 ? 0 : i & 1, next = kBufs == 1 ? 0 : buf ^ 1;
+      if (active && mine(i)) compute(masked, buf, i);
+      if (mine(i + 1)) put(next, i + 1);
+      if (mine(i + 2)) load(raw, i + 2);  // in flight during the next block's products
+      if constexpr (kC > 1) moe::lds_barrier();
+    }
+  };
+  // steps whose block every token of the wave sees whole: from whole0 to whole1
+  auto step_of = [&](int block) {
+    return min(max((block - begin - kg + kK - 1) / kK, 0), steps);
+  };
+  const int whole1 = step_of(max(cached / kTreeBlock, begin));
+  const int whole0 = min(whole1, step_of(max(seen_from >= 0 ? seen_from / kTreeBlock + 1 : 0, begin)));
+  run(std::true_type{}, whole0);
+  run(std::false_type{}, whole1);
+  run(std::true_type{}, steps);
+
+  float lt = l + __shfl_xor(l, 32, kWave);
+  if constexpr (kK > 1) {
+    // the groups' states into the first group's, in order, through the tiles' LDS
+    __shared__ float2 ml[kK - 1][kC][32];
+    if constexpr (kC == 1) moe::lds_barrier();  // every wave is done with its tile
+    f32x4* const part = (f32x4*)&lds[0][0][0][0] + cw * 8 * kWave + lane;
+    if (kg > 0) {
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        part[((kg - 1) * kC * 8 + q) * kWave] =
+            f32x4{o[q >> 2][4 * (q & 3)], o[q >> 2][4 * (q & 3) + 1],
+                  o[q >> 2][4 * (q & 3) + 2], o[q >> 2][4 * (q & 3) + 3]};
+      if (h == 0) ml[kg - 1][cw][c] = make_float2(-mneg, lt);
+    }
+    moe::lds_barrier();
+    if (kg > 0) return;
+    float top = -mneg;
+#pragma unroll
+    for (int g = 0; g < kK - 1; ++g) top = fmaxf(top, ml[g][cw][c].x);
+    const float w0 = tree_weight(-mneg, lt, top);
+    lt *= w0;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] *= w0;
+#pragma unroll
+    for (int g = 0; g < kK - 1; ++g) {
+      const float2 other = ml[g][cw][c];
+      const float w = tree_weight(other.x, other.y, top);
+      lt = fmaf(other.y, w, lt);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const f32x4 po = part[(g * kC * 8 + q) * kWave];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          o[q >> 2][4 * (q & 3) + j] = fmaf(po[j], w, o[q >> 2][4 * (q & 3) + j]);
+      }
+    }
+    mneg = -top;
+  }
+  if (4 * cw + (c >> 3) >= nt) return;
+  if (span.used <= 1) {
+    const float f = tree_share(lt, -mneg, sink);
+    uint16_t* const out = a.out + ((size_t)row * kHq + hk * kGroup + (c & 7)) * kD;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        uint16_t v4[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v4[j] = f2bf(o[dt][i + j] * f);
+        *(uint2*)(out + 32 * dt + 2 * i + 4 * h) =
+            make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
+                       (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
+      }
+  } else {
+    const size_t pt = ((size_t)share * a.rows + (b * a.tiles + tile) * 4 * kC + token) * kHq +
+                      hk * kGroup + (c & 7);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *(f32x4*)(a.part_o + pt * kD + 32 * dt + 2 * i + 4 * h) =
+            f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+    if (h == 0) *(float2*)(a.part_ml + pt * 2) = make_float2(-mneg, lt);
+  }
+}
+
+// The splits of a tile merged, in order: 16 threads a row (token, head), four dimensions each, eight
+// splits' loads in flight.  `tokens`: of a tile.
+__global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens) {
+  const int b = blockIdx.x / a.tiles, t0 = blockIdx.x % a.tiles * tokens;
+  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
+  const int i = blockIdx.y * 16 + (threadIdx.x >> 4);  // (token of the tile, head)
+  const int token = i / kHq, head = i % kHq, d = (threadIdx.x & 15) * 4;
+  if (token >= tokens || t0 + token >= qn) return;
+  const int L = a.page_indptr[b + 1] > a.page_indptr[b] ? a.kv_len[b] : 0;
+  const int used = TreeSpan(max(L - qn, 0), L, a.window, a.splits, a.least).used;
+  if (used <= 1) return;  // written already
+  const size_t at = ((size_t)blockIdx.x * tokens + token) * kHq + head;
+  const size_t step = (size_t)a.rows * kHq;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < used; s0 += 8) {
+    float2 ml[8];
+    f32x4 po[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const size_t pt = at + (size_t)min(s0 + j, used - 1) * step;
+      ml[j] = *(const float2*)(a.part_ml + pt * 2);
+      po[j] = *(const f32x4*)(a.part_o + pt * kD + d);
+    }
+    float mn = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mn = s0 + j < used ? fmaxf(mn, ml[j].x) : mn;
+    const float alpha = tree_weight(m, l, mn);
+    l *= alpha;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] *= alpha;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (s0 + j >= used) continue;
+      const float w = tree_weight(ml[j].x, ml[j].y, mn);
+      l = fmaf(ml[j].y, w, l);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = fmaf(po[j][q], w, o[q]);
+    }
+    m = mn;
+  }
+  const float f = tree_share(l, m, a.sinks[head]);
+  uint16_t v4[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) v4[q] = f2bf(o[q] * f);
+  *(uint2*)(a.out + ((size_t)(qb + t0 + token) * kHq + head) * kD + d) =
+      make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
+                 (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
 }
 
 }  // namespace attn
 
 extern "C" {
 
+// tokens: of a tile, 4, 8, 16 or 32; splits > 1: part_o [splits][rows][64][64], part_ml
+// [splits][rows][64][2], rows = batch * tiles * tokens.
 int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_len,
                      const void* mask, int words, const int* positions, const void* cache,
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
                      const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
+                     int tokens, int splits, int least, float* part_o, float* part_ml,
                      hipStream_t s) {
+  if (splits < 1 || splits > 65535 || least < 1) return -6;
+  const int tiles = (max_q_len + tokens - 1) / tokens;
   const attn::TreeArgs a{(const uint16_t*)q, q_indptr, (const uint32_t*)mask, positions,
                          (const uint8_t*)cache, page_indptr, page_indices, kv_len,
-                         (const uint16_t*)sinks, (uint16_t*)out, words, num_pages, window,
+                         (const uint16_t*)sinks, (uint16_t*)out, part_o, part_ml, words,
+                         num_pages, window, tiles, splits, least, batch * tiles * tokens,
                          sm_scale * attn::kTreeLog2e};
-  const dim3 grid(attn::kHkv * max_q_len, batch);
-  if (fp8)
-    hipLaunchKernelGGL(attn::tree_kernel<true>, grid, dim3(256), 0, s, a);
+  const dim3 grid(attn::kHkv * batch * tiles, splits);
+  auto go = [&](auto kernel, int waves) {
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, a);
+  };
+  if (tokens == 4)
+    fp8 ? go(attn::tree_kernel<true, 1, 4>, 4) : go(attn::tree_kernel<false, 1, 4>, 4);
+  else if (tokens == 8)
+    fp8 ? go(attn::tree_kernel<true, 2, 2>, 4) : go(attn::tree_kernel<false, 2, 2>, 4);
+  else if (tokens == 16)
+    fp8 ? go(attn::tree_kernel<true, 4, 2>, 8) : go(attn::tree_kernel<false, 4, 2>, 8);
+  else if (tokens == 32)
+    fp8 ? go(attn::tree_kernel<true, 8, 1>, 8) : go(attn::tree_kernel<false, 8, 1>, 8);
   else
-    hipLaunchKernelGGL(attn::tree_kernel<false>, grid, dim3(256), 0, s, a);
+    return -6;
+  if (hipGetLastError() != hipSuccess) return -6;
+  if (splits > 1)
+    hipLaunchKernelGGL(attn::tree_merge_kernel, dim3(batch * tiles, tokens * attn::kHq / 16),
+                       dim3(256), 0, s, a, tokens);
   return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
