@@ -65,7 +65,7 @@ int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_le
                      const void* mask, int words, const int* positions, const void* cache,
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
                      const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
-                     int tokens, int splits, int least, float* part_o, float* part_ml,
+                     int tokens, int workers, int least, float* part_o, float* part_ml,
                      hipStream_t s);
 int attn_launch_tree_commit(void* cache, int layers, int num_pages, bool fp8,
                             const int* page_indptr, const int* page_indices, const int* kv_len,
@@ -74,7 +74,7 @@ int attn_launch_tree_commit(void* cache, int layers, int num_pages, bool fp8,
                             int* count, int* next, hipStream_t s);
 int attn_launch_copy_pages(void* cache, int layers, int num_pages, int page_bytes, const int* src,
                            const int* dst, int n, hipStream_t s);
-size_t attn_beam_state_bytes(int rows, int vocab, int k);
+size_t attn_beam_state_bytes(int64_t rows, int vocab, int k);
 int attn_launch_beam(const void* logits, bool f32, const float* scores, int batch, int width,
                      int vocab, int k, float* out_scores, int* out_beams, int* out_tokens,
                      void* state, hipStream_t s);
@@ -599,21 +599,22 @@ constexpr int64_t kTreeNodes = 1024;  // of a sequence
 constexpr int64_t kBeams = 64;        // of a request, and continuations of one that are chosen
 constexpr int64_t kMaxBatch = 65535, kMaxLayers = 65535;
 
-// Tokens of a tree's tile, and how many splits its keys are shared out over: as many as let its
-// workgroups fit the chip at once (two a CU), each of kTreeLeast blocks or more.
-constexpr int64_t kTreeLeast = 4, kTreeWgs = 512, kTreeMaxSplits = 64;
+// Tokens of a tree's tile, and how many workgroups of a kv head its keys are shared out over:
+// as many as fit the chip at once (two a CU), each of kTreeLeast blocks or more; 0: a workgroup a
+// tile, where there are tiles enough to fill it twice over, more than 64 sequences or no bound.
+constexpr int64_t kTreeLeast = 4, kTreeWorkers = 64;
 struct TreePlan {
-  int64_t tokens, tiles, splits;
+  int64_t tokens, tiles, workers;
 };
 TreePlan tree_plan(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t window) {
   const int64_t tokens = max_q_len <= 4 ? 4 : max_q_len <= 8 ? 8 : max_q_len <= 16 ? 16 : 32;
   const int64_t tiles = (max_q_len + tokens - 1) / tokens;
   max_kv_len = std::min(max_kv_len, kMaxPages * kPage);  // (and no overflow below)
   const int64_t keys = window > 0 ? std::min(max_kv_len, window + max_q_len) : max_kv_len;
-  if (keys <= 0) return TreePlan{tokens, tiles, 1};
-  const int64_t most = std::min(kTreeMaxSplits, kTreeWgs / (tiles * batch * kKvHeads));
-  return TreePlan{tokens, tiles,
-                  std::max<int64_t>(1, std::min(most, fp8_blocks(keys) / kTreeLeast))};
+  if (keys <= 0 || batch > 64 || batch * tiles > 2 * kTreeWorkers) return TreePlan{tokens, tiles, 0};
+  const int64_t pieces = (batch * tiles * fp8_blocks(keys) + kTreeLeast - 1) / kTreeLeast;
+  if (pieces <= batch * tiles) return TreePlan{tokens, tiles, 0};
+  return TreePlan{tokens, tiles, std::min(kTreeWorkers, pieces)};
 }
 
 int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
@@ -641,11 +642,11 @@ int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch
   if (workspace_bytes < need) return MOE_ERR_WORKSPACE;
   const TreePlan plan = tree_plan(batch, max_q_len, max_kv_len, window);
   float* part_o = (float*)workspace;
-  const int64_t parts = plan.splits * plan.tokens * plan.tiles * batch;
+  const int64_t parts = (plan.workers + plan.tiles * batch) * plan.tokens;
   return status(attn_launch_tree(q, q_indptr, (int)batch, (int)max_q_len, tree_mask,
                                  (int)mask_words, positions, kv_cache, fp8, page_indptr,
                                  page_indices, (int)num_pages, kv_len, window, sm_scale, sinks, out,
-                                 (int)plan.tokens, (int)plan.splits, (int)kTreeLeast, part_o,
+                                 (int)plan.tokens, (int)plan.workers, (int)kTreeLeast, part_o,
                                  need ? part_o + parts * kQHeads * kHeadDim : nullptr,
                                  as_stream(stream)));
 }
@@ -677,8 +678,8 @@ size_t attn_tree_workspace_bytes(int64_t batch, int64_t max_q_len, int64_t max_k
                                  int32_t window) {
   if (batch <= 0 || batch > kMaxBatch || max_q_len <= 0 || max_q_len > kTreeNodes) return 0;
   const TreePlan plan = tree_plan(batch, max_q_len, max_kv_len, window);
-  if (plan.splits <= 1) return 0;
-  return (size_t)(plan.splits * plan.tokens * plan.tiles * batch * kQHeads * (kHeadDim + 2)) *
+  if (plan.workers == 0) return 0;
+  return (size_t)((plan.workers + plan.tiles * batch) * plan.tokens * kQHeads * (kHeadDim + 2)) *
          sizeof(float);
 }
 
@@ -742,7 +743,7 @@ size_t attn_beam_workspace_bytes(int64_t batch, int64_t width, int64_t vocab, in
   if (batch <= 0 || batch > kMaxBatch || width <= 0 || width > kBeams || vocab <= 0 ||
       vocab >= ((int64_t)1 << 30) || k <= 0 || k > kBeams || k > width * vocab)
     return 0;
-  return attn_beam_state_bytes((int)(batch * width), (int)vocab, (int)k);
+  return attn_beam_state_bytes(batch * width, (int)vocab, (int)k);
 }
 
 int attn_beam_top_k(const void* logits, int32_t logits_f32, int64_t batch, int64_t width,
@@ -760,8 +761,9 @@ int attn_beam_top_k(const void* logits, int32_t logits_f32, int64_t batch, int64
   if (!a16(logits) || !a4(scores) || !a4(out_scores) || !a4(out_beams) || !a4(out_tokens) ||
       !a16(workspace))
     return MOE_ERR_ALIGN;
-  if (workspace_bytes < attn_beam_workspace_bytes(batch, width, vocab, k))
-    return MOE_ERR_WORKSPACE;
+  const size_t need = attn_beam_workspace_bytes(batch, width, vocab, k);
+  if (need == 0) return MOE_ERR_SHAPE;
+  if (workspace_bytes < need) return MOE_ERR_WORKSPACE;
   return status(attn_launch_beam(logits, logits_f32 != 0, scores, (int)batch, (int)width,
                                  (int)vocab, (int)k, out_scores, out_beams, out_tokens, workspace,
                                  as_stream(stream)));

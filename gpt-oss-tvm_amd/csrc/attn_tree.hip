@@ -5,6 +5,8 @@
 //   out = sum_j p_j v_j / (sum_j p_j + exp(sink)),  p_j = exp(sm_scale q . k_j)
 // rounded to bf16 once; a node that sees no key gets 0.  Scores, sums and outputs in fp32,
 // exponents in units of log2.
+#include <stdint.h>
+
 #include <type_traits>
 
 #include "attn_common.h"
@@ -33,9 +35,9 @@ struct TreeArgs {
   const int* kv_len;
   const uint16_t* sinks;
   uint16_t* out;
-  float* part_o;   // [splits][tiles' tokens][64][64]
-  float* part_ml;  // [splits][tiles' tokens][64][2]
-  int words, num_pages, window, tiles, splits, least, rows;
+  float* part_o;   // [workers + tiles][tokens of a tile][64][64]
+  float* part_ml;  // [workers + tiles][tokens of a tile][64][2]
+  int words, num_pages, window, batch, tiles, workers, least;
   float c2;        // sm_scale log2(e)
 };
 
@@ -43,20 +45,58 @@ __device__ __forceinline__ f32x16 tree_mfma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// The blocks of 64 keys that a sequence's nodes look at, and how they are shared out: over
-// as many splits as have `least` blocks, at most `most`.  It follows from the keys and not
-// from the caller's bound on them, which only trims the grid.
+// The blocks of 64 keys that a sequence's nodes look at.
 struct TreeSpan {
-  int first, blocks;  // first block, number of blocks
-  int each, used;     // blocks of a split, splits with any
-  __device__ __forceinline__ TreeSpan(int cached, int total, int window, int most, int least) {
+  int first, blocks;
+  __device__ __forceinline__ TreeSpan(int cached, int total, int window) {
     // positions are at or past the cached tokens' end
     const int lo = window > 0 ? max(0, cached - window + 1) : 0;
     first = lo / kTreeBlock;
     blocks = total > lo ? (total - 1) / kTreeBlock - first + 1 : 0;
-    const int n = min(most, (blocks + least - 1) / least);
-    each = n > 0 ? (blocks + n - 1) / n : 0;
-    used = each > 0 ? (blocks + each - 1) / each : 0;
+  }
+};
+
+// The work of a kv head in one line: the blocks of every tile of every sequence (up to 64, one a
+// lane; a tile without keys counts as one), one after the other, cut into equal pieces of at least
+// `least`, a worker each.  Sequences of all lengths and few of them fill the chip alike, and it
+// follows from the keys and not from the caller's bound on them, which only trims the workers.
+// A worker's part of tile g (counted over all sequences) that it does not have whole goes to place
+// worker + g of the workspace: two parts never share one, as one step in the line moves on
+// to the next worker, the next tile or both.
+struct TreeLine {
+  int64_t before, after;  // the line up to the lane's sequence and with it
+  int64_t all, piece;
+  int blocks;             // of one of its tiles
+  int tiles_before;       // of the sequences before it
+  TreeLine() = default;
+  __device__ __forceinline__ TreeLine(const TreeArgs& a, int tokens) {
+    const int lane = threadIdx.x & 63, b = min(lane, a.batch - 1);
+    const int qn = lane < a.batch ? a.q_indptr[b + 1] - a.q_indptr[b] : 0;
+    const int total = a.page_indptr[b + 1] > a.page_indptr[b] ? a.kv_len[b] : 0;
+    blocks = max(1, TreeSpan(max(total - qn, 0), total, a.window).blocks);
+    const int tiles = min(max((qn + tokens - 1) / tokens, 0), a.tiles);
+    const int64_t mine = (int64_t)tiles * blocks;
+    after = mine;
+    int tiles_after = tiles;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t x = __shfl_up(after, off, kWave);
+      const int y = __shfl_up(tiles_after, off, kWave);
+      after += lane >= off ? x : 0;
+      tiles_after += lane >= off ? y : 0;
+    }
+    before = after - mine;
+    tiles_before = tiles_after - tiles;
+    all = lane_of(after, 63);
+    // (exact: far below 2^53, and a quotient is an integer or 1 / workers away from the next)
+    piece = max((int64_t)a.least, (int64_t)((double)(all + a.workers - 1) / (double)a.workers));
+  }
+  static __device__ __forceinline__ int64_t lane_of(int64_t x, int l) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l) |
+                     (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32);
+  }
+  __device__ __forceinline__ int worker_of(int64_t at) const {
+    return (int)((double)at / (double)piece);  // (as above)
   }
 };
 
@@ -85,29 +125,30 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //    sees, and is renewed only when a tile's sum passes 2^24.
 //  * Blocks that every token of a wave sees whole take no mask; in the others (the tree's own, a
 //    window's edge) a lane has its token's 32 bits of a tile.
+template <int kC, int kK>
+struct TreeLds {
+  static constexpr int kBufs = kC == 1 ? 1 : 2;  // one wave needs no second buffer
+  __align__(16) uint8_t tiles[kK][kBufs][2][kTreeHalf];
+  float2 ml[kK][kC][32];
+};
+
+// Blocks begin .. end - 1 of a tile whose sequence has qn nodes from row qb on and L tokens in all;
+// the result goes to out, or where it is a part to `place` of the workspace.
 template <bool kFp8, int kC, int kK>
-__global__ __launch_bounds__(64 * kC * kK)
-__attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs a) {
-  constexpr int kBufs = kC == 1 ? 1 : 2;        // one wave needs no second buffer
+__device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& lds, int hk, int b,
+                                           int tile, int qb, int qn, int L, int begin, int end,
+                                           int place) {
+  constexpr int kBufs = TreeLds<kC, kK>::kBufs;
   constexpr int kUnits = (kFp8 ? 8 : 16) / kC;  // 1 KB loads of a block that a wave makes
-  __shared__ __align__(16) uint8_t lds[kK][kBufs][2][kTreeHalf];
-  // x: (sequence, tile, kv head), y: split
-  const int hk = blockIdx.x % kHkv, share = blockIdx.y;
-  const int b = blockIdx.x / kHkv / a.tiles, tile = blockIdx.x / kHkv % a.tiles;
-  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb, t0 = tile * 4 * kC;
-  if (t0 >= qn) return;
-  const int nt = min(4 * kC, qn - t0), row0 = qb + t0;
-  const PageList pages{a.page_indices + a.page_indptr[b],
-                       a.page_indptr[b + 1] - a.page_indptr[b], a.num_pages};
-  const int L = pages.count > 0 ? a.kv_len[b] : 0, cached = max(L - qn, 0);
-  const TreeSpan span(cached, L, a.window, a.splits, a.least);
-  if (share >= max(span.used, 1)) return;
-  const int t = threadIdx.x, lane = t & 63, c = lane & 31, h = lane >> 5;
+  int t = threadIdx.x;
+  asm volatile("" : "+v"(t));  // (what follows from it is not carried over to the next piece)
+  const int lane = t & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), cw = wave % kC, kg = wave / kC;
+  const int t0 = tile * 4 * kC, nt = min(4 * kC, qn - t0), row0 = qb + t0;
+  const int cached = max(L - qn, 0), page0 = a.page_indptr[b];
+  const PageList pages{a.page_indices + page0, a.page_indptr[b + 1] - page0, a.num_pages};
   const bool active = 4 * cw < nt;
   const int last_page = max(0, min(pages.count - 1, (L - 1) / kPage));
-  const int begin = span.first + share * span.each;
-  const int end = min(begin + span.each, span.first + span.blocks);
   const int steps = (end - begin + kK - 1) / kK;  // of every group
   constexpr int kPageSize = kFp8 ? kFp8Page : kBfPage;
 
@@ -319,6 +360,7 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
 #pragma unroll
       for (int dt = 0; dt < 2; ++dt) {
         bf16x8 va;
+        if constexpr (kMasked) __builtin_amdgcn_sched_barrier(0);  // (registers)
         if constexpr (kFp8) {
           va = *(const bf16x8*)(vt + 4096 * dt + (v_at ^ (32 * m + 64 * kt32)));
         } else {
@@ -360,7 +402,7 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
   };
   auto compute = [&](auto masked, int buf, int i) __attribute__((always_inline)) {
     const int kb = (begin + kg + kK * i) * kTreeBlock;
-    const uint8_t *kt = lds[kg][buf][0], *vt = lds[kg][buf][1];
+    const uint8_t *kt = lds.tiles[kg][buf][0], *vt = lds.tiles[kg][buf][1];
     if constexpr (decltype(masked)::value) {
 #pragma unroll 1  // (registers)
       for (int kt32 = 0; kt32 < 2; ++kt32) tile32(masked, kt, vt, kb, kt32);
@@ -370,7 +412,8 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
     }
   };
   auto put = [&](int buf, int i) __attribute__((always_inline)) {
-    store(raw, lds[kg][buf][0], lds[kg][buf][1], (begin + kg + kK * i) * kTreeBlock);
+    store(raw, lds.tiles[kg][buf][0], lds.tiles[kg][buf][1],
+          (begin + kg + kK * i) * kTreeBlock);
   };
 
   if (mine(0)) put(0, 0);
@@ -399,22 +442,21 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
   float lt = l + __shfl_xor(l, 32, kWave);
   if constexpr (kK > 1) {
     // the groups' states into the first group's, in order, through the tiles' LDS
-    __shared__ float2 ml[kK - 1][kC][32];
     if constexpr (kC == 1) moe::lds_barrier();  // every wave is done with its tile
-    f32x4* const part = (f32x4*)&lds[0][0][0][0] + cw * 8 * kWave + lane;
+    f32x4* const part = (f32x4*)&lds.tiles[0][0][0][0] + cw * 8 * kWave + lane;
     if (kg > 0) {
 #pragma unroll
       for (int q = 0; q < 8; ++q)
         part[((kg - 1) * kC * 8 + q) * kWave] =
             f32x4{o[q >> 2][4 * (q & 3)], o[q >> 2][4 * (q & 3) + 1],
                   o[q >> 2][4 * (q & 3) + 2], o[q >> 2][4 * (q & 3) + 3]};
-      if (h == 0) ml[kg - 1][cw][c] = make_float2(-mneg, lt);
+      if (h == 0) lds.ml[kg][cw][c] = make_float2(-mneg, lt);
     }
     moe::lds_barrier();
     if (kg > 0) return;
     float top = -mneg;
 #pragma unroll
-    for (int g = 0; g < kK - 1; ++g) top = fmaxf(top, ml[g][cw][c].x);
+    for (int g = 1; g < kK; ++g) top = fmaxf(top, lds.ml[g][cw][c].x);
     const float w0 = tree_weight(-mneg, lt, top);
     lt *= w0;
 #pragma unroll
@@ -422,13 +464,13 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[dt][i] *= w0;
 #pragma unroll
-    for (int g = 0; g < kK - 1; ++g) {
-      const float2 other = ml[g][cw][c];
+    for (int g = 1; g < kK; ++g) {
+      const float2 other = lds.ml[g][cw][c];
       const float w = tree_weight(other.x, other.y, top);
       lt = fmaf(other.y, w, lt);
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        const f32x4 po = part[(g * kC * 8 + q) * kWave];
+        const f32x4 po = part[((g - 1) * kC * 8 + q) * kWave];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           o[q >> 2][4 * (q & 3) + j] = fmaf(po[j], w, o[q >> 2][4 * (q & 3) + j]);
@@ -437,7 +479,7 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
     mneg = -top;
   }
   if (4 * cw + (c >> 3) >= nt) return;
-  if (span.used <= 1) {
+  if (place < 0) {
     const float f = tree_share(lt, -mneg, sink);
     uint16_t* const out = a.out + ((size_t)row * kHq + hk * kGroup + (c & 7)) * kD;
 #pragma unroll
@@ -452,8 +494,7 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
                        (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
       }
   } else {
-    const size_t pt = ((size_t)share * a.rows + (b * a.tiles + tile) * 4 * kC + token) * kHq +
-                      hk * kGroup + (c & 7);
+    const size_t pt = ((size_t)place * 4 * kC + token) * kHq + hk * kGroup + (c & 7);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
@@ -464,19 +505,63 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
   }
 }
 
-// The splits of a tile merged, in order: 16 threads a row (token, head), four dimensions each, eight
-// splits' loads in flight.  `tokens`: of a tile.
+template <bool kFp8, int kC, int kK>
+__global__ __launch_bounds__(64 * kC * kK)
+__attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs a) {
+  __shared__ TreeLds<kC, kK> lds;
+  __shared__ TreeLine lines[kWave];  // (out of the registers)
+  // x: (worker, kv head); without workers (sequence, tile, kv head)
+  const int hk = blockIdx.x % kHkv, worker = blockIdx.x / kHkv, lane = threadIdx.x & 63;
+  int64_t at = 0, stop = 1;
+  if (a.workers > 0) {
+    const TreeLine line(a, 4 * kC);
+    const int64_t piece = TreeLine::lane_of(line.piece, 0);
+    at = worker * piece;
+    stop = min(at + piece, line.all);
+    if (at >= stop) return;
+    if (threadIdx.x < kWave) lines[lane] = line;
+    moe::lds_barrier();
+  }
+  do {
+    int b = worker / a.tiles, tile = worker % a.tiles, first = 0, place = -1;
+    int64_t n = INT32_MAX;
+    if (a.workers > 0) {
+      b = __builtin_ctzll(__ballot(lines[lane].after > at));
+      const int blocks = __builtin_amdgcn_readfirstlane(lines[b].blocks);
+      const int from = (int)(at - TreeLine::lane_of(lines[b].before, 0));
+      tile = from / blocks;
+      first = from - tile * blocks;
+      n = min((int64_t)(blocks - first), stop - at);
+      if (n < blocks)
+        place = worker + __builtin_amdgcn_readfirstlane(lines[b].tiles_before) + tile;
+    }
+    const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
+    const int L = a.page_indptr[b + 1] > a.page_indptr[b] ? a.kv_len[b] : 0;
+    if (tile * 4 * kC >= qn) return;  // (only without workers)
+    const TreeSpan span(max(L - qn, 0), L, a.window);
+    tree_piece<kFp8, kC, kK>(a, lds, hk, b, tile, qb, qn, L, span.first + first,
+                             span.first + (int)min(first + n, (int64_t)span.blocks), place);
+    at += n;
+    if (at < stop) moe::lds_barrier();  // the next piece's tiles go where this one's parts lie
+  } while (at < stop);
+}
+
+// The parts of a tile merged, in order: 16 threads a row (token, head), four dimensions each, eight
+// parts' loads in flight.  `tokens`: of a tile.
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens) {
-  const int b = blockIdx.x / a.tiles, t0 = blockIdx.x % a.tiles * tokens;
-  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
   const int i = blockIdx.y * 16 + (threadIdx.x >> 4);  // (token of the tile, head)
   const int token = i / kHq, head = i % kHq, d = (threadIdx.x & 15) * 4;
-  if (token >= tokens || t0 + token >= qn) return;
-  const int L = a.page_indptr[b + 1] > a.page_indptr[b] ? a.kv_len[b] : 0;
-  const int used = TreeSpan(max(L - qn, 0), L, a.window, a.splits, a.least).used;
-  if (used <= 1) return;  // written already
-  const size_t at = ((size_t)blockIdx.x * tokens + token) * kHq + head;
-  const size_t step = (size_t)a.rows * kHq;
+  const int b = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
+  const TreeLine line(a, tokens);
+  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
+  const int blocks = __builtin_amdgcn_readlane(line.blocks, b);
+  if (tile * tokens >= qn) return;
+  const int64_t from = TreeLine::lane_of(line.before, b) + (int64_t)tile * blocks;
+  const int first = line.worker_of(from), used = line.worker_of(from + blocks - 1) - first + 1;
+  if (used <= 1 || token >= tokens || tile * tokens + token >= qn) return;  // (written already)
+  const int place = first + __builtin_amdgcn_readlane(line.tiles_before, b) + tile;
+  const size_t at = ((size_t)place * tokens + token) * kHq + head;
+  const size_t step = (size_t)tokens * kHq;
   float m = -INFINITY, l = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < used; s0 += 8) {
@@ -509,7 +594,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
   uint16_t v4[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) v4[q] = f2bf(o[q] * f);
-  *(uint2*)(a.out + ((size_t)(qb + t0 + token) * kHq + head) * kD + d) =
+  *(uint2*)(a.out + ((size_t)(qb + tile * tokens + token) * kHq + head) * kD + d) =
       make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
                  (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
 }
@@ -518,24 +603,24 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
 
 extern "C" {
 
-// tokens: of a tile, 4, 8, 16 or 32; splits > 1: part_o [splits][rows][64][64], part_ml
-// [splits][rows][64][2], rows = batch * tiles * tokens.
+// tokens: of a tile, 4, 8, 16 or 32; workers: of a kv head, 0: a workgroup a tile (more than 64
+// sequences); else part_o [workers + batch * tiles][tokens][64][64], part_ml [.. ][2] in its place.
 int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_len,
                      const void* mask, int words, const int* positions, const void* cache,
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
                      const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
-                     int tokens, int splits, int least, float* part_o, float* part_ml,
+                     int tokens, int workers, int least, float* part_o, float* part_ml,
                      hipStream_t s) {
-  if (splits < 1 || splits > 65535 || least < 1) return -6;
+  if (workers < 0 || (workers > 0 && batch > 64) || least < 1) return -6;
   const int tiles = (max_q_len + tokens - 1) / tokens;
   const attn::TreeArgs a{(const uint16_t*)q, q_indptr, (const uint32_t*)mask, positions,
                          (const uint8_t*)cache, page_indptr, page_indices, kv_len,
                          (const uint16_t*)sinks, (uint16_t*)out, part_o, part_ml, words,
-                         num_pages, window, tiles, splits, least, batch * tiles * tokens,
+                         num_pages, window, batch, tiles, workers, least,
                          sm_scale * attn::kTreeLog2e};
-  const dim3 grid(attn::kHkv * batch * tiles, splits);
+  const int grid = attn::kHkv * (workers > 0 ? workers : batch * tiles);
   auto go = [&](auto kernel, int waves) {
-    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, s, a);
   };
   if (tokens == 4)
     fp8 ? go(attn::tree_kernel<true, 1, 4>, 4) : go(attn::tree_kernel<false, 1, 4>, 4);
@@ -548,7 +633,7 @@ int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_le
   else
     return -6;
   if (hipGetLastError() != hipSuccess) return -6;
-  if (splits > 1)
+  if (workers > 0)
     hipLaunchKernelGGL(attn::tree_merge_kernel, dim3(batch * tiles, tokens * attn::kHq / 16),
                        dim3(256), 0, s, a, tokens);
   return hipGetLastError() == hipSuccess ? 0 : -6;

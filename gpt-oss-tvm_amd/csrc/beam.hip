@@ -1,135 +1,479 @@
 // Beam search's selection (gfx950): the k best of a request's beams x vocabulary continuations.
 //
 // The score of (beam b, token t) is scores[b] + x_t - log sum exp(x), x the beam's logits, in
-// fp64; a beam whose logits have no maximum (NaN, +inf, nothing but -inf), or a score that is NaN,
-// gives -inf.  The order is by score, then beam, then token, ascending.
+// fp64; a beam whose logits have no maximum (NaN, +inf, nothing but -inf), or whose own score is
+// not finite, gives -inf.  The order is by score, then beam, then logit, then token.
+//
+// Two launches.  part_kernel reads the logits once, a workgroup a stretch of a row: its maximum m,
+// the sum of exp(x - m), and its k best by logit (within a row the order is the logits').
+// merge_kernel, a workgroup a request, joins the sums and picks the k best of all stretches' lists.
+// Both find a bound first.  Of q waves that hold numbers, each takes the ceil(k / q)-th largest
+// of its lanes' maxima, by bits from above with a ballot each: where q waves reach a bound there
+// are k numbers that do.  With q half of the waves (and the q-th largest of their values) about 2 k
+// numbers of a stretch reach it, with q = 1 ten times k.  They go to LDS, and take their
+// places by counting those before them.
+#include <stdint.h>
+
+#include <algorithm>
 #include <type_traits>
 
 #include "moe_common.h"
 
 namespace beam {
 
-using moe::bf2f;
+using moe::u32x4;
+using moe::u32x4_any;
 
-constexpr int kThreads = 1024;
+constexpr int kMost = 64;        // k at most: the lanes of a wave
+constexpr int kBoundBits = 18;   // of the bounds: 2^-9 of a value lets few more through
 
-template <class T>
-__device__ __forceinline__ float logit(const T* x, int i) {
-  if constexpr (sizeof(T) == 2) return bf2f(x[i]);
-  return x[i];
+struct Stat {  // of a stretch
+  double sum;  // of exp(x - m), m = 0 where there is nothing but -inf
+  float m;
+};
+struct Item {
+  float x;
+  int token;  // -1: none
+};
+
+// order-preserving image of a float (both zeros alike)
+__device__ __forceinline__ uint32_t image(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+// a bound on the k-th largest of a wave's values from below: its upper kBits bits
+template <int kBits>
+__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t mine, int k) {
+  uint32_t t = 0u;
+#pragma unroll
+  for (int bit = 31; bit >= 32 - kBits; --bit) {
+    const uint32_t next = t | 1u << bit;
+    if (__popcll(__ballot(mine >= next)) >= k) t = next;
+  }
+  return t;
+}
+// the q-th largest of n values, n <= 64, q <= n
+__device__ __forceinline__ uint32_t nth_of(const uint32_t* x, int n, int q) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t mine = x[min(lane, n - 1)];
+  int before = 0;
+  for (int i = 0; i < n; ++i) {
+    const uint32_t o = (uint32_t)__builtin_amdgcn_readlane((int)mine, i);
+    before += o > mine || (o == mine && i < lane) ? 1 : 0;
+  }
+  return (uint32_t)__builtin_amdgcn_readlane(
+      (int)mine, __builtin_ctzll(__ballot(lane < n && before == q - 1)));
+}
+// max over the wave, by register moves: pairs, quads, rows of 16, then across the rows
+template <int kCtrl, int kRows>
+__device__ __forceinline__ float max_with(float x) {
+  const int u = __float_as_int(x);
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(u, u, kCtrl, kRows, 0xF, false)));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = max_with<0xB1, 0xF>(x);   // quad_perm [1,0,3,2]
+  x = max_with<0x4E, 0xF>(x);   // quad_perm [2,3,0,1]
+  x = max_with<0x141, 0xF>(x);  // row_half_mirror
+  x = max_with<0x140, 0xF>(x);  // row_mirror
+  x = max_with<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+  x = max_with<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
-// maximum and log of the sum of exp(x - maximum) of each row
-template <class T>
-__global__ __launch_bounds__(kThreads) void stats_kernel(const T* __restrict__ logits, int V,
-                                                         double* __restrict__ stats) {
-  __shared__ double tmp[kThreads / 64];
-  const T* x = logits + (size_t)blockIdx.x * V;
+// Adds to ranks[i] how many of n things come before thing i: the fewer things, the more threads
+// share out one's comparisons.
+template <int kThreads, class At, class Before>
+__device__ __forceinline__ void rank_all(int n, int* ranks, At at, Before before) {
   const int t = threadIdx.x;
-  float m = -INFINITY;
-  for (int i = t; i < V; i += kThreads) {
-    const float v = logit(x, i);
-    m = v != v ? INFINITY : fmaxf(m, v);
+  int share = 1;  // threads a thing
+  while (share < 16 && n * share * 2 <= kThreads) share *= 2;
+  const int step = kThreads / share, from = t / step;
+  for (int i = t % step; i < n; i += step) {
+    const auto mine = at(i);
+    int rank = 0;
+    for (int j = from; j < n; j += share) rank += before(at(j), mine) ? 1 : 0;
+    if (rank) atomicAdd(&ranks[i], rank);
   }
+}
+
+// exp(d), d <= 0: exp2 of the product with log2(e) in two pieces, so that it is off by a few
+// 2^-24 of itself however small it is
+__device__ __forceinline__ float exp_of(float d) {
+  return __builtin_amdgcn_exp2f(fmaf(d, 1.9259630e-8f, d * 1.44269502f));
+}
+
+// T: float or uint16_t (bf16).  A stretch is `chunks` chunks, of which a thread holds 16 elements
+// and the next one's loads, wherever the row begins.  The bound is taken after the first, then after
+// 8, 16, .. and after the last; a thread whose maximum of a chunk reaches it only notes that (looking at each number there
+// cost twice the time), and what reaches the last bound is picked out of the noted ones' 16 numbers,
+// from memory, at the end.
+constexpr int kPartThreads = 512, kPartElems = 16, kChunk = kPartThreads * kPartElems;
+constexpr int kPartList = 1024, kWaveList = kPartList / (kPartThreads / 64);
+template <class T>
+__global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6))) void part_kernel(
+    const T* __restrict__ logits, int V, int k, int parts, int chunks, Stat* __restrict__ stats,
+    Item* __restrict__ items) {
+  constexpr int kEach = 16 / sizeof(T), kElems = kPartElems, kLoads = kElems / kEach;
+  constexpr int kWaves = kPartThreads / 64;
+  __shared__ int found[kWaves][kWaveList];  // (chunk, thread) whose maximum reached the bound
+  __shared__ Item list[kPartList];
+  __shared__ int ranks[kPartList], kept;
+  __shared__ double wsum[kWaves];
+  __shared__ float wm[kWaves];
+  __shared__ uint32_t wbound[2][kWaves];
+  __shared__ int wcount[2][kWaves];
+  const int part = blockIdx.x % parts, t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const T* const x = logits + (size_t)(blockIdx.x / parts) * V;
+  const int begin = part * chunks * kChunk, end = min(V, begin + chunks * kChunk);
+  struct Raw {
+    u32x4 w[kLoads];
+    __device__ __forceinline__ float operator()(int e) const {
+      const uint32_t u = w[e / kEach][sizeof(T) == 2 ? (e % kEach) >> 1 : e % kEach];
+      if constexpr (sizeof(T) == 2) return __uint_as_float(e & 1 ? u & 0xFFFF0000u : u << 16);
+      return __uint_as_float(u);
+    }
+  };
+  // The stretch's whole 16-byte units are loaded without a branch (one would wait for its load
+  // before the next), past the last the last again, which then counts as -inf; the few numbers
+  // behind them have a thread each.
+  const int units = (end - begin) / kEach, tail = end - begin - units * kEach;
+  auto load = [&](Raw& raw, int chunk) __attribute__((always_inline)) {
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  if ((t & 63) == 0) tmp[t >> 6] = m;
-  __syncthreads();
-  for (int i = 0; i < kThreads / 64; ++i) m = fmaxf(m, (float)tmp[i]);
-  __syncthreads();
-  double s = 0.0;
-  for (int i = t; i < V; i += kThreads) s += exp((double)logit(x, i) - (double)m);
-  s = moe::wave_sum(s);
-  if ((t & 63) == 0) tmp[t >> 6] = s;
+    for (int j = 0; j < kLoads; ++j) {
+      const int u = min((chunk * kLoads + j) * kPartThreads + t, units - 1);
+      raw.w[j] = *(const u32x4_any*)(x + begin + u * kEach);
+    }
+  };
+  auto outside = [&](Raw& raw, int chunk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const bool in = (chunk * kLoads + j) * kPartThreads + t < units;
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        raw.w[j][w] = in ? raw.w[j][w] : sizeof(T) == 2 ? 0xFF80FF80u : 0xFF800000u;
+    }
+  };
+  auto number = [&](int p) {
+    return sizeof(T) == 2 ? moe::bf2f((uint16_t)x[p]) : (float)x[p];
+  };
+  Raw raw, next;
+  if (units > 0) load(raw, 0);
+  const float extra = t < tail ? number(end - tail + t) : -INFINITY;
+  for (int i = t; i < kPartList; i += kPartThreads) ranks[i] = 0;
+  // the lane's maximum (it passes over NaN; the sum does not) and sum of exp(x - maximum)
+  float lm = fmaxf(extra, -INFINITY), least = -INFINITY;
+  float s = exp_of(extra - (lm == -INFINITY ? 0.0f : lm));
+  int noted = 0;  // by the wave
+  // waves with fewer numbers than lanes are not counted on for the bound
+  const int full = min(kWaves, max(1, (end - begin) / (64 * kEach))), q = (full + 1) / 2;
+  auto bound = [&](int turn) __attribute__((always_inline)) {
+    const uint32_t mine = kth_of_lanes<kBoundBits>(image(lm), (k + q - 1) / q);
+    if (lane == 0) wbound[turn][wave] = mine;
+    __syncthreads();
+    const uint32_t top = nth_of(wbound[turn], kWaves, q);
+    // the image back, where there are k numbers (below -inf's image it would be a NaN)
+    least = top <= 0x007FFFFFu
+                ? -INFINITY : __uint_as_float(top & 0x80000000u ? top & 0x7FFFFFFFu : ~top);
+  };
+  int chunk = 0;
+  for (; chunk * kLoads * kPartThreads < units; ++chunk) {
+    load(next, chunk + 1);
+    if ((chunk + 1) * kLoads * kPartThreads > units) outside(raw, chunk);
+    float cm = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) cm = fmaxf(cm, raw(e));
+    const float old = lm, base = fmaxf(old, cm) == -INFINITY ? 0.0f : fmaxf(old, cm);
+    lm = fmaxf(old, cm);
+    s *= exp_of(old - base);
+#pragma unroll
+    for (int e = 0; e < kElems; ++e) s += exp_of(raw(e) - base);
+    if ((chunk & (chunk + 1)) == 0 && (chunk == 0 || chunk >= 7)) bound(__builtin_ctz(chunk + 1) & 1);
+    const uint64_t who = __ballot(cm >= least);
+    const int at = noted + __builtin_amdgcn_mbcnt_hi(
+                               (uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+    if (cm >= least && at < kWaveList) found[wave][at] = chunk * kPartThreads + t;
+    noted += __popcll(who);
+    raw = next;
+  }
+  if (t == 0) kept = 0;
+  float m = wave_max(lm);
+  if (lane == 0) {
+    wm[wave] = m;
+    wcount[0][wave] = noted;
+  }
+  if (chunk == 1 && tail == 0)
+    __syncthreads();  // (as it was taken)
+  else
+    bound(chunk < 8 ? 1 : (32 - __builtin_clz(chunk)) & 1);  // (the other turn than the last one's)
+  bool fits = true;
+  int records = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    m = fmaxf(m, wm[w]);
+    records += wcount[0][w];
+    fits = fits && wcount[0][w] <= kWaveList;
+  }
+  auto keep = [&](float v, int p) {  // (in any order: their places are found by comparing)
+    const int at = atomicAdd(&kept, 1);
+    if (at < kPartList) list[at] = Item{v, p};
+  };
+  if (fits) {
+    for (int i = t; i < records * kLoads; i += kPartThreads) {
+      int r = i / kLoads, w = 0;
+      for (; r >= wcount[0][w]; ++w) r -= wcount[0][w];
+      const int note = found[w][r];
+      const int u = (note / kPartThreads * kLoads + i % kLoads) * kPartThreads + note % kPartThreads;
+      if (u >= units) continue;
+      Raw again;
+      again.w[0] = *(const u32x4_any*)(x + begin + u * kEach);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (again(e) >= least) keep(again(e), begin + u * kEach + e);
+    }
+    if (t < tail && extra >= least) keep(extra, end - tail + t);
+  }
+  const double sum = moe::wave_sum_f64((double)(lm == -INFINITY ? s : s * exp_of(lm - m)));
+  if (lane == 0) wsum[wave] = sum;
   __syncthreads();
   if (t == 0) {
-    s = 0.0;
-    for (int i = 0; i < kThreads / 64; ++i) s += tmp[i];
-    stats[2 * blockIdx.x] = m;
-    stats[2 * blockIdx.x + 1] = log(s);
+    double all = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all += wsum[w];
+    stats[blockIdx.x] = Stat{all, m};
+  }
+  int n = kept;
+  if (!fits || n > kPartList) {
+    // Too many reach a bound (equal logits, or a row in order): the k-th best by bits, of the
+    // images and then of the places among those equal to it, counting the whole stretch each time
+    // (from memory: a copy in registers would cost every call a third of its waves).
+    auto count = [&](auto which, int turn) {
+      int c = 0;
+#pragma unroll 1
+      for (int p = begin + t; p < end; p += kPartThreads) c += which(image(number(p)), p) ? 1 : 0;
+#pragma unroll
+      for (int off = 32; off >= 1; off >>= 1) c += __shfl_xor(c, off, 64);
+      if (lane == 0) wcount[turn & 1][wave] = c;
+      __syncthreads();
+      c = 0;
+      for (int w = 0; w < kWaves; ++w) c += wcount[turn & 1][w];
+      return c;
+    };
+    __syncthreads();
+    int turn = 0;
+    uint32_t kth = 0u;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit, ++turn) {
+      const uint32_t next = kth | 1u << bit;
+      if (count([&](uint32_t y, int) { return y >= next; }, turn) >= k) kth = next;
+    }
+    int last = begin - 1;  // places up to `last` + 1 of those equal to it
+    const int rest = k - count([&](uint32_t y, int) { return y > kth; }, turn++);
+#pragma unroll 1
+    for (int step = 1 << (31 - __builtin_clz(end - begin)); step; step >>= 1, ++turn)
+      if (count([&](uint32_t y, int p) { return y == kth && p <= last + step; }, turn) < rest)
+        last += step;
+    if (t == 0) wcount[turn & 1][0] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int p = begin + t; p < end; p += kPartThreads) {
+      const uint32_t y = image(number(p));
+      if (y > kth || (y == kth && p <= last + 1)) {  // k of them, in any order
+        const int at = atomicAdd(&wcount[turn & 1][0], 1);
+        if (at < kPartList)
+          list[at] = Item{number(p), p};
+      }
+    }
+    __syncthreads();
+    n = min(wcount[turn & 1][0], kPartList);
+  }
+  rank_all<kPartThreads>(n, ranks, [&](int i) { return list[i]; },
+                         [](const Item& a, const Item& b) {
+                           return a.x > b.x || (a.x == b.x && a.token < b.token);
+                         });
+  __syncthreads();
+  Item* const out = items + (size_t)blockIdx.x * k;
+  for (int i = t; i < n; i += kPartThreads)
+    if (ranks[i] < k) out[ranks[i]] = list[i];
+  for (int i = n + t; i < k; i += kPartThreads) out[i] = Item{0.f, -1};
+}
+
+// One workgroup a request: its rows' sums, then the k best of its lists.
+constexpr int kMergeThreads = 1024, kMergeList = kMergeThreads;
+struct Best {
+  double v;
+  float x;
+  int beam, token;
+  __device__ __forceinline__ bool before(const Best& o) const {
+    if (v != o.v) return v > o.v;
+    if (beam != o.beam) return beam < o.beam;
+    if (x != o.x) return x > o.x;
+    return token < o.token;
+  }
+};
+
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(
+    const Stat* __restrict__ stats, const Item* __restrict__ items,
+    const float* __restrict__ scores, int W, int V, int k, int parts,
+    float* __restrict__ out_scores, int* __restrict__ out_beams, int* __restrict__ out_tokens) {
+  constexpr int kWaves = kMergeThreads / 64;
+  __shared__ double row_m[kMost], row_lse[kMost];  // row_lse NaN: a beam without continuations
+  __shared__ Best list[kMergeList];
+  __shared__ int ranks[kMergeList];
+  __shared__ uint32_t wbound[kWaves];
+  __shared__ int found;
+  const int r = blockIdx.x, t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  for (int b = wave; b < W; b += kWaves) {
+    const Stat* const st = stats + ((size_t)r * W + b) * parts;
+    float m = -INFINITY;
+    for (int p = lane; p < parts; p += 64) m = fmaxf(m, st[p].m);
+    m = wave_max(m);
+    double s = 0.0;
+    for (int p = lane; p < parts; p += 64) {
+      const Stat x = st[p];
+      s += x.sum * (x.m == m || x.sum == 0.0 ? 1.0 : exp((double)x.m - (double)m));
+    }
+    s = moe::wave_sum_f64(s);
+    if (lane == 0) {
+      const float score = scores[(size_t)r * W + b];
+      const bool good = m > -INFINITY && m < INFINITY && s == s &&
+                        score > -INFINITY && score < INFINITY;
+      row_m[b] = m;
+      row_lse[b] = good ? log(s) : __builtin_nan("");
+    }
+  }
+  __syncthreads();
+  const int each = parts * k, total = W * each;
+  // candidate i of the request's lists; of a beam without continuations the first k tokens
+  auto candidate = [&](int i, Best& c) {
+    const int b = i / each, j = i - b * each;
+    const Item x = items[((size_t)r * W + b) * each + j];
+    const double lse = row_lse[b];
+    c.beam = b;
+    if (lse != lse) {
+      c.v = -INFINITY;
+      c.x = -INFINITY;
+      c.token = j;
+      return j < min(k, V);
+    }
+    c.x = x.x;
+    c.token = x.token;
+    c.v = (double)scores[(size_t)r * W + b] + (((double)x.x - row_m[b]) - lse);
+    return x.token >= 0;
+  };
+  auto high = [](double v) {  // order-preserving image of its upper half
+    const uint32_t u = (uint32_t)(__builtin_bit_cast(uint64_t, v + 0.0) >> 32);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+  };
+  // The first kHeld candidates of a thread stay in registers: most calls' all.
+  constexpr int kHeld = 2;
+  Best c, held[kHeld];
+  uint32_t lm = 0u, image[kHeld];  // 0: none
+  const int rest = t + kHeld * kMergeThreads;
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) {
+    const int i = t + j * kMergeThreads;
+    image[j] = i < total && candidate(i, held[j]) ? high(held[j].v) : 0u;
+    lm = max(lm, image[j]);
+  }
+  for (int i = rest; i < total; i += kMergeThreads)
+    if (candidate(i, c)) lm = max(lm, high(c.v));
+  // (q = 1: beams' scores lie far apart, and one wave may hold all of the best)
+  const uint32_t bound = kth_of_lanes<kBoundBits + 3>(lm, k);
+  if (lane == 0) wbound[wave] = bound;
+  if (t == 0) found = 0;
+  ranks[t] = 0;
+  __syncthreads();
+  const uint32_t top = max(nth_of(wbound, kWaves, 1), 1u);
+  auto keep = [&](const Best& x) {
+    const int at = atomicAdd(&found, 1);
+    if (at < kMergeList) list[at] = x;
+  };
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j)
+    if (image[j] >= top) keep(held[j]);
+  for (int i = rest; i < total; i += kMergeThreads)
+    if (candidate(i, c) && high(c.v) >= top) keep(c);
+  __syncthreads();
+  const int n = found;
+  auto write = [&](int rank, const Best& x) {
+    out_scores[(size_t)r * k + rank] = (float)x.v;
+    out_beams[(size_t)r * k + rank] = x.beam;
+    out_tokens[(size_t)r * k + rank] = x.token;
+  };
+  if (n <= kMergeList) {
+    rank_all<kMergeThreads>(n, ranks, [&](int i) { return list[i]; },
+                            [](const Best& x, const Best& y) { return x.before(y); });
+    __syncthreads();
+    for (int i = t; i < n; i += kMergeThreads)
+      if (ranks[i] < k) write(ranks[i], list[i]);
+    return;
+  }
+  // Too many (equal scores): one after the other, each the best of those behind the last
+  Best last{INFINITY, INFINITY, -1, -1};
+  const Best none{-INFINITY, -INFINITY, INT32_MAX, INT32_MAX};
+  for (int rank = 0; rank < k; ++rank) {
+    Best best = none;
+    for (int i = t; i < total; i += kMergeThreads)
+      if (candidate(i, c) && last.before(c) && c.before(best)) best = c;
+    __syncthreads();
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) {
+      const Best o{__shfl_xor(best.v, off, 64), __shfl_xor(best.x, off, 64),
+                   __shfl_xor(best.beam, off, 64), __shfl_xor(best.token, off, 64)};
+      if (o.before(best)) best = o;
+    }
+    if (lane == 0) list[wave] = best;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w)
+      if (list[w].before(best)) best = list[w];
+    last = best;
+    if (t == 0) write(rank, best);
   }
 }
 
-// the k best of a request, one after the other: each the best of those behind the last
-template <class T>
-__global__ __launch_bounds__(kThreads) void select_kernel(
-    const T* __restrict__ logits, const float* __restrict__ scores, int W, int V, int k,
-    const double* __restrict__ stats, float* __restrict__ out_scores, int* __restrict__ out_beams,
-    int* __restrict__ out_tokens) {
-  __shared__ double bv[kThreads / 64];
-  __shared__ int64_t bi[kThreads / 64];
-  const int r = blockIdx.x, t = threadIdx.x;
-  double last_v = INFINITY;
-  int64_t last_i = -1;
-  auto before = [](double v, int64_t i, double w, int64_t j) { return v > w || (v == w && i < j); };
-  for (int n = 0; n < k; ++n) {
-    double best = -INFINITY;
-    int64_t at = INT64_MAX;
-    for (int b = 0; b < W; ++b) {
-      const double m = stats[2 * (r * W + b)], lse = stats[2 * (r * W + b) + 1];
-      const double score = scores[r * W + b];
-      const T* x = logits + (size_t)(r * W + b) * V;
-      for (int i = t; i < V; i += kThreads) {
-        double v = score + (((double)logit(x, i) - m) - lse);
-        if (v != v) v = -INFINITY;
-        const int64_t idx = (int64_t)b * V + i;
-        if (before(last_v, last_i, v, idx) && before(v, idx, best, at)) {
-          best = v;
-          at = idx;
-        }
-      }
-    }
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) {
-      const double v = __shfl_xor(best, off, 64);
-      const int64_t i = __shfl_xor(at, off, 64);
-      if (before(v, i, best, at)) {
-        best = v;
-        at = i;
-      }
-    }
-    if ((t & 63) == 0) {
-      bv[t >> 6] = best;
-      bi[t >> 6] = at;
-    }
-    __syncthreads();
-    for (int i = 0; i < kThreads / 64; ++i)
-      if (before(bv[i], bi[i], best, at)) {
-        best = bv[i];
-        at = bi[i];
-      }
-    __syncthreads();
-    last_v = best;
-    last_i = at;
-    if (t == 0) {
-      out_scores[r * k + n] = (float)best;
-      out_beams[r * k + n] = (int)(at / V);
-      out_tokens[r * k + n] = (int)(at % V);
-    }
-  }
+// Chunks of a stretch: as many as leave 512 workgroups, two a CU, of a call's rows.  us of both
+// launches
+inline int chunks_of(int64_t rows, int vocab) {
+  const int64_t all = ((int64_t)vocab + kChunk - 1) / kChunk;
+  const int64_t parts = std::min(all, std::max<int64_t>(1, (512 + rows - 1) / rows));
+  return (int)((all + parts - 1) / parts);
 }
+inline int64_t parts_of(int64_t rows, int vocab) {
+  const int64_t each = (int64_t)chunks_of(rows, vocab) * kChunk;
+  return (vocab + each - 1) / each;
+}
+inline size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
 }  // namespace beam
 
 extern "C" {
 
-size_t attn_beam_state_bytes(int rows, int vocab, int k) { return (size_t)rows * 16; }
+// 0 where there are too many stretches for a launch
+size_t attn_beam_state_bytes(int64_t rows, int vocab, int k) {
+  const int64_t n = rows * beam::parts_of(rows, vocab);
+  if (n * k >= (int64_t)1 << 31 || n * beam::kPartThreads >= (int64_t)1 << 32) return 0;
+  return beam::round256(n * sizeof(beam::Stat)) + n * k * sizeof(beam::Item);
+}
 
 int attn_launch_beam(const void* logits, bool f32, const float* scores, int batch, int width,
                      int vocab, int k, float* out_scores, int* out_beams, int* out_tokens,
                      void* state, hipStream_t s) {
-  double* stats = (double*)state;
-  auto go = [&](auto* x) {
-    using T = std::remove_pointer_t<decltype(x)>;
-    hipLaunchKernelGGL((beam::stats_kernel<std::remove_const_t<T>>), dim3(batch * width),
-                       dim3(beam::kThreads), 0, s, x, vocab, stats);
-    if (hipGetLastError() != hipSuccess) return -6;
-    hipLaunchKernelGGL((beam::select_kernel<std::remove_const_t<T>>), dim3(batch),
-                       dim3(beam::kThreads), 0, s, x, scores, width, vocab, k, stats, out_scores,
-                       out_beams, out_tokens);
-    return hipGetLastError() == hipSuccess ? 0 : -6;
-  };
-  return f32 ? go((const float*)logits) : go((const uint16_t*)logits);
+  const int64_t rows = (int64_t)batch * width;
+  const int parts = (int)beam::parts_of(rows, vocab), chunks = beam::chunks_of(rows, vocab);
+  beam::Stat* stats = (beam::Stat*)state;
+  beam::Item* items =
+      (beam::Item*)((char*)state + beam::round256(rows * parts * sizeof(beam::Stat)));
+  const dim3 grid((unsigned)(rows * parts)), threads(beam::kPartThreads);
+  if (f32)
+    hipLaunchKernelGGL(beam::part_kernel<float>, grid, threads, 0, s, (const float*)logits, vocab,
+                       k, parts, chunks, stats, items);
+  else
+    hipLaunchKernelGGL(beam::part_kernel<uint16_t>, grid, threads, 0, s, (const uint16_t*)logits,
+                       vocab, k, parts, chunks, stats, items);
+  if (hipGetLastError() != hipSuccess) return -6;
+  hipLaunchKernelGGL(beam::merge_kernel, dim3(batch), dim3(beam::kMergeThreads), 0, s, stats,
+                     items, scores, width, vocab, k, parts, out_scores, out_beams, out_tokens);
+  return hipGetLastError() == hipSuccess ? 0 : -6;
 }
 
 }  // extern "C"

@@ -331,12 +331,14 @@ MOE_API int attn_kv_copy_pages(void* kv_cache, int64_t layers, int64_t num_pages
 /* The k best continuations of each request over its beams and the vocabulary: logits [batch,
  * width, vocab] bf16, or fp32 where logits_f32 is not 0; scores [batch, width] fp32, the beams'
  * own (-inf: a beam that has ended, or is not there yet).  The score of token t after beam b is
- * scores[b] + logits[b][t] - log sum exp(logits[b]), summed and compared in fp64 and rounded once
- * to fp32; a row of logits without a maximum (a NaN, +inf, nothing but -inf) and a score of
- * NaN give -inf.  In descending order, equal ones by beam, then token: out_scores, out_beams (0
- * .. width - 1 within the request) and out_tokens [batch, k].  width and k up to 64, k at
- * most width * vocab.  The workspace needs no initialisation; calls on one have to follow
- * one another. */
+ * scores[b] + logits[b][t] - log sum exp(logits[b]), summed and compared in fp64 (the
+ * exponentials off by a few 2^-24 of themselves) and rounded once to fp32; a row of
+ * logits without a maximum (a NaN, +inf, nothing but -inf) and a beam whose own score is not
+ * finite give -inf.  In descending order, equal ones by beam, then logit, then token: out_scores,
+ * out_beams (0 .. width - 1 within the request) and out_tokens [batch, k].  width and k up to
+ * 64, k at most width * vocab, fewer than 2^22 stretches of 16384 logits of a row (2^31 / k
+ * where k is more).  Rows of logits may begin at any element.  The workspace needs no initialisation; calls on one have to
+ * follow one another.  attn_beam_workspace_bytes is 0 where the call would be refused. */
 MOE_API size_t attn_beam_workspace_bytes(int64_t batch, int64_t width, int64_t vocab, int64_t k);
 MOE_API int attn_beam_top_k(const void* logits, int32_t logits_f32, int64_t batch, int64_t width,
                             int64_t vocab, const float* scores, int64_t k, float* out_scores,
