@@ -9,6 +9,11 @@ A chat loop drives it exactly as the reference's chat.py does: ``prefill``
 (or ``extend``) the prompt, ``sample``, then ``decode`` + ``sample`` per
 generated token, ``popn`` to roll the cache back.  ``kv_dtype`` torch.float8_e4m3fn
 keeps the cache in 8 bits: half its bytes in memory and in every decode step.
+
+Beyond one continuation at a time: ``decode_tree`` verifies a tree of drafted tokens in one
+forward and gives the tokens that ``decode`` and ``sample`` would have given one by one (up to
+the kernels' rounding), and ``beam_search`` follows the best continuations by their
+probability (``max_batch`` beams).
 """
 from __future__ import annotations
 
@@ -27,7 +32,7 @@ class Engine:
 
     def __init__(self, model_path: str | Path | None = None, config: GPTOssConfig | None = None,
                  device: str = "cuda", max_total_seq_len: int | None = None,
-                 kv_dtype: torch.dtype = torch.bfloat16):
+                 kv_dtype: torch.dtype = torch.bfloat16, max_batch: int = 1):
         if model_path is not None:
             self.model_path = Path(model_path)
             self.config = config or GPTOssConfig.from_file(self.model_path / "config.json")
@@ -42,11 +47,12 @@ class Engine:
             weights.TorchCheckpoint(self.model_path, self.device).load_into(self.model)
         cw = self.config.context_window_size or 40960
         self.paged_kv_cache = self.model.create_paged_kv_cache(
-            1, max_total_seq_len or cw, self.config.prefill_chunk_size, 16, self.device,
+            max_batch, max_total_seq_len or cw, self.config.prefill_chunk_size, 16, self.device,
             dtype=kv_dtype)
         self.sample_parameters = {"temperature": 0.7, "top_p": 0.9, "random_seed": 0.5}
         self._sample_ws = A.sample_workspace(1, self.device)
         self._token = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._tree_ws: torch.Tensor | None = None  # the sampler's, for a tree's nodes
 
     # -- sequences (engine.py:109-131) ---------------------------------------------
     def clear_kv_cache(self) -> None:
@@ -95,6 +101,100 @@ class Engine:
     @torch.no_grad()
     def extend(self, input_tokens, sequence_id: int = 0) -> torch.Tensor:
         return self._run(self.model.extend, input_tokens, sequence_id)
+
+    # -- several continuations at once ---------------------------------------------------
+    @torch.no_grad()
+    def decode_tree(self, input_tokens, parents, sequence_id: int = 0) -> list[int]:
+        """One step over a tree of drafted tokens: ``input_tokens[0]`` is the last sampled token
+        (as ``decode`` takes it), every other one a draft for the place after
+        ``parents[i]`` < i (``parents[0]`` is -1).  Each node's next token is sampled as
+        ``sample`` does; the nodes on the way from the root that were sampled stay in the
+        cache.  Returns the new tokens, the accepted ones and the one sampled after the last
+        of them: at least one, and the next call's root is the last."""
+        ids, parents = self._ids(input_tokens), list(parents)
+        n, cache, p = len(parents), self.paged_kv_cache, self.sample_parameters
+        if ids.numel() != n:
+            raise ValueError(f"{ids.numel()} tokens and {n} parents")
+        if self._tree_ws is None or self._tree_ws.numel() < n * self._sample_ws.numel():
+            self._tree_ws = A.sample_workspace(n, self.device)
+        tables = cache.begin_tree([sequence_id], [parents])
+        try:
+            logits = self.model.decode_logits_bf16(self.model.embed(ids), cache)
+            chosen = A.sample_top_p(logits, p["temperature"], p["top_p"], p["random_seed"],
+                                    self._tree_ws)
+            path, count, after = A.tree_commit(
+                cache.data, tables.page_indptr, tables.page_indices, tables.kv_len,
+                tables.q_indptr, n, ids, tables.parents, chosen)
+            self._token.copy_(after)
+            new = torch.cat([count, after, ids[path.clamp(min=0).long()]]).tolist()
+        except Exception:
+            cache.popn(sequence_id, n)
+            raise
+        finally:
+            cache.end_forward()
+        accepted = new[0]
+        cache.popn(sequence_id, n - accepted)
+        return new[3:2 + accepted] + [new[1]]
+
+    @torch.no_grad()
+    def beam_search(self, input_tokens, width: int, max_new_tokens: int, stop_tokens=(),
+                    length_penalty: float = 0.0) -> list[tuple[list[int], float]]:
+        """The ``width`` best continuations of a prompt found by beam search: at most
+        ``max_new_tokens`` tokens each (a stop token ends one), with the sum of their log
+        probabilities, best first by that sum over length ** ``length_penalty``.  The
+        beams share the prompt's pages and each other's; the engine's cache needs room for
+        ``width`` sequences (``max_batch``) and is left as it was."""
+        cache, stops = self.paged_kv_cache, set(int(t) for t in stop_tokens)
+        vocab = self.config.vocab_size
+        # of the best width (1 + stops) continuations no more than width stops end
+        k = min(width * (1 + len(stops)), width * vocab)
+        if not 1 <= width <= cache.max_batch or k > A.MAX_BEAMS or max_new_tokens < 1:
+            raise ValueError(f"beam search of width {width} with {len(stops)} stop tokens and "
+                             f"{max_new_tokens} new tokens: the cache has room for "
+                             f"{cache.max_batch} sequences, the selection for {A.MAX_BEAMS}")
+        beams = [([], 0.0)]
+        ended: list[tuple[list[int], float]] = []
+        seqs = [self.begin_sequence()]
+
+        def worth(beam):
+            return beam[1] / max(1, len(beam[0])) ** length_penalty
+
+        try:
+            logits = self.prefill(input_tokens, seqs[0]).view(1, vocab)
+            for step in range(max_new_tokens):
+                scores = torch.tensor([[s for _, s in beams]], dtype=torch.float32,
+                                      device=self.device)
+                best = A.beam_top_k(logits, scores, min(k, len(beams) * vocab))
+                best = zip(*(t[0].tolist() for t in best))
+                live, parents = [], []
+                for score, parent, token in best:
+                    if score == float("-inf") or len(live) == width:
+                        break
+                    if token in stops:
+                        ended.append((beams[parent][0] + [token], score))
+                    else:
+                        live.append((beams[parent][0] + [token], score))
+                        parents.append(parent)
+                beams = live
+                if not live or len(ended) >= width or step == max_new_tokens - 1:
+                    break
+                new = seqs[:len(live)]
+                while len(new) < len(live):
+                    new.append(self.__class__.next_seq_id)
+                    self.__class__.next_seq_id += 1
+                cache.branch(seqs, parents, new)
+                seqs = new
+                embed = self.model.embed(self._ids([tokens[-1] for tokens, _ in live]))
+                cache.begin_forward(seqs, [1] * len(live))
+                try:
+                    logits = self.model.decode_logits_bf16(embed, cache)
+                finally:
+                    cache.end_forward()
+        finally:
+            for sid in seqs:
+                if sid in cache.seqs:
+                    cache.remove_sequence(sid)
+        return sorted(ended + beams, key=worth, reverse=True)[:width]
 
     # -- the decode step in one HIP graph ---------------------------------------------
     def _step_body(self) -> None:

@@ -19,6 +19,9 @@ Over an 8-bit cache (``PagedKVCache(dtype=torch.float8_e4m3fn)``) k and v are
 quantised as they are written -- by the RoPE epilogue, or from the bf16 rows
 that the fused projections leave in the cache's staging pages -- and the 8-bit
 forms of the attention kernels read them.
+
+A forward of trees of drafted tokens (``PagedKVCache.begin_tree``) is the same but for the
+attention, which takes each node's mask over its tree.
 """
 from __future__ import annotations
 
@@ -178,6 +181,11 @@ class AttentionBlock(torch.nn.Module):
             decode = A.decode_fp8 if cache.fp8 else A.decode
             decode(q, layer, tables.page_indptr, tables.page_indices, tables.kv_len, span,
                    window, self.sm_scale, self.sinks, o, ws)
+        elif tables.tree_mask is not None:
+            tree = A.tree_fp8 if cache.fp8 else A.tree
+            tree(q, tables.q_indptr, tables.max_q_len, tables.tree_mask, tables.positions, layer,
+                 tables.page_indptr, tables.page_indices, tables.kv_len, window, self.sm_scale,
+                 self.sinks, o, tables.max_kv_len)
         else:
             prefill = A.prefill_fp8 if cache.fp8 else A.prefill
             prefill(q, tables.q_indptr, tables.max_q_len, layer, tables.page_indptr,

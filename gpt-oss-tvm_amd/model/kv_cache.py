@@ -26,16 +26,25 @@ With ``dtype=torch.float8_e4m3fn`` the cache holds 8-bit rows with a scale byte
 each (the format of include/attn_gfx950.h): one uint8 tensor [layers, pages,
 16640], half a bf16 cache's bytes, quantised as it is written and read by the
 8-bit attention kernels.  The tables are the same.
+
+Sequences may share pages: ``branch`` lets several go on from what one holds (beams), at
+no cost but the page lists'.  A page that others hold too and that a forward would write to is
+copied first, in all layers by one launch.
+
+``begin_tree`` appends a tree of drafted tokens to each sequence in place of a chunk: the tables
+then also have each node's mask over its tree, and positions by depth.
 """
 from __future__ import annotations
 
 import dataclasses
 
+import numpy as np
 import torch
 
 PAGE_SIZE = 16
 FP8_PAGE_BYTES = 16640  # of a page of an 8-bit cache
 STAGED = 64             # tokens of the largest fused decode projection
+TREE_MAX_NODES = 1024   # of a sequence's tree of drafted tokens
 
 
 @dataclasses.dataclass
@@ -59,10 +68,14 @@ class ForwardTables:
     page_indices: torch.Tensor  # [pages] int32
     kv_len: torch.Tensor        # [batch] int32
     windows: tuple              # per sequence: sliding window (0 = none)
+    # of a forward of trees: bit j % 32 of word j / 32, node i sees node j of its sequence;
+    # each node's parent in its tree (-1: the root)
+    tree_mask: torch.Tensor | None = None  # [num_tokens, words] int32
+    parents: torch.Tensor | None = None    # [num_tokens] int32
 
     @property
     def is_decode(self) -> bool:
-        return self.max_q_len == 1
+        return self.max_q_len == 1 and self.tree_mask is None
 
 
 class PagedKVCache:
@@ -90,6 +103,7 @@ class PagedKVCache:
             self.data = torch.zeros((num_layers, num_pages, 2, kv_heads, PAGE_SIZE, head_dim),
                                     dtype=dtype, device=device)
         self.free = list(range(num_pages - 1, -1, -1))  # pop() hands out page 0 first
+        self._refs = [0] * num_pages                     # sequences that hold a page
         self.seqs: dict[int, _Seq] = {}
         # The forward tables live in one device buffer at fixed offsets (kernels
         # captured in a graph keep their addresses), uploaded from a pinned
@@ -97,9 +111,10 @@ class PagedKVCache:
         # tokens (every decode step) keeps its positions and slots in short
         # arrays ahead of the page indices, so its tables are one contiguous
         # range and one copy; a longer forward uses the long arrays at the end
-        # (three copies, each spanning only what the forward uses).
+        # (three copies, each spanning only what the forward uses).  Last the pages that a
+        # forward copies before it writes to them, sources and then destinations.
         sizes = (max_batch + 1, max_batch + 1, max_batch, max_batch, max_batch, num_pages,
-                 max_tokens, max_tokens)
+                 max_tokens, max_tokens, 2 * max_batch)
         self._tables_dev = torch.zeros(sum(sizes), dtype=torch.int32, device=device)
         # two staging buffers used in turn: a forward waits only for the copy
         # made from its buffer two forwards ago (an event), not for the stream
@@ -113,7 +128,8 @@ class PagedKVCache:
             views.append(self._tables_dev[off:off + k])
             off += k
         (self._q_indptr, self._page_indptr, self._kv_len, self._positions_short,
-         self._slots_short, self._page_indices, self._positions, self._slots) = views
+         self._slots_short, self._page_indices, self._positions, self._slots,
+         self._copies) = views
         self.tables: ForwardTables | None = None
         self._decode_ws: torch.Tensor | None = None
         self._decode_ws_held: list = []
@@ -157,8 +173,43 @@ class PagedKVCache:
                              "the reference runs with 0 (engine.py:62, 120)")
         self.seqs[seq_id].window = int(window)
 
+    def _take(self) -> int:
+        page = self.free.pop()
+        self._refs[page] = 1
+        return page
+
+    def _drop(self, pages) -> None:
+        for page in reversed(pages):
+            self._refs[page] -= 1
+            if self._refs[page] == 0:
+                self.free.append(page)
+
     def remove_sequence(self, seq_id: int) -> None:
-        self.free.extend(reversed(self.seqs.pop(seq_id).pages))
+        self._drop(self.seqs.pop(seq_id).pages)
+
+    def branch(self, seq_ids, parents, new_ids=None) -> None:
+        """Sequence ``new_ids[i]`` goes on from what ``seq_ids[parents[i]]`` holds, sharing its
+        pages; the sequences ``seq_ids`` end (``new_ids``, by default the first of them, may
+        name them again)."""
+        seq_ids, parents = list(seq_ids), [int(p) for p in parents]
+        new_ids = seq_ids[:len(parents)] if new_ids is None else list(new_ids)
+        if len(new_ids) != len(parents) or len(set(new_ids)) != len(new_ids):
+            raise ValueError(f"{len(parents)} branches need as many different sequences, "
+                             f"not {new_ids}")
+        if len(set(seq_ids)) != len(seq_ids) or any(s not in self.seqs for s in seq_ids):
+            raise ValueError(f"sequences {seq_ids} are not all there, or not different")
+        if any(not 0 <= p < len(seq_ids) for p in parents):
+            raise ValueError(f"parents {parents} of {len(seq_ids)} sequences")
+        taken = [s for s in new_ids if s in self.seqs and s not in seq_ids]
+        if taken:
+            raise ValueError(f"sequence {taken[0]} exists")
+        old = [self.seqs.pop(s) for s in seq_ids]
+        for sid, p in zip(new_ids, parents):
+            self.seqs[sid] = _Seq(old[p].length, list(old[p].pages), old[p].window)
+            for page in old[p].pages:
+                self._refs[page] += 1
+        for s in old:
+            self._drop(s.pages)
 
     def clear(self) -> None:
         for sid in list(self.seqs):
@@ -170,7 +221,7 @@ class PagedKVCache:
             raise ValueError(f"popn({n}) on a sequence of {s.length} tokens")
         s.length -= n
         keep = -(-s.length // PAGE_SIZE)
-        self.free.extend(reversed(s.pages[keep:]))
+        self._drop(s.pages[keep:])
         del s.pages[keep:]
 
     def total_sequence_length(self) -> int:
@@ -218,7 +269,7 @@ class PagedKVCache:
             raise MemoryError(f"KV cache full: {need} pages needed, {len(self.free)} free")
         self.add_sequence(seq_id)
         s = self.seqs[seq_id]
-        s.pages = [self.free.pop() for _ in range(need)]
+        s.pages = [self._take() for _ in range(need)]
         s.length, s.window = old.length, old.window
         try:
             if s.length:
@@ -229,10 +280,51 @@ class PagedKVCache:
             self.remove_sequence(seq_id)
             raise
 
+    def _copy_pages(self, src: torch.Tensor, dst: torch.Tensor) -> None:
+        if self.data.is_cuda and (self.fp8 or self.data.dtype == torch.bfloat16):
+            import attn_native
+            attn_native.kv_copy_pages(self.data, src, dst)
+        else:
+            self.data[:, dst.long()] = self.data[:, src.long()]
+
     # -- one forward ---------------------------------------------------------------
-    def begin_forward(self, seq_ids, append_lengths) -> ForwardTables:
+    def _shares_last(self, s: _Seq) -> bool:
+        """Whether a sequence's next token goes to a page that others hold too."""
+        return s.length % PAGE_SIZE != 0 and self._refs[s.pages[-1]] > 1
+
+    def begin_tree(self, seq_ids, parents) -> ForwardTables:
+        """``begin_forward`` for a tree of drafted tokens each: ``parents[i]`` lists its nodes'
+        parents within the tree, -1 first (the last sampled token) and every other one
+        before its node.  Nodes lie one after the other behind the cached tokens; a node's
+        position is the number of those plus its depth.  ``popn`` takes back what is not
+        accepted, after ``attn_native.tree_commit`` has moved what is."""
+        parents = [[int(p) for p in tree] for tree in parents]
+        seq_ids = list(seq_ids)
+        longest = max((len(tree) for tree in parents), default=0)
+        words = max(1, -(-longest // 32))
+        if longest > TREE_MAX_NODES:
+            raise ValueError(f"a tree of {longest} nodes, at most {TREE_MAX_NODES}")
+        depths, masks = [], []
+        for sid, tree in zip(seq_ids, parents):
+            if tree[:1] != [-1] or any(not 0 <= p < i for i, p in enumerate(tree) if i):
+                raise ValueError("a tree's nodes come after their parents, the root (-1) first")
+            depth, sees = [0] * len(tree), [1] * len(tree)
+            for i, p in enumerate(tree):
+                if i:
+                    depth[i], sees[i] = depth[p] + 1, sees[p] | 1 << i
+            depths.append(depth)
+            masks += [[(x >> (32 * w)) & 0xFFFFFFFF for w in range(words)] for x in sees]
+        tables = self.begin_forward(seq_ids, [len(tree) for tree in parents], depths)
+        flat = np.array([p for tree in parents for p in tree], dtype=np.int32)
+        mask = np.array(masks, dtype=np.uint32).view(np.int32).reshape(-1, words)
+        tables.parents = torch.from_numpy(flat).to(self.data.device)
+        tables.tree_mask = torch.from_numpy(mask).to(self.data.device)
+        return tables
+
+    def begin_forward(self, seq_ids, append_lengths, depths=None) -> ForwardTables:
         """Append ``append_lengths[i]`` tokens to sequence ``seq_ids[i]``
-        (pages allocated as needed) and upload the tables of this forward."""
+        (pages allocated as needed) and upload the tables of this forward.  ``depths[i]``: the
+        tokens' positions behind the sequence's end, where they do not follow one another."""
         seq_ids, append_lengths = list(seq_ids), [int(a) for a in append_lengths]
         batch, n = len(seq_ids), sum(append_lengths)
         if batch > self.max_batch or n > self.max_tokens:
@@ -241,16 +333,23 @@ class PagedKVCache:
         if min(append_lengths, default=1) < 1:
             raise ValueError("every sequence of a forward appends at least one token")
         need = sum(max(0, -(-(self.seqs[s].length + a) // PAGE_SIZE) - len(self.seqs[s].pages))
-                   for s, a in zip(seq_ids, append_lengths))
+                   + self._shares_last(self.seqs[s]) for s, a in zip(seq_ids, append_lengths))
         if need > len(self.free):
             raise MemoryError(f"KV cache full: {need} pages needed, {len(self.free)} free")
         q_indptr, positions, slots, page_indptr, page_indices, kv_len = [0], [], [], [0], [], []
-        for sid, a in zip(seq_ids, append_lengths):
+        copies = []
+        for i, (sid, a) in enumerate(zip(seq_ids, append_lengths)):
             s = self.seqs[sid]
+            if self._shares_last(s):  # others keep that page
+                shared = s.pages[-1]
+                s.pages[-1] = self._take()
+                self._drop([shared])
+                copies.append((shared, s.pages[-1]))
             while len(s.pages) * PAGE_SIZE < s.length + a:
-                s.pages.append(self.free.pop())
+                s.pages.append(self._take())
+            positions.extend(range(s.length, s.length + a) if depths is None
+                             else (s.length + d for d in depths[i]))
             for p in range(s.length, s.length + a):
-                positions.append(p)
                 slots.append(s.pages[p // PAGE_SIZE] * PAGE_SIZE + p % PAGE_SIZE)
             s.length += a
             q_indptr.append(q_indptr[-1] + a)
@@ -270,6 +369,9 @@ class PagedKVCache:
         ranges = [(0, offs[5] + len(page_indices))]
         if not short:
             ranges += [(pos_off, pos_off + n), (slot_off, slot_off + n)]
+        if copies:
+            ranges.append((offs[8], offs[8] + 2 * len(copies)))
+            host[offs[8]:offs[8] + 2 * len(copies)] = torch.tensor(copies, dtype=torch.int32).t().flatten()
         for a, b in ranges:
             self._tables_dev[a:b].copy_(host[a:b], non_blocking=True)
         if self.data.is_cuda:
@@ -277,6 +379,8 @@ class PagedKVCache:
             ev.record()
             self._stage_events[j] = ev
             self._stage = j ^ 1
+        if copies:
+            self._copy_pages(*self._copies[:2 * len(copies)].split(len(copies)))
         self.tables = ForwardTables(
             batch=batch, num_tokens=n, max_q_len=max(append_lengths),
             max_kv_len=max(kv_len), q_indptr=self._q_indptr[:batch + 1],

@@ -155,3 +155,118 @@ def test_oracle_attention_seen_is_the_causal_one():
         for a, b in zip(AO.attention_seen(q, k, v, mask, sinks),
                         AO.attention_sink(q, k, v, np.array([6, 7, 8]), window, sinks)):
             np.testing.assert_allclose(a, b, rtol=1e-12)
+
+
+# -- the cache's host side ---------------------------------------------------------------------
+
+def make(pages=12, batch=4, tokens=64):
+    from model.kv_cache import PagedKVCache
+    return PagedKVCache(num_layers=2, num_pages=pages, max_batch=batch, max_tokens=tokens,
+                        device="cpu", dtype=torch.float32)
+
+
+def write(c, t, values):
+    """Row i of a forward's tokens gets values[i] in k and -values[i] in v, in every layer."""
+    for i, slot in enumerate(t.slots.tolist()):
+        c.data[:, slot // 16, 0, :, slot % 16] = float(values[i])
+        c.data[:, slot // 16, 1, :, slot % 16] = -float(values[i])
+    c.end_forward()
+
+
+def rows(c, sid):
+    out = []
+    for layer in range(2):
+        k, v = c.read(sid, layer)
+        assert torch.equal(k, -v) and (k == k[:, :1, :1]).all()
+        out.append(k[:, 0, 0].tolist())
+    assert out[0] == out[1]
+    return out[0]
+
+
+def test_branches_share_pages_until_they_write():
+    c = make()
+    c.add_sequence(0)
+    c.enable_sliding_window(0, 128)
+    write(c, c.begin_forward([0], [20]), range(20))
+    c.branch([0], [0, 0, 0], [5, 6, 0])
+    assert len(c.free) == 10 and c.total_sequence_length() == 60
+    assert c.seqs[5].pages == c.seqs[6].pages == c.seqs[0].pages
+    t = c.begin_forward([5, 6, 0], [1, 1, 1])       # two of three copy the part-filled page
+    assert len(c.free) == 8 and t.windows == (128,) * 3
+    write(c, t, [100, 101, 102])
+    for sid, last in ((5, 100), (6, 101), (0, 102)):
+        assert rows(c, sid) == list(range(20)) + [last]
+    # beams 6 and 0 end, 5 goes on twice
+    c.branch([5, 6, 0], [0, 0, 1], [5, 6, 0])
+    assert len(c.free) == 9
+    write(c, c.begin_forward([5, 6, 0], [1, 1, 13]), [200, 201] + list(range(300, 313)))
+    assert rows(c, 5) == list(range(20)) + [100, 200]
+    assert rows(c, 6) == list(range(20)) + [100, 201]
+    assert rows(c, 0) == list(range(20)) + [101] + list(range(300, 313))
+    for sid in (5, 0, 6):
+        c.remove_sequence(sid)
+    assert sorted(c.free) == list(range(12)) and not any(c._refs)
+
+
+def test_branch_at_a_page_end_and_popn_into_shared_pages():
+    c = make()
+    c.add_sequence(0)
+    write(c, c.begin_forward([0], [32]), range(32))
+    c.branch([0], [0, 0], [0, 1])
+    write(c, c.begin_forward([0, 1], [1, 1]), [50, 51])     # pages of their own: nothing to copy
+    assert len(c.free) == 8
+    c.popn(1, 13)                                            # into the shared second page
+    assert len(c.free) == 9
+    write(c, c.begin_forward([1], [2]), [60, 61])            # which is copied first
+    assert len(c.free) == 8
+    assert rows(c, 1) == list(range(20)) + [60, 61]
+    assert rows(c, 0) == list(range(32)) + [50]
+    c.popn(0, 33)
+    write(c, c.begin_forward([0], [1]), [7])
+    assert rows(c, 0) == [7] and rows(c, 1) == list(range(20)) + [60, 61]
+    c.clear()
+    assert sorted(c.free) == list(range(12)) and not any(c._refs)
+
+
+def test_branch_refusals():
+    c = make(pages=3)
+    c.add_sequence(0)
+    c.add_sequence(1)
+    write(c, c.begin_forward([0], [17]), range(17))
+    for args in (([0], [0, 0]), ([0], [1]), ([0], [-1]), ([0, 0], [0]), ([7], [0]),
+                 ([0], [0, 0], [2, 2]), ([0], [0, 0], [0, 1]), ([0], [0, 0], [2])):
+        with pytest.raises(ValueError):
+            c.branch(*args)
+    assert c.seqs[0].length == 17 and sorted(c.seqs) == [0, 1] and len(c.free) == 1
+    c.branch([0], [0, 0, 0], [0, 2, 3])
+    with pytest.raises(MemoryError):                 # two copies needed, one page free
+        c.begin_forward([0, 2, 3], [1, 1, 1])
+    assert c.seqs[0].pages == c.seqs[2].pages == c.seqs[3].pages and len(c.free) == 1
+    c.branch([0, 2, 3], [], [])                      # no branch: all of them end
+    assert sorted(c.seqs) == [1] and len(c.free) == 3
+
+
+def test_begin_tree_tables():
+    c = make()
+    c.add_sequence(0)
+    c.add_sequence(1)
+    write(c, c.begin_forward([0, 1], [20, 3]), range(23))
+    wide = [-1] + [0] * 39
+    t = c.begin_tree([0, 1], [[-1, 0, 0, 1, 3], wide])
+    assert not t.is_decode and t.max_q_len == 40 and t.kv_len.tolist() == [25, 43]
+    assert t.positions.tolist() == [20, 21, 21, 22, 23] + [3] + [4] * 39
+    assert t.parents.tolist() == [-1, 0, 0, 1, 3] + wide
+    ids = c.seqs[0].pages
+    assert t.slots[:5].tolist() == [ids[1] * 16 + 4 + i for i in range(5)]
+    m = t.tree_mask.numpy().view(np.uint32)
+    assert m.shape == (45, 2)
+    assert m[:5, 0].tolist() == [1, 3, 5, 11, 27] and not m[:5, 1].any()
+    assert m[5 + 31].tolist() == [1 | 1 << 31, 0] and m[5 + 32].tolist() == [1, 1]
+    c.end_forward()
+    c.popn(0, 3)
+    assert c.seq_len(0) == 22
+    for bad in ([], [0], [-1, 1], [-1, -1], [-1, 0, 5], [-1] + [0] * 1024):
+        with pytest.raises(ValueError):
+            c.begin_tree([0], [bad])
+    assert c.seq_len(0) == 22 and c.tables is None
+    assert not c.begin_tree([0], [[-1]]).is_decode
