@@ -3,7 +3,7 @@
 
 Same rules as ``moe_native``: GPU tensors only, dtype / shape / contiguity
 checked before anything is launched, torch's current stream, RuntimeError on
-a non-zero status, no fallback when the library is missing.
+a non-zero status, no fallback when a library is missing.
 """
 from __future__ import annotations
 
@@ -13,6 +13,12 @@ import torch
 
 import moe_native
 from moe_native import _check, _expect, _ptr, _stream
+
+try:
+    import attn_binding  # csrc/attn_binding.cpp, over the library that moe_native loaded
+except ImportError as e:
+    raise ImportError("attn_binding.so is missing or does not load: build it with "
+                      "`python gpt-oss-tvm_amd/build_native.py` (or __graft_entry__.build())") from e
 
 _lib = moe_native.lib()
 
@@ -498,36 +504,10 @@ def prefill_fp8(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, kv_cach
 
 
 # -- several continuations: trees of drafted tokens, beams -----------------------------------------
+# Their checks and calls are in csrc/attn_binding.cpp: in Python they take longer than the kernels
+# of a small call.
 
-BF16_PAGE_BYTES = 2 * KV_HEADS * PAGE * HEAD_DIM * 2
 TREE_MAX_NODES, MAX_BEAMS = 1024, 64
-
-
-def _on_current(t, name, dtype):
-    """The index of the device that `t` is on, the current one, and the stream."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _expect(t, name, dtype)
-    index = torch.cuda.current_device()
-    if t.get_device() != index:
-        raise ValueError(f"{name}: on {t.device}, expected cuda:{index}, the current device")
-    return index, _stream()
-
-
-def _tree(fn, what, q, q_indptr, max_q_len, tree_mask, positions, kv_cache, pages, dev, stream,
-          page_indptr, page_indices, kv_len, window, sm_scale, sinks, out, max_kv_len):
-    n, batch = _count(q, "q", _BF16), _count(q_indptr, "q_indptr", _I32T) - 1
-    _need(q_indptr, "q_indptr", _I32T, (batch + 1,), dev)
-    _need_tables(q, page_indptr, page_indices, kv_len, sinks, out, batch, dev)
-    words = _shape(tree_mask)[-1] if _shape(tree_mask) else 0
-    _need(tree_mask, "tree_mask", _I32T, (n, words), dev)
-    _need(positions, "positions", _I32T, (n,), dev)
-    need = _lib.attn_tree_workspace_bytes(batch, max_q_len, max_kv_len, window)
-    ws = torch.empty(need, dtype=_U8, device=q.device) if need else None
-    _check(fn(q.data_ptr(), n, q_indptr.data_ptr(), batch, max_q_len, tree_mask.data_ptr(), words,
-              positions.data_ptr(), kv_cache.data_ptr(), pages, page_indptr.data_ptr(),
-              page_indices.data_ptr(), kv_len.data_ptr(), max_kv_len, window, sm_scale,
-              sinks.data_ptr(), out.data_ptr(), _ptr(ws), need, stream), what)
-    return out
 
 
 def tree(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, tree_mask: torch.Tensor,
@@ -539,12 +519,8 @@ def tree(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, tree_mask: tor
     % 32 of word j / 32 for node j of its sequence.  ``positions`` [n]: the cached tokens' number
     plus a node's depth.  The softmax has the sink as a further logit and rounds once.
     ``max_q_len`` (at most 1024) bounds the trees; ``max_kv_len`` as in ``prefill``."""
-    dev, stream = _on_current(kv_cache, "kv_cache", _BF16)
-    pages = _count(kv_cache, "kv_cache", _BF16)
-    _need(kv_cache, "kv_cache", _BF16, (pages, 2, KV_HEADS, PAGE, HEAD_DIM), dev)
-    return _tree(_lib.attn_tree, "attn_tree", q, q_indptr, max_q_len, tree_mask, positions,
-                 kv_cache, pages, dev, stream, page_indptr, page_indices, kv_len, window, sm_scale,
-                 sinks, out, max_kv_len)
+    return attn_binding.tree(q, q_indptr, max_q_len, tree_mask, positions, kv_cache, page_indptr,
+                             page_indices, kv_len, window, sm_scale, sinks, out, max_kv_len, False)
 
 
 def tree_fp8(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, tree_mask: torch.Tensor,
@@ -552,20 +528,8 @@ def tree_fp8(q: torch.Tensor, q_indptr: torch.Tensor, max_q_len: int, tree_mask:
              page_indices: torch.Tensor, kv_len: torch.Tensor, window: int, sm_scale: float,
              sinks: torch.Tensor, out: torch.Tensor, max_kv_len: int = 0) -> torch.Tensor:
     """``tree`` over the 8-bit cache."""
-    pages, dev, stream = _need_fp8(kv_cache)
-    return _tree(_lib.attn_tree_fp8, "attn_tree_fp8", q, q_indptr, max_q_len, tree_mask, positions,
-                 kv_cache, pages, dev, stream, page_indptr, page_indices, kv_len, window, sm_scale,
-                 sinks, out, max_kv_len)
-
-
-def _layers(kv_cache):
-    """Of all layers of a cache: its layers, pages, bytes of a page, device and stream."""
-    fp8 = getattr(kv_cache, "dtype", None) is _U8
-    dev, stream = _on_current(kv_cache, "kv_cache", _U8 if fp8 else _BF16)
-    layers, pages = kv_cache.shape[:2] if kv_cache.dim() > 1 else (0, 0)
-    shape = (FP8_PAGE_BYTES,) if fp8 else (2, KV_HEADS, PAGE, HEAD_DIM)
-    _need(kv_cache, "kv_cache", _U8 if fp8 else _BF16, (layers, pages, *shape), dev)
-    return layers, pages, FP8_PAGE_BYTES if fp8 else BF16_PAGE_BYTES, dev, stream
+    return attn_binding.tree(q, q_indptr, max_q_len, tree_mask, positions, kv_cache, page_indptr,
+                             page_indices, kv_len, window, sm_scale, sinks, out, max_kv_len, True)
 
 
 def tree_commit(kv_cache: torch.Tensor, page_indptr: torch.Tensor, page_indices: torch.Tensor,
@@ -576,24 +540,8 @@ def tree_commit(kv_cache: torch.Tensor, page_indptr: torch.Tensor, page_indices:
     the accepted nodes' rows moved behind the cached ones in all layers of ``kv_cache`` [layers,
     pages, ...] (bf16 or 8-bit).  Returns path [n] (each sequence's accepted nodes in order, then
     -1), count [batch] and next [batch], the token chosen after the last accepted node."""
-    layers, pages, page_bytes, dev, stream = _layers(kv_cache)
-    n, batch = _count(tokens, "tokens", _I32T), _count(q_indptr, "q_indptr", _I32T) - 1
-    _need(q_indptr, "q_indptr", _I32T, (batch + 1,), dev)
-    _need(page_indptr, "page_indptr", _I32T, (batch + 1,), dev)
-    _need(page_indices, "page_indices", _I32T, _shape(page_indices), dev)
-    _need(kv_len, "kv_len", _I32T, (batch,), dev)
-    _need(tokens, "tokens", _I32T, (n,), dev)
-    _need(parents, "parents", _I32T, (n,), dev)
-    _need(chosen, "chosen", _I32T, (n,), dev)
-    out = torch.empty(n + 2 * batch, dtype=_I32T, device=kv_cache.device)
-    path, count, after = out.split((n, batch, batch))
-    fn, what = ((_lib.attn_tree_commit, "attn_tree_commit") if page_bytes == BF16_PAGE_BYTES else
-                (_lib.attn_tree_commit_fp8, "attn_tree_commit_fp8"))
-    _check(fn(kv_cache.data_ptr(), layers, pages, page_indptr.data_ptr(), page_indices.data_ptr(),
-              kv_len.data_ptr(), q_indptr.data_ptr(), batch, n, max_q_len, tokens.data_ptr(),
-              parents.data_ptr(), chosen.data_ptr(), path.data_ptr(), count.data_ptr(),
-              after.data_ptr(), stream), what)
-    return path, count, after
+    return attn_binding.tree_commit(kv_cache, page_indptr, page_indices, kv_len, q_indptr,
+                                    max_q_len, tokens, parents, chosen)
 
 
 def kv_copy_pages(kv_cache: torch.Tensor, src_pages: torch.Tensor,
@@ -601,14 +549,7 @@ def kv_copy_pages(kv_cache: torch.Tensor, src_pages: torch.Tensor,
     """Pages ``src_pages`` [n] copied to ``dst_pages`` [n] in all layers of ``kv_cache`` [layers,
     pages, ...] (bf16 or 8-bit).  Destinations have to differ, from one another and from the
     sources."""
-    layers, pages, page_bytes, dev, stream = _layers(kv_cache)
-    n = _count(src_pages, "src_pages", _I32T)
-    _need(src_pages, "src_pages", _I32T, (n,), dev)
-    _need(dst_pages, "dst_pages", _I32T, (n,), dev)
-    _check(_lib.attn_kv_copy_pages(kv_cache.data_ptr(), layers, pages, page_bytes,
-                                   src_pages.data_ptr(), dst_pages.data_ptr(), n, stream),
-           "attn_kv_copy_pages")
-    return kv_cache
+    return attn_binding.kv_copy_pages(kv_cache, src_pages, dst_pages)
 
 
 def beam_top_k(logits: torch.Tensor, scores: torch.Tensor,
@@ -617,21 +558,4 @@ def beam_top_k(logits: torch.Tensor, scores: torch.Tensor,
     fp32, ``scores`` [batch, width] fp32 (-inf: a beam that has ended or is not there yet).
     Returns scores [batch, k] fp32, the beams and the tokens [batch, k] int32, best first; equal
     ones by beam, then token.  width and k up to 64."""
-    f32 = getattr(logits, "dtype", None) is _F32T
-    dev, stream = _on_current(logits, "logits", _F32T if f32 else _BF16)
-    batch, width = _shape(scores) if len(_shape(scores) or ()) == 2 else (0, 0)
-    _need(scores, "scores", _F32T, (batch, width), dev)
-    vocab = logits.shape[-1] if logits.dim() else 0
-    _need(logits, "logits", _F32T if f32 else _BF16, (batch * width, vocab), dev)
-    if not 1 <= k <= min(MAX_BEAMS, width * vocab) or width > MAX_BEAMS:
-        raise ValueError(f"k: {k} of {width} beams and {vocab} tokens; both up to {MAX_BEAMS}")
-    need = _lib.attn_beam_workspace_bytes(batch, width, vocab, k)
-    ws = torch.empty(need, dtype=_U8, device=logits.device)
-    out = torch.empty((3, batch, k), dtype=_I32T, device=logits.device)
-    values, beams, tokens = out.unbind()
-    values = values.view(_F32T)
-    _check(_lib.attn_beam_top_k(logits.data_ptr(), int(f32), batch, width, vocab,
-                                scores.data_ptr(), k, values.data_ptr(), beams.data_ptr(),
-                                tokens.data_ptr(), ws.data_ptr(), need, stream),
-           "attn_beam_top_k")
-    return values, beams, tokens
+    return attn_binding.beam_top_k(logits, scores, k)

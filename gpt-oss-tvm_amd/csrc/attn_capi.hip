@@ -614,7 +614,7 @@ TreePlan tree_plan(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t
   if (keys <= 0 || batch > 64 || batch * tiles > 2 * kTreeWorkers) return TreePlan{tokens, tiles, 0};
   const int64_t pieces = (batch * tiles * fp8_blocks(keys) + kTreeLeast - 1) / kTreeLeast;
   if (pieces <= batch * tiles) return TreePlan{tokens, tiles, 0};
-  return TreePlan{tokens, tiles, std::min(kTreeWorkers, pieces)};
+  return TreePlan{tokens, tiles, std::min(tokens == 32 ? kTreeWorkers / 2 : kTreeWorkers, pieces)};
 }
 
 int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,

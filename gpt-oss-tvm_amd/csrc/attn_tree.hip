@@ -68,13 +68,18 @@ struct TreeLine {
   int64_t all, piece;
   int blocks;             // of one of its tiles
   int tiles_before;       // of the sequences before it
+  int row, nodes, total, page, pages;  // its tables
   TreeLine() = default;
   __device__ __forceinline__ TreeLine(const TreeArgs& a, int tokens) {
     const int lane = threadIdx.x & 63, b = min(lane, a.batch - 1);
-    const int qn = lane < a.batch ? a.q_indptr[b + 1] - a.q_indptr[b] : 0;
-    const int total = a.page_indptr[b + 1] > a.page_indptr[b] ? a.kv_len[b] : 0;
-    blocks = max(1, TreeSpan(max(total - qn, 0), total, a.window).blocks);
-    const int tiles = min(max((qn + tokens - 1) / tokens, 0), a.tiles);
+    row = a.q_indptr[b];
+    nodes = a.q_indptr[b + 1] - row;
+    page = a.page_indptr[b];
+    pages = a.page_indptr[b + 1] - page;
+    total = a.kv_len[b];
+    if (pages <= 0) total = 0;
+    blocks = max(1, TreeSpan(max(total - nodes, 0), total, a.window).blocks);
+    const int tiles = lane < a.batch ? min(max((nodes + tokens - 1) / tokens, 0), a.tiles) : 0;
     const int64_t mine = (int64_t)tiles * blocks;
     after = mine;
     int tiles_after = tiles;
@@ -130,14 +135,15 @@ struct TreeLds {
   static constexpr int kBufs = kC == 1 ? 1 : 2;  // one wave needs no second buffer
   __align__(16) uint8_t tiles[kK][kBufs][2][kTreeHalf];
   float2 ml[kK][kC][32];
+  int bad[kK][kBufs][kC];  // by each wave: an infinity or a NaN in what it staged of v (bf16)
 };
 
 // Blocks begin .. end - 1 of a tile whose sequence has qn nodes from row qb on and L tokens in all;
 // the result goes to out, or where it is a part to `place` of the workspace.
 template <bool kFp8, int kC, int kK>
-__device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& lds, int hk, int b,
-                                           int tile, int qb, int qn, int L, int begin, int end,
-                                           int place) {
+__device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& lds, int hk,
+                                           const PageList& pages, int tile, int qb, int qn, int L,
+                                           int begin, int end, int place) {
   constexpr int kBufs = TreeLds<kC, kK>::kBufs;
   constexpr int kUnits = (kFp8 ? 8 : 16) / kC;  // 1 KB loads of a block that a wave makes
   int t = threadIdx.x;
@@ -145,8 +151,7 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
   const int lane = t & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), cw = wave % kC, kg = wave / kC;
   const int t0 = tile * 4 * kC, nt = min(4 * kC, qn - t0), row0 = qb + t0;
-  const int cached = max(L - qn, 0), page0 = a.page_indptr[b];
-  const PageList pages{a.page_indices + page0, a.page_indptr[b + 1] - page0, a.num_pages};
+  const int cached = max(L - qn, 0);
   const bool active = 4 * cw < nt;
   const int last_page = max(0, min(pages.count - 1, (L - 1) / kPage));
   const int steps = (end - begin + kK - 1) / kK;  // of every group
@@ -184,7 +189,18 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
       }
     }
   };
-  auto store = [&](Raw& x, uint8_t* kt, uint8_t* vt, int kb) __attribute__((always_inline)) {
+  auto store = [&](Raw& x, uint8_t* kt, uint8_t* vt, int kb, int* bad)
+      __attribute__((always_inline)) {
+    if constexpr (!kFp8) {
+      uint32_t full = 0u;  // bits 15 and 31: an exponent of all ones
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u)
+        if ((u * kC + cw) >> 3)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) full |= (x.data[u][j] & 0x7F807F80u) + 0x00800080u;
+      const bool any = __any(full & 0x80008000u);
+      if (lane == 0) bad[cw] = any;
+    }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       const int id = u * kC + cw;
@@ -303,41 +319,54 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
   const int v_at = kFp8 ? k_at
                         : (4 * h + ((lane >> 2) & 3)) * 128 + ((lane >> 4) & 1) * 32 +
                               (lane & 3) * 8 + ((lane >> 3) & 1) * 64;
-  auto tile32 = [&](auto masked, const uint8_t* kt, const uint8_t* vt, int kb, int kt32)
-      __attribute__((always_inline)) {
+  // kN tiles of 32 keys from tile kt32 of a block on; both of a block in one go let one's products
+  // run under the other's exponentials
+  auto keys32 = [&](auto masked, auto many, const uint8_t* kt, const uint8_t* vt, int kb, int kt32,
+                    bool bad) __attribute__((always_inline)) {
     constexpr bool kMasked = decltype(masked)::value;
-    f32x16 s;
+    constexpr int kN = decltype(many)::value;
+    f32x16 s[kN];
+    uint32_t see[kN];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = 0.f;
+    for (int n = 0; n < kN; ++n) {
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      const bf16x8 ka = *(const bf16x8*)(kt + 4096 * kt32 + (k_at ^ (32 * st)));
-      s = tree_mfma(ka, qv[st], s);
+      for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const bf16x8 ka = *(const bf16x8*)(kt + 4096 * (kt32 + n) + (k_at ^ (32 * st)));
+        s[n] = tree_mfma(ka, qv[st], s[n]);
+      }
     }
-    uint32_t see = ~0u;
     if constexpr (kMasked) {
-      see = seen(kb + 32 * kt32);
-      const uint32_t mine = see >> (4 * h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
+      for (int n = 0; n < kN; ++n) {
+        see[n] = seen(kb + 32 * (kt32 + n));
+        const uint32_t mine = see[n] >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[n][i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? s[n][i] : -INFINITY;
+      }
     }
-    moe::bf16x2 p[8];
+    moe::bf16x2 p[kN][8];
     float ps;
     auto exps = [&](float mn) __attribute__((always_inline)) {
       ps = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i][0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i], a.c2, mn));
-        p[i][1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], a.c2, mn));
-        ps = __builtin_amdgcn_fdot2_f32_bf16(p[i], ones, ps, false);
-      }
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          p[n][i][0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[n][2 * i], a.c2, mn));
+          p[n][i][1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[n][2 * i + 1], a.c2, mn));
+          ps = __builtin_amdgcn_fdot2_f32_bf16(p[n][i], ones, ps, false);
+        }
     };
     exps(mneg);
     if (__any(!(ps < kTreeMost))) {
-      float mx = s[0];
+      float mx = s[0][0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+      for (int n = 0; n < kN; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
       const uint32_t u = __float_as_uint(mx);
       const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
       mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
@@ -353,69 +382,82 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
     }
     l += ps;
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      bf16x8 pb;
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pb[j] = p[4 * m + (j >> 1)][j & 1];
+      for (int m = 0; m < 2; ++m) {
+        bf16x8 pb;
 #pragma unroll
-      for (int dt = 0; dt < 2; ++dt) {
-        bf16x8 va;
-        if constexpr (kMasked) __builtin_amdgcn_sched_barrier(0);  // (registers)
-        if constexpr (kFp8) {
-          va = *(const bf16x8*)(vt + 4096 * dt + (v_at ^ (32 * m + 64 * kt32)));
-        } else {
-          u32x4 w;  // dim c of 32 dt of the keys 16 m + 8 j + 4 h ..
+        for (int j = 0; j < 8; ++j) pb[j] = p[n][4 * m + (j >> 1)][j & 1];
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (lds_s16x4)(vt + 4096 * kt32 + 2048 * m + 1024 * j + (v_at ^ (64 * dt))));
-            const uint2 pair = __builtin_bit_cast(uint2, four);
-            w[2 * j] = pair.x;
-            w[2 * j + 1] = pair.y;
-          }
-          va = moe::as_bf16x8(w);
-          if constexpr (kMasked) {
-            // An infinity or a NaN must not meet the probability 0 of who does not see its key: it
-            // goes in by a product of its own, the largest number for it and for who sees it,
-            // whose square is past fp32's range
-            const __bf16 big = (__bf16)3.3895314e38f, none = (__bf16)0.0f;
-            bool bad = false;
+        for (int dt = 0; dt < 2; ++dt) {
+          bf16x8 va;
+          if constexpr (kMasked && kC > 4) __builtin_amdgcn_sched_barrier(0);  // (registers)
+          if constexpr (kFp8) {
+            va = *(const bf16x8*)(vt + 4096 * dt + (v_at ^ (32 * m + 64 * (kt32 + n))));
+          } else {
+            u32x4 w;  // dim c of 32 dt of the keys 16 m + 8 j + 4 h ..
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              bad |= ((w[j >> 1] >> (16 * (j & 1))) & 0x7F80u) == 0x7F80u;
-            if (__any(bad)) {
-              bf16x8 marks, who;
+            for (int j = 0; j < 2; ++j) {
+              const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (lds_s16x4)(vt + 4096 * (kt32 + n) + 2048 * m + 1024 * j + (v_at ^ (64 * dt))));
+              const uint2 pair = __builtin_bit_cast(uint2, four);
+              w[2 * j] = pair.x;
+              w[2 * j + 1] = pair.y;
+            }
+            va = moe::as_bf16x8(w);
+            if constexpr (kMasked) {
+              if (bad) {
+                // An infinity or a NaN must not meet the probability 0 of who does not see its
+                // key: it goes in by a product of its own, the largest number for it and for who
+                // sees it, whose square is past fp32's range
+                const __bf16 big = (__bf16)3.3895314e38f, none = (__bf16)0.0f;
+                bf16x8 marks, who;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const bool x = ((w[j >> 1] >> (16 * (j & 1))) & 0x7F80u) == 0x7F80u;
-                marks[j] = x ? big : none;
-                va[j] = x ? none : va[j];
-                who[j] = see >> (16 * m + 8 * (j >> 2) + 4 * h + (j & 3)) & 1u ? big : none;
+                for (int j = 0; j < 8; ++j) {
+                  const bool x = ((w[j >> 1] >> (16 * (j & 1))) & 0x7F80u) == 0x7F80u;
+                  marks[j] = x ? big : none;
+                  va[j] = x ? none : va[j];
+                  who[j] =
+                      see[n] >> (16 * m + 8 * (j >> 2) + 4 * h + (j & 3)) & 1u ? big : none;
+                }
+                o[dt] = tree_mfma(marks, who, o[dt]);
               }
-              o[dt] = tree_mfma(marks, who, o[dt]);
             }
           }
+          o[dt] = tree_mfma(va, pb, o[dt]);
         }
-        o[dt] = tree_mfma(va, pb, o[dt]);
       }
-    }
   };
   auto compute = [&](auto masked, int buf, int i) __attribute__((always_inline)) {
     const int kb = (begin + kg + kK * i) * kTreeBlock;
     const uint8_t *kt = lds.tiles[kg][buf][0], *vt = lds.tiles[kg][buf][1];
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
     if constexpr (decltype(masked)::value) {
+      int bad = 0;
+      if constexpr (!kFp8) {
+#pragma unroll
+        for (int w = 0; w < kC; ++w) bad |= lds.bad[kg][buf][w];
+        bad = __builtin_amdgcn_readfirstlane(bad);
+      }
 #pragma unroll 1  // (registers)
-      for (int kt32 = 0; kt32 < 2; ++kt32) tile32(masked, kt, vt, kb, kt32);
+      for (int kt32 = 0; kt32 < 2; ++kt32) keys32(masked, one, kt, vt, kb, kt32, bad != 0);
+    } else if constexpr (kC <= 4) {
+      keys32(masked, two, kt, vt, kb, 0, false);
     } else {
-      tile32(masked, kt, vt, kb, 0);
-      tile32(masked, kt, vt, kb, 1);
+      keys32(masked, one, kt, vt, kb, 0, false);
+      keys32(masked, one, kt, vt, kb, 1, false);
     }
   };
   auto put = [&](int buf, int i) __attribute__((always_inline)) {
-    store(raw, lds.tiles[kg][buf][0], lds.tiles[kg][buf][1],
-          (begin + kg + kK * i) * kTreeBlock);
+    store(raw, lds.tiles[kg][buf][0], lds.tiles[kg][buf][1], (begin + kg + kK * i) * kTreeBlock,
+          lds.bad[kg][buf]);
   };
 
+  // every load before the loop (the first block, q, the mask) done: the compiler then waits for
+  // nothing but the next block there (it waited for them, and so for the loads behind them, before
+  // each block's products: 146 us of two trees of 26 nodes over up to 131072 tokens, now 115)
+  moe::wait_vmcnt<0>();
   if (mine(0)) put(0, 0);
   if (mine(1)) load(raw, 1);
   if constexpr (kC > 1) moe::lds_barrier();
@@ -507,7 +549,7 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
 
 template <bool kFp8, int kC, int kK>
 __global__ __launch_bounds__(64 * kC * kK)
-__attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs a) {
+__attribute__((amdgpu_waves_per_eu(kC <= 4 ? 2 : 4))) void tree_kernel(TreeArgs a) {
   __shared__ TreeLds<kC, kK> lds;
   __shared__ TreeLine lines[kWave];  // (out of the registers)
   // x: (worker, kv head); without workers (sequence, tile, kv head)
@@ -523,23 +565,34 @@ __attribute__((amdgpu_waves_per_eu(kC <= 2 ? 2 : 4))) void tree_kernel(TreeArgs 
     moe::lds_barrier();
   }
   do {
-    int b = worker / a.tiles, tile = worker % a.tiles, first = 0, place = -1;
+    int tile = worker % a.tiles, first = 0, place = -1, qb, qn, L, page, pages;
     int64_t n = INT32_MAX;
     if (a.workers > 0) {
-      b = __builtin_ctzll(__ballot(lines[lane].after > at));
-      const int blocks = __builtin_amdgcn_readfirstlane(lines[b].blocks);
-      const int from = (int)(at - TreeLine::lane_of(lines[b].before, 0));
+      const TreeLine& line = lines[__builtin_ctzll(__ballot(lines[lane].after > at))];
+      auto one = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+      const int blocks = one(line.blocks);
+      const int from = (int)(at - TreeLine::lane_of(line.before, 0));
       tile = from / blocks;
       first = from - tile * blocks;
       n = min((int64_t)(blocks - first), stop - at);
-      if (n < blocks)
-        place = worker + __builtin_amdgcn_readfirstlane(lines[b].tiles_before) + tile;
+      if (n < blocks) place = worker + one(line.tiles_before) + tile;
+      qb = one(line.row);
+      qn = one(line.nodes);
+      L = one(line.total);
+      page = one(line.page);
+      pages = one(line.pages);
+    } else {
+      const int b = worker / a.tiles;
+      qb = a.q_indptr[b];
+      qn = a.q_indptr[b + 1] - qb;
+      if (tile * 4 * kC >= qn) return;
+      page = a.page_indptr[b];
+      pages = a.page_indptr[b + 1] - page;
+      L = pages > 0 ? a.kv_len[b] : 0;
     }
-    const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
-    const int L = a.page_indptr[b + 1] > a.page_indptr[b] ? a.kv_len[b] : 0;
-    if (tile * 4 * kC >= qn) return;  // (only without workers)
     const TreeSpan span(max(L - qn, 0), L, a.window);
-    tree_piece<kFp8, kC, kK>(a, lds, hk, b, tile, qb, qn, L, span.first + first,
+    tree_piece<kFp8, kC, kK>(a, lds, hk, PageList{a.page_indices + page, pages, a.num_pages}, tile,
+                             qb, qn, L, span.first + first,
                              span.first + (int)min(first + n, (int64_t)span.blocks), place);
     at += n;
     if (at < stop) moe::lds_barrier();  // the next piece's tiles go where this one's parts lie
@@ -553,7 +606,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
   const int token = i / kHq, head = i % kHq, d = (threadIdx.x & 15) * 4;
   const int b = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const TreeLine line(a, tokens);
-  const int qb = a.q_indptr[b], qn = a.q_indptr[b + 1] - qb;
+  const int qb = __builtin_amdgcn_readlane(line.row, b);
+  const int qn = __builtin_amdgcn_readlane(line.nodes, b);
   const int blocks = __builtin_amdgcn_readlane(line.blocks, b);
   if (tile * tokens >= qn) return;
   const int64_t from = TreeLine::lane_of(line.before, b) + (int64_t)tile * blocks;
@@ -629,7 +683,7 @@ int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_le
   else if (tokens == 16)
     fp8 ? go(attn::tree_kernel<true, 4, 2>, 8) : go(attn::tree_kernel<false, 4, 2>, 8);
   else if (tokens == 32)
-    fp8 ? go(attn::tree_kernel<true, 8, 1>, 8) : go(attn::tree_kernel<false, 8, 1>, 8);
+    fp8 ? go(attn::tree_kernel<true, 8, 2>, 16) : go(attn::tree_kernel<false, 8, 2>, 16);
   else
     return -6;
   if (hipGetLastError() != hipSuccess) return -6;
