@@ -557,5 +557,5 @@ def beam_top_k(logits: torch.Tensor, scores: torch.Tensor,
     """The ``k`` best continuations of each request: ``logits`` [batch * width, vocab] bf16 or
     fp32, ``scores`` [batch, width] fp32 (-inf: a beam that has ended or is not there yet).
     Returns scores [batch, k] fp32, the beams and the tokens [batch, k] int32, best first; equal
-    ones by beam, then token.  width and k up to 64."""
+    ones by beam, then logit, then token.  width and k up to 64."""
     return attn_binding.beam_top_k(logits, scores, k)

@@ -42,12 +42,13 @@ __device__ __forceinline__ uint32_t image(float x) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 // a bound on the k-th largest of a wave's values from below: its upper kBits bits
-template <int kBits>
-__device__ __forceinline__ uint32_t kth_of_lanes(uint32_t mine, int k) {
-  uint32_t t = 0u;
+template <int kBits, class U>
+__device__ __forceinline__ U kth_of_lanes(U mine, int k) {
+  constexpr int kAll = 8 * sizeof(U);
+  U t = 0u;
 #pragma unroll
-  for (int bit = 31; bit >= 32 - kBits; --bit) {
-    const uint32_t next = t | 1u << bit;
+  for (int bit = kAll - 1; bit >= kAll - kBits; --bit) {
+    const U next = t | (U)1 << bit;
     if (__popcll(__ballot(mine >= next)) >= k) t = next;
   }
   return t;
@@ -104,9 +105,9 @@ __device__ __forceinline__ float exp_of(float d) {
 
 // T: float or uint16_t (bf16).  A stretch is `chunks` chunks, of which a thread holds 16 elements
 // and the next one's loads, wherever the row begins.  The bound is taken after the first, then after
-// 8, 16, .. and after the last; a thread whose maximum of a chunk reaches it only notes that (looking at each number there
-// cost twice the time), and what reaches the last bound is picked out of the noted ones' 16 numbers,
-// from memory, at the end.
+// 8, 16, .. and after the last; a thread whose maximum of a chunk reaches it only notes that
+// (looking at each number there cost twice the time), and what reaches the last bound is picked out
+// of the noted ones' 16 numbers, from memory, at the end.
 constexpr int kPartThreads = 512, kPartElems = 16, kChunk = kPartThreads * kPartElems;
 constexpr int kPartList = 1024, kWaveList = kPartList / (kPartThreads / 64);
 template <class T>
@@ -166,8 +167,8 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
   int noted = 0;  // by the wave
   // waves with fewer numbers than lanes are not counted on for the bound
   const int full = min(kWaves, max(1, (end - begin) / (64 * kEach))), q = (full + 1) / 2;
-  auto bound = [&](int turn) __attribute__((always_inline)) {
-    const uint32_t mine = kth_of_lanes<kBoundBits>(image(lm), (k + q - 1) / q);
+  auto bound = [&](auto bits, int turn) __attribute__((always_inline)) {
+    const uint32_t mine = kth_of_lanes<decltype(bits)::value>(image(lm), (k + q - 1) / q);
     if (lane == 0) wbound[turn][wave] = mine;
     __syncthreads();
     const uint32_t top = nth_of(wbound[turn], kWaves, q);
@@ -175,6 +176,7 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
     least = top <= 0x007FFFFFu
                 ? -INFINITY : __uint_as_float(top & 0x80000000u ? top & 0x7FFFFFFFu : ~top);
   };
+  constexpr std::integral_constant<int, kBoundBits> coarse;
   int chunk = 0;
   for (; chunk * kLoads * kPartThreads < units; ++chunk) {
     load(next, chunk + 1);
@@ -187,7 +189,8 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
     s *= exp_of(old - base);
 #pragma unroll
     for (int e = 0; e < kElems; ++e) s += exp_of(raw(e) - base);
-    if ((chunk & (chunk + 1)) == 0 && (chunk == 0 || chunk >= 7)) bound(__builtin_ctz(chunk + 1) & 1);
+    if ((chunk & (chunk + 1)) == 0 && (chunk == 0 || chunk >= 7))
+      bound(coarse, __builtin_ctz(chunk + 1) & 1);
     const uint64_t who = __ballot(cm >= least);
     const int at = noted + __builtin_amdgcn_mbcnt_hi(
                                (uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
@@ -204,7 +207,7 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
   if (chunk == 1 && tail == 0)
     __syncthreads();  // (as it was taken)
   else
-    bound(chunk < 8 ? 1 : (32 - __builtin_clz(chunk)) & 1);  // (the other turn than the last one's)
+    bound(coarse, chunk < 8 ? 1 : (32 - __builtin_clz(chunk)) & 1);  // (the other turn than the last one's)
   bool fits = true;
   int records = 0;
 #pragma unroll
@@ -242,10 +245,70 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
     stats[blockIdx.x] = Stat{all, m};
   }
   int n = kept;
-  if (!fits || n > kPartList) {
-    // Too many reach a bound (equal logits, or a row in order): the k-th best by bits, of the
-    // images and then of the places among those equal to it, counting the whole stretch each time
-    // (from memory: a copy in registers would cost every call a third of its waves).
+  bool chosen = fits && n <= kPartList;
+  if (!chosen) {
+    // Too many reach a bound (most logits equal, as where a mask leaves few tokens, or a row in
+    // ascending order): with the last bound exact, those above it, and of those equal to it the
+    // first ones that make k.  128 rows of 201088 logits, bf16, of which a mask leaves 100: both
+    // launches 32 us, by bits as below 1824; without a mask 23.
+    __syncthreads();
+    if (t == 0) kept = 0;
+    bound(std::integral_constant<int, 32>(), 0);
+    const int rounds = (units + kPartThreads - 1) / kPartThreads;
+    auto unit = [&](Raw& x16, int u) {
+      x16.w[0] = *(const u32x4_any*)(x + begin + min(u, units - 1) * kEach);
+      return u < units;
+    };
+#pragma unroll 4
+    for (int r = 0; r < rounds; ++r) {
+      Raw again;
+      const int u = r * kPartThreads + t;
+      const bool in = unit(again, u);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (in && again(e) > least) keep(again(e), begin + u * kEach + e);
+    }
+    if (t < tail && extra > least) keep(extra, end - tail + t);
+    __syncthreads();
+    n = kept;
+    chosen = n <= kPartList - kMost;
+    // (the last round: the numbers behind the units)
+    for (int r = 0; chosen && r <= rounds && n < k; ++r) {
+      Raw again;
+      const int u = r * kPartThreads + t;
+      const bool in = r < rounds && unit(again, u);
+      int mine = r == rounds && t < tail && extra == least ? 1 : 0;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) mine += in && again(e) == least ? 1 : 0;
+      int upto = mine;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(upto, off, 64);
+        upto += lane >= off ? o : 0;
+      }
+      if (lane == 63) wcount[r & 1][wave] = upto;
+      __syncthreads();
+      int at = n + upto - mine, all = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        at += w < wave ? wcount[r & 1][w] : 0;
+        all += wcount[r & 1][w];
+      }
+      if (r == rounds && mine && at < k) list[at] = Item{extra, end - tail + t};
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (in && again(e) == least) {
+          if (at < k) list[at] = Item{again(e), begin + u * kEach + e};
+          ++at;
+        }
+      n = min(n + all, k);
+    }
+    __syncthreads();
+  }
+  if (!chosen) {
+    // Too many are above it (a few lanes hold them all): the k-th best by bits, of the images and
+    // then of the places among those equal to it, counting the whole stretch each time (from
+    // memory: a copy in registers would cost every call a third of its waves).
     auto count = [&](auto which, int turn) {
       int c = 0;
 #pragma unroll 1
@@ -299,6 +362,10 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
 
 // One workgroup a request: its rows' sums, then the k best of its lists.
 constexpr int kMergeThreads = 1024, kMergeList = kMergeThreads;
+// As many are compared with one another at once; us of both launches for 4 beams (k = 8) and for 128
+// (k = 16) of which a mask leaves 3 tokens: up to 128 or 256 25.6 and 39, 512 25.6 and 78, all 1024
+// 179 and 78.
+constexpr int kMergeFew = 256;
 struct Best {
   double v;
   float x;
@@ -320,6 +387,8 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(
   __shared__ Best list[kMergeList];
   __shared__ int ranks[kMergeList];
   __shared__ uint32_t wbound[kWaves];
+  __shared__ uint64_t wexact[kWaves];
+  __shared__ uint32_t logit[2];  // of those equal to the bound, from .. to
   __shared__ int found;
   const int r = blockIdx.x, t = threadIdx.x, wave = t >> 6, lane = t & 63;
   for (int b = wave; b < W; b += kWaves) {
@@ -394,12 +463,56 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(
   for (int i = rest; i < total; i += kMergeThreads)
     if (candidate(i, c) && high(c.v) >= top) keep(c);
   __syncthreads();
-  const int n = found;
+  int n = found;
   auto write = [&](int rank, const Best& x) {
     out_scores[(size_t)r * k + rank] = (float)x.v;
     out_beams[(size_t)r * k + rank] = x.beam;
     out_tokens[(size_t)r * k + rank] = x.token;
   };
+  if (n > kMergeFew) {
+    // Many reach the bound (scores equal, as -inf is where a mask leaves few tokens): with it
+    // exact, those above it, and of those equal to it the first ones that make k: where
+    // their logits are equal too, the lists' order is theirs (beam, stretch, token).
+    auto all_bits = [](double v) {
+      const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
+      return u >> 63 ? ~u : u | (uint64_t)1 << 63;
+    };
+    uint64_t most = 0u;  // (no number's)
+    for (int i = t; i < total; i += kMergeThreads)
+      if (candidate(i, c)) most = max(most, all_bits(c.v));
+    most = kth_of_lanes<64>(most, k);
+    __syncthreads();
+    if (t == 0) {
+      found = 0;
+      logit[0] = ~0u;
+      logit[1] = 0u;
+    }
+    if (lane == 0) wexact[wave] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) most = max(most, wexact[w]);
+    for (int i = t; i < total; i += kMergeThreads)
+      if (candidate(i, c)) {
+        const uint64_t u = all_bits(c.v);
+        if (u > most) keep(c);
+        if (u == most) {
+          atomicMin(&logit[0], beam::image(c.x));
+          atomicMax(&logit[1], beam::image(c.x));
+        }
+      }
+    __syncthreads();
+    n = found;
+    if (n < k && logit[0] != logit[1]) n = kMergeList + 1;  // (their own order is wanted)
+    for (int i0 = 0; n < k && i0 < total; i0 += 64) {  // (each wave for itself, the first writes)
+      const bool is = i0 + lane < total && candidate(i0 + lane, c) && all_bits(c.v) == most;
+      const uint64_t who = __ballot(is);
+      const int at = n + __builtin_amdgcn_mbcnt_hi(
+                             (uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+      if (wave == 0 && is && at < k) list[at] = c;
+      n = min(n + (int)__popcll(who), k);
+    }
+    __syncthreads();
+  }
   if (n <= kMergeList) {
     rank_all<kMergeThreads>(n, ranks, [&](int i) { return list[i]; },
                             [](const Best& x, const Best& y) { return x.before(y); });
@@ -408,7 +521,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(
       if (ranks[i] < k) write(ranks[i], list[i]);
     return;
   }
-  // Too many (equal scores): one after the other, each the best of those behind the last
+  // Too many: one after the other, each the best of those behind the last
   Best last{INFINITY, INFINITY, -1, -1};
   const Best none{-INFINITY, -INFINITY, INT32_MAX, INT32_MAX};
   for (int rank = 0; rank < k; ++rank) {
@@ -431,8 +544,9 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(
   }
 }
 
-// Chunks of a stretch: as many as leave 512 workgroups, two a CU, of a call's rows.  us of both
-// launches
+// Chunks of a stretch: as many as leave 512 workgroups, two a CU, of a call's rows.  16 requests of
+// 8 beams of 201088 logits, us of both launches: 256 workgroups 34, 512 25, 1024 29 (more lists for
+// the second one).
 inline int chunks_of(int64_t rows, int vocab) {
   const int64_t all = ((int64_t)vocab + kChunk - 1) / kChunk;
   const int64_t parts = std::min(all, std::max<int64_t>(1, (512 + rows - 1) / rows));

@@ -173,3 +173,60 @@ def test_copy_pages(A, fp8, n, layers):
     np.testing.assert_array_equal(dev.cpu().numpy() if fp8 else host_bf16(dev), cache)
     e = torch.empty(0, dtype=torch.int32, device="cuda")
     A.kv_copy_pages(dev, e, e)
+
+
+@TYPES
+@pytest.mark.parametrize("batch,vocab", [(1, 20001), (16, 30011)])  # (a chunk a stretch, several)
+def test_few_tokens_left(A, batch, vocab, f32):
+    """A mask that leaves no, fewer than k, k or some more tokens, by -inf, the type's lowest value
+    and a number: the rest counts too, in its order."""
+    rng = np.random.default_rng(vocab)
+    x, s = draw(rng, batch, 8, vocab, f32)
+    s[:, 1] = s[:, 0]
+    low = np.finfo(np.float32).min if f32 else np.float32(-3.3895314e38)
+    for masked in (-np.inf, low, np.float32(-32768.0)):
+        for left in (0, 1, 15, 16, 17, 100, 2000):
+            y = np.full_like(x, masked)
+            for b in range(batch):
+                at = rng.choice(vocab, left, replace=False)
+                y[b, :, at] = x[b, :, at]
+            y[:, 1] = y[:, 0]                         # equal scores in two beams
+            select(A, y, s, 16, f32)
+    y = np.full_like(x, -np.inf)                      # what is left differs from beam to beam
+    for b in range(batch):
+        for w in range(8):
+            at = rng.choice(vocab, w * w // 3, replace=False)
+            y[b, w, at] = x[b, w, at]
+    for k in (1, 8, 64):
+        select(A, y, s, k, f32)
+
+
+@TYPES
+def test_best_in_few_lanes(A, f32):
+    """The largest numbers in a few columns of 16 bytes that come again and again: most lanes' maxima
+    say little of them."""
+    rng = np.random.default_rng(8)
+    for vocab in (8192, 50001):
+        x, s = draw(rng, 1, 4, vocab, f32)
+        column = np.arange(vocab) // (4 if f32 else 8) % 64
+        x[:, :, column < 10] += 40.0
+        x = x if f32 else O.bf16_to_f32(O.f32_to_bf16(x))
+        select(A, x, s, 64, f32)
+        select(A, x, s, 16, f32)
+
+
+@TYPES
+def test_scores_equal_and_logits_not(A, f32):
+    """Beside a logit of 1e38 all others' scores are the same number, -1e38 in fp64 too: equal scores
+    go by beam, then by the logits, then by token."""
+    rng = np.random.default_rng(9)
+    for vocab, width in ((3000, 3), (VOCAB, 8)):
+        x = O.bf16_to_f32(O.f32_to_bf16(rng.standard_normal((1, width, vocab)).astype(np.float32)))
+        x[0, :, vocab // 3] = O.bf16_to_f32(O.f32_to_bf16(np.array([1e38], np.float32)))
+        dev = f32_dev(x[0]) if f32 else bf16_dev(O.f32_to_bf16(x[0]))
+        score, beams, tokens = [t.cpu().numpy()[0] for t in
+                                A.beam_top_k(dev, f32_dev(np.zeros((1, width), np.float32)), 16)]
+        best = np.argsort(-x[0, 0], kind="stable")[:17 - width]       # of the first beam
+        np.testing.assert_array_equal(beams, [*range(width), *[0] * (16 - width)])
+        np.testing.assert_array_equal(tokens, [*[vocab // 3] * width, *best[1:]])
+        assert (score[:width] == 0).all() and (score[width:] == -x[0, 0, vocab // 3]).all()
