@@ -37,6 +37,7 @@ then also have each node's mask over its tree, and positions by depth.
 from __future__ import annotations
 
 import dataclasses
+from collections import Counter
 
 import numpy as np
 import torch
@@ -300,6 +301,8 @@ class PagedKVCache:
         accepted, after ``attn_native.tree_commit`` has moved what is."""
         parents = [[int(p) for p in tree] for tree in parents]
         seq_ids = list(seq_ids)
+        if len(seq_ids) != len(parents) or len(set(seq_ids)) != len(seq_ids):
+            raise ValueError(f"{len(parents)} trees need as many different sequences, not {seq_ids}")
         longest = max((len(tree) for tree in parents), default=0)
         words = max(1, -(-longest // 32))
         if longest > TREE_MAX_NODES:
@@ -333,7 +336,11 @@ class PagedKVCache:
         if min(append_lengths, default=1) < 1:
             raise ValueError("every sequence of a forward appends at least one token")
         need = sum(max(0, -(-(self.seqs[s].length + a) // PAGE_SIZE) - len(self.seqs[s].pages))
-                   + self._shares_last(self.seqs[s]) for s, a in zip(seq_ids, append_lengths))
+                   for s, a in zip(seq_ids, append_lengths))
+        # a copy for each that writes to a shared page; the last of its holders keeps it
+        writers = Counter(self.seqs[s].pages[-1] for s in set(seq_ids)
+                          if self._shares_last(self.seqs[s]))
+        need += sum(n - (n == self._refs[page]) for page, n in writers.items())
         if need > len(self.free):
             raise MemoryError(f"KV cache full: {need} pages needed, {len(self.free)} free")
         q_indptr, positions, slots, page_indptr, page_indices, kv_len = [0], [], [], [0], [], []

@@ -270,3 +270,30 @@ def test_begin_tree_tables():
             c.begin_tree([0], [bad])
     assert c.seq_len(0) == 22 and c.tables is None
     assert not c.begin_tree([0], [[-1]]).is_decode
+
+
+def test_trees_of_as_many_different_sequences():
+    c = make()
+    c.add_sequence(0)
+    c.add_sequence(1)
+    for ids, trees in (([0, 0], [[-1], [-1]]), ([0, 1], [[-1]]), ([0], [[-1], [-1]])):
+        with pytest.raises(ValueError):
+            c.begin_tree(ids, trees)
+    assert c.seq_len(0) == c.seq_len(1) == 0 and len(c.free) == 12
+
+
+def test_last_holder_of_a_page_needs_no_copy():
+    c = make(pages=2)
+    c.add_sequence(0)
+    write(c, c.begin_forward([0], [5]), range(5))
+    c.branch([0], [0, 0], [0, 1])
+    write(c, c.begin_forward([0, 1], [1, 1]), [10, 11])      # one copy, the one page there is
+    assert not c.free and rows(c, 0) == [*range(5), 10] and rows(c, 1) == [*range(5), 11]
+    c.clear()
+    c.add_sequence(0)
+    write(c, c.begin_forward([0], [5]), range(5))
+    c.branch([0], [0, 0, 0], [0, 1, 2])
+    with pytest.raises(MemoryError):                         # sequence 2 keeps it: two copies
+        c.begin_forward([0, 1], [1, 1])
+    write(c, c.begin_forward([1], [1]), [20])
+    assert not c.free and rows(c, 1) == [*range(5), 20] and rows(c, 0) == rows(c, 2) == [*range(5)]

@@ -488,3 +488,28 @@ def test_commit_graph(A):
             torch.cuda.synchronize()
             for a, b in zip((*held, cache), want):
                 assert torch.equal(a, b)
+
+
+@BOTH
+@pytest.mark.parametrize("cached,nodes", [([100], [1024]), ([0, 1000], [513, 40])])
+def test_large_trees(A, fp8, cached, nodes):
+    """Masks of up to 32 words; a chain's deepest node sees a thousand others."""
+    see, pos = zip(*(tree_bits(list(range(-1, m - 1)) if b == 0 else
+                               random_tree(np.random.default_rng(m), m))
+                     for b, m in enumerate(nodes)))
+    c = Case(11, fp8, cached, nodes, see, [n + p for n, p in zip(cached, pos)])
+    rows = np.array([0, 1, 31, 32, 39, 63, 64, 200, 511, 512, 800, 1022, 1023])
+    for window in (0, 128):
+        c.check(c.run(A, window), window, rows)
+
+
+@BOTH
+def test_many_tiles(A, fp8):
+    """More tiles than are shared out, of sequences of several tiles each."""
+    rng = np.random.default_rng(12)
+    nodes = rng.integers(1, 130, 48).tolist()
+    nodes[3], nodes[7] = 129, 0
+    c = Case(12, fp8, rng.integers(0, 60, 48).tolist(), nodes)
+    rows = np.array([0, 1, 30, 31, 32, 64, 95, 96, 128])
+    c.check(c.run(A), 0, rows)
+    c.check(c.run(A, 20), 20, rows)
