@@ -602,6 +602,11 @@ constexpr int64_t kMaxBatch = 65535, kMaxLayers = 65535;
 // Tokens of a tree's tile, and how many workgroups of a kv head its keys are shared out over:
 // as many as fit the chip at once (two a CU), each of kTreeLeast blocks or more; 0: a workgroup a
 // tile, where there are tiles enough to fill it twice over, more than 64 sequences or no bound.
+// us of the kernel, for 16 trees of 8 nodes over up to 4000 tokens with 32, 64, 128 workgroups: 28,
+// 25, 30; of at least 2, 4, 8, 16 blocks: 24.7, 25, 25, 29, and one tree of 5 nodes over 777
+// tokens 8.6, 8.2, 11, 14 (then without the merge's 3.8).  Tiles of 32 tokens take a CU each:
+// two trees of 26 nodes over up to 131072 tokens, 32 of 16 waves 146, 64 of 8 waves 150 and a merge
+// of twice the parts.
 constexpr int64_t kTreeLeast = 4, kTreeWorkers = 64;
 struct TreePlan {
   int64_t tokens, tiles, workers;

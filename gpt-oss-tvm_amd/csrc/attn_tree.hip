@@ -130,6 +130,24 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //    sees, and is renewed only when a tile's sum passes 2^24.
 //  * Blocks that every token of a wave sees whole take no mask; in the others (the tree's own, a
 //    window's edge) a lane has its token's 32 bits of a tile.
+//
+// What bounds it, with us of the kernel alone at four sizes: 1 tree of 5 nodes over 777 tokens, 16
+// of 8 over up to 4000 (bf16), 1 of 64 over 16000, 2 of 26 over up to 131072 (8-bit): 8.2, 24, 42,
+// 146.
+//  * Few nodes: the keys' bytes, and at the smallest calls the loads that wait for one another
+//    (tables, page ids, keys, parts).  16 x 8: 80 MB, 3.3 TB/s; a copy reaches 5.0.
+//  * Many nodes: the products and the exponentials beside them.  2 x 26: 85 GFLOP for tokens that
+//    are there, 590 TFLOP/s of the 1280 that a large bf16 product reaches; a wave's 32 keys take
+//    260 cycles of matrix instructions and 250 of others, 160 of them exponentials.  Without
+//    its exponentials it takes 128, without the second product 135, without staging 153: no part
+//    carries it alone.  Two 32-key tiles at once, the operands of a tile read ahead, four buffers
+//    and half the barriers, sums by additions and raised wave priorities were each timed
+//    and gained nothing (144 .. 175).
+//  * kC: a tile as wide as the tree, so that its keys are staged once, up to 32 tokens.  kK:
+//    8-token tiles with 1, 2, 4 groups: 16 x 8 28, 25, 32, one of 5 nodes 10.4, 8.2, 9.7; 32-token
+//    tiles with 1, 2: 2 x 26 175, 146 (with as many workgroups).
+//  * Registers: up to 16 tokens 256 a lane (32 trees of 16 nodes in a window: 13; with 128,
+//    spilled, 21); 32 tokens take 16 waves and so 128.
 template <int kC, int kK>
 struct TreeLds {
   static constexpr int kBufs = kC == 1 ? 1 : 2;  // one wave needs no second buffer
@@ -319,54 +337,42 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
   const int v_at = kFp8 ? k_at
                         : (4 * h + ((lane >> 2) & 3)) * 128 + ((lane >> 4) & 1) * 32 +
                               (lane & 3) * 8 + ((lane >> 3) & 1) * 64;
-  // kN tiles of 32 keys from tile kt32 of a block on; both of a block in one go let one's products
-  // run under the other's exponentials
-  auto keys32 = [&](auto masked, auto many, const uint8_t* kt, const uint8_t* vt, int kb, int kt32,
-                    bool bad) __attribute__((always_inline)) {
+  // the 32 keys from 32 kt32 of a block on
+  auto keys32 = [&](auto masked, const uint8_t* kt, const uint8_t* vt, int kb, int kt32, bool bad)
+      __attribute__((always_inline)) {
     constexpr bool kMasked = decltype(masked)::value;
-    constexpr int kN = decltype(many)::value;
-    f32x16 s[kN];
-    uint32_t see[kN];
+    f32x16 s;
+    uint32_t see = ~0u;
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
+    for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        const bf16x8 ka = *(const bf16x8*)(kt + 4096 * (kt32 + n) + (k_at ^ (32 * st)));
-        s[n] = tree_mfma(ka, qv[st], s[n]);
-      }
+    for (int st = 0; st < 4; ++st) {
+      const bf16x8 ka = *(const bf16x8*)(kt + 4096 * kt32 + (k_at ^ (32 * st)));
+      s = tree_mfma(ka, qv[st], s);
     }
     if constexpr (kMasked) {
+      see = seen(kb + 32 * kt32);
+      const uint32_t mine = see >> (4 * h);
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        see[n] = seen(kb + 32 * (kt32 + n));
-        const uint32_t mine = see[n] >> (4 * h);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[n][i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? s[n][i] : -INFINITY;
-      }
+      for (int i = 0; i < 16; ++i)
+        s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
     }
-    moe::bf16x2 p[kN][8];
+    moe::bf16x2 p[8];
     float ps;
     auto exps = [&](float mn) __attribute__((always_inline)) {
       ps = 0.f;
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          p[n][i][0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[n][2 * i], a.c2, mn));
-          p[n][i][1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[n][2 * i + 1], a.c2, mn));
-          ps = __builtin_amdgcn_fdot2_f32_bf16(p[n][i], ones, ps, false);
-        }
+      for (int i = 0; i < 8; ++i) {
+        p[i][0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i], a.c2, mn));
+        p[i][1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], a.c2, mn));
+        ps = __builtin_amdgcn_fdot2_f32_bf16(p[i], ones, ps, false);
+      }
     };
     exps(mneg);
     if (__any(!(ps < kTreeMost))) {
-      float mx = s[0][0];
+      float mx = s[0];
 #pragma unroll
-      for (int n = 0; n < kN; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[n][i]);
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
       const uint32_t u = __float_as_uint(mx);
       const auto x = __builtin_amdgcn_permlane32_swap(u, u, false, false);
       mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
@@ -382,57 +388,53 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
     }
     l += ps;
 #pragma unroll
-    for (int n = 0; n < kN; ++n)
+    for (int m = 0; m < 2; ++m) {
+      bf16x8 pb;
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        bf16x8 pb;
+      for (int j = 0; j < 8; ++j) pb[j] = p[4 * m + (j >> 1)][j & 1];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pb[j] = p[n][4 * m + (j >> 1)][j & 1];
+      for (int dt = 0; dt < 2; ++dt) {
+        bf16x8 va;
+        if constexpr (kMasked && kC > 4) __builtin_amdgcn_sched_barrier(0);  // (registers)
+        if constexpr (kFp8) {
+          va = *(const bf16x8*)(vt + 4096 * dt + (v_at ^ (32 * m + 64 * kt32)));
+        } else {
+          u32x4 w;  // dim c of 32 dt of the keys 16 m + 8 j + 4 h ..
 #pragma unroll
-        for (int dt = 0; dt < 2; ++dt) {
-          bf16x8 va;
-          if constexpr (kMasked && kC > 4) __builtin_amdgcn_sched_barrier(0);  // (registers)
-          if constexpr (kFp8) {
-            va = *(const bf16x8*)(vt + 4096 * dt + (v_at ^ (32 * m + 64 * (kt32 + n))));
-          } else {
-            u32x4 w;  // dim c of 32 dt of the keys 16 m + 8 j + 4 h ..
+          for (int j = 0; j < 2; ++j) {
+            const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (lds_s16x4)(vt + 4096 * kt32 + 2048 * m + 1024 * j + (v_at ^ (64 * dt))));
+            const uint2 pair = __builtin_bit_cast(uint2, four);
+            w[2 * j] = pair.x;
+            w[2 * j + 1] = pair.y;
+          }
+          va = moe::as_bf16x8(w);
+          if constexpr (kMasked) {
+            if (bad) {
+              // An infinity or a NaN must not meet the probability 0 of who does not see its
+              // key: it goes in by a product of its own, the largest number for it and for who
+              // sees it, whose square is past fp32's range
+              const __bf16 big = (__bf16)3.3895314e38f, none = (__bf16)0.0f;
+              bf16x8 marks, who;
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const s16x4 four = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (lds_s16x4)(vt + 4096 * (kt32 + n) + 2048 * m + 1024 * j + (v_at ^ (64 * dt))));
-              const uint2 pair = __builtin_bit_cast(uint2, four);
-              w[2 * j] = pair.x;
-              w[2 * j + 1] = pair.y;
-            }
-            va = moe::as_bf16x8(w);
-            if constexpr (kMasked) {
-              if (bad) {
-                // An infinity or a NaN must not meet the probability 0 of who does not see its
-                // key: it goes in by a product of its own, the largest number for it and for who
-                // sees it, whose square is past fp32's range
-                const __bf16 big = (__bf16)3.3895314e38f, none = (__bf16)0.0f;
-                bf16x8 marks, who;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const bool x = ((w[j >> 1] >> (16 * (j & 1))) & 0x7F80u) == 0x7F80u;
-                  marks[j] = x ? big : none;
-                  va[j] = x ? none : va[j];
-                  who[j] =
-                      see[n] >> (16 * m + 8 * (j >> 2) + 4 * h + (j & 3)) & 1u ? big : none;
-                }
-                o[dt] = tree_mfma(marks, who, o[dt]);
+              for (int j = 0; j < 8; ++j) {
+                const bool x = ((w[j >> 1] >> (16 * (j & 1))) & 0x7F80u) == 0x7F80u;
+                marks[j] = x ? big : none;
+                va[j] = x ? none : va[j];
+                who[j] =
+                    see >> (16 * m + 8 * (j >> 2) + 4 * h + (j & 3)) & 1u ? big : none;
               }
+              o[dt] = tree_mfma(marks, who, o[dt]);
             }
           }
-          o[dt] = tree_mfma(va, pb, o[dt]);
         }
+        o[dt] = tree_mfma(va, pb, o[dt]);
       }
+    }
   };
   auto compute = [&](auto masked, int buf, int i) __attribute__((always_inline)) {
     const int kb = (begin + kg + kK * i) * kTreeBlock;
     const uint8_t *kt = lds.tiles[kg][buf][0], *vt = lds.tiles[kg][buf][1];
-    constexpr std::integral_constant<int, 1> one;
-    constexpr std::integral_constant<int, 2> two;
     if constexpr (decltype(masked)::value) {
       int bad = 0;
       if constexpr (!kFp8) {
@@ -441,12 +443,10 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
         bad = __builtin_amdgcn_readfirstlane(bad);
       }
 #pragma unroll 1  // (registers)
-      for (int kt32 = 0; kt32 < 2; ++kt32) keys32(masked, one, kt, vt, kb, kt32, bad != 0);
-    } else if constexpr (kC <= 4) {
-      keys32(masked, two, kt, vt, kb, 0, false);
+      for (int kt32 = 0; kt32 < 2; ++kt32) keys32(masked, kt, vt, kb, kt32, bad != 0);
     } else {
-      keys32(masked, one, kt, vt, kb, 0, false);
-      keys32(masked, one, kt, vt, kb, 1, false);
+      keys32(masked, kt, vt, kb, 0, false);
+      keys32(masked, kt, vt, kb, 1, false);
     }
   };
   auto put = [&](int buf, int i) __attribute__((always_inline)) {
@@ -455,8 +455,7 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
   };
 
   // every load before the loop (the first block, q, the mask) done: the compiler then waits for
-  // nothing but the next block there (it waited for them, and so for the loads behind them, before
-  // each block's products: 146 us of two trees of 26 nodes over up to 131072 tokens, now 115)
+  // nothing but the next block there
   moe::wait_vmcnt<0>();
   if (mine(0)) put(0, 0);
   if (mine(1)) load(raw, 1);
@@ -476,7 +475,8 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
     return min(max((block - begin - kg + kK - 1) / kK, 0), steps);
   };
   const int whole1 = step_of(max(cached / kTreeBlock, begin));
-  const int whole0 = min(whole1, step_of(max(seen_from >= 0 ? seen_from / kTreeBlock + 1 : 0, begin)));
+  const int window0 = seen_from >= 0 ? seen_from / kTreeBlock + 1 : 0;
+  const int whole0 = min(whole1, step_of(max(window0, begin)));
   run(std::true_type{}, whole0);
   run(std::false_type{}, whole1);
   run(std::true_type{}, steps);
