@@ -18,6 +18,7 @@ constexpr int kBfPage = 2 * kHkv * kHeadBytes;
 constexpr float kTreeLog2e = 1.4426950408889634f;
 constexpr float kTreeMost = 16777216.0f;    // 2^24
 constexpr int kTreeBlock = 64;              // keys
+constexpr int kTreePart = 8 * kWave * 4;    // numbers of a wave's part
 constexpr int kTreeHalf = kTreeBlock * kD * 2;  // bytes of a block's k or v in LDS
 
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
@@ -35,8 +36,9 @@ struct TreeArgs {
   const int* kv_len;
   const uint16_t* sinks;
   uint16_t* out;
-  float* part_o;   // [workers + tiles][tokens of a tile][64][64]
-  float* part_ml;  // [workers + tiles][tokens of a tile][64][2]
+  // parts, as a wave's lanes hold them (rows of 16 bytes 256 bytes apart took twice the time):
+  float* part_o;   // [workers + tiles][kv head][tokens of a tile / 4][8][lane][4]
+  float* part_ml;  // [workers + tiles][kv head][tokens of a tile / 4][32 columns][2]
   int words, num_pages, window, batch, tiles, workers, least;
   float c2;        // sm_scale log2(e)
 };
@@ -536,14 +538,13 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
                        (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
       }
   } else {
-    const size_t pt = ((size_t)place * 4 * kC + token) * kHq + hk * kGroup + (c & 7);
+    const size_t at = ((size_t)place * kHkv + hk) * kC + cw;
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *(f32x4*)(a.part_o + pt * kD + 32 * dt + 2 * i + 4 * h) =
-            f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
-    if (h == 0) *(float2*)(a.part_ml + pt * 2) = make_float2(-mneg, lt);
+    for (int q = 0; q < 8; ++q)
+      *(f32x4*)(a.part_o + at * kTreePart + (q * kWave + lane) * 4) =
+          f32x4{o[q >> 2][4 * (q & 3)], o[q >> 2][4 * (q & 3) + 1], o[q >> 2][4 * (q & 3) + 2],
+                o[q >> 2][4 * (q & 3) + 3]};
+    if (h == 0) *(float2*)(a.part_ml + (at * 32 + c) * 2) = make_float2(-mneg, lt);
   }
 }
 
@@ -599,11 +600,14 @@ __attribute__((amdgpu_waves_per_eu(kC <= 4 ? 2 : 4))) void tree_kernel(TreeArgs 
   } while (at < stop);
 }
 
-// The parts of a tile merged, in order: 16 threads a row (token, head), four dimensions each, eight
-// parts' loads in flight.  `tokens`: of a tile.
+// The parts of a tile merged, in order: a wave a quarter of a half (q) of a wave's 4 tokens of a kv
+// head, in the lanes that wrote them; eight parts' loads in flight.  `tokens`: of a tile.
 __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens) {
-  const int i = blockIdx.y * 16 + (threadIdx.x >> 4);  // (token of the tile, head)
-  const int token = i / kHq, head = i % kHq, d = (threadIdx.x & 15) * 4;
+  const int waves = tokens / 4, lane = threadIdx.x & 63, c = lane & 31;
+  const int group = blockIdx.y >> 1, hk = group / waves, cw = group % waves;
+  const int q = 4 * (blockIdx.y & 1) + (threadIdx.x >> 6);
+  const int token = 4 * cw + (c >> 3), head = hk * kGroup + (c & 7);
+  const int d = 32 * (q >> 2) + 8 * (q & 3) + 4 * (lane >> 5);
   const int b = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
   const TreeLine line(a, tokens);
   const int qb = __builtin_amdgcn_readlane(line.row, b);
@@ -612,10 +616,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
   if (tile * tokens >= qn) return;
   const int64_t from = TreeLine::lane_of(line.before, b) + (int64_t)tile * blocks;
   const int first = line.worker_of(from), used = line.worker_of(from + blocks - 1) - first + 1;
-  if (used <= 1 || token >= tokens || tile * tokens + token >= qn) return;  // (written already)
+  // (read before any lane leaves: one that has left need not hold its values)
   const int place = first + __builtin_amdgcn_readlane(line.tiles_before, b) + tile;
-  const size_t at = ((size_t)place * tokens + token) * kHq + head;
-  const size_t step = (size_t)tokens * kHq;
+  if (used <= 1 || tile * tokens + token >= qn) return;  // (written already, or no token)
+  const size_t step = (size_t)kHkv * waves, at = place * step + group;
   float m = -INFINITY, l = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < used; s0 += 8) {
@@ -624,8 +628,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const size_t pt = at + (size_t)min(s0 + j, used - 1) * step;
-      ml[j] = *(const float2*)(a.part_ml + pt * 2);
-      po[j] = *(const f32x4*)(a.part_o + pt * kD + d);
+      ml[j] = *(const float2*)(a.part_ml + (pt * 32 + c) * 2);
+      po[j] = *(const f32x4*)(a.part_o + pt * kTreePart + (q * kWave + lane) * 4);
     }
     float mn = m;
 #pragma unroll
@@ -658,7 +662,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
 extern "C" {
 
 // tokens: of a tile, 4, 8, 16 or 32; workers: of a kv head, 0: a workgroup a tile (more than 64
-// sequences); else part_o [workers + batch * tiles][tokens][64][64], part_ml [.. ][2] in its place.
+// sequences); else part_o of 64 x 64 and part_ml of 64 x 2 numbers for each token of
+// workers + batch * tiles tiles.
 int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_len,
                      const void* mask, int words, const int* positions, const void* cache,
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
@@ -688,7 +693,7 @@ int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_le
     return -6;
   if (hipGetLastError() != hipSuccess) return -6;
   if (workers > 0)
-    hipLaunchKernelGGL(attn::tree_merge_kernel, dim3(batch * tiles, tokens * attn::kHq / 16),
+    hipLaunchKernelGGL(attn::tree_merge_kernel, dim3(batch * tiles, attn::kHkv * tokens / 2),
                        dim3(256), 0, s, a, tokens);
   return hipGetLastError() == hipSuccess ? 0 : -6;
 }
