@@ -65,7 +65,7 @@ int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_le
                      const void* mask, int words, const int* positions, const void* cache,
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
                      const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
-                     int tokens, int workers, int least, float* part_o, float* part_ml,
+                     int tokens, int workers, int least, int lead, float* part_o, float* part_ml,
                      hipStream_t s);
 int attn_launch_tree_commit(void* cache, int layers, int num_pages, bool fp8,
                             const int* page_indptr, const int* page_indices, const int* kv_len,
@@ -600,14 +600,17 @@ constexpr int64_t kBeams = 64;        // of a request, and continuations of one 
 constexpr int64_t kMaxBatch = 65535, kMaxLayers = 65535;
 
 // Tokens of a tree's tile, and how many workgroups of a kv head its keys are shared out over:
-// as many as fit the chip at once (two a CU), each of kTreeLeast blocks or more; 0: a workgroup a
-// tile, where there are tiles enough to fill it twice over, more than 64 sequences or no bound.
-// us of the kernel, for 16 trees of 8 nodes over up to 4000 tokens with 32, 64, 128 workgroups: 28,
-// 25, 30; of at least 2, 4, 8, 16 blocks: 24.7, 25, 25, 29, and one tree of 5 nodes over 777
-// tokens 8.6, 8.2, 11, 14 (then without the merge's 3.8).  Tiles of 32 tokens take a CU each:
-// two trees of 26 nodes over up to 131072 tokens, 32 of 16 waves 146, 64 of 8 waves 150 and a merge
-// of twice the parts.
-constexpr int64_t kTreeLeast = 4, kTreeWorkers = 64;
+// as many as the chip holds at once (two a CU; of tiles of 16 tokens and more, whose waves and
+// registers fill one, one a CU), each of kTreeLeast blocks or more; 0: a workgroup a tile, where
+// there are tiles enough to fill it twice over, more than 64 sequences or no bound.
+// us of a call (with the parts' merge) at sizes of trees x nodes over up to so many tokens:
+//  * 32 instead of 64 workgroups of 8-token tiles: 16 x 8 over 4000 28 and 25, 48 of them 28;
+//    64 instead of 32 of 16-token tiles: 4 x 16 over 8000 31 and 24, 40 x 16 over 700 38 and 31.
+//  * kTreeLeast 2, 4, 6, 8: 1 x 5 over 777 11.6, 11.9, 13.0, 13.9; 1 x 32 over 1000 18.1, 18.4, 19.8,
+//    21.8; 3 x 8 over 300 12.6, 12.2, 9.6, 9.7 (no merge).
+//  * kTreeLead (blocks that beginning another tile counts for) 0, 2, 4, 8, 12: 16 x 8 over 4000
+//    28, 27, 26, 25, 26; 1 x 64 over 16000 45, 44, 41, 40, 41; 64 x 26 over 500 69, 64, 63, 59, 57.
+constexpr int64_t kTreeLeast = 4, kTreeLead = 8, kTreeWorkers = 64;
 struct TreePlan {
   int64_t tokens, tiles, workers;
 };
@@ -619,7 +622,7 @@ TreePlan tree_plan(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t
   if (keys <= 0 || batch > 64 || batch * tiles > 2 * kTreeWorkers) return TreePlan{tokens, tiles, 0};
   const int64_t pieces = (batch * tiles * fp8_blocks(keys) + kTreeLeast - 1) / kTreeLeast;
   if (pieces <= batch * tiles) return TreePlan{tokens, tiles, 0};
-  return TreePlan{tokens, tiles, std::min(tokens == 32 ? kTreeWorkers / 2 : kTreeWorkers, pieces)};
+  return TreePlan{tokens, tiles, std::min(tokens >= 16 ? kTreeWorkers / 2 : kTreeWorkers, pieces)};
 }
 
 int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,
@@ -651,7 +654,8 @@ int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch
   return status(attn_launch_tree(q, q_indptr, (int)batch, (int)max_q_len, tree_mask,
                                  (int)mask_words, positions, kv_cache, fp8, page_indptr,
                                  page_indices, (int)num_pages, kv_len, window, sm_scale, sinks, out,
-                                 (int)plan.tokens, (int)plan.workers, (int)kTreeLeast, part_o,
+                                 (int)plan.tokens, (int)plan.workers, (int)kTreeLeast,
+                                 (int)kTreeLead, part_o,
                                  need ? part_o + parts * kQHeads * kHeadDim : nullptr,
                                  as_stream(stream)));
 }

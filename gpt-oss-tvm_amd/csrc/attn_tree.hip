@@ -39,7 +39,7 @@ struct TreeArgs {
   // parts, as a wave's lanes hold them (rows of 16 bytes 256 bytes apart took twice the time):
   float* part_o;   // [workers + tiles][kv head][tokens of a tile / 4][8][lane][4]
   float* part_ml;  // [workers + tiles][kv head][tokens of a tile / 4][32 columns][2]
-  int words, num_pages, window, batch, tiles, workers, least;
+  int words, num_pages, window, batch, tiles, workers, least, lead;
   float c2;        // sm_scale log2(e)
 };
 
@@ -60,8 +60,9 @@ struct TreeSpan {
 
 // The work of a kv head in one line: the blocks of every tile of every sequence (up to 64, one a
 // lane; a tile without keys counts as one), one after the other, cut into equal pieces of at least
-// `least`, a worker each.  Sequences of all lengths and few of them fill the chip alike, and it
-// follows from the keys and not from the caller's bound on them, which only trims the workers.
+// `least`, a worker each; before every tile but the first `lead` blocks that nobody has, for what
+// beginning another tile costs.  Sequences of all lengths and few of them fill the chip alike, and
+// it follows from the keys and not from the caller's bound on them, which only trims the workers.
 // A worker's part of tile g (counted over all sequences) that it does not have whole goes to place
 // worker + g of the workspace: two parts never share one, as one step in the line moves on
 // to the next worker, the next tile or both.
@@ -70,6 +71,7 @@ struct TreeLine {
   int64_t all, piece;
   int blocks;             // of one of its tiles
   int tiles_before;       // of the sequences before it
+  int lead;
   int row, nodes, total, page, pages;  // its tables
   TreeLine() = default;
   __device__ __forceinline__ TreeLine(const TreeArgs& a, int tokens) {
@@ -82,7 +84,7 @@ struct TreeLine {
     if (pages <= 0) total = 0;
     blocks = max(1, TreeSpan(max(total - nodes, 0), total, a.window).blocks);
     const int tiles = lane < a.batch ? min(max((nodes + tokens - 1) / tokens, 0), a.tiles) : 0;
-    const int64_t mine = (int64_t)tiles * blocks;
+    const int64_t mine = (int64_t)tiles * (a.lead + blocks);
     after = mine;
     int tiles_after = tiles;
 #pragma unroll
@@ -94,7 +96,8 @@ struct TreeLine {
     }
     before = after - mine;
     tiles_before = tiles_after - tiles;
-    all = lane_of(after, 63);
+    all = max((int64_t)0, lane_of(after, 63) - a.lead);  // (it begins at a.lead)
+    lead = a.lead;
     // (exact: far below 2^53, and a quotient is an integer or 1 / workers away from the next)
     piece = max((int64_t)a.least, (int64_t)((double)(all + a.workers - 1) / (double)a.workers));
   }
@@ -103,7 +106,7 @@ struct TreeLine {
                      (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32);
   }
   __device__ __forceinline__ int worker_of(int64_t at) const {
-    return (int)((double)at / (double)piece);  // (as above)
+    return (int)((double)(at - lead) / (double)piece);  // (as above)
   }
 };
 
@@ -134,20 +137,21 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //    window's edge) a lane has its token's 32 bits of a tile.
 //
 // What bounds it, with us of the kernel alone at four sizes: 1 tree of 5 nodes over 777 tokens, 16
-// of 8 over up to 4000 (bf16), 1 of 64 over 16000, 2 of 26 over up to 131072 (8-bit): 8.2, 24, 42,
-// 146.
+// of 8 over up to 4000 (bf16), 1 of 64 over 16000, 2 of 26 over up to 131072 (8-bit): 8.2, 21,
+// 33, 137.
 //  * Few nodes: the keys' bytes, and at the smallest calls the loads that wait for one another
-//    (tables, page ids, keys, parts).  16 x 8: 80 MB, 3.3 TB/s; a copy reaches 5.0.
+//    (tables, page ids, keys, parts).  16 x 8: 80 MB, 3.9 TB/s; a copy reaches 5.0.
 //  * Many nodes: the products and the exponentials beside them.  2 x 26: 85 GFLOP for tokens that
-//    are there, 590 TFLOP/s of the 1280 that a large bf16 product reaches; a wave's 32 keys take
-//    260 cycles of matrix instructions and 250 of others, 160 of them exponentials.  Without
-//    its exponentials it takes 128, without the second product 135, without staging 153: no part
-//    carries it alone.  Two 32-key tiles at once, the operands of a tile read ahead, four buffers
-//    and half the barriers, sums by additions and raised wave priorities were each timed
-//    and gained nothing (144 .. 175).
-//  * kC: a tile as wide as the tree, so that its keys are staged once, up to 32 tokens.  kK:
-//    8-token tiles with 1, 2, 4 groups: 16 x 8 28, 25, 32, one of 5 nodes 10.4, 8.2, 9.7; 32-token
-//    tiles with 1, 2: 2 x 26 175, 146 (with as many workgroups).
+//    are there, 620 TFLOP/s of the 1280 that a large bf16 product reaches; a wave's 32 keys take
+//    260 cycles of matrix instructions and 250 of others, 160 of them exponentials.  At 146 in
+//    all it was 128 without the exponentials, 135 without the second product, 153 without
+//    staging: no part carries it alone.  Two 32-key tiles at once, the operands of a tile read
+//    ahead, four buffers and half the barriers, sums by additions and raised wave priorities were
+//    each timed and gained nothing (144 .. 175).
+//  * kC: a tile as wide as the tree, so that its keys are staged once, up to 32 tokens.  kK, with
+//    as many waves on the chip, both launches: 8-token tiles of 2 and 4 groups, 16 x 8 25.5 and 28,
+//    64 x 8 over up to 1000 34 and 41; 4-token tiles of 4 and 8, 64 x 4 over up to 500 24 and 30;
+//    32-token tiles of 2 and 1, 2 x 26 153 and 160.
 //  * Registers: up to 16 tokens 256 a lane (32 trees of 16 nodes in a window: 13; with 128,
 //    spilled, 21); 32 tokens take 16 waves and so 128.
 template <int kC, int kK>
@@ -559,8 +563,8 @@ __attribute__((amdgpu_waves_per_eu(kC <= 4 ? 2 : 4))) void tree_kernel(TreeArgs 
   if (a.workers > 0) {
     const TreeLine line(a, 4 * kC);
     const int64_t piece = TreeLine::lane_of(line.piece, 0);
-    at = worker * piece;
-    stop = min(at + piece, line.all);
+    at = worker * piece + a.lead;
+    stop = min(at + piece, line.all + a.lead);
     if (at >= stop) return;
     if (threadIdx.x < kWave) lines[lane] = line;
     moe::lds_barrier();
@@ -573,8 +577,13 @@ __attribute__((amdgpu_waves_per_eu(kC <= 4 ? 2 : 4))) void tree_kernel(TreeArgs 
       auto one = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
       const int blocks = one(line.blocks);
       const int from = (int)(at - TreeLine::lane_of(line.before, 0));
-      tile = from / blocks;
-      first = from - tile * blocks;
+      tile = from / (a.lead + blocks);
+      first = from - tile * (a.lead + blocks) - a.lead;
+      if (first < 0) {  // the blocks before a tile
+        at -= first;
+        if (at >= stop) return;
+        first = 0;
+      }
       n = min((int64_t)(blocks - first), stop - at);
       if (n < blocks) place = worker + one(line.tiles_before) + tile;
       qb = one(line.row);
@@ -614,7 +623,8 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
   const int qn = __builtin_amdgcn_readlane(line.nodes, b);
   const int blocks = __builtin_amdgcn_readlane(line.blocks, b);
   if (tile * tokens >= qn) return;
-  const int64_t from = TreeLine::lane_of(line.before, b) + (int64_t)tile * blocks;
+  const int64_t from = TreeLine::lane_of(line.before, b) +
+                       (int64_t)tile * (a.lead + blocks) + a.lead;
   const int first = line.worker_of(from), used = line.worker_of(from + blocks - 1) - first + 1;
   // (read before any lane leaves: one that has left need not hold its values)
   const int place = first + __builtin_amdgcn_readlane(line.tiles_before, b) + tile;
@@ -668,14 +678,14 @@ int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_le
                      const void* mask, int words, const int* positions, const void* cache,
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
                      const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
-                     int tokens, int workers, int least, float* part_o, float* part_ml,
+                     int tokens, int workers, int least, int lead, float* part_o, float* part_ml,
                      hipStream_t s) {
   if (workers < 0 || (workers > 0 && batch > 64) || least < 1) return -6;
   const int tiles = (max_q_len + tokens - 1) / tokens;
   const attn::TreeArgs a{(const uint16_t*)q, q_indptr, (const uint32_t*)mask, positions,
                          (const uint8_t*)cache, page_indptr, page_indices, kv_len,
                          (const uint16_t*)sinks, (uint16_t*)out, part_o, part_ml, words,
-                         num_pages, window, batch, tiles, workers, least,
+                         num_pages, window, batch, tiles, workers, least, lead,
                          sm_scale * attn::kTreeLog2e};
   const int grid = attn::kHkv * (workers > 0 ? workers : batch * tiles);
   auto go = [&](auto kernel, int waves) {
