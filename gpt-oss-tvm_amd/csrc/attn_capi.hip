@@ -66,7 +66,7 @@ int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_le
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
                      const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
                      int tokens, int workers, int least, int lead, float* part_o, float* part_ml,
-                     hipStream_t s);
+                     void* line, hipStream_t s);
 int attn_launch_tree_commit(void* cache, int layers, int num_pages, bool fp8,
                             const int* page_indptr, const int* page_indices, const int* kv_len,
                             const int* q_indptr, int batch, int rows, int max_q_len,
@@ -649,15 +649,16 @@ int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch
   if (need && !a16(workspace)) return MOE_ERR_ALIGN;
   if (workspace_bytes < need) return MOE_ERR_WORKSPACE;
   const TreePlan plan = tree_plan(batch, max_q_len, max_kv_len, window);
+  // parts of o, their (m, l), and what the merge needs to know of the tiles
   float* part_o = (float*)workspace;
-  const int64_t parts = (plan.workers + plan.tiles * batch) * plan.tokens;
+  const int64_t parts = (plan.workers + plan.tiles * batch) * plan.tokens * kQHeads;
+  float* part_ml = need ? part_o + parts * kHeadDim : nullptr;
   return status(attn_launch_tree(q, q_indptr, (int)batch, (int)max_q_len, tree_mask,
                                  (int)mask_words, positions, kv_cache, fp8, page_indptr,
                                  page_indices, (int)num_pages, kv_len, window, sm_scale, sinks, out,
                                  (int)plan.tokens, (int)plan.workers, (int)kTreeLeast,
-                                 (int)kTreeLead, part_o,
-                                 need ? part_o + parts * kQHeads * kHeadDim : nullptr,
-                                 as_stream(stream)));
+                                 (int)kTreeLead, part_o, part_ml,
+                                 need ? part_ml + parts * 2 : nullptr, as_stream(stream)));
 }
 
 int tree_commit(void* kv_cache, int64_t layers, int64_t num_pages, const int32_t* page_indptr,
@@ -689,7 +690,8 @@ size_t attn_tree_workspace_bytes(int64_t batch, int64_t max_q_len, int64_t max_k
   const TreePlan plan = tree_plan(batch, max_q_len, max_kv_len, window);
   if (plan.workers == 0) return 0;
   return (size_t)((plan.workers + plan.tiles * batch) * plan.tokens * kQHeads * (kHeadDim + 2)) *
-         sizeof(float);
+             sizeof(float) +
+         (size_t)(plan.tiles * batch) * 16;
 }
 
 int attn_tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,

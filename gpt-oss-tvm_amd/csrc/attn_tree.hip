@@ -39,6 +39,7 @@ struct TreeArgs {
   // parts, as a wave's lanes hold them (rows of 16 bytes 256 bytes apart took twice the time):
   float* part_o;   // [workers + tiles][kv head][tokens of a tile / 4][8][lane][4]
   float* part_ml;  // [workers + tiles][kv head][tokens of a tile / 4][32 columns][2]
+  int4* line;      // [batch][tiles]: first part, parts (0 or 1: none to merge), row, rows
   int words, num_pages, window, batch, tiles, workers, least, lead;
   float c2;        // sm_scale log2(e)
 };
@@ -46,6 +47,9 @@ struct TreeArgs {
 __device__ __forceinline__ f32x16 tree_mfma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
+
+template <int kValue>
+using Const = std::integral_constant<int, kValue>;
 
 // The blocks of 64 keys that a sequence's nodes look at.
 struct TreeSpan {
@@ -71,7 +75,6 @@ struct TreeLine {
   int64_t all, piece;
   int blocks;             // of one of its tiles
   int tiles_before;       // of the sequences before it
-  int lead;
   int row, nodes, total, page, pages;  // its tables
   TreeLine() = default;
   __device__ __forceinline__ TreeLine(const TreeArgs& a, int tokens) {
@@ -87,17 +90,25 @@ struct TreeLine {
     const int64_t mine = (int64_t)tiles * (a.lead + blocks);
     after = mine;
     int tiles_after = tiles;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t x = __shfl_up(after, off, kWave);
-      const int y = __shfl_up(tiles_after, off, kWave);
-      after += lane >= off ? x : 0;
-      tiles_after += lane >= off ? y : 0;
-    }
+    // (by register moves: within rows of 16 lanes, then across them; through LDS 0.4 us more)
+    auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+      auto moved = [&](int x) {
+        return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF,
+                                           false);
+      };
+      const uint64_t low = (uint32_t)moved((int)(uint32_t)after);
+      after += (int64_t)(low | (uint64_t)(uint32_t)moved((int)(after >> 32)) << 32);
+      tiles_after += moved(tiles_after);
+    };
+    step(Const<0x111>(), Const<0xF>());  // row_shr:1, 2, 4, 8
+    step(Const<0x112>(), Const<0xF>());
+    step(Const<0x114>(), Const<0xF>());
+    step(Const<0x118>(), Const<0xF>());
+    step(Const<0x142>(), Const<0xA>());  // row_bcast:15 into rows 1 and 3
+    step(Const<0x143>(), Const<0xC>());  // row_bcast:31 into rows 2 and 3
     before = after - mine;
     tiles_before = tiles_after - tiles;
     all = max((int64_t)0, lane_of(after, 63) - a.lead);  // (it begins at a.lead)
-    lead = a.lead;
     // (exact: far below 2^53, and a quotient is an integer or 1 / workers away from the next)
     piece = max((int64_t)a.least, (int64_t)((double)(all + a.workers - 1) / (double)a.workers));
   }
@@ -105,8 +116,20 @@ struct TreeLine {
     return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, l) |
                      (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32);
   }
-  __device__ __forceinline__ int worker_of(int64_t at) const {
-    return (int)((double)(at - lead) / (double)piece);  // (as above)
+  // what the merge needs to know of the lane's sequence's tiles
+  __device__ __forceinline__ void write(const TreeArgs& a, int tokens) const {
+    const int b = threadIdx.x & 63, used = (nodes + tokens - 1) / tokens;
+    if (b >= a.batch) return;
+    for (int i = 0; i < a.tiles; ++i) {
+      const int64_t from = before + (int64_t)i * (a.lead + blocks);  // (less lead: it begins there)
+      // (exact, as above)
+      const int first = (int)((double)from / (double)piece);
+      const int last = (int)((double)(from + blocks - 1) / (double)piece);
+      a.line[b * a.tiles + i] =
+          i < used ? make_int4(first + tiles_before + i, last - first + 1, row + i * tokens,
+                               min(tokens, nodes - i * tokens))
+                   : make_int4(0, 0, 0, 0);
+    }
   }
 };
 
@@ -565,6 +588,7 @@ __attribute__((amdgpu_waves_per_eu(kC <= 4 ? 2 : 4))) void tree_kernel(TreeArgs 
     const int64_t piece = TreeLine::lane_of(line.piece, 0);
     at = worker * piece + a.lead;
     stop = min(at + piece, line.all + a.lead);
+    if (blockIdx.x == 0 && threadIdx.x < kWave) line.write(a, 4 * kC);
     if (at >= stop) return;
     if (threadIdx.x < kWave) lines[lane] = line;
     moe::lds_barrier();
@@ -617,19 +641,10 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
   const int q = 4 * (blockIdx.y & 1) + (threadIdx.x >> 6);
   const int token = 4 * cw + (c >> 3), head = hk * kGroup + (c & 7);
   const int d = 32 * (q >> 2) + 8 * (q & 3) + 4 * (lane >> 5);
-  const int b = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
-  const TreeLine line(a, tokens);
-  const int qb = __builtin_amdgcn_readlane(line.row, b);
-  const int qn = __builtin_amdgcn_readlane(line.nodes, b);
-  const int blocks = __builtin_amdgcn_readlane(line.blocks, b);
-  if (tile * tokens >= qn) return;
-  const int64_t from = TreeLine::lane_of(line.before, b) +
-                       (int64_t)tile * (a.lead + blocks) + a.lead;
-  const int first = line.worker_of(from), used = line.worker_of(from + blocks - 1) - first + 1;
-  // (read before any lane leaves: one that has left need not hold its values)
-  const int place = first + __builtin_amdgcn_readlane(line.tiles_before, b) + tile;
-  if (used <= 1 || tile * tokens + token >= qn) return;  // (written already, or no token)
-  const size_t step = (size_t)kHkv * waves, at = place * step + group;
+  const int4 tile = a.line[blockIdx.x];
+  const int used = tile.y;
+  if (used <= 1 || token >= tile.w) return;  // (written already, or no token)
+  const size_t step = (size_t)kHkv * waves, at = tile.x * step + group;
   float m = -INFINITY, l = 0.f;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < used; s0 += 8) {
@@ -662,7 +677,7 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(TreeArgs a, int tokens)
   uint16_t v4[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) v4[q] = f2bf(o[q] * f);
-  *(uint2*)(a.out + ((size_t)(qb + tile * tokens + token) * kHq + head) * kD + d) =
+  *(uint2*)(a.out + ((size_t)(tile.z + token) * kHq + head) * kD + d) =
       make_uint2((uint32_t)v4[0] | ((uint32_t)v4[1] << 16),
                  (uint32_t)v4[2] | ((uint32_t)v4[3] << 16));
 }
@@ -673,18 +688,18 @@ extern "C" {
 
 // tokens: of a tile, 4, 8, 16 or 32; workers: of a kv head, 0: a workgroup a tile (more than 64
 // sequences); else part_o of 64 x 64 and part_ml of 64 x 2 numbers for each token of
-// workers + batch * tiles tiles.
+// workers + batch * tiles tiles, and line of 16 bytes for each of batch * tiles.
 int attn_launch_tree(const void* q, const int* q_indptr, int batch, int max_q_len,
                      const void* mask, int words, const int* positions, const void* cache,
                      bool fp8, const int* page_indptr, const int* page_indices, int num_pages,
                      const int* kv_len, int window, float sm_scale, const void* sinks, void* out,
                      int tokens, int workers, int least, int lead, float* part_o, float* part_ml,
-                     hipStream_t s) {
+                     void* line, hipStream_t s) {
   if (workers < 0 || (workers > 0 && batch > 64) || least < 1) return -6;
   const int tiles = (max_q_len + tokens - 1) / tokens;
   const attn::TreeArgs a{(const uint16_t*)q, q_indptr, (const uint32_t*)mask, positions,
                          (const uint8_t*)cache, page_indptr, page_indices, kv_len,
-                         (const uint16_t*)sinks, (uint16_t*)out, part_o, part_ml, words,
+                         (const uint16_t*)sinks, (uint16_t*)out, part_o, part_ml, (int4*)line, words,
                          num_pages, window, batch, tiles, workers, least, lead,
                          sm_scale * attn::kTreeLog2e};
   const int grid = attn::kHkv * (workers > 0 ? workers : batch * tiles);
