@@ -143,13 +143,15 @@ std::tuple<Tensor, Tensor, Tensor> tree_commit(
   const auto* tk = (const int32_t*)need(call, tokens, "tokens", kInt, {n});
   const auto* pa = (const int32_t*)need(call, parents, "parents", kInt, {n});
   const auto* ch = (const int32_t*)need(call, chosen, "chosen", kInt, {n});
+  const at::AutoDispatchBelowADInplaceOrView below;  // (of integers: nothing to differentiate)
   const Tensor out = at::empty({n + 2 * batch}, tokens.options());
   auto* p = (int32_t*)out.data_ptr();
   check((c.fp8 ? attn_tree_commit_fp8 : attn_tree_commit)(
             c.data, c.layers, c.pages, pi, ids, len, qi, batch, n, max_q_len, tk, pa, ch, p, p + n,
             p + n + batch, call.handle()),
         c.fp8 ? "attn_tree_commit_fp8" : "attn_tree_commit");
-  return {out.narrow(0, 0, n), out.narrow(0, n, batch), out.narrow(0, n + batch, batch)};
+  return {at::as_strided(out, {n}, {1}, 0), at::as_strided(out, {batch}, {1}, n),
+          at::as_strided(out, {batch}, {1}, n + batch)};
 }
 
 Tensor kv_copy_pages(const Tensor& kv_cache, const Tensor& src_pages, const Tensor& dst_pages) {
