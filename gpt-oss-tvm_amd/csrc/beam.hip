@@ -12,6 +12,11 @@
 // are k numbers that do.  With q half of the waves (and the q-th largest of their values) about 2 k
 // numbers of a stretch reach it, with q = 1 ten times k.  They go to LDS, and take their
 // places by counting those before them.
+//
+// What bounds it, us of the two launches at rows of 201088: 128 bf16 rows (51 MB, k = 16) 16.4 + 6.3,
+// 20 fp32 rows (16 MB, k = 10) 9 + 5.9, 4 bf16 rows (k = 8) 6.5 + 5.5.  The first is 3.1 TB/s: the
+// same loop without bounds and lists takes 10.6, the exponentials and the bounds the rest.
+// Few rows: loads and barriers that wait for one another, in both launches.
 #include <stdint.h>
 
 #include <algorithm>
@@ -104,8 +109,8 @@ __device__ __forceinline__ float exp_of(float d) {
 }
 
 // T: float or uint16_t (bf16).  A stretch is `chunks` chunks, of which a thread holds 16 elements
-// and the next one's loads, wherever the row begins.  The bound is taken after the first, then after
-// 8, 16, .. and after the last; a thread whose maximum of a chunk reaches it only notes that
+// and the next one's loads, wherever the row begins.  The bound is taken after the first, then
+// after 8, 16, .. and after the last; a thread whose maximum of a chunk reaches it only notes that
 // (looking at each number there cost twice the time), and what reaches the last bound is picked out
 // of the noted ones' 16 numbers, from memory, at the end.
 constexpr int kPartThreads = 512, kPartElems = 16, kChunk = kPartThreads * kPartElems;
@@ -207,7 +212,7 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
   if (chunk == 1 && tail == 0)
     __syncthreads();  // (as it was taken)
   else
-    bound(coarse, chunk < 8 ? 1 : (32 - __builtin_clz(chunk)) & 1);  // (the other turn than the last one's)
+    bound(coarse, chunk < 8 ? 1 : (32 - __builtin_clz(chunk)) & 1);  // (not the last one's turn)
   bool fits = true;
   int records = 0;
 #pragma unroll
@@ -225,7 +230,8 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
       int r = i / kLoads, w = 0;
       for (; r >= wcount[0][w]; ++w) r -= wcount[0][w];
       const int note = found[w][r];
-      const int u = (note / kPartThreads * kLoads + i % kLoads) * kPartThreads + note % kPartThreads;
+      const int u =
+          (note / kPartThreads * kLoads + i % kLoads) * kPartThreads + note % kPartThreads;
       if (u >= units) continue;
       Raw again;
       again.w[0] = *(const u32x4_any*)(x + begin + u * kEach);
@@ -362,9 +368,9 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
 
 // One workgroup a request: its rows' sums, then the k best of its lists.
 constexpr int kMergeThreads = 1024, kMergeList = kMergeThreads;
-// As many are compared with one another at once; us of both launches for 4 beams (k = 8) and for 128
-// (k = 16) of which a mask leaves 3 tokens: up to 128 or 256 25.6 and 39, 512 25.6 and 78, all 1024
-// 179 and 78.
+// As many are compared with one another at once; us of both launches for 4 beams (k = 8) and for
+// 128 (k = 16) of which a mask leaves 3 tokens: up to 128 or 256 25.6 and 39, 512 25.6 and 78, all
+// 1024 179 and 78.
 constexpr int kMergeFew = 256;
 struct Best {
   double v;
@@ -384,6 +390,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(
     float* __restrict__ out_scores, int* __restrict__ out_beams, int* __restrict__ out_tokens) {
   constexpr int kWaves = kMergeThreads / 64;
   __shared__ double row_m[kMost], row_lse[kMost];  // row_lse NaN: a beam without continuations
+  __shared__ float row_score[kMost];
   __shared__ Best list[kMergeList];
   __shared__ int ranks[kMergeList];
   __shared__ uint32_t wbound[kWaves];
@@ -391,8 +398,16 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(
   __shared__ uint32_t logit[2];  // of those equal to the bound, from .. to
   __shared__ int found;
   const int r = blockIdx.x, t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const int each = parts * k, total = W * each;
+  // the first kHeld candidates of a thread stay in registers, most calls' all; their loads go first
+  constexpr int kHeld = 2;
+  const Item* const mine = items + (size_t)r * total;
+  Item first[kHeld];
+#pragma unroll
+  for (int j = 0; j < kHeld; ++j) first[j] = mine[min(t + j * kMergeThreads, total - 1)];
   for (int b = wave; b < W; b += kWaves) {
     const Stat* const st = stats + ((size_t)r * W + b) * parts;
+    const float score = scores[(size_t)r * W + b];
     float m = -INFINITY;
     for (int p = lane; p < parts; p += 64) m = fmaxf(m, st[p].m);
     m = wave_max(m);
@@ -403,19 +418,17 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(
     }
     s = moe::wave_sum_f64(s);
     if (lane == 0) {
-      const float score = scores[(size_t)r * W + b];
       const bool good = m > -INFINITY && m < INFINITY && s == s &&
                         score > -INFINITY && score < INFINITY;
       row_m[b] = m;
+      row_score[b] = score;
       row_lse[b] = good ? log(s) : __builtin_nan("");
     }
   }
   __syncthreads();
-  const int each = parts * k, total = W * each;
   // candidate i of the request's lists; of a beam without continuations the first k tokens
-  auto candidate = [&](int i, Best& c) {
+  auto made = [&](int i, const Item& x, Best& c) {
     const int b = i / each, j = i - b * each;
-    const Item x = items[((size_t)r * W + b) * each + j];
     const double lse = row_lse[b];
     c.beam = b;
     if (lse != lse) {
@@ -426,22 +439,21 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(
     }
     c.x = x.x;
     c.token = x.token;
-    c.v = (double)scores[(size_t)r * W + b] + (((double)x.x - row_m[b]) - lse);
+    c.v = (double)row_score[b] + (((double)x.x - row_m[b]) - lse);
     return x.token >= 0;
   };
+  auto candidate = [&](int i, Best& c) { return made(i, mine[i], c); };
   auto high = [](double v) {  // order-preserving image of its upper half
     const uint32_t u = (uint32_t)(__builtin_bit_cast(uint64_t, v + 0.0) >> 32);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
   };
-  // The first kHeld candidates of a thread stay in registers: most calls' all.
-  constexpr int kHeld = 2;
   Best c, held[kHeld];
   uint32_t lm = 0u, image[kHeld];  // 0: none
   const int rest = t + kHeld * kMergeThreads;
 #pragma unroll
   for (int j = 0; j < kHeld; ++j) {
     const int i = t + j * kMergeThreads;
-    image[j] = i < total && candidate(i, held[j]) ? high(held[j].v) : 0u;
+    image[j] = i < total && made(i, first[j], held[j]) ? high(held[j].v) : 0u;
     lm = max(lm, image[j]);
   }
   for (int i = rest; i < total; i += kMergeThreads)
