@@ -513,3 +513,58 @@ def test_many_tiles(A, fp8):
     rows = np.array([0, 1, 30, 31, 32, 64, 95, 96, 128])
     c.check(c.run(A), 0, rows)
     c.check(c.run(A, 20), 20, rows)
+
+
+@BOTH
+def test_commit_replayed_on_other_rows(A, fp8):
+    """Each replay, with eager calls between, moves the rows that are there then."""
+    rng = np.random.default_rng(66)
+    trees = [random_tree(rng, m, 6) for m in (9, 26)]
+    n, shape = 35, (4, 5, AO.FP8_PAGE_BYTES) if fp8 else (4, 5, 2, HKV, PAGE, D)
+    parents, tokens = i32_dev(np.concatenate(trees)), i32_dev(rng.integers(0, 3, n))
+    chosen = i32_dev(np.zeros(n))
+    cache = torch.zeros(shape, dtype=torch.uint8 if fp8 else torch.bfloat16, device="cuda")
+    tables = (i32_dev(np.array([0, 2, 5])), i32_dev(np.array([3, 0, 4, 1, 2])),
+              i32_dev(np.array([20, 40])), i32_dev(np.array([0, 9, 35])), 26)
+
+    def call():
+        return A.tree_commit(cache, *tables, tokens, parents, chosen)
+
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = call()
+    moved = 0
+    for _ in range(6):
+        before = torch.randint(0, 250, shape, device="cuda").to(cache.dtype)
+        chosen.copy_(torch.randint(0, 3, (n,), device="cuda", dtype=torch.int32))
+        cache.copy_(before)
+        want = [t.clone() for t in call()]
+        rows = cache.clone()
+        moved += not torch.equal(rows, before)
+        cache.copy_(before)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)) and torch.equal(cache, rows)
+    assert moved
+
+
+@BOTH
+def test_moves_past_32_bits(A, fp8):
+    """Rows and pages of the last layer of caches of more than 4 GB (and 2^31 elements)."""
+    page = (AO.FP8_PAGE_BYTES,) if fp8 else (2, HKV, PAGE, D)
+    pool = (1 << 31) // (AO.FP8_PAGE_BYTES if fp8 else 32768) + 3000
+    cache = torch.empty((3, pool, *page), dtype=torch.uint8 if fp8 else torch.bfloat16,
+                        device="cuda")
+    ids = [pool - 1, pool - 5, 7, pool - 2]
+    small = torch.randint(0, 250, (3, 4, *page), device="cuda").to(cache.dtype)
+    cache[:, ids] = small
+    i32 = lambda x: i32_dev(np.array(x))  # noqa: E731
+    args = (i32([23]), i32([0, 5]), 5, i32([1, 2, 3, 4, 5]), i32([-1, 0, 0, 2, 3]),
+            i32([3, 0, 4, 5, 9]))
+    for data, pages in ((cache, ids), (small, [0, 1, 2, 3])):
+        path, count, after = A.tree_commit(data, i32([0, 2]), i32(pages[:2]), *args)
+        assert path.tolist() == [0, 2, 3, 4, -1] and (int(count), int(after)) == (4, 9)
+        A.kv_copy_pages(data, i32([pages[1], pages[2]]), i32([pages[3], pages[0]]))
+    assert torch.equal(cache[:, ids], small)
