@@ -602,15 +602,21 @@ constexpr int64_t kMaxBatch = 65535, kMaxLayers = 65535;
 // Tokens of a tree's tile, and how many workgroups of a kv head its keys are shared out over:
 // as many as the chip holds at once (two a CU; of tiles of 16 tokens and more, whose waves and
 // registers fill one, one a CU), each of kTreeLeast blocks or more; 0: a workgroup a tile, where
-// there are tiles enough to fill it twice over, more than 64 sequences or no bound.
+// there are tiles enough to fill it twice over, more than 64 sequences or no bound, or where the
+// longest sequence the bound allows has few blocks and a share of them would save few.
 // us of a call (with the parts' merge) at sizes of trees x nodes over up to so many tokens:
 //  * 32 instead of 64 workgroups of 8-token tiles: 16 x 8 over 4000 28 and 25, 48 of them 28;
 //    64 instead of 32 of 16-token tiles: 4 x 16 over 8000 31 and 24, 40 x 16 over 700 38 and 31.
-//  * kTreeLeast 2, 4, 6, 8: 1 x 5 over 777 11.6, 11.9, 13.0, 13.9; 1 x 32 over 1000 18.1, 18.4, 19.8,
-//    21.8; 3 x 8 over 300 12.6, 12.2, 9.6, 9.7 (no merge).
+//  * kTreeLeast 2, 4, 6, 8: 1 x 5 over 777 11.6, 11.9, 13.0, 13.9; 1 x 32 over 1000 18.1, 18.4,
+//    19.8, 21.8.
 //  * kTreeLead (blocks that beginning another tile counts for) 0, 2, 4, 8, 12: 16 x 8 over 4000
 //    28, 27, 26, 25, 26; 1 x 64 over 16000 45, 44, 41, 40, 41; 64 x 26 over 500 69, 64, 63, 59, 57.
-constexpr int64_t kTreeLeast = 4, kTreeLead = 8, kTreeWorkers = 64;
+//  * shared out, and a workgroup a tile: 32 x 26 over 1000 45, 31 (over 2000 57, 47), 64 x 8 over
+//    1000 33, 25 (over 2000 43, 39), 40 x 16 over 700 29, 27, 3 x 8 over 300 11.9, 9.8.  With one
+//    long sequence among short ones, 2500 tokens beside 31 or 63 of 64, 34 and 25 both ways;
+//    kTreeFew bounds what longer ones could cost.  kTreeGain 3, 6, 10: 1 x 8 over 500 11.5, 10.8,
+//    10.8, 1 x 32 over 500 16.7, 16.7, 19.6.
+constexpr int64_t kTreeLeast = 4, kTreeLead = 8, kTreeWorkers = 64, kTreeFew = 40, kTreeGain = 6;
 struct TreePlan {
   int64_t tokens, tiles, workers;
 };
@@ -619,10 +625,13 @@ TreePlan tree_plan(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t
   const int64_t tiles = (max_q_len + tokens - 1) / tokens;
   max_kv_len = std::min(max_kv_len, kMaxPages * kPage);  // (and no overflow below)
   const int64_t keys = window > 0 ? std::min(max_kv_len, window + max_q_len) : max_kv_len;
-  if (keys <= 0 || batch > 64 || batch * tiles > 2 * kTreeWorkers) return TreePlan{tokens, tiles, 0};
-  const int64_t pieces = (batch * tiles * fp8_blocks(keys) + kTreeLeast - 1) / kTreeLeast;
-  if (pieces <= batch * tiles) return TreePlan{tokens, tiles, 0};
-  return TreePlan{tokens, tiles, std::min(tokens >= 16 ? kTreeWorkers / 2 : kTreeWorkers, pieces)};
+  if (keys <= 0 || batch > 64 || batch * tiles > 2 * kTreeWorkers)
+    return TreePlan{tokens, tiles, 0};
+  const int64_t most = tokens >= 16 ? kTreeWorkers / 2 : kTreeWorkers;
+  const int64_t blocks = fp8_blocks(keys), all = batch * tiles * blocks;
+  const int64_t piece = std::max(kTreeLeast, (all + most - 1) / most);
+  if (blocks <= kTreeFew && blocks - piece < kTreeGain) return TreePlan{tokens, tiles, 0};
+  return TreePlan{tokens, tiles, std::min(most, (all + kTreeLeast - 1) / kTreeLeast)};
 }
 
 int tree(const uint16_t* q, int64_t rows, const int32_t* q_indptr, int64_t batch,

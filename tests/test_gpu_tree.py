@@ -568,3 +568,25 @@ def test_moves_past_32_bits(A, fp8):
         assert path.tolist() == [0, 2, 3, 4, -1] and (int(count), int(after)) == (4, 9)
         A.kv_copy_pages(data, i32([pages[1], pages[2]]), i32([pages[3], pages[0]]))
     assert torch.equal(cache[:, ids], small)
+
+
+@BOTH
+@pytest.mark.parametrize("window", [0, 3, 100])
+def test_shared_out(A, fp8, window):
+    """A bound far above the lengths: the keys of every tile go to as many workgroups as there are,
+    whose shares begin and end anywhere; sequences without nodes or keys, of one and of several
+    tiles."""
+    rng = np.random.default_rng(13)
+    for seed, (cached, nodes) in enumerate((
+            ([0, 1, 15, 16, 17, 63, 64, 130, 40, 700], [1, 5, 8, 2, 33, 64, 7, 12, 0, 20]),
+            ([0, 2000, 3, 0, 900], [0, 4, 0, 1, 3]),
+            (rng.integers(0, 600, 64).tolist(), rng.integers(0, 9, 64).tolist()),
+            (rng.integers(0, 300, 30).tolist(), rng.integers(9, 17, 30).tolist()),
+            ([1500, 40], [70, 100]), ([5], [1]))):
+        c = Case(100 + seed, fp8, cached, nodes)
+        n, lengths = int(c.starts[-1]), list(c.lengths)
+        c.lengths = [*lengths, 100000]                 # (what run takes its bound from)
+        got = c.run(A, window)
+        c.lengths = lengths
+        assert got.shape[0] == n
+        c.check(got, window)
