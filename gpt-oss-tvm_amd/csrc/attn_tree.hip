@@ -157,7 +157,8 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //  * No running maximum: the reference point is the maximum of the first keys that a column
 //    sees, and is renewed only when a tile's sum passes 2^24.
 //  * Blocks that every token of a wave sees whole take no mask; in the others (the tree's own, a
-//    window's edge) a lane has its token's 32 bits of a tile.
+//    window's edge) a lane has its token's 32 bits of a tile, and tiles of which nobody sees a key
+//    are passed over (32 trees of 16 nodes in a window 12.2 -> 10.9).
 //
 // What bounds it, with us of the kernel alone at four sizes: 1 tree of 5 nodes over 777 tokens, 16
 // of 8 over up to 4000 (bf16), 1 of 64 over 16000, 2 of 26 over up to 131072 (8-bit): 8.2, 21,
@@ -175,8 +176,8 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //    as many waves on the chip, both launches: 8-token tiles of 2 and 4 groups, 16 x 8 25.5 and 28,
 //    64 x 8 over up to 1000 34 and 41; 4-token tiles of 4 and 8, 64 x 4 over up to 500 24 and 30;
 //    32-token tiles of 2 and 1, 2 x 26 153 and 160.
-//  * Registers: up to 16 tokens 256 a lane (32 trees of 16 nodes in a window: 13; with 128,
-//    spilled, 21); 32 tokens take 16 waves and so 128.
+//  * Registers: up to 16 tokens 256 a lane (32 trees of 16 nodes in a window: 14 when this was
+//    chosen; with 128, spilled, 21); 32 tokens take 16 waves and so 128.
 template <int kC, int kK>
 struct TreeLds {
   static constexpr int kBufs = kC == 1 ? 1 : 2;  // one wave needs no second buffer
@@ -352,6 +353,7 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
   };
 
   f32x16 o[2];
+  bool fresh = true;  // no tile yet
   float mneg = INFINITY, l = 0.f;  // minus the column's reference point (not set: inf)
 #pragma unroll
   for (int dt = 0; dt < 2; ++dt)
@@ -372,6 +374,10 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
     constexpr bool kMasked = decltype(masked)::value;
     f32x16 s;
     uint32_t see = ~0u;
+    if constexpr (kMasked) {
+      see = seen(kb + 32 * kt32);
+      if (!__any(see != 0u)) return;
+    }
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.f;
 #pragma unroll
@@ -380,11 +386,12 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
       s = tree_mfma(ka, qv[st], s);
     }
     if constexpr (kMasked) {
-      see = seen(kb + 32 * kt32);
       const uint32_t mine = see >> (4 * h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        s[i] = (mine >> (8 * (i >> 2) + (i & 3))) & 1u ? s[i] : -INFINITY;
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t keep = __builtin_amdgcn_sbfe((int)mine, 8 * (i >> 2) + (i & 3), 1);
+        s[i] = __uint_as_float((keep & __float_as_uint(s[i])) | (~keep & 0xFF800000u));
+      }
     }
     moe::bf16x2 p[8];
     float ps;
@@ -397,8 +404,8 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
         ps = __builtin_amdgcn_fdot2_f32_bf16(p[i], ones, ps, false);
       }
     };
-    exps(mneg);
-    if (__any(!(ps < kTreeMost))) {
+    if (!fresh) exps(mneg);
+    if (fresh || __any(!(ps < kTreeMost))) {
       float mx = s[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
@@ -407,11 +414,13 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
       mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
       const float m = -mneg, mn = fmaxf(m, mx * a.c2);
       const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+      if (!fresh)
 #pragma unroll
-      for (int dt = 0; dt < 2; ++dt)
+        for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+          for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
       l *= alpha;
+      fresh = false;
       mneg = -mn;
       exps(mn == -INFINITY ? 0.0f : -mn);
     }
