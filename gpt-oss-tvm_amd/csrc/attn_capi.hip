@@ -615,7 +615,9 @@ constexpr int64_t kMaxBatch = 65535, kMaxLayers = 65535;
 //    1000 33, 25 (over 2000 43, 39), 40 x 16 over 700 29, 27, 3 x 8 over 300 11.9, 9.8.  With one
 //    long sequence among short ones, 2500 tokens beside 31 or 63 of 64, 34 and 25 both ways;
 //    kTreeFew bounds what longer ones could cost.  kTreeGain 3, 6, 10: 1 x 8 over 500 11.5, 10.8,
-//    10.8, 1 x 32 over 500 16.7, 16.7, 19.6.
+//    10.8, 1 x 32 over 500 16.7, 16.7, 19.6.  6 and 10 for 4-token tiles, whose workgroups share
+//    keys out among four groups: 4 x 4 over 700 11.2, 9.4, 1 x 1 over 700 10.3, 9.3; for 8-token
+//    ones 1 x 5 over 600 11.1, 12.1, 4 x 8 over 700 12.5, 13.4.
 constexpr int64_t kTreeLeast = 4, kTreeLead = 8, kTreeWorkers = 64, kTreeFew = 40, kTreeGain = 6;
 struct TreePlan {
   int64_t tokens, tiles, workers;
@@ -630,7 +632,8 @@ TreePlan tree_plan(int64_t batch, int64_t max_q_len, int64_t max_kv_len, int64_t
   const int64_t most = tokens >= 16 ? kTreeWorkers / 2 : kTreeWorkers;
   const int64_t blocks = fp8_blocks(keys), all = batch * tiles * blocks;
   const int64_t piece = std::max(kTreeLeast, (all + most - 1) / most);
-  if (blocks <= kTreeFew && blocks - piece < kTreeGain) return TreePlan{tokens, tiles, 0};
+  const int64_t gain = tokens == 4 ? kTreeGain + 4 : kTreeGain;
+  if (blocks <= kTreeFew && blocks - piece < gain) return TreePlan{tokens, tiles, 0};
   return TreePlan{tokens, tiles, std::min(most, (all + kTreeLeast - 1) / kTreeLeast)};
 }
 
