@@ -55,20 +55,13 @@ VOCAB = 201088
 SHARED = 512                                # tokens of a prompt that sequences share
 
 
-_module = None
-
-
 def _native():
-    """The framework's binding, imported by the first call that wants it."""
-    global _module
-    if _module is None:
-        pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                           "gpt-oss-tvm_amd")
-        if pkg not in sys.path:
-            sys.path.insert(1, pkg)
-        import attn_native
-        _module = attn_native
-    return _module
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                       "gpt-oss-tvm_amd")
+    if pkg not in sys.path:
+        sys.path.insert(1, pkg)
+    import attn_native
+    return attn_native
 
 
 # -- the cases ---------------------------------------------------------------------------
