@@ -152,8 +152,14 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //  * S^T = K Q^T: lane (column l % 32, half h = l / 32) has the keys 8 (i / 4) + 4 h + i % 4 of a
 //    32-key tile in elements i = 0 .. 15, which are, packed to bf16, the operands of two
 //    products O^T += V^T P^T over 16 keys each.
-//  * p enters as one bf16 rounding, and the sum takes the rounded p: a weight is off by at most
-//    half a bf16 step, as the output's own rounding is.
+//  * p enters as two bf16 pieces, off by 2^-16 of itself at most, as the framework's other
+//    attention over few tokens or a bf16 cache has it; the sum takes both.  Tiles of 32 tokens of
+//    the 8-bit cache round it once, as its long chunks do (a weight off by half a bf16 step at
+//    most, where the cached values are off by up to 16 times as much): errors against 64 bits
+//    0.0020 to 0.0021 instead of 0.0017, but two pieces would take 192 us instead of 132 for 2
+//    trees of 26 over up to 131072, 49 instead of 40 for one of 64 over 16000.  What they cost
+//    the others, graph replays, us with one and with two: 16 x 8 over 4000 29 and 32, 1 x 5 over 777
+//    16.1 and 16.4, 32 x 16 in a window 17.0 and 17.4, 64 x 26 over 500 57 and 76 (bf16).
 //  * No running maximum: the reference point is the maximum of the first keys that a column
 //    sees, and is renewed only when a tile's sum passes 2^24.
 //  * Blocks that every token of a wave sees whole take no mask; in the others (the tree's own, a
@@ -194,6 +200,7 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
                                            int begin, int end, int place) {
   constexpr int kBufs = TreeLds<kC, kK>::kBufs;
   constexpr int kUnits = (kFp8 ? 8 : 16) / kC;  // 1 KB loads of a block that a wave makes
+  constexpr int kPieces = kFp8 && kC == 8 ? 1 : 2;  // of p
   int t = threadIdx.x;
   asm volatile("" : "+v"(t));  // (what follows from it is not carried over to the next piece)
   const int lane = t & 63, c = lane & 31, h = lane >> 5;
@@ -393,15 +400,20 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
         s[i] = __uint_as_float((keep & __float_as_uint(s[i])) | (~keep & 0xFF800000u));
       }
     }
-    moe::bf16x2 p[8];
+    moe::bf16x2 p[kPieces][8];
     float ps;
     auto exps = [&](float mn) __attribute__((always_inline)) {
       ps = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        p[i][0] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i], a.c2, mn));
-        p[i][1] = (__bf16)__builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], a.c2, mn));
-        ps = __builtin_amdgcn_fdot2_f32_bf16(p[i], ones, ps, false);
+        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[2 * i], a.c2, mn));
+        const float e1 = __builtin_amdgcn_exp2f(fmaf(s[2 * i + 1], a.c2, mn));
+        p[0][i] = moe::bf16x2{(__bf16)e0, (__bf16)e1};
+        ps = __builtin_amdgcn_fdot2_f32_bf16(p[0][i], ones, ps, false);
+        if constexpr (kPieces == 2) {
+          p[1][i] = moe::bf16x2{(__bf16)(e0 - (float)p[0][i][0]), (__bf16)(e1 - (float)p[0][i][1])};
+          ps = __builtin_amdgcn_fdot2_f32_bf16(p[1][i], ones, ps, false);
+        }
       }
     };
     if (!fresh) exps(mneg);
@@ -427,9 +439,11 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
     l += ps;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-      bf16x8 pb;
+      bf16x8 pb[kPieces];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) pb[j] = p[4 * m + (j >> 1)][j & 1];
+      for (int n = 0; n < kPieces; ++n)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pb[n][j] = p[n][4 * m + (j >> 1)][j & 1];
 #pragma unroll
       for (int dt = 0; dt < 2; ++dt) {
         bf16x8 va;
@@ -466,7 +480,8 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
             }
           }
         }
-        o[dt] = tree_mfma(va, pb, o[dt]);
+#pragma unroll
+        for (int n = 0; n < kPieces; ++n) o[dt] = tree_mfma(va, pb[n], o[dt]);
       }
     }
   };

@@ -269,7 +269,9 @@ MOE_API int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_i
  * keys of positions above its own minus the window, a node's position being positions[row] (one
  * before the cached tokens' end counts as their end).  out = sum_j p_j v_j / (sum_j p_j +
  * exp(sinks[h])), p_j = exp(sm_scale q . k_j), with one rounding to bf16 as attn_decode_fp8 has it
- * (attn_decode and attn_prefill round o, the sink's factor and their product); a row that
+ * (attn_decode and attn_prefill round o, the sink's factor and their product).  The p_j enter
+ * to about 16 bits; in attn_tree_fp8 with max_q_len above 16 they are rounded to bf16, as in
+ * attn_prefill_fp8's longer chunks (their sum is taken of the rounded ones).  A row that
  * sees no key gets 0.  Keys that a row does not see do not affect it, whatever they
  * hold; infinities and NaN in those that it sees go where the formula takes them (8-bit cache:
  * their rows stand for NaN).  Rows outside q_indptr's ranges are left as they are.
