@@ -29,7 +29,9 @@ each (the format of include/attn_gfx950.h): one uint8 tensor [layers, pages,
 
 Sequences may share pages: ``branch`` lets several go on from what one holds (beams), at
 no cost but the page lists'.  A page that others hold too and that a forward would write to is
-copied first, in all layers by one launch.
+copied first, in all layers by one launch.  A forward lists a shared page once a sequence, so its
+lists may be longer than the pool: the tables have room for ``max_listed`` entries (by default a
+whole pool a sequence, up to 2^22 more than the pool has), and a forward that lists more is refused.
 
 ``begin_tree`` appends a tree of drafted tokens to each sequence in place of a chunk: the tables
 then also have each node's mask over its tree, and positions by depth.
@@ -44,6 +46,7 @@ import torch
 
 PAGE_SIZE = 16
 FP8_PAGE_BYTES = 16640  # of a page of an 8-bit cache
+SHARED_LISTED = 1 << 22  # entries of a forward's page lists beyond the pool's size
 STAGED = 64             # tokens of the largest fused decode projection
 TREE_MAX_NODES = 1024   # of a sequence's tree of drafted tokens
 
@@ -82,11 +85,14 @@ class ForwardTables:
 class PagedKVCache:
     def __init__(self, num_layers: int, num_pages: int, max_batch: int, max_tokens: int,
                  kv_heads: int = 8, head_dim: int = 64, device="cuda",
-                 dtype=torch.bfloat16):
+                 dtype=torch.bfloat16, max_listed: int | None = None):
         self.num_layers = num_layers
         self.num_pages = num_pages
         self.max_batch = max_batch
         self.max_tokens = max_tokens
+        if max_listed is None:
+            max_listed = min(max_batch * num_pages, num_pages + SHARED_LISTED)
+        self.max_listed = max(max_listed, num_pages)  # (without sharing it is never more)
         self.fp8 = dtype == torch.float8_e4m3fn
         if self.fp8:
             if (kv_heads, head_dim) != (8, 64):
@@ -114,7 +120,7 @@ class PagedKVCache:
         # range and one copy; a longer forward uses the long arrays at the end
         # (three copies, each spanning only what the forward uses).  Last the pages that a
         # forward copies before it writes to them, sources and then destinations.
-        sizes = (max_batch + 1, max_batch + 1, max_batch, max_batch, max_batch, num_pages,
+        sizes = (max_batch + 1, max_batch + 1, max_batch, max_batch, max_batch, self.max_listed,
                  max_tokens, max_tokens, 2 * max_batch)
         self._tables_dev = torch.zeros(sum(sizes), dtype=torch.int32, device=device)
         # two staging buffers used in turn: a forward waits only for the copy
@@ -335,12 +341,18 @@ class PagedKVCache:
                              f"{self.max_batch} / {self.max_tokens}")
         if min(append_lengths, default=1) < 1:
             raise ValueError("every sequence of a forward appends at least one token")
-        need = sum(max(0, -(-(self.seqs[s].length + a) // PAGE_SIZE) - len(self.seqs[s].pages))
-                   for s, a in zip(seq_ids, append_lengths))
+        grown, listed = {}, 0  # the sequences' lengths, and the page lists' entries
+        for s, a in zip(seq_ids, append_lengths):
+            grown[s] = grown.get(s, self.seqs[s].length) + a
+            listed += -(-grown[s] // PAGE_SIZE)
+        if listed > self.max_listed:
+            raise MemoryError(f"the forward's sequences list {listed} pages, the cache's tables "
+                              f"have room for {self.max_listed} (max_listed)")
+        need = sum(max(0, -(-n // PAGE_SIZE) - len(self.seqs[s].pages)) for s, n in grown.items())
         # a copy for each that writes to a shared page; the last of its holders keeps it
         writers = Counter(self.seqs[s].pages[-1] for s in set(seq_ids)
                           if self._shares_last(self.seqs[s]))
-        need += sum(n - (n == self._refs[page]) for page, n in writers.items())
+        need += sum(w - (w == self._refs[page]) for page, w in writers.items())
         if need > len(self.free):
             raise MemoryError(f"KV cache full: {need} pages needed, {len(self.free)} free")
         q_indptr, positions, slots, page_indptr, page_indices, kv_len = [0], [], [], [0], [], []
