@@ -141,9 +141,11 @@ class Engine:
                     length_penalty: float = 0.0) -> list[tuple[list[int], float]]:
         """The ``width`` best continuations of a prompt found by beam search: at most
         ``max_new_tokens`` tokens each (a stop token ends one), with the sum of their log
-        probabilities, best first by that sum over length ** ``length_penalty``.  The
-        beams share the prompt's pages and each other's; the engine's cache needs room for
-        ``width`` sequences (``max_batch``) and is left as it was."""
+        probabilities, best first by that sum over length ** ``length_penalty``.  It goes on
+        until no beam can come to more than the ``width`` best that have ended; beams that
+        have not are results only with all ``max_new_tokens`` tokens.  The beams share
+        the prompt's pages and each other's; the engine's cache needs room for ``width``
+        sequences (``max_batch``) and is left as it was."""
         cache, stops = self.paged_kv_cache, set(int(t) for t in stop_tokens)
         vocab = self.config.vocab_size
         # of the best width (1 + stops) continuations no more than width stops end
@@ -158,6 +160,11 @@ class Engine:
 
         def worth(beam):
             return beam[1] / max(1, len(beam[0])) ** length_penalty
+
+        def settled():  # sums only fall, so a beam comes to no more than this one's at best
+            longest = max_new_tokens if length_penalty > 0 else len(beams[0][0]) + 1
+            best = beams[0][1] / longest ** length_penalty
+            return len(ended) >= width and sorted(map(worth, ended))[-width] >= best
 
         try:
             logits = self.prefill(input_tokens, seqs[0]).view(1, vocab)
@@ -176,7 +183,10 @@ class Engine:
                         live.append((beams[parent][0] + [token], score))
                         parents.append(parent)
                 beams = live
-                if not live or len(ended) >= width or step == max_new_tokens - 1:
+                if not live or step == max_new_tokens - 1:
+                    break
+                if settled():
+                    beams = []
                     break
                 new = seqs[:len(live)]
                 while len(new) < len(live):
