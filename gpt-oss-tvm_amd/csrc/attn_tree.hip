@@ -159,7 +159,7 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //    0.0020 to 0.0021 instead of 0.0017, but two pieces would take 192 us instead of 132 for 2
 //    trees of 26 over up to 131072, 49 instead of 40 for one of 64 over 16000.  What they cost
 //    the others, graph replays, us with one and with two: 16 x 8 over 4000 29 and 32, 1 x 5 over 777
-//    16.1 and 16.4, 32 x 16 in a window 17.0 and 17.4, 64 x 26 over 500 57 and 76 (bf16).
+//    16.1 and 16.4, 32 x 16 in a window 17.0 and 17.4.
 //  * No running maximum: the reference point is the maximum of the first keys that a column
 //    sees, and is renewed only when a tile's sum passes 2^24.
 //  * Blocks that every token of a wave sees whole take no mask; in the others (the tree's own, a
@@ -189,7 +189,7 @@ struct TreeLds {
   static constexpr int kBufs = kC == 1 ? 1 : 2;  // one wave needs no second buffer
   __align__(16) uint8_t tiles[kK][kBufs][2][kTreeHalf];
   float2 ml[kK][kC][32];
-  int bad[kK][kBufs][kC];  // by each wave: an infinity or a NaN in what it staged of v (bf16)
+  int2 bad[kK][kC];  // a wave's first and last block with an infinity or a NaN in v (bf16)
 };
 
 // Blocks begin .. end - 1 of a tile whose sequence has qn nodes from row qb on and L tokens in all;
@@ -244,8 +244,9 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
       }
     }
   };
-  auto store = [&](Raw& x, uint8_t* kt, uint8_t* vt, int kb, int* bad)
-      __attribute__((always_inline)) {
+  int2 bad = make_int2(INT32_MAX, -1);
+  auto store = [&](Raw& x, uint8_t* kt, uint8_t* vt, int i) __attribute__((always_inline)) {
+    const int kb = (begin + kg + kK * i) * kTreeBlock;
     if constexpr (!kFp8) {
       uint32_t full = 0u;  // bits 15 and 31: an exponent of all ones
 #pragma unroll
@@ -253,8 +254,19 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
         if ((u * kC + cw) >> 3)
 #pragma unroll
           for (int j = 0; j < 4; ++j) full |= (x.data[u][j] & 0x7F807F80u) + 0x00800080u;
-      const bool any = __any(full & 0x80008000u);
-      if (lane == 0) bad[cw] = any;
+      if (__any(full & 0x80008000u)) {
+        bad = make_int2(min(bad.x, i), i);
+        if (lane == 0) lds.bad[kg][cw] = bad;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u)
+          if ((u * kC + cw) >> 3)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t y = x.data[u][j];
+              x.data[u][j] = ((y & 0x7F80u) == 0x7F80u ? 0u : y & 0xFFFFu) |
+                             ((y & 0x7F800000u) == 0x7F800000u ? 0u : y & 0xFFFF0000u);
+            }
+      }
     }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
@@ -376,7 +388,7 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
                         : (4 * h + ((lane >> 2) & 3)) * 128 + ((lane >> 4) & 1) * 32 +
                               (lane & 3) * 8 + ((lane >> 3) & 1) * 64;
   // the 32 keys from 32 kt32 of a block on
-  auto keys32 = [&](auto masked, const uint8_t* kt, const uint8_t* vt, int kb, int kt32, bool bad)
+  auto keys32 = [&](auto masked, const uint8_t* kt, const uint8_t* vt, int kb, int kt32)
       __attribute__((always_inline)) {
     constexpr bool kMasked = decltype(masked)::value;
     f32x16 s;
@@ -461,24 +473,6 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
             w[2 * j + 1] = pair.y;
           }
           va = moe::as_bf16x8(w);
-          if constexpr (kMasked) {
-            if (bad) {
-              // An infinity or a NaN must not meet the probability 0 of who does not see its
-              // key: it goes in by a product of its own, the largest number for it and for who
-              // sees it, whose square is past fp32's range
-              const __bf16 big = (__bf16)3.3895314e38f, none = (__bf16)0.0f;
-              bf16x8 marks, who;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const bool x = ((w[j >> 1] >> (16 * (j & 1))) & 0x7F80u) == 0x7F80u;
-                marks[j] = x ? big : none;
-                va[j] = x ? none : va[j];
-                who[j] =
-                    see >> (16 * m + 8 * (j >> 2) + 4 * h + (j & 3)) & 1u ? big : none;
-              }
-              o[dt] = tree_mfma(marks, who, o[dt]);
-            }
-          }
         }
 #pragma unroll
         for (int n = 0; n < kPieces; ++n) o[dt] = tree_mfma(va, pb[n], o[dt]);
@@ -489,27 +483,68 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
     const int kb = (begin + kg + kK * i) * kTreeBlock;
     const uint8_t *kt = lds.tiles[kg][buf][0], *vt = lds.tiles[kg][buf][1];
     if constexpr (decltype(masked)::value) {
-      int bad = 0;
-      if constexpr (!kFp8) {
-#pragma unroll
-        for (int w = 0; w < kC; ++w) bad |= lds.bad[kg][buf][w];
-        bad = __builtin_amdgcn_readfirstlane(bad);
-      }
 #pragma unroll 1  // (registers)
-      for (int kt32 = 0; kt32 < 2; ++kt32) keys32(masked, kt, vt, kb, kt32, bad != 0);
+      for (int kt32 = 0; kt32 < 2; ++kt32) keys32(masked, kt, vt, kb, kt32);
     } else {
-      keys32(masked, kt, vt, kb, 0, false);
-      keys32(masked, kt, vt, kb, 1, false);
+      keys32(masked, kt, vt, kb, 0);
+      keys32(masked, kt, vt, kb, 1);
     }
   };
   auto put = [&](int buf, int i) __attribute__((always_inline)) {
-    store(raw, lds.tiles[kg][buf][0], lds.tiles[kg][buf][1], (begin + kg + kK * i) * kTreeBlock,
-          lds.bad[kg][buf]);
+    store(raw, lds.tiles[kg][buf][0], lds.tiles[kg][buf][1], i);
+  };
+  // Infinities and NaN in v of a bf16 cache.  They must not meet the probability 0 of who does not
+  // see their key, nor the second piece of one, which may be 0 or negative: staged as 0, they
+  // go in behind the loop (blocks first to last of the group, again from memory) by products of
+  // their own.  The largest number for them and for who sees them, whose square is past fp32's range:
+  // +inf and NaN by one, -inf and NaN by another.  (At the products, in a branch of masked blocks,
+  // they took registers of every call: 64 x 26 over 500 73 us and not 52, 2 x 26 over 40000 119
+  // and not 79.)
+  auto add_bad = [&](int first, int last) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (int at = 4 * first; at < 4 * last + 4; ++at) {  // 16 keys, a page, at a time
+      const int k0 = (begin + kg + kK * (at >> 2)) * kTreeBlock + kPage * (at & 3);
+      const uint8_t* const page =
+          a.cache +
+          (size_t)(unsigned)pages.clamp(pages.ids[min(k0 / kPage, last_page)]) * kPageSize +
+          (kHkv + hk) * kHeadBytes;
+      const uint32_t see = seen(k0);
+      const __bf16 big = (__bf16)3.3895314e38f, none = (__bf16)0.0f;
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt) {
+        uint32_t x[8];
+        bf16x8 marks, who;
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = 8 * (j >> 2) + 4 * h + (j & 3);
+          x[j] = *(const uint16_t*)(page + key * (kD * 2) + (32 * dt + c) * 2);
+          any |= (x[j] & 0x7F80u) == 0x7F80u;
+          who[j] = see >> key & 1u ? big : none;
+        }
+        if (!__any(any)) continue;
+#pragma unroll
+        for (int sign = 0; sign < 2; ++sign) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const bool is = (x[j] & 0x7FFFu) > 0x7F80u || x[j] == (sign ? 0xFF80u : 0x7F80u);
+            marks[j] = is ? sign ? -big : big : none;
+          }
+          f32x16 inf;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) inf[i] = 0.f;
+          inf = tree_mfma(marks, who, inf);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[dt][i] += inf[i];
+        }
+      }
+    }
   };
 
   // every load before the loop (the first block, q, the mask) done: the compiler then waits for
   // nothing but the next block there
   moe::wait_vmcnt<0>();
+  if (!kFp8 && lane == 0) lds.bad[kg][cw] = bad;
   if (mine(0)) put(0, 0);
   if (mine(1)) load(raw, 1);
   if constexpr (kC > 1) moe::lds_barrier();
@@ -534,6 +569,18 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
   run(std::false_type{}, whole1);
   run(std::true_type{}, steps);
 
+  if constexpr (!kFp8) {
+    if (active) {
+#pragma unroll
+      for (int w = 0; w < kC; ++w) {
+        const int2 other = lds.bad[kg][w];
+        bad = make_int2(min(bad.x, other.x), max(bad.y, other.y));
+      }
+      const int first = __builtin_amdgcn_readfirstlane(bad.x);
+      const int last = __builtin_amdgcn_readfirstlane(bad.y);
+      if (last >= 0) add_bad(first, last);
+    }
+  }
   float lt = l + __shfl_xor(l, 32, kWave);
   if constexpr (kK > 1) {
     // the groups' states into the first group's, in order, through the tiles' LDS

@@ -274,7 +274,9 @@ MOE_API int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_i
  * attn_prefill_fp8's longer chunks (their sum is taken of the rounded ones).  A row that
  * sees no key gets 0.  Keys that a row does not see do not affect it, whatever they
  * hold; infinities and NaN in those that it sees go where the formula takes them (8-bit cache:
- * their rows stand for NaN).  Rows outside q_indptr's ranges are left as they are.
+ * their rows stand for NaN), but that an infinity in v whose probability is below fp32's range
+ * beside the largest may give NaN.  The sums are fp32 with weights of up to 2^24: |v| above
+ * 2^80 may give an infinity.  Rows outside q_indptr's ranges are left as they are.
  * max_q_len bounds every q_len: at most 1024, and 32 mask_words.  max_kv_len bounds kv_len;
  * it only chooses how the keys are shared out over workgroups (0: unknown, not shared
  * out), so last bits may change with it and with the other sequences of the call.  The
