@@ -1,8 +1,9 @@
 // Beam search's selection (gfx950): the k best of a request's beams x vocabulary continuations.
 //
 // The score of (beam b, token t) is scores[b] + x_t - log sum exp(x), x the beam's logits, in
-// fp64; a beam whose logits have no maximum (NaN, +inf, nothing but -inf), or whose own score is
-// not finite, gives -inf.  The order is by score, then beam, then logit, then token.
+// fp64 but for the exponentials (fp32, added up sixteen at a time); a beam whose logits have no
+// maximum (NaN, +inf, nothing but -inf), or whose own score is not finite, gives -inf.  The order
+// is by score, then beam, then logit, then token.
 //
 // Two launches.  part_kernel reads the logits once, a workgroup a stretch of a row: its maximum m,
 // the sum of exp(x - m), and its k best by logit (within a row the order is the logits').
@@ -102,10 +103,10 @@ __device__ __forceinline__ void rank_all(int n, int* ranks, At at, Before before
   }
 }
 
-// exp(d), d <= 0: exp2 of the product with log2(e) in two pieces, so that it is off by a few
-// 2^-24 of itself however small it is
+// exp(d): off by up to (2 + 1.3 |d|) 2^-24 of itself (the instruction's step, the product's half of
+// one, log2(e)'s own rounding)
 __device__ __forceinline__ float exp_of(float d) {
-  return __builtin_amdgcn_exp2f(fmaf(d, 1.9259630e-8f, d * 1.44269502f));
+  return __builtin_amdgcn_exp2f(d * 1.44269502f);
 }
 
 // T: float or uint16_t (bf16).  A stretch is `chunks` chunks, of which a thread holds 16 elements
@@ -166,9 +167,13 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
   if (units > 0) load(raw, 0);
   const float extra = t < tail ? number(end - tail + t) : -INFINITY;
   for (int i = t; i < kPartList; i += kPartThreads) ranks[i] = 0;
-  // the lane's maximum (it passes over NaN; the sum does not) and sum of exp(x - maximum)
-  float lm = fmaxf(extra, -INFINITY), least = -INFINITY;
-  float s = exp_of(extra - (lm == -INFINITY ? 0.0f : lm));
+  // The lane's maximum (it passes over NaN; the sum does not) and sum of exp(x - base).  Each chunk's
+  // sixteen are added up in fp32 by fours and go to an fp64 sum: in an fp32 one of a whole row
+  // (201088 numbers, few distinct) the logarithm was off by 2e-5.  The base is a maximum of the
+  // lane's and is renewed where a chunk's is more than 1 above: as many rescalings then lie
+  // behind a number as its exponent is low, however the row ascends.
+  float lm = fmaxf(extra, -INFINITY), base = lm, least = -INFINITY;
+  double s = exp_of(extra - (lm == -INFINITY ? 0.0f : lm));
   int noted = 0;  // by the wave
   // waves with fewer numbers than lanes are not counted on for the bound
   const int full = min(kWaves, max(1, (end - begin) / (64 * kEach))), q = (full + 1) / 2;
@@ -189,11 +194,14 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
     float cm = -INFINITY;
 #pragma unroll
     for (int e = 0; e < kElems; ++e) cm = fmaxf(cm, raw(e));
-    const float old = lm, base = fmaxf(old, cm) == -INFINITY ? 0.0f : fmaxf(old, cm);
-    lm = fmaxf(old, cm);
-    s *= exp_of(old - base);
+    const float old = base;
+    base = cm > old + 1.0f ? cm : old;
+    lm = fmaxf(lm, cm);
+    const float from = base == -INFINITY ? 0.0f : base;
+    float four[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < kElems; ++e) s += exp_of(raw(e) - base);
+    for (int e = 0; e < kElems; ++e) four[e & 3] += exp_of(raw(e) - from);
+    s = s * (double)exp_of(old - from) + (double)((four[0] + four[1]) + (four[2] + four[3]));
     if ((chunk & (chunk + 1)) == 0 && (chunk == 0 || chunk >= 7))
       bound(coarse, __builtin_ctz(chunk + 1) & 1);
     const uint64_t who = __ballot(cm >= least);
@@ -241,7 +249,7 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
     }
     if (t < tail && extra >= least) keep(extra, end - tail + t);
   }
-  const double sum = moe::wave_sum_f64((double)(lm == -INFINITY ? s : s * exp_of(lm - m)));
+  const double sum = moe::wave_sum_f64(base == -INFINITY ? s : s * (double)exp_of(base - m));
   if (lane == 0) wsum[wave] = sum;
   __syncthreads();
   if (t == 0) {

@@ -336,7 +336,9 @@ MOE_API int attn_kv_copy_pages(void* kv_cache, int64_t layers, int64_t num_pages
  * width, vocab] bf16, or fp32 where logits_f32 is not 0; scores [batch, width] fp32, the beams'
  * own (-inf: a beam that has ended, or is not there yet).  The score of token t after beam b is
  * scores[b] + logits[b][t] - log sum exp(logits[b]), summed and compared in fp64 (the
- * exponentials off by a few 2^-24 of themselves) and rounded once to fp32; a row of
+ * exponentials, sixteen at a time, in fp32: off by a few 2^-24 of themselves and of their
+ * exponents, which puts the logarithm off by less than 2^-21 (2 + ln vocab), of the rows
+ * measured by less than 2^-20) and rounded once to fp32; a row of
  * logits without a maximum (a NaN, +inf, nothing but -inf) and a beam whose own score is not
  * finite give -inf.  In descending order, equal ones by beam, then logit, then token: out_scores,
  * out_beams (0 .. width - 1 within the request) and out_tokens [batch, k].  width and k up to
