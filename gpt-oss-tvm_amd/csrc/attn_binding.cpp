@@ -178,6 +178,8 @@ std::tuple<Tensor, Tensor, Tensor> beam_top_k(const Tensor& logits, const Tensor
   const int64_t vocab = logits.dim() ? logits.size(-1) : 0;
   const auto* sc = (const float*)need(call, scores, "scores", kFloat, {batch, width});
   const void* x = need(call, logits, "logits", f32 ? kFloat : kBf16, {batch * width, vocab});
+  Tensor moved;  // rows of bf16 from an odd element on: the entry point wants 4-byte words
+  if ((uintptr_t)x & 3u) x = (moved = logits.clone()).data_ptr();
   if (k < 1 || k > kBeams || k > width * vocab || width > kBeams)
     throw py::value_error("k: " + std::to_string(k) + " of " + std::to_string(width) +
                           " beams and " + std::to_string(vocab) + " tokens; both up to " +

@@ -781,7 +781,7 @@ int attn_beam_top_k(const void* logits, int32_t logits_f32, int64_t batch, int64
   if (batch == 0) return MOE_OK;
   if (!logits || !scores || !out_scores || !out_beams || !out_tokens || !workspace)
     return MOE_ERR_NULL;
-  if (!a16(logits) || !a4(scores) || !a4(out_scores) || !a4(out_beams) || !a4(out_tokens) ||
+  if (!a4(logits) || !a4(scores) || !a4(out_scores) || !a4(out_beams) || !a4(out_tokens) ||
       !a16(workspace))
     return MOE_ERR_ALIGN;
   const size_t need = attn_beam_workspace_bytes(batch, width, vocab, k);

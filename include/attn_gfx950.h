@@ -342,8 +342,8 @@ MOE_API int attn_kv_copy_pages(void* kv_cache, int64_t layers, int64_t num_pages
  * logits without a maximum (a NaN, +inf, nothing but -inf) and a beam whose own score is not
  * finite give -inf.  In descending order, equal ones by beam, then logit, then token: out_scores,
  * out_beams (0 .. width - 1 within the request) and out_tokens [batch, k].  width and k up to
- * 64, k at most width * vocab, batch up to 65535, vocab below 2^30.  Rows of logits may begin
- * at any element.  The workspace needs no initialisation; calls on one have to follow one
+ * 64, k at most width * vocab, batch up to 65535, vocab below 2^30.  Logits need an alignment
+ * of 4 bytes only, the rows behind the first may begin at any element.  The workspace needs no initialisation; calls on one have to follow one
  * another.  attn_beam_workspace_bytes is 0 where the call would be refused. */
 MOE_API size_t attn_beam_workspace_bytes(int64_t batch, int64_t width, int64_t vocab, int64_t k);
 MOE_API int attn_beam_top_k(const void* logits, int32_t logits_f32, int64_t batch, int64_t width,
