@@ -3,7 +3,8 @@
 
 Same rules as ``moe_native``: GPU tensors only, dtype / shape / contiguity
 checked before anything is launched, torch's current stream, RuntimeError on
-a non-zero status, no fallback when a library is missing.
+a non-zero status, no fallback when a library is missing (the binding's functions raise
+ImportError when they are called, libmoe_gfx950.so's absence on import).
 """
 from __future__ import annotations
 
@@ -16,9 +17,20 @@ from moe_native import _check, _expect, _ptr, _stream
 
 try:
     import attn_binding  # csrc/attn_binding.cpp, over the library that moe_native loaded
-except ImportError as e:
-    raise ImportError("attn_binding.so is missing or does not load: build it with "
-                      "`python gpt-oss-tvm_amd/build_native.py` (or __graft_entry__.build())") from e
+except ImportError as _error:
+
+    class _Missing:
+        """In place of the binding: its functions raise, everything else works without them."""
+
+        def __init__(self, cause: ImportError):
+            self._cause = cause
+
+        def __getattr__(self, name: str):
+            raise ImportError(f"{name}: attn_binding.so is missing or does not load; build it with "
+                              "`python gpt-oss-tvm_amd/build_native.py` (or "
+                              "__graft_entry__.build())") from self._cause
+
+    attn_binding = _Missing(_error)
 
 _lib = moe_native.lib()
 
