@@ -340,7 +340,8 @@ MOE_API int attn_kv_copy_pages(void* kv_cache, int64_t layers, int64_t num_pages
  * exponents, which puts the logarithm off by less than 2^-21 (2 + ln vocab), of the rows
  * measured by less than 2^-20) and rounded once to fp32; a row of
  * logits without a maximum (a NaN, +inf, nothing but -inf) and a beam whose own score is not
- * finite give -inf.  In descending order, equal ones by beam, then logit, then token: out_scores,
+ * finite give -inf.  In descending order, equal ones by beam, then logit, then token (those of
+ * -inf by beam and token): out_scores,
  * out_beams (0 .. width - 1 within the request) and out_tokens [batch, k].  width and k up to
  * 64, k at most width * vocab, batch up to 65535, vocab below 2^30.  Logits need an alignment
  * of 4 bytes only, the rows behind the first may begin at any element.  The workspace needs no initialisation; calls on one have to follow one

@@ -310,14 +310,17 @@ def tree_walk(tokens, parents, chosen) -> list:
 
 def beam_top_k(logits: np.ndarray, scores: np.ndarray, k: int):
     """logits [width, vocab], scores [width] -> (scores fp64, beams, tokens) of the k best
-    continuations: by score in fp64, then beam, then token."""
+    continuations: by score in fp64, then beam, then logit (scores of different logits may be
+    equal), then token; scores of -inf by beam and token."""
     x = logits.astype(np.float64)
     with np.errstate(all="ignore"):
         top = x.max(axis=1, keepdims=True)
         s = scores.astype(np.float64)[:, None] + (
             (x - top) - np.log(np.exp(x - top).sum(axis=1, keepdims=True)))
-    s = np.where(np.isnan(s), -np.inf, s).ravel()
-    order = np.argsort(-s, kind="stable")[:k]
+    s = np.where(np.isnan(s), -np.inf, s)
+    beam = np.broadcast_to(np.arange(len(x))[:, None], s.shape)
+    order = np.lexsort((-np.where(s == -np.inf, -np.inf, x).ravel(), beam.ravel(), -s.ravel()))[:k]
+    s = s.ravel()
     return s[order], order // x.shape[1], order % x.shape[1]
 
 
