@@ -34,7 +34,8 @@ lists may be longer than the pool: the tables have room for ``max_listed`` entri
 whole pool a sequence, up to 2^22 more than the pool has), and a forward that lists more is refused.
 
 ``begin_tree`` appends a tree of drafted tokens to each sequence in place of a chunk: the tables
-then also have each node's mask over its tree, and positions by depth.
+then also have each node's mask over its tree, and positions by depth.  Masks and parents are new
+tensors, built on the host in each call: a forward of trees is not for capture in a graph.
 """
 from __future__ import annotations
 
