@@ -351,16 +351,16 @@ class PagedKVCache:
                               f"have room for {self.max_listed} (max_listed)")
         need = sum(max(0, -(-n // PAGE_SIZE) - len(self.seqs[s].pages)) for s, n in grown.items())
         # a copy for each that writes to a shared page; the last of its holders keeps it
-        writers = Counter(self.seqs[s].pages[-1] for s in set(seq_ids)
-                          if self._shares_last(self.seqs[s]))
-        need += sum(w - (w == self._refs[page]) for page, w in writers.items())
+        writers = [self.seqs[s].pages[-1] for s in grown if self._shares_last(self.seqs[s])]
+        if writers:
+            need += sum(w - (w == self._refs[page]) for page, w in Counter(writers).items())
         if need > len(self.free):
             raise MemoryError(f"KV cache full: {need} pages needed, {len(self.free)} free")
         q_indptr, positions, slots, page_indptr, page_indices, kv_len = [0], [], [], [0], [], []
         copies = []
         for i, (sid, a) in enumerate(zip(seq_ids, append_lengths)):
             s = self.seqs[sid]
-            if self._shares_last(s):  # others keep that page
+            if writers and self._shares_last(s):  # others keep that page
                 shared = s.pages[-1]
                 s.pages[-1] = self._take()
                 self._drop([shared])
