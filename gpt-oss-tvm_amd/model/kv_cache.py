@@ -324,11 +324,11 @@ class PagedKVCache:
                     depth[i], sees[i] = depth[p] + 1, sees[p] | 1 << i
             depths.append(depth)
             masks += [[(x >> (32 * w)) & 0xFFFFFFFF for w in range(words)] for x in sees]
-        tables = self.begin_forward(seq_ids, [len(tree) for tree in parents], depths)
         flat = np.array([p for tree in parents for p in tree], dtype=np.int32)
         mask = np.array(masks, dtype=np.uint32).view(np.int32).reshape(-1, words)
-        tables.parents = torch.from_numpy(flat).to(self.data.device)
-        tables.tree_mask = torch.from_numpy(mask).to(self.data.device)
+        flat, mask = (torch.from_numpy(x).to(self.data.device) for x in (flat, mask))
+        tables = self.begin_forward(seq_ids, [len(tree) for tree in parents], depths)
+        tables.parents, tables.tree_mask = flat, mask
         return tables
 
     def begin_forward(self, seq_ids, append_lengths, depths=None) -> ForwardTables:

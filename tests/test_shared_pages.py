@@ -87,3 +87,17 @@ def test_lists_that_do_not_fit_are_refused_whole():
 def test_room_of_the_tables():
     assert make(24, 4, 64)._page_indices.numel() == 96
     assert make(24, 1, 64)._page_indices.numel() == 24
+
+
+def test_trees_whose_upload_fails_change_nothing(monkeypatch):
+    c = branched(20, 2, 24)
+
+    def fails(_):
+        raise MemoryError("no memory")
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "from_numpy", fails)
+        with pytest.raises(MemoryError):
+            c.begin_tree([0, 1], [[-1, 0], [-1]])
+    assert c.seq_len(0) == c.seq_len(1) == 20 and c.tables is None
+    assert c.begin_tree([0, 1], [[-1, 0], [-1]]).parents.tolist() == [-1, 0, -1]
