@@ -1,7 +1,7 @@
 // The wrappers of the trees' and beams' entry points (attn_native.py), in C++: their argument
 // checks, the buffers that they allocate and the call.  A call's host time with its launches, us in
-// Python and here: a tree 17, 9.4, a selection 17, 11, a page copy 8.1, 4.6, a commit 14, 6.5; a
-// small one's kernels take 3 to 12.
+// Python and here: a tree 17, 9.4, a selection 17, 11, a page copy 8.1, 4.6, a commit 14, 6.5 (on
+// another machine here 11.8, 13.5, 7.1, 8.6); a small one's kernels take 3 to 12.
 //
 // The rules are attn_native's: GPU tensors on the current device, dtype, shape and contiguity
 // checked before anything is launched (TypeError, ValueError), torch's current stream,

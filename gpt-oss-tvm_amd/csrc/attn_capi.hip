@@ -604,7 +604,8 @@ constexpr int64_t kMaxBatch = 65535, kMaxLayers = 65535;
 // registers fill one, one a CU), each of kTreeLeast blocks or more; 0: a workgroup a tile, where
 // there are tiles enough to fill it twice over, more than 64 sequences or no bound, or where the
 // longest sequence the bound allows has few blocks and a share of them would save few.
-// us of a call (with the parts' merge) at sizes of trees x nodes over up to so many tokens:
+// us of a call (with the parts' merge) at sizes of trees x nodes over up to so many tokens
+// (probabilities in one piece; two add up to 3 us on either side):
 //  * 32 instead of 64 workgroups of 8-token tiles: 16 x 8 over 4000 28 and 25, 48 of them 28;
 //    64 instead of 32 of 16-token tiles: 4 x 16 over 8000 31 and 24, 40 x 16 over 700 38 and 31.
 //  * kTreeLeast 2, 4, 6, 8: 1 x 5 over 777 11.6, 11.9, 13.0, 13.9; 1 x 32 over 1000 18.1, 18.4,

@@ -167,12 +167,12 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //    are passed over (32 trees of 16 nodes in a window 12.2 -> 10.9).
 //
 // What bounds it, with us of the kernel alone at four sizes: 1 tree of 5 nodes over 777 tokens, 16
-// of 8 over up to 4000 (bf16), 1 of 64 over 16000, 2 of 26 over up to 131072 (8-bit): 8.2, 21,
-// 33, 137.
+// of 8 over up to 4000 (bf16), 1 of 64 over 16000, 2 of 26 over up to 131072 (8-bit): 8.7, 24,
+// 32, 134.  (Comparisons below at 4 to 16 tokens are of probabilities in one piece.)
 //  * Few nodes: the keys' bytes, and at the smallest calls the loads that wait for one another
-//    (tables, page ids, keys, parts).  16 x 8: 80 MB, 3.9 TB/s; a copy reaches 5.0.
+//    (tables, page ids, keys, parts).  16 x 8: 80 MB, 3.4 TB/s; a copy reaches 5.0.
 //  * Many nodes: the products and the exponentials beside them.  2 x 26: 85 GFLOP for tokens that
-//    are there, 620 TFLOP/s of the 1280 that a large bf16 product reaches; a wave's 32 keys take
+//    are there, 630 TFLOP/s of the 1280 that a large bf16 product reaches; a wave's 32 keys take
 //    260 cycles of matrix instructions and 250 of others, 160 of them exponentials.  At 146 in
 //    all it was 128 without the exponentials, 135 without the second product, 153 without
 //    staging: no part carries it alone.  Two 32-key tiles at once, the operands of a tile read

@@ -14,8 +14,8 @@
 // numbers of a stretch reach it, with q = 1 ten times k.  They go to LDS, and take their
 // places by counting those before them.
 //
-// What bounds it, us of the two launches at rows of 201088: 128 bf16 rows (51 MB, k = 16) 16.4 +
-// 6.3, 20 fp32 rows (16 MB, k = 10) 9 + 5.9, 4 bf16 rows (k = 8) 6.5 + 5.5.  The first is 3.1 TB/s:
+// What bounds it, us of the two launches at rows of 201088: 128 bf16 rows (51 MB, k = 16) 16.7 +
+// 6.0, 20 fp32 rows (16 MB, k = 10) 9 + 6.4, 4 bf16 rows (k = 8) 6.5 + 5.5.  The first is 3.1 TB/s:
 // a pass that only reads takes 10.6, the exponentials, bounds and lists the rest.  Few rows: loads
 // and barriers that wait for one another, in both launches.
 #include <stdint.h>

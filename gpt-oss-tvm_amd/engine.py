@@ -11,9 +11,9 @@ generated token, ``popn`` to roll the cache back.  ``kv_dtype`` torch.float8_e4m
 keeps the cache in 8 bits: half its bytes in memory and in every decode step.
 
 Beyond one continuation at a time: ``decode_tree`` verifies a tree of drafted tokens in one
-forward and gives the tokens that ``decode`` and ``sample`` would have given one by one (but where
-the kernels' rounding, another over a tree, decides between two), and ``beam_search`` follows the best continuations by their
-probability (``max_batch`` beams).
+forward and gives the tokens that ``decode`` and ``sample`` would have given one by one (but
+where the kernels' rounding, another over a tree, decides between two), and ``beam_search``
+follows the best continuations by their probability (``max_batch`` beams).
 """
 from __future__ import annotations
 

@@ -279,7 +279,9 @@ MOE_API int attn_prefill_fp8(const uint16_t* q, int64_t rows, const int32_t* q_i
  * 2^80 may give an infinity.  Rows outside q_indptr's ranges are left as they are.
  * max_q_len bounds every q_len: at most 1024, and 32 mask_words.  max_kv_len bounds kv_len;
  * it only chooses how the keys are shared out over workgroups (0: unknown, not shared
- * out), so last bits may change with it and with the other sequences of the call.  The
+ * out, nor are those of more than 64 sequences or of trees of more than 128 tiles, of 32
+ * nodes each, or of 16, 8 or 4 where max_q_len is as low), so last bits may change with
+ * it and with the other sequences of the call.  The
  * workspace (none where attn_tree_workspace_bytes is 0) needs no initialisation; calls on
  * one have to follow one another.  sm_scale > 0. */
 MOE_API size_t attn_tree_workspace_bytes(int64_t batch, int64_t max_q_len, int64_t max_kv_len,
