@@ -158,8 +158,8 @@ __device__ __forceinline__ float tree_weight(float m, float l, float top) {
 //    most, where the cached values are off by up to 16 times as much): errors against 64 bits
 //    0.0020 to 0.0021 instead of 0.0017, but two pieces would take 192 us instead of 132 for 2
 //    trees of 26 over up to 131072, 49 instead of 40 for one of 64 over 16000.  What they cost
-//    the others, graph replays, us with one and with two: 16 x 8 over 4000 29 and 32, 1 x 5 over 777
-//    16.1 and 16.4, 32 x 16 in a window 17.0 and 17.4.
+//    the others, graph replays, us with one and with two: 16 x 8 over 4000 29 and 32, 1 x 5
+//    over 777 16.1 and 16.4, 32 x 16 in a window 17.0 and 17.4.
 //  * No running maximum: the reference point is the maximum of the first keys that a column
 //    sees, and is renewed only when a tile's sum passes 2^24.
 //  * Blocks that every token of a wave sees whole take no mask; in the others (the tree's own, a
@@ -496,8 +496,8 @@ __device__ __forceinline__ void tree_piece(const TreeArgs& a, TreeLds<kC, kK>& l
   // Infinities and NaN in v of a bf16 cache.  They must not meet the probability 0 of who does not
   // see their key, nor the second piece of one, which may be 0 or negative: staged as 0, they
   // go in behind the loop (blocks first to last of the group, again from memory) by products of
-  // their own.  The largest number for them and for who sees them, whose square is past fp32's range:
-  // +inf and NaN by one, -inf and NaN by another.  (At the products, in a branch of masked blocks,
+  // their own.  The largest number for them and for who sees them, whose square is past fp32's
+  // range: +inf and NaN by one, -inf and NaN by another.  (At the products, in a branch of masked blocks,
   // they took registers of every call: 64 x 26 over 500 73 us and not 52, 2 x 26 over 40000 119
   // and not 79.)
   auto add_bad = [&](int first, int last) __attribute__((always_inline)) {

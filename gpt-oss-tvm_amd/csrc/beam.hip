@@ -167,8 +167,8 @@ __global__ __launch_bounds__(kPartThreads) __attribute__((amdgpu_waves_per_eu(6)
   if (units > 0) load(raw, 0);
   const float extra = t < tail ? number(end - tail + t) : -INFINITY;
   for (int i = t; i < kPartList; i += kPartThreads) ranks[i] = 0;
-  // The lane's maximum (it passes over NaN; the sum does not) and sum of exp(x - base).  Each chunk's
-  // sixteen are added up in fp32 by fours and go to an fp64 sum: in an fp32 one of a whole row
+  // The lane's maximum (it passes over NaN; the sum does not) and sum of exp(x - base).  Each
+  // chunk's sixteen are added up in fp32 by fours and go to an fp64 sum: in an fp32 one of a whole row
   // (201088 numbers, few distinct) the logarithm was off by 2e-5.  The base is a maximum of the
   // lane's and is renewed where a chunk's is more than 1 above: as many rescalings then lie
   // behind a number as its exponent is low, however the row ascends.
